@@ -187,6 +187,147 @@ int q4gpu_lm_head_argmax_noalloc(const int32_t *act, const uint8_t *packed, cons
                                  void *stream);
 
 /* =========================================================================
+ * 16-bit paged serving operators (device pointers).  No reference
+ * counterpart: the reference runs one token at a time in fixed point, with a
+ * flat cache of 256 positions.  They are the floating-point companions of the
+ * kernels above for callers that hold activations in bf16 or f16: a layer step
+ * adds the residual and norms it, rotates the new queries and keys and stores
+ * keys and values in the pages of their sequences, and attends from the new
+ * tokens to everything stored; between steps sequences are forked and the
+ * pages in use are packed together.
+ *
+ * Every function checks its arguments on the host before any device work,
+ * enqueues on `stream` and returns without synchronising.  Strides count
+ * elements.  Sums, softmax statistics and rotations are held in 32 bits and
+ * each result is rounded once.  What only the device can check (a position, a
+ * row, a page or a slot named in device memory) is checked there: the access
+ * is skipped and *err_flag (an optional device int that the caller zeroes) is
+ * set to 1.
+ * ======================================================================= */
+enum { Q4GPU_F32 = 0, Q4GPU_F16 = 1, Q4GPU_BF16 = 2, Q4GPU_E4M3 = 3, Q4GPU_S8 = 4 };
+
+/* Residual addition and root-mean-square norm over `rows` rows of n values:
+ *   h = x + residual (or x);  y = h / sqrt(mean(h^2) + eps) * weight.
+ * dtype (F32, F16, BF16) is that of x, residual, weight and residual_out; the
+ * norm uses h before its rounding to residual_out (optional).  out_dtype is
+ * dtype, or E4M3 / S8: then every `group` columns (8, 16, .. 256, a divisor of
+ * n; 0 = the whole row) share one float32 scale = max|y| / M (M = 448 or 127),
+ * scale [rows, n / group] contiguous, and out = round(y * (M / max|y|)), ties
+ * to even; a group of zeros has scale 0.  1 <= n <= Q4GPU_NORM_MAX_N.
+ * residual_out may be x or residual, out may be x, with the same strides.
+ * With group > 0 every row of x, residual, residual_out, weight and out starts
+ * on a 16-byte (out: 8-byte) boundary, or Q4GPU_ERR_ALIGN. */
+#define Q4GPU_NORM_MAX_N 32768
+typedef struct q4gpu_norm_args {
+    const void *x, *residual, *weight;
+    void *out, *residual_out;
+    float *scale;
+    int64_t rows, x_stride, residual_stride, out_stride, residual_out_stride;
+    int32_t n, group, dtype, out_dtype;
+    float eps;
+    int32_t reserved;
+} q4gpu_norm_args;
+int q4gpu_add_rmsnorm(const q4gpu_norm_args *a, void *stream);
+
+/* Rotary positions of new tokens and their storage in a paged cache.
+ * q [tokens, q_heads, dim], k and v [tokens, kv_heads, dim] (F16 or BF16, head
+ * vectors contiguous).  With q_gamma / k_gamma [dim] each head vector is
+ * normed first (x / sqrt(mean(x^2) + eps) * gamma).  Then its first rot_dim
+ * values are rotated by the angle whose cosine and sine stand in row
+ * positions[token] of cos / sin (float32 [table_positions, rot_dim / 2]):
+ *   (a, b) -> (a cos - b sin, b cos + a sin),
+ * pair i being values (i, i + rot_dim / 2), or (2i, 2i + 1) with interleaved.
+ * Rotated queries go to q_out (may be q); rotated keys and unchanged values
+ * go to cache row rows[token] = page * page_tokens + offset, at
+ *   cache + page * page_stride + head * head_stride + offset * row_stride;
+ * a negative row stores nothing.  q, k or v may be NULL (with its outputs).
+ * rot_dim is a multiple of 16, dim a multiple of 8 up to 512; every head
+ * vector starts on a 16-byte boundary. */
+typedef struct q4gpu_rope_args {
+    const void *q, *k, *v;
+    void *q_out, *k_cache, *v_cache;
+    const void *q_gamma, *k_gamma;
+    const float *cos, *sin;
+    const int32_t *positions;
+    const int64_t *rows;
+    int32_t *err_flag;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t q_out_token_stride, q_out_head_stride, page_stride, head_stride, row_stride;
+    int64_t n_rows; /* rows of the cache: pages * page_tokens */
+    int32_t tokens, q_heads, kv_heads, dim, rot_dim, interleaved, dtype, page_tokens, table_positions;
+    float eps;
+} q4gpu_rope_args;
+int q4gpu_rope_append(const q4gpu_rope_args *a, void *stream);
+
+/* Attention of each sequence's newest tokens to its pages.  Sequence i owns
+ * query tokens [cu_q[i], cu_q[i + 1]) (int32 [n_seqs + 1], at most max_q
+ * each) and slot s = seq_ids[i] (NULL: i): keys 0 .. lens[s] - 1 stand in the
+ * pages table[s][0 ..] (int32, table_stride entries a slot), page_tokens each
+ * (16, 32, 64 or 128), at cache + page * page_stride + kv_head * head_stride +
+ * offset * row_stride.  The new tokens are the last of those keys: query t of
+ * n stands at position p = lens[s] - n + t and sees keys j <= p, with
+ * window > 0 only j > p - window.  Query head h reads key head
+ * h / (q_heads / kv_heads).
+ *   out = sum_j softmax_j(scale * q.k_j) v_j,  lse = log sum_j exp(scale * q.k_j)
+ * out [tokens, q_heads, dim]; lse (optional) float32 [tokens, q_heads]
+ * contiguous.  A query that sees no key (p < 0, or pages whose table entry is
+ * outside 0 .. n_pages - 1, which hold no keys) gets zeros and -infinity.
+ * What stands in a key or value row that a query does not see does not reach
+ * its result.  dim is 64 or 128; F16 or BF16; query and cache head vectors
+ * start on 16-byte boundaries.
+ * max_ctx bounds lens[s]; it only decides how the work is split.
+ * workspace: q4gpu_paged_attention_workspace_bytes(a) bytes, 16-byte aligned
+ * (0 bytes: may be NULL), zeroed once before its first use (each call leaves
+ * its counters at zero) and not shared by calls that can overlap. */
+typedef struct q4gpu_attn_args {
+    const void *q, *k_cache, *v_cache;
+    void *out;
+    float *lse;
+    const int32_t *table, *lens, *cu_q, *seq_ids;
+    void *workspace;
+    uint64_t workspace_bytes;
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    int64_t page_stride, head_stride, row_stride, table_stride;
+    int32_t n_seqs, n_slots, tokens, max_q, max_ctx, q_heads, kv_heads, dim, page_tokens, n_pages, window, dtype;
+    float scale;
+    int32_t reserved;
+} q4gpu_attn_args;
+size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args *a);
+int q4gpu_paged_attention(const q4gpu_attn_args *a, void *stream);
+
+/* A pool of pages and the tables that name them.  A page is page_bytes long:
+ * blocks of block_bytes (one per layer, K/V and head), each page_tokens rows.
+ * Slot s holds lens[s] tokens in pages table[s][0 .. ceil(lens[s] / page_tokens)).
+ * Pages, blocks and rows are multiples of 16 bytes. */
+typedef struct q4gpu_pages_args {
+    void *pool;
+    int32_t *table; /* [n_slots, table_stride] */
+    int32_t *lens;  /* [n_slots] */
+    int32_t *err_flag;
+    int64_t page_bytes, block_bytes, table_stride;
+    int32_t n_pages, page_tokens, n_slots, reserved;
+} q4gpu_pages_args;
+
+/* n sequences branch off (device int32 arrays of n): slot children[i] gets the
+ * pages of slot parents[i]; where the last of them is partly filled, its filled
+ * rows are copied to page fresh[i], which takes its place.  Full pages are
+ * shared.  Entries past the last page are set to -1.  Children are distinct,
+ * no child is a parent, no fresh page is in use. */
+int q4gpu_pages_fork(const q4gpu_pages_args *a, const int32_t *parents, const int32_t *children,
+                     const int32_t *fresh, int32_t n, void *stream);
+
+/* Packs the pages in use (named in any slot's first ceil(lens / page_tokens)
+ * entries; shared pages once) into pages 0 .. n_live - 1: the i-th used page
+ * from n_live on, in ascending order, moves to the i-th unused page below it.
+ * new_table (may be a->table) gets the renumbered entries, -1 past each
+ * slot's last; remap[old page] (int32 [n_pages]) the new number or -1; *n_live
+ * the number of pages in use.  All arrays are device memory; workspace:
+ * q4gpu_pages_compact_workspace_bytes(n_pages) bytes, 16-byte aligned. */
+size_t q4gpu_pages_compact_workspace_bytes(int32_t n_pages);
+int q4gpu_pages_compact(const q4gpu_pages_args *a, int32_t *new_table, int32_t *remap, int32_t *n_live,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* =========================================================================
  * Runner seam: types of the reference's host runtime
  * (FPGA_Project/software/qmap_one_token_runtime/qmap_one_token_runtime.h:17-82),
  * declared here with the same names and layout unless that header is

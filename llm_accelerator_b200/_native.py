@@ -90,6 +90,44 @@ class QmapTensor(C.Structure):
                 ("rows", C.c_int32), ("cols", C.c_int32), ("elem_stride", C.c_int32), ("elem_kind", C.c_int32)]
 
 
+class NormArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "weight", "out", "residual_out", "scale")] + \
+               [(n, C.c_int64) for n in ("rows", "x_stride", "residual_stride", "out_stride",
+                                         "residual_out_stride")] + \
+               [(n, C.c_int32) for n in ("n", "group", "dtype", "out_dtype")] + \
+               [("eps", C.c_float), ("reserved", C.c_int32)]
+
+
+class RopeArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "q_gamma", "k_gamma", "cos",
+                                          "sin", "positions", "rows", "err_flag")] + \
+               [(n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                         "v_token_stride", "v_head_stride", "q_out_token_stride",
+                                         "q_out_head_stride", "page_stride", "head_stride", "row_stride",
+                                         "n_rows")] + \
+               [(n, C.c_int32) for n in ("tokens", "q_heads", "kv_heads", "dim", "rot_dim", "interleaved", "dtype",
+                                         "page_tokens", "table_positions")] + [("eps", C.c_float)]
+
+
+class AttnArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "out", "lse", "table", "lens", "cu_q", "seq_ids",
+                                          "workspace")] + [("workspace_bytes", C.c_uint64)] + \
+               [(n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride",
+                                         "page_stride", "head_stride", "row_stride", "table_stride")] + \
+               [(n, C.c_int32) for n in ("n_seqs", "n_slots", "tokens", "max_q", "max_ctx", "q_heads", "kv_heads",
+                                         "dim", "page_tokens", "n_pages", "window", "dtype")] + \
+               [("scale", C.c_float), ("reserved", C.c_int32)]
+
+
+class PagesArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("pool", "table", "lens", "err_flag")] + \
+               [(n, C.c_int64) for n in ("page_bytes", "block_bytes", "table_stride")] + \
+               [(n, C.c_int32) for n in ("n_pages", "page_tokens", "n_slots", "reserved")]
+
+
+# element types of the 16-bit paged operators (Q4GPU_F32 ..)
+DT_F32, DT_F16, DT_BF16, DT_E4M3, DT_S8 = range(5)
+
 QMAP_PACKED_Q4, QMAP_S16, QMAP_U16, QMAP_U32 = range(4)
 
 P = C.c_void_p
@@ -116,6 +154,13 @@ SIGNATURES = {
     "q4gpu_lm_head_workspace_bytes": (SZ, [I32]),
     "q4gpu_lm_head_argmax": (C.c_int, [P, P, P, I32, P, P, SZ, P, P, P]),
     "q4gpu_lm_head_argmax_noalloc": (C.c_int, [P, P, P, I32, P, P, P, P]),
+    "q4gpu_add_rmsnorm": (C.c_int, [C.POINTER(NormArgs), P]),
+    "q4gpu_rope_append": (C.c_int, [C.POINTER(RopeArgs), P]),
+    "q4gpu_paged_attention_workspace_bytes": (SZ, [C.POINTER(AttnArgs)]),
+    "q4gpu_paged_attention": (C.c_int, [C.POINTER(AttnArgs), P]),
+    "q4gpu_pages_fork": (C.c_int, [C.POINTER(PagesArgs), P, P, P, I32, P]),
+    "q4gpu_pages_compact_workspace_bytes": (SZ, [I32]),
+    "q4gpu_pages_compact": (C.c_int, [C.POINTER(PagesArgs), P, P, P, P, SZ, P]),
     "q4gpu_model_create": (C.c_int, [C.POINTER(ModelConfig), C.POINTER(P)]),
     "q4gpu_model_destroy": (None, [P]),
     "q4gpu_model_init_synthetic": (C.c_int, [P, U64, C.c_float, C.c_float]),

@@ -1,0 +1,360 @@
+"""16-bit paged serving operators on torch CUDA tensors.
+
+The floating-point companions of the fixed-point kernels, for callers that
+hold activations in bf16 or f16: the operators of one layer step over a paged
+K/V cache, and what happens to the cache's pages between steps.
+
+* ``AddRmsNorm``  residual addition + RMS norm, 16-bit or 8-bit output with scales
+* ``RopeAppend``  q/k head norm, rotary positions, K/V stored in their pages
+* ``Attention``   a chunk of new tokens per sequence (or one) over the pages
+* ``Pages``       forking sequences, packing the pages in use
+* ``PagedCache``  a pool with its tables, and which pages are free
+
+Each operator is an object that holds what a serving loop keeps (weights,
+tables, cache, workspace) and is called with the step's tensors.  Calls
+enqueue on torch's current stream and do not synchronise; a workspace belongs
+to its object, so one object's calls run on one stream at a time.  Nothing has
+a reference counterpart (the reference decodes one token at a time in fixed
+point with a flat cache of 256 positions,
+``FPGA_Project/software/qmap_one_token_runtime/qmap_one_token_runtime.h:369-500``).
+Wrong arguments raise ``ValueError`` here or ``_native.Q4GpuError`` from the
+library, both before any device work; there is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _native
+
+_DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.bfloat16: _native.DT_BF16,
+           torch.float8_e4m3fn: _native.DT_E4M3, torch.int8: _native.DT_S8}
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on(t: torch.Tensor, device: torch.device, name: str, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """`t`, if it is a CUDA tensor of this device (and type)."""
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
+    return t
+
+
+def _cuda(t: torch.Tensor, name: str) -> torch.device:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU fallback)")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return t.device
+
+
+class AddRmsNorm:
+    """h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight, per row.
+
+    ``out_dtype`` is the weight's type (default), ``torch.float8_e4m3fn`` or
+    ``torch.int8``; an 8-bit output has one float32 scale per ``group`` columns
+    (0: per row), y = out * scale.
+    """
+
+    def __init__(self, weight: torch.Tensor, eps: float = 1e-6, out_dtype: Optional[torch.dtype] = None,
+                 group: int = 0):
+        self.lib = _native.load()
+        self.device = _cuda(weight, "weight")
+        _need(weight.dim() == 1 and weight.is_contiguous(), "weight must be a contiguous vector")
+        _need(weight.dtype in (torch.float32, torch.float16, torch.bfloat16), f"weight is {weight.dtype}")
+        self.weight, self.n, self.dtype = weight, weight.shape[0], weight.dtype
+        self.out_dtype = out_dtype or weight.dtype
+        _need(self.out_dtype in _DTYPES, f"unsupported output type {self.out_dtype}")
+        self.narrow = self.out_dtype in (torch.float8_e4m3fn, torch.int8)
+        self.groups = self.n // group if group else 1
+        self.args = _native.NormArgs(weight=weight.data_ptr(), n=self.n, group=group, dtype=_DTYPES[weight.dtype],
+                                     out_dtype=_DTYPES[self.out_dtype], eps=eps)
+
+    def _rows(self, t: torch.Tensor, rows: int, name: str, dtype: torch.dtype) -> int:
+        if t.dtype != dtype or t.device != self.device:
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {dtype} on {self.device}")
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != self.n or (t.stride(1) != 1 and self.n > 1):
+            raise ValueError(f"{name} must be [{rows}, {self.n}] with contiguous rows")
+        return t.stride(0)
+
+    def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                 residual_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
+        """x, residual, residual_out, out: [rows, n]; returns out, or (out, scale) for 8 bits."""
+        _need(x.dim() == 2, "x must be [rows, n]")
+        rows = x.shape[0]
+        a = self.args
+        if out is None:
+            out = torch.empty(rows, self.n, dtype=self.out_dtype, device=self.device)
+        a.rows = rows
+        a.x, a.x_stride = x.data_ptr(), self._rows(x, rows, "x", self.dtype)
+        a.out, a.out_stride = out.data_ptr(), self._rows(out, rows, "out", self.out_dtype)
+        a.residual = a.residual_out = a.scale = None
+        if residual is not None:
+            a.residual, a.residual_stride = residual.data_ptr(), self._rows(residual, rows, "residual", self.dtype)
+        if residual_out is not None:
+            a.residual_out = residual_out.data_ptr()
+            a.residual_out_stride = self._rows(residual_out, rows, "residual_out", self.dtype)
+        if self.narrow:
+            if scale is None:
+                scale = torch.empty(rows, self.groups, dtype=torch.float32, device=self.device)
+            _on(scale, self.device, "scale", torch.float32)
+            _need(scale.shape == (rows, self.groups) and scale.is_contiguous(),
+                  f"scale must be contiguous [{rows}, {self.groups}]")
+            a.scale = scale.data_ptr()
+        rc = self.lib.q4gpu_add_rmsnorm(a, _stream())
+        if rc:
+            _native.check(rc, "q4gpu_add_rmsnorm")
+        return (out, scale) if self.narrow else out
+
+
+class _Err:
+    """The device error word of an operator: `check` waits for the stream and raises once."""
+
+    def _new_err(self) -> None:
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+
+    def check(self) -> None:
+        if int(self.err.item()):
+            self.err.zero_()
+            raise _native.Q4GpuError(f"{type(self).__name__}: a position, row, page or slot was out of range; "
+                                     "what it named was left untouched")
+
+
+class RopeAppend(_Err):
+    """Rotary positions of new tokens, keys and values stored in their pages.
+
+    ``cos`` / ``sin`` float32 [positions, rot_dim / 2] (``tables.rope_float_tables``);
+    ``q_gamma`` / ``k_gamma`` [dim] norm each head vector first.
+    """
+
+    def __init__(self, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False,
+                 q_gamma: Optional[torch.Tensor] = None, k_gamma: Optional[torch.Tensor] = None, eps: float = 1e-6):
+        self.lib = _native.load()
+        self.device = _cuda(cos, "cos")
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            _on(t, self.device, name, torch.float32)
+            _need(t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape, f"{name} must be [positions, rot / 2]")
+        self.cos, self.sin, self.q_gamma, self.k_gamma = cos, sin, q_gamma, k_gamma
+        self._new_err()
+        a = self.args = _native.RopeArgs(cos=cos.data_ptr(), sin=sin.data_ptr(), table_positions=cos.shape[0],
+                                         rot_dim=2 * cos.shape[1], interleaved=int(interleaved), eps=eps,
+                                         err_flag=self.err.data_ptr())
+        self.gamma_dim = None
+        for g, name in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+            if g is not None:
+                _on(g, self.device, name)
+                _need(g.dim() == 1 and g.is_contiguous(), f"{name} must be a contiguous vector")
+                _need(self.gamma_dim in (None, (g.shape[0], g.dtype)), "q_gamma and k_gamma differ in size or type")
+                self.gamma_dim = (g.shape[0], g.dtype)
+                setattr(a, name, g.data_ptr())
+
+    def __call__(self, q: Optional[torch.Tensor], k: Optional[torch.Tensor], v: Optional[torch.Tensor],
+                 positions: torch.Tensor, rows: Optional[torch.Tensor], k_cache: Optional[torch.Tensor],
+                 v_cache: Optional[torch.Tensor], q_out: Optional[torch.Tensor] = None):
+        """q [tokens, q_heads, dim], k / v [tokens, kv_heads, dim] (any of them None);
+        positions int32 [tokens]; rows int64 [tokens], the cache row of each token
+        (page * page_tokens + offset, negative: not stored); k_cache / v_cache
+        [pages, kv_heads, page_tokens, dim].  Returns q_out (default: q in place)."""
+        ref = q if q is not None else k if k is not None else v
+        _need(ref is not None, "one of q, k, v is needed")
+        tokens, _, dim = ref.shape
+        dtype, a = ref.dtype, self.args
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"head vectors are {dtype}, expected float16 or bfloat16")
+        _need(self.gamma_dim in (None, (dim, dtype)), f"gamma does not match head vectors of {dim} x {dtype}")
+        a.tokens, a.dim, a.dtype, a.q_heads, a.kv_heads = tokens, dim, _DTYPES[dtype], 0, 0
+        a.q = a.k = a.v = a.q_out = a.k_cache = a.v_cache = a.positions = a.rows = None
+        if q is not None or k is not None:
+            _on(positions, self.device, "positions", torch.int32)
+            _need(positions.shape == (tokens,) and positions.is_contiguous(), f"positions must be [{tokens}]")
+            a.positions = positions.data_ptr()
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            a.q_heads = q.shape[1]
+            a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, a.q_heads, dim, dtype, "q")
+            a.q_out, a.q_out_token_stride, a.q_out_head_stride = self._heads(q_out, tokens, a.q_heads, dim, dtype,
+                                                                             "q_out")
+        if k is not None or v is not None:
+            _on(rows, self.device, "rows", torch.int64)
+            _need(rows.shape == (tokens,) and rows.is_contiguous(), f"rows must be [{tokens}]")
+            a.rows = rows.data_ptr()
+            a.kv_heads = (k if k is not None else v).shape[1]
+            cache = k_cache if k is not None else v_cache
+            for t, c, name in ((k, k_cache, "k"), (v, v_cache, "v")):
+                if t is None:
+                    continue
+                p, ts, hs = self._heads(t, tokens, a.kv_heads, dim, dtype, name)
+                setattr(a, name, p)
+                setattr(a, name + "_token_stride", ts)
+                setattr(a, name + "_head_stride", hs)
+                _on(c, self.device, name + "_cache", dtype)
+                st = c.stride()
+                if c.dim() != 4 or c.shape != cache.shape or st != cache.stride() or st[3] != 1 or \
+                        c.shape[1] != a.kv_heads or c.shape[3] != dim:
+                    raise ValueError(f"{name}_cache must be [pages, {a.kv_heads}, page_tokens, {dim}] with contiguous "
+                                     "head vectors, K and V laid out alike")
+                setattr(a, name + "_cache", c.data_ptr())
+            a.page_stride, a.head_stride, a.row_stride, _ = cache.stride()
+            a.page_tokens, a.n_rows = cache.shape[2], cache.shape[0] * cache.shape[2]
+        rc = self.lib.q4gpu_rope_append(a, _stream())
+        if rc:
+            _native.check(rc, "q4gpu_rope_append")
+        return q_out
+
+    def _heads(self, t: torch.Tensor, tokens: int, heads: int, dim: int, dtype: torch.dtype, name: str):
+        if t.device != self.device or t.dtype != dtype:
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {dtype} on {self.device}")
+        ts, hs, ds = t.stride()
+        if t.shape != (tokens, heads, dim) or ds != 1:
+            raise ValueError(f"{name} must be [{tokens}, {heads}, {dim}] with contiguous head vectors")
+        return t.data_ptr(), ts, hs
+
+
+class Attention:
+    """Attention of each sequence's newest tokens to its pages.
+
+    ``k_cache`` / ``v_cache`` [pages, kv_heads, page_tokens, dim] (bf16 or f16, K and
+    V laid out alike), ``table`` int32 [slots, pages per slot], ``lens`` int32 [slots]:
+    the keys a slot holds, the new ones included.  ``scale`` defaults to
+    dim ** -0.5; with ``window`` a query sees the last ``window`` keys up to its own.
+    """
+
+    def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                 q_heads: int, scale: Optional[float] = None, window: int = 0):
+        self.lib = _native.load()
+        self.device = _cuda(k_cache, "k_cache")
+        self.dtype = k_cache.dtype
+        _need(self.dtype in (torch.float16, torch.bfloat16), f"the cache is {self.dtype}")
+        _on(v_cache, self.device, "v_cache", self.dtype)
+        _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride() and
+              k_cache.stride(3) == 1, "k_cache and v_cache must be [pages, kv_heads, page_tokens, dim], laid out alike")
+        _on(table, self.device, "table", torch.int32)
+        _on(lens, self.device, "lens", torch.int32)
+        _need(table.dim() == 2 and table.stride(1) == 1 and lens.dim() == 1 and lens.is_contiguous() and
+              lens.shape[0] == table.shape[0], "table must be [slots, pages] and lens [slots]")
+        pages, kv_heads, page_tokens, dim = k_cache.shape
+        self.q_heads, self.dim, self.slots = q_heads, dim, table.shape[0]
+        self.k_cache, self.v_cache, self.table, self.lens = k_cache, v_cache, table, lens
+        self.workspace = None
+        # a row of the table is as long as its stride lets it name
+        self.args = _native.AttnArgs(
+            k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr(),
+            page_stride=k_cache.stride(0), head_stride=k_cache.stride(1), row_stride=k_cache.stride(2),
+            table_stride=table.stride(0) if self.slots > 1 else table.shape[1], n_slots=self.slots, q_heads=q_heads,
+            kv_heads=kv_heads, dim=dim, page_tokens=page_tokens, n_pages=pages, window=window,
+            dtype=_DTYPES[self.dtype], scale=dim ** -0.5 if scale is None else scale)
+
+    def __call__(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
+                 max_q: int = 1, max_ctx: int = 0, lse: Optional[torch.Tensor] = None,
+                 seq_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q [tokens, q_heads, dim]; cu_q int32 [sequences + 1]: sequence i has the query
+        tokens cu_q[i] .. cu_q[i + 1] - 1, at most max_q; seq_ids int32 [sequences]: their
+        slots (default: 0, 1, ..); max_ctx: no lens is larger (0: the table's width).
+        lse (optional) float32 [tokens, q_heads] receives log sum exp of the scores."""
+        a, tokens = self.args, q.shape[0]
+        if cu_q is None:
+            raise ValueError("cu_q is needed")
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, "q")
+        a.out, a.out_token_stride, a.out_head_stride = self._heads(out, tokens, "out")
+        if cu_q.dtype != torch.int32 or cu_q.device != self.device or cu_q.dim() != 1 or cu_q.shape[0] < 1 or \
+                not cu_q.is_contiguous():
+            raise ValueError(f"cu_q must be a contiguous int32 vector on {self.device}")
+        n = cu_q.shape[0] - 1
+        a.cu_q, a.n_seqs, a.tokens, a.max_q = cu_q.data_ptr(), n, tokens, max_q
+        a.max_ctx = max_ctx or int(min(a.table_stride * a.page_tokens, 2 ** 31 - 1))
+        a.seq_ids = a.lse = None
+        if seq_ids is not None:
+            _on(seq_ids, self.device, "seq_ids", torch.int32)
+            _need(seq_ids.shape == (n,) and seq_ids.is_contiguous(), f"seq_ids must be [{n}]")
+            a.seq_ids = seq_ids.data_ptr()
+        elif n > self.slots:
+            raise ValueError(f"{n} sequences over {self.slots} slots")
+        if lse is not None:
+            _on(lse, self.device, "lse", torch.float32)
+            _need(lse.shape == (tokens, self.q_heads) and lse.is_contiguous(), f"lse must be [{tokens}, {self.q_heads}]")
+            a.lse = lse.data_ptr()
+        need = self.lib.q4gpu_paged_attention_workspace_bytes(a)
+        if need > a.workspace_bytes:
+            # the old one stays alive until the work queued on this stream is done with it
+            self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = self.workspace.data_ptr(), need
+        rc = self.lib.q4gpu_paged_attention(a, _stream())
+        if rc:
+            _native.check(rc, "q4gpu_paged_attention")
+        return out
+
+    def _heads(self, t: torch.Tensor, tokens: int, name: str):
+        if t.device != self.device or t.dtype != self.dtype:
+            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {self.dtype} on {self.device}")
+        if t.shape != (tokens, self.q_heads, self.dim) or t.stride(2) != 1:
+            raise ValueError(f"{name} must be [{tokens}, {self.q_heads}, {self.dim}] with contiguous head vectors")
+        return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+class Pages(_Err):
+    """A pool of pages [pages, ..blocks.., page_tokens, dim] and the tables that name them.
+
+    ``table`` int32 [slots, pages per slot], ``lens`` int32 [slots]; slot s holds lens[s]
+    tokens in the pages of its first ceil(lens[s] / page_tokens) entries.
+    """
+
+    def __init__(self, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, page_tokens: int):
+        self.lib = _native.load()
+        self.device = _cuda(pool, "pool")
+        _need(pool.dim() >= 3 and pool.is_contiguous() and pool.shape[-2] == page_tokens,
+              "pool must be contiguous [pages, .., page_tokens, dim]")
+        _on(table, self.device, "table", torch.int32)
+        _on(lens, self.device, "lens", torch.int32)
+        _need(table.dim() == 2 and table.is_contiguous() and lens.is_contiguous() and
+              lens.shape == (table.shape[0],), "table must be contiguous [slots, pages] and lens [slots]")
+        self.pool, self.table, self.lens = pool, table, lens
+        self._new_err()
+        es = pool.element_size()
+        self.args = _native.PagesArgs(pool=pool.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr(),
+                                      err_flag=self.err.data_ptr(), page_bytes=pool.stride(0) * es,
+                                      block_bytes=page_tokens * pool.shape[-1] * es, table_stride=table.shape[1],
+                                      n_pages=pool.shape[0], page_tokens=page_tokens, n_slots=table.shape[0])
+        self.workspace = None
+
+    def _ids(self, t: torch.Tensor, n: int, name: str) -> int:
+        if t.dtype != torch.int32 or t.device != self.device or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector of {n} on {self.device}")
+        return t.data_ptr()
+
+    def fork(self, parents: torch.Tensor, children: torch.Tensor, fresh: torch.Tensor) -> None:
+        """Slot children[i] gets the pages of slot parents[i]; a partly filled last page is
+        copied (its filled rows) to page fresh[i].  int32 [n] each."""
+        n = parents.shape[0]
+        rc = self.lib.q4gpu_pages_fork(self.args, self._ids(parents, n, "parents"), self._ids(children, n, "children"),
+                                       self._ids(fresh, n, "fresh"), n, _stream())
+        if rc:
+            _native.check(rc, "q4gpu_pages_fork")
+
+    def compact(self, new_table: torch.Tensor, remap: torch.Tensor, n_live: torch.Tensor) -> None:
+        """Moves the pages in use into the first n_live pages.  new_table (may be the table
+        itself) int32 [slots, pages per slot], remap int32 [pages] (old -> new, -1 unused),
+        n_live int32 [1]."""
+        _on(new_table, self.device, "new_table", torch.int32)
+        _need(new_table.shape == self.table.shape and new_table.is_contiguous(),
+              f"new_table must be contiguous {tuple(self.table.shape)}")
+        if self.workspace is None:
+            self.workspace = torch.empty(self.lib.q4gpu_pages_compact_workspace_bytes(self.args.n_pages),
+                                         dtype=torch.uint8, device=self.device)
+        rc = self.lib.q4gpu_pages_compact(self.args, new_table.data_ptr(), self._ids(remap, self.args.n_pages, "remap"),
+                                          self._ids(n_live, 1, "n_live"), self.workspace.data_ptr(),
+                                          self.workspace.numel(), _stream())
+        if rc:
+            _native.check(rc, "q4gpu_pages_compact")
