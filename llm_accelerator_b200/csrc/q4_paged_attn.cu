@@ -25,6 +25,324 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int token) 
   return lo;
 }
 
+// What a CTA needs to know of sequence i.
+struct Seq {
+  int slot, len, first, n;  // cache slot, stored keys, first query token, query tokens
+};
+__device__ __forceinline__ Seq sequence(const q4gpu_attn_args& a, int i) {
+  Seq s;
+  s.first = max(0, min(a.cu_q[i], a.tokens));
+  s.n = max(0, min(a.cu_q[i + 1], a.tokens) - s.first);
+  s.slot = a.seq_ids ? a.seq_ids[i] : i;
+  const bool known = s.slot >= 0 && s.slot < a.n_slots;
+  s.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[s.slot], a.table_stride * a.page_tokens)) : 0;
+  return s;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------------------
+// few query rows (decode): at most 16 (token, head) pairs share a key head
+// ---------------------------------------------------------------------------
+constexpr int kRows = 16;        // rows of one mma.sync tile
+constexpr int kTileKeys = 16;    // keys of a warp's step; a page holds whole steps
+constexpr int kRowWarps = 4;
+constexpr int kRowStages = 3;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int D>
+constexpr int row_smem() { return kRowWarps * kRowStages * 2 * kTileKeys * D * 2; }
+
+// 16-byte piece c of row r in a tile of D-value rows: pieces are exchanged
+// inside each 128-byte line by the row number, so the eight rows that an
+// ldmatrix phase reads lie in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)(r * D * 2 + ((c ^ (r & 7)) * 16)); }
+
+__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at));
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && __is_same(T, __half))
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes to shared memory, or zeros where `there` is false.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// How the keys are split over CTAs, and where the parts of a row are joined.
+struct SplitPlan {
+  int chunk;      // keys of one part, a multiple of 64
+  int parts;      // most parts of a sequence
+  float* o;       // [item][part][kRows][D] unnormalised sums
+  float2* ml;     // [item][part][kRows] running maximum (log2 units) and sum
+  int32_t* done;  // [item] finished parts
+};
+
+// blockIdx = (part, key head, sequence).  Each warp runs over its own 16-key
+// steps of the part with its own running maximum and sum, so no barrier stands
+// in the loop; the four are joined at the end, and the parts of a long
+// sequence by the CTA that finishes last, in the order of the parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, SplitPlan plan) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ float s_m[kRowWarps][kRows], s_l[kRowWarps][kRows];
+  __shared__ int s_last;
+  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Seq s = sequence(a, seq);
+  const int group = a.q_heads / a.kv_heads;
+  if (s.n == 0 || s.n > kRows / group) return;
+  const int rows = s.n * group;
+  const int pos0 = s.len - s.n, pos1 = s.len - 1;  // of the first and the last query
+  const int lo = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) & ~(kTileKeys - 1);
+  // a sequence longer than max_ctx said still gets no more than plan.parts parts
+  const int chunk = max(plan.chunk, ((s.len - lo + plan.parts - 1) / plan.parts + 63) & ~63);
+  const int parts = max(1, (s.len - lo + chunk - 1) / chunk);
+  if (part >= parts) return;
+  const int begin = lo + part * chunk, end = min(s.len, begin + chunk);
+
+  // the queries as A fragments: row g and g + 8, 16 values of a head per step
+  const int g = lane >> 2, tq = lane & 3;
+  uint32_t qf[D / 16][4];
+  int row_pos[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = g + 8 * h, t = r / group;
+    row_pos[h] = r < rows ? pos0 + t : -1;
+    const T* qp = static_cast<const T*>(a.q) + (int64_t)(s.first + t) * a.q_token_stride +
+                  (int64_t)(kvh * group + r - t * group) * a.q_head_stride + 2 * tq;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      qf[k][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
+      qf[k][h + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
+    }
+  }
+
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kRowStages * 2 * kTileKeys * D * 2);
+  constexpr int kTileBytes = kTileKeys * D * 2;
+  const int32_t* table = a.table + (int64_t)max(0, min(s.slot, a.n_slots - 1)) * a.table_stride;
+  const int steps = begin < end ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
+  const int mine = steps > warp ? (steps - warp + kRowWarps - 1) / kRowWarps : 0;
+  const int shift = 31 - __clz(a.page_tokens);
+  auto page_of = [&](int i) {
+    if (i >= mine) return -1;
+    const int p = table[(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
+    return p < a.n_pages ? p : -1;
+  };
+  int next_page = page_of(0);
+  uint32_t valid = 0;  // bit i % 32: step i's page exists
+  auto load = [&](int i) {
+    const int page = next_page;
+    next_page = page_of(i + 1);
+    if (i < mine) valid = (valid & ~(1u << (i & 31))) | ((page >= 0 ? 1u : 0u) << (i & 31));
+    if (i < mine && page >= 0) {
+      const int key = begin + kTileKeys * (warp + kRowWarps * i);
+      const int64_t off = page * a.page_stride + kvh * a.head_stride + (key & (a.page_tokens - 1)) * a.row_stride;
+      const uint32_t at = ring + (i % kRowStages) * 2 * kTileBytes;
+      constexpr int kPieces = D / 8, kPer = 32 / kPieces;  // lanes per row, rows per pass
+      const int c = lane % kPieces;
+#pragma unroll
+      for (int r0 = 0; r0 < kTileKeys; r0 += kPer) {
+        const int r = r0 + lane / kPieces;
+        // rows past the last key are zeros: whatever the page holds there meets a zero weight
+        const bool there = key + r < end;
+        const int64_t o = off + (there ? r : 0) * a.row_stride + c * 8;
+        cp16(at + piece<D>(r, c), static_cast<const T*>(a.k_cache) + o, there);
+        cp16(at + kTileBytes + piece<D>(r, c), static_cast<const T*>(a.v_cache) + o, there);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kRowStages - 1; ++i) load(i);
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  const float c2 = a.scale * kLog2e;
+  for (int i = 0; i < mine; ++i) {
+    cp_wait<kRowStages - 2>();
+    __syncwarp();
+    load(i + kRowStages - 1);
+    if (!((valid >> (i & 31)) & 1u)) continue;
+    const uint32_t kt = ring + (i % kRowStages) * 2 * kTileBytes, vt = kt + kTileBytes;
+    const int key = begin + kTileKeys * (warp + kRowWarps * i);
+    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t b[4];  // keys 0-7: b[0], b[1]; keys 8-15: b[2], b[3]
+      ldsm4(b, kt + piece<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+      mma16816<T>(sc[0], qf[k], b[0], b[1]);
+      mma16816<T>(sc[1], qf[k], b[2], b[3]);
+    }
+    // element e of sc[n]: row g + 8 (e / 2), key 8 n + 2 tq + e % 2
+    const bool whole = key + kTileKeys <= pos0 + 1 && (a.window == 0 || key > pos1 - a.window);
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = sc[n][e] * c2;
+        if (!whole) {
+          const int j = key + 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
+          if (j > p || (a.window > 0 && j <= p - a.window)) v = -INFINITY;
+        }
+        sc[n][e] = v;
+        top[e >> 1] = fmaxf(top[e >> 1], v);
+      }
+    float shrink[2], base[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+      base[h] = top[h] == -INFINITY ? 0.f : top[h];  // nothing seen yet
+      shrink[h] = ex2(m[h] - base[h]);
+      m[h] = top[h];
+      l[h] *= shrink[h];
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[n][e] = ex2(sc[n][e] - base[e >> 1]);
+        l[e >> 1] += sc[n][e];  // this lane's keys; the four lanes of a row are added at the end
+      }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][e] *= shrink[e >> 1];
+    // Some rows see a key of this step and some do not: an infinity or NaN in its value row may reach only the
+    // former, and a product would carry it to both (0 times infinity).  Such values are added by hand and zeroed.
+    if (key + kTileKeys > pos0 + 1 || (a.window > 0 && key <= pos1 - a.window)) {
+      unsigned char* v = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
+      bool odd = false;
+      for (int x = lane; x < kTileKeys * D; x += 32)
+        odd |= !isfinite(to_f32(*reinterpret_cast<const T*>(v + x * 2)));
+      if (__any_sync(~0u, odd)) {
+        for (int j = 0; j < kTileKeys; ++j)
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int col = 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
+              const float x = to_f32(*reinterpret_cast<const T*>(v + piece<D>(j, col / 8) + (col % 8) * 2));
+              if (!isfinite(x) && key + j <= p && (a.window == 0 || key + j > p - a.window)) o[n][e] += x;
+            }
+        __syncwarp();
+        for (int x = lane; x < kTileKeys * D; x += 32) {
+          T* at = reinterpret_cast<T*>(v + x * 2);
+          if (!isfinite(to_f32(*at))) *at = from_f32<T>(0.f);
+        }
+        __syncwarp();
+      }
+    }
+    // weights rounded to the cache's type for the tensor cores (their sum is not)
+    const uint32_t pf[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]), pack2<T>(sc[1][0], sc[1][1]),
+                            pack2<T>(sc[1][2], sc[1][3])};
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      uint32_t b[4];  // 16 keys x 16 values
+      ldsm4_t(b, vt + piece<D>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
+      mma16816<T>(o[2 * n], pf, b[0], b[1]);
+      mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+    }
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(~0u, l[h], 1);
+    l[h] += __shfl_xor_sync(~0u, l[h], 2);
+    if (tq == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
+  }
+  __syncthreads();  // every warp is done with its ring
+  // the warps' sums, side by side in the ring's memory
+  float* so = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (g + 8 * h < rows)
+        *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
+            make_float2(o[n][2 * h], o[n][2 * h + 1]);
+  __syncthreads();
+  const int64_t item = (int64_t)seq * a.kv_heads + kvh;
+  auto put = [&](int r, int d, float m_all, float l_all, float v) {
+    const int t = r / group, head = kvh * group + r - t * group;
+    static_cast<T*>(a.out)[(int64_t)(s.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride + d] =
+        from_f32<T>(l_all == 0.f ? 0.f : v / l_all);
+    if (a.lse && d == 0)
+      a.lse[(int64_t)(s.first + t) * a.q_heads + head] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+  };
+  for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
+    const int r = x / D, d = x - r * D;
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float f = ex2(s_m[w][r] - base);
+      sum = fmaf(s_l[w][r], f, sum);
+      v = fmaf(so[(w * kRows + r) * D + d], f, v);
+    }
+    if (parts == 1) {
+      put(r, d, base, sum, v);
+    } else {
+      const int64_t at = (item * plan.parts + part) * kRows + r;
+      plan.o[at * D + d] = v;
+      if (d == 0) plan.ml[at] = make_float2(top, sum);
+    }
+  }
+  if (parts == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_last = atomicAdd(plan.done + item, 1) == parts - 1;
+    if (s_last) plan.done[item] = 0;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
+    const int r = x / D, d = x - r * D;
+    const int64_t at = item * plan.parts * kRows + r;
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[at + k * kRows]).x);
+    const float base = top == -INFINITY ? 0.f : top;
+    for (int k = 0; k < parts; ++k) {
+      const float2 w = __ldcg(&plan.ml[at + k * kRows]);
+      const float f = ex2(w.x - base);
+      sum = fmaf(w.y, f, sum);
+      v = fmaf(__ldcg(&plan.o[(at + k * kRows) * D + d]), f, v);
+    }
+    put(r, d, base, sum, v);
+  }
+}
+
 // One warp per (token, query head): 32 keys at a time, lane k scoring key k,
 // with the running maximum and sum of the softmax in 32 bits.
 template <typename T, int D>
@@ -38,6 +356,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(q4gpu_attn_args a) {
   for (int d = lane; d < D; d += 32) q[d] = to_f32(qp[d]);
   __syncwarp();
   const int i = sequence_of(a.cu_q, a.n_seqs, token);
+  if (a.cu_q[i + 1] - a.cu_q[i] <= kRows / (a.q_heads / a.kv_heads)) return;  // attn_rows_kernel's
   const int slot = a.seq_ids ? a.seq_ids[i] : i;
   int len = slot >= 0 && slot < a.n_slots ? a.lens[slot] : 0;
   len = (int)min((int64_t)len, a.table_stride * a.page_tokens);
@@ -94,9 +413,8 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(q4gpu_attn_args a) {
   if (a.lse && lane == 0) a.lse[(int64_t)token * a.q_heads + head] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + logf(sum);
 }
 
-int check_attn(const q4gpu_attn_args* a) {
-  if (!a || !a->k_cache || !a->v_cache || !a->table || !a->lens || !a->cu_q)
-    return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null pointer");
+int check_sizes(const q4gpu_attn_args* a) {
+  if (!a) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null arguments");
   if (a->dtype != Q4GPU_F16 && a->dtype != Q4GPU_BF16)
     return q4gpu_fail(Q4GPU_ERR_ARG, "attention: dtype is F16 or BF16");
   if (a->dim != 64 && a->dim != 128) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: dim = %d is not 64 or 128", a->dim);
@@ -109,6 +427,14 @@ int check_attn(const q4gpu_attn_args* a) {
   if (a->n_seqs < 0 || a->n_seqs > 65535 || a->tokens < 0 || a->max_q < 0 || a->max_ctx < 0 || a->window < 0 ||
       a->n_slots < 1 || a->n_pages < 1 || a->table_stride < 1)
     return q4gpu_fail(Q4GPU_ERR_ARG, "attention: negative or empty size");
+  return Q4GPU_OK;
+}
+
+int check_attn(const q4gpu_attn_args* a) {
+  const int rc = check_sizes(a);
+  if (rc != Q4GPU_OK) return rc;
+  if (!a->k_cache || !a->v_cache || !a->table || !a->lens || !a->cu_q)
+    return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null pointer");
   if (a->tokens != 0 && (!a->q || !a->out)) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null pointer");
   if (!(a->scale == a->scale)) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: scale is not a number");
   if (!aligned(a->q, 16) || !aligned(a->k_cache, 16) || !aligned(a->v_cache, 16) || !aligned(a->out, 16) ||
@@ -118,30 +444,85 @@ int check_attn(const q4gpu_attn_args* a) {
   return Q4GPU_OK;
 }
 
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+constexpr int kSms = 148;
+
+// Keys of one part of a split sequence.  Joining the parts costs about as much
+// as a CTA's pass over 400 keys, so a part is not shorter than that; beyond it
+// the parts are as short as gives every SM eight of them, and at most 2048
+// keys, so that sequences of different lengths even out.
+SplitPlan row_plan(const q4gpu_attn_args& a, size_t* bytes) {
+  SplitPlan p{};
+  const int64_t span = a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + a.max_q + kTileKeys) : a.max_ctx;
+  const int64_t items = (int64_t)a.n_seqs * a.kv_heads;
+  int64_t chunk = (span * items / (kSms * 8) + 63) / 64 * 64;
+  chunk = std::max<int64_t>(384, std::min<int64_t>(2048, chunk));
+  p.chunk = (int)chunk;
+  p.parts = (int)std::max<int64_t>(1, (span + chunk - 1) / chunk);
+  if (bytes) {
+    const size_t rows = p.parts > 1 ? (size_t)items * p.parts * kRows : 0;
+    *bytes = p.parts > 1 ? ((size_t)items * 4 + 15) / 16 * 16 + rows * (8 + (size_t)a.dim * 4) : 0;
+  }
+  return p;
+}
+void place(SplitPlan* p, const q4gpu_attn_args& a, char* ws) {
+  const size_t items = (size_t)a.n_seqs * a.kv_heads;
+  p->done = reinterpret_cast<int32_t*>(ws);
+  p->ml = reinterpret_cast<float2*>(ws + (items * 4 + 15) / 16 * 16);
+  p->o = reinterpret_cast<float*>(p->ml + items * p->parts * kRows);
+}
+
+// Raises a kernel's shared-memory limit once per device.
+int allow_smem(const void* kernel, int bytes, unsigned char* ready) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < Q4GPU_MAX_DEVICES && ready[dev]) return Q4GPU_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: shared memory: %s", cudaGetErrorString(e));
+  if (dev < Q4GPU_MAX_DEVICES) ready[dev] = 1;
+  return Q4GPU_OK;
+}
+
+template <typename T, int D>
+int launch(const q4gpu_attn_args& a, cudaStream_t s) {
+  if (a.max_q > 0) {
+    SplitPlan plan = row_plan(a, nullptr);
+    place(&plan, a, static_cast<char*>(a.workspace));
+    static unsigned char ready[Q4GPU_MAX_DEVICES];
+    const int rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D>), row_smem<D>(), ready);
+    if (rc != Q4GPU_OK) return rc;
+    attn_rows_kernel<T, D>
+        <<<dim3(plan.parts, a.kv_heads, a.n_seqs), kRowWarps * 32, row_smem<D>(), s>>>(a, plan);
+  }
+  if ((int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows)
+    paged_attn_kernel<T, D><<<dim3(a.tokens, (a.q_heads + 3) / 4), 128, 0, s>>>(a);
+  return q4gpu_check_launch();
+}
+
 }  // namespace
 
 extern "C" {
 
-size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args*) { return 0; }
+size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args* a) {
+  if (check_sizes(a) != Q4GPU_OK) return 0;
+  size_t rows;
+  row_plan(*a, &rows);
+  return rows;
+}
 
 int q4gpu_paged_attention(const q4gpu_attn_args* a, void* stream) {
   const int rc = check_attn(a);
   if (rc != Q4GPU_OK) return rc;
   if (a->n_seqs == 0 || a->tokens == 0) return Q4GPU_OK;
-  const dim3 grid(a->tokens, (a->q_heads + 3) / 4);
+  const size_t need = q4gpu_paged_attention_workspace_bytes(a);
+  if (a->workspace_bytes < need || (need && !a->workspace))
+    return q4gpu_fail(Q4GPU_ERR_WORKSPACE, "attention: needs a workspace of %zu bytes", need);
+  if (!aligned(a->workspace, 16)) return q4gpu_fail(Q4GPU_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
   cudaStream_t s = as_stream(stream);
-  if (a->dtype == Q4GPU_F16) {
-    if (a->dim == 64)
-      paged_attn_kernel<__half, 64><<<grid, 128, 0, s>>>(*a);
-    else
-      paged_attn_kernel<__half, 128><<<grid, 128, 0, s>>>(*a);
-  } else {
-    if (a->dim == 64)
-      paged_attn_kernel<__nv_bfloat16, 64><<<grid, 128, 0, s>>>(*a);
-    else
-      paged_attn_kernel<__nv_bfloat16, 128><<<grid, 128, 0, s>>>(*a);
-  }
-  return q4gpu_check_launch();
+  if (a->dtype == Q4GPU_F16) return a->dim == 64 ? launch<__half, 64>(*a, s) : launch<__half, 128>(*a, s);
+  return a->dim == 64 ? launch<__nv_bfloat16, 64>(*a, s) : launch<__nv_bfloat16, 128>(*a, s);
 }
 
 }  // extern "C"
