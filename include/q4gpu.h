@@ -278,13 +278,16 @@ int q4gpu_rope_append(const q4gpu_rope_args *a, void *stream);
  * max_ctx bounds lens[s]; it only decides how the work is split.
  * workspace: q4gpu_paged_attention_workspace_bytes(a) bytes, 16-byte aligned
  * (0 bytes: may be NULL), zeroed once before its first use (each call leaves
- * its counters at zero) and not shared by calls that can overlap. */
+ * its counters at zero) and not shared by calls that can overlap.
+ * Every wait in the kernels has a limit; one that runs out sets *err_flag
+ * (optional) to 2 and leaves the output incomplete. */
 typedef struct q4gpu_attn_args {
     const void *q, *k_cache, *v_cache;
     void *out;
     float *lse;
     const int32_t *table, *lens, *cu_q, *seq_ids;
     void *workspace;
+    int32_t *err_flag;
     uint64_t workspace_bytes;
     int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
     int64_t page_stride, head_stride, row_stride, table_stride;

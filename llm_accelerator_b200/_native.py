@@ -111,7 +111,7 @@ class RopeArgs(C.Structure):
 
 class AttnArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "out", "lse", "table", "lens", "cu_q", "seq_ids",
-                                          "workspace")] + [("workspace_bytes", C.c_uint64)] + \
+                                          "workspace", "err_flag")] + [("workspace_bytes", C.c_uint64)] + \
                [(n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride",
                                          "page_stride", "head_stride", "row_stride", "table_stride")] + \
                [(n, C.c_int32) for n in ("n_seqs", "n_slots", "tokens", "max_q", "max_ctx", "q_heads", "kv_heads",

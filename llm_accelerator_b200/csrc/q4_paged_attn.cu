@@ -1,8 +1,12 @@
 // Attention of each sequence's newest tokens to its pages (16-bit paged
 // serving operators, include/q4gpu.h: q4gpu_paged_attention).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <cstdint>
 
 #include "q4_paged.cuh"
+#include "q4_paged_chunk.cuh"
 #include "q4gpu_internal.h"
 
 using namespace q4::paged;
@@ -11,19 +15,6 @@ namespace {
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-
-// Sequence that owns a query token: the last i with cu_q[i] <= token.
-__device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int token) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= token)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
-}
 
 // What a CTA needs to know of sequence i.
 struct Seq {
@@ -37,12 +28,6 @@ __device__ __forceinline__ Seq sequence(const q4gpu_attn_args& a, int i) {
   const bool known = s.slot >= 0 && s.slot < a.n_slots;
   s.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[s.slot], a.table_stride * a.page_tokens)) : 0;
   return s;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // ---------------------------------------------------------------------------
@@ -343,76 +328,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   }
 }
 
-// One warp per (token, query head): 32 keys at a time, lane k scoring key k,
-// with the running maximum and sum of the softmax in 32 bits.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_attn_kernel(q4gpu_attn_args a) {
-  const int lane = threadIdx.x & 31;
-  const int token = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5);
-  __shared__ float s_q[4][D];
-  if (head >= a.q_heads) return;
-  float* q = s_q[threadIdx.x >> 5];
-  const T* qp = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
-  for (int d = lane; d < D; d += 32) q[d] = to_f32(qp[d]);
-  __syncwarp();
-  const int i = sequence_of(a.cu_q, a.n_seqs, token);
-  if (a.cu_q[i + 1] - a.cu_q[i] <= kRows / (a.q_heads / a.kv_heads)) return;  // attn_rows_kernel's
-  const int slot = a.seq_ids ? a.seq_ids[i] : i;
-  int len = slot >= 0 && slot < a.n_slots ? a.lens[slot] : 0;
-  len = (int)min((int64_t)len, a.table_stride * a.page_tokens);
-  const int pos = len - (a.cu_q[i + 1] - a.cu_q[i]) + (token - a.cu_q[i]);
-  const int kvh = head / (a.q_heads / a.kv_heads);
-  const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  float top = -INFINITY, sum = 0.f, acc[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
-  for (int k0 = first; k0 <= pos; k0 += 32) {
-    const int key = k0 + lane;
-    int64_t off = -1;
-    if (key <= pos) {
-      const int page = a.table[slot * a.table_stride + key / a.page_tokens];
-      if (page >= 0 && page < a.n_pages)
-        off = page * a.page_stride + kvh * a.head_stride + (key % a.page_tokens) * a.row_stride;
-    }
-    float s = -INFINITY;
-    if (off >= 0) {
-      const T* kp = static_cast<const T*>(a.k_cache) + off;
-      s = 0.f;
-      for (int d = 0; d < D; d += 8) {
-        float f[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(kp + d), f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = fmaf(f[j], q[d + j], s);
-      }
-      s *= a.scale;
-    }
-    float m = s;
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    m = fmaxf(m, top);
-    if (__all_sync(~0u, off < 0)) continue;
-    const float base = m == -INFINITY ? 0.f : m;  // a row of NaN scores has no maximum
-    const float p = off < 0 ? 0.f : expf(s - base), shrink = expf(top - base);
-    top = m;
-    float ps = p;
-    for (int o = 16; o; o >>= 1) ps += __shfl_xor_sync(~0u, ps, o);
-    sum = sum * shrink + ps;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) acc[c] *= shrink;
-    for (int k = 0; k < 32; ++k) {
-      const int64_t o = __shfl_sync(~0u, off, k);
-      const float w = __shfl_sync(~0u, p, k);
-      if (o < 0) continue;
-      const T* vp = static_cast<const T*>(a.v_cache) + o;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(w, to_f32(vp[c * 32 + lane]), acc[c]);
-    }
-  }
-  T* o = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride;
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) o[c * 32 + lane] = from_f32<T>(sum == 0.f ? 0.f : acc[c] / sum);
-  if (a.lse && lane == 0) a.lse[(int64_t)token * a.q_heads + head] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + logf(sum);
-}
-
 int check_sizes(const q4gpu_attn_args* a) {
   if (!a) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null arguments");
   if (a->dtype != Q4GPU_F16 && a->dtype != Q4GPU_BF16)
@@ -474,6 +389,49 @@ void place(SplitPlan* p, const q4gpu_attn_args& a, char* ws) {
   p->o = reinterpret_cast<float*>(p->ml + items * p->parts * kRows);
 }
 
+// Parts of a chunk's keys: one where the row pairs alone fill the GPU, else as
+// many as fill it once, each of at least 512 keys.
+ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
+  ChunkPlan p{};
+  const int64_t group = a.q_heads / a.kv_heads;
+  if (a.max_q * group <= kRows) {
+    if (bytes) *bytes = 0;
+    return p;
+  }
+  const int64_t rows = a.tokens * group;
+  p.tiles = (int)std::min<int64_t>(a.n_seqs == 1 ? (rows + kPair - 1) / kPair : rows / kPair + a.n_seqs, INT32_MAX);
+  const int64_t items = (int64_t)p.tiles * a.kv_heads;
+  const int64_t span = a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + kPair + kNTile) : a.max_ctx;
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kSms / items, span / 512));
+  p.chunk = (int)std::max<int64_t>(kNTile, ((span + parts - 1) / parts + kNTile - 1) / kNTile * kNTile);
+  p.parts = (int)parts;
+  if (bytes) *bytes = parts > 1 ? (size_t)(items * parts * kPair) * (8 + (size_t)a.dim * 4) : 0;
+  return p;
+}
+
+int encode_map(CUtensorMap* map, const q4gpu_attn_args& a, const void* base) {
+  static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  if (!encode) {
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", reinterpret_cast<void**>(&encode), cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess || !encode)
+      return q4gpu_fail(Q4GPU_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  }
+  // one 128-byte line of every row of a page per box
+  const cuuint64_t dims[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.page_tokens, (cuuint64_t)a.kv_heads,
+                              (cuuint64_t)a.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.row_stride * 2, (cuuint64_t)a.head_stride * 2,
+                                 (cuuint64_t)a.page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)a.page_tokens, 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, a.dtype == Q4GPU_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                            4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return Q4GPU_OK;
+}
+
 // Raises a kernel's shared-memory limit once per device.
 int allow_smem(const void* kernel, int bytes, unsigned char* ready) {
   int dev = 0;
@@ -496,8 +454,24 @@ int launch(const q4gpu_attn_args& a, cudaStream_t s) {
     attn_rows_kernel<T, D>
         <<<dim3(plan.parts, a.kv_heads, a.n_seqs), kRowWarps * 32, row_smem<D>(), s>>>(a, plan);
   }
-  if ((int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows)
-    paged_attn_kernel<T, D><<<dim3(a.tokens, (a.q_heads + 3) / 4), 128, 0, s>>>(a);
+  if ((int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows) {
+    size_t rows_bytes;
+    row_plan(a, &rows_bytes);
+    ChunkPlan plan = chunk_plan(a, nullptr);
+    if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
+    char* ws = static_cast<char*>(a.workspace) + (rows_bytes + 15) / 16 * 16;
+    plan.ml = reinterpret_cast<float2*>(ws);
+    plan.o = reinterpret_cast<float*>(plan.ml + (size_t)plan.tiles * a.kv_heads * plan.parts * kPair);
+    CUtensorMap kmap, vmap;
+    int rc = encode_map(&kmap, a, a.k_cache);
+    if (rc == Q4GPU_OK) rc = encode_map(&vmap, a, a.v_cache);
+    static unsigned char ready[Q4GPU_MAX_DEVICES];
+    if (rc == Q4GPU_OK) rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D>), chunk_smem<D>(), ready);
+    if (rc != Q4GPU_OK) return rc;
+    attn_chunk_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, plan.parts), kChunkThreads, chunk_smem<D>(), s>>>(kmap, vmap,
+                                                                                                           a, plan);
+    if (plan.parts > 1) attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
+  }
   return q4gpu_check_launch();
 }
 
@@ -507,9 +481,10 @@ extern "C" {
 
 size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args* a) {
   if (check_sizes(a) != Q4GPU_OK) return 0;
-  size_t rows;
+  size_t rows, chunks;
   row_plan(*a, &rows);
-  return rows;
+  chunk_plan(*a, &chunks);
+  return chunks ? (rows + 15) / 16 * 16 + chunks : rows;
 }
 
 int q4gpu_paged_attention(const q4gpu_attn_args* a, void* stream) {

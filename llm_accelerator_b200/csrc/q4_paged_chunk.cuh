@@ -1,0 +1,520 @@
+// Attention of a chunk of query tokens over a paged cache on the 5th-generation
+// tensor cores: the kernel of q4gpu_paged_attention for sequences with more
+// than 16 (token, head) rows per key head.
+#pragma once
+#include "q4_paged.cuh"
+#include "q4_umma.cuh"
+#include "q4gpu_internal.h"
+
+namespace q4 {
+namespace paged {
+
+constexpr int kMTile = 128;             // query rows of one accumulator
+constexpr int kPair = 2 * kMTile;       // query rows of a CTA
+constexpr int kNTile = 128;             // keys of one step
+constexpr int kChunkThreads = 10 * 32;  // two softmax warpgroups, a TMA warp, an MMA warp
+
+template <int D>
+__host__ __device__ constexpr int chunk_stages() { return D == 128 ? 5 : 10; }
+template <int D>
+__host__ __device__ constexpr int chunk_smem() { return 1024 + (2 * kMTile + chunk_stages<D>() * kNTile) * D * 2; }
+
+struct ChunkPlan {
+  int tiles;  // grid of query row pairs over all sequences, an upper bound
+  int chunk;  // keys of one part, a multiple of kNTile
+  int parts;
+  float* o;    // [tile * kv_heads + head][part][kPair][D] unnormalised sums (parts > 1)
+  float2* ml;  // the same rows: running maximum (log2 units) and sum
+};
+
+// Sequence and row pair of one grid index; sequences with few rows have none.
+// Later rows see more keys, so pairs are handed out from the last to the first.
+struct ChunkTile {
+  int seq, row0, index;
+};
+__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int group) {
+  const int n = max(0, min(a.cu_q[i + 1], a.tokens) - max(0, min(a.cu_q[i], a.tokens)));
+  return n <= 16 / group ? 0 : (int)(((int64_t)n * group + kPair - 1) / kPair);
+}
+// By one full warp; seq = -1 where the index is past the last pair.
+__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int y) {
+  const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
+  int total = 0;
+  for (int i = lane; i < a.n_seqs; i += 32) total += pairs_of(a, i, group);
+  total = __reduce_add_sync(~0u, total);
+  ChunkTile t{-1, 0, total - 1 - y};
+  if (y >= total) return t;
+  int before = 0;
+  for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
+    const int mine = i0 + lane < a.n_seqs ? pairs_of(a, i0 + lane, group) : 0;
+    int run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(~0u, run, o);
+      if (lane >= o) run += v;
+    }
+    const unsigned hit = __ballot_sync(~0u, before + run > t.index);
+    if (hit) {
+      const int k = __ffs(hit) - 1;
+      t.seq = i0 + k;
+      t.row0 = (t.index - before - __shfl_sync(~0u, run - mine, k)) * kPair;
+      return t;
+    }
+    before += __shfl_sync(~0u, run, 31);
+  }
+  return t;
+}
+
+// ---- tensor memory, 32 columns at a time ---------------------------------------
+__device__ __forceinline__ void tm_ld32(uint32_t at, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(u[0]),
+      "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+      "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
+      "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]),
+      "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- products --------------------------------------------------------------------
+// kind::f16 instruction descriptor: float32 accumulator, both operands f16 or
+// bf16, M x N; the B operand K-major, or MN-major (values: keys are its rows).
+__host__ __device__ constexpr uint32_t f16_idesc(bool bf16, int M, int N, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// An MN-major tile in 128-byte swizzled lines of 64 values: 8-row groups 1024
+// bytes apart (stride), the next 64 columns `chunk` bytes on (leading).
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t chunk) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(chunk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* b) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(umma::smem_addr(b))
+      : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// One CTA: 256 query rows (row = token * group + head of the group) of one
+// sequence and key head against one part of its keys.  Two accumulators of 128
+// rows take turns: while one warpgroup works on the softmax of its 128 x 128
+// scores, the tensor cores multiply for the other.  Per step and tile
+//   S = Q K^T (shared x shared -> TMEM);  P = exp2(S c - m) -> TMEM, over S;
+//   O += P V (TMEM x shared -> TMEM),
+// a thread holding one row of S.  O is rescaled only when a row's maximum grows
+// by more than 8 (in log2): until then P <= 2^8, which 16-bit weights and
+// 32-bit sums hold without loss.
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    attn_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ q4gpu_attn_args a, const __grid_constant__ ChunkPlan plan) {
+  using namespace umma;
+  constexpr int kStages = chunk_stages<D>();
+  constexpr int kLines = D / 64;                  // 128-byte lines of a head vector
+  constexpr uint32_t kLineTile = kNTile * 128;    // bytes of one line of a 128-row tile
+  constexpr uint32_t kTile = kLineTile * kLines;  // bytes of a 128-row tile
+  constexpr bool kBf16 = !__is_same(T, __half);
+  constexpr uint32_t kSCol = 0, kOCol = 2 * kNTile;  // TMEM columns: S0, S1, O0, O1
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t full[kStages], empty[kStages], s_full[2], p_full[2], o_full, care;
+  __shared__ uint32_t tmem_slot;
+  __shared__ ChunkTile s_tile;
+  __shared__ int s_bad, s_odd, s_dead;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x, part = blockIdx.z;
+  if (warp == 0) {
+    const ChunkTile t = find_tile(a, blockIdx.y);
+    if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
+  }
+  __syncthreads();
+  const ChunkTile tile = s_tile;
+  if (tile.seq < 0) return;
+  const int group = a.q_heads / a.kv_heads;
+  const int first = max(0, min(a.cu_q[tile.seq], a.tokens));
+  const int n = min(a.cu_q[tile.seq + 1], a.tokens) - first;
+  const int slot = a.seq_ids ? a.seq_ids[tile.seq] : tile.seq;
+  const bool known = slot >= 0 && slot < a.n_slots;
+  const int len = known ? (int)max((int64_t)0, min((int64_t)a.lens[slot], a.table_stride * a.page_tokens)) : 0;
+  const int64_t all_rows = (int64_t)n * group;
+  const int rows = (int)min((int64_t)kPair, all_rows - tile.row0);
+  const int t0 = tile.row0 / group, t1 = (tile.row0 + rows - 1) / group;  // first and last query of the pair
+  const int pos0 = len - n + t0, pos1 = len - n + t1;
+  // keys that some row sees, and those that every row sees
+  const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1);
+  const int all_lo = a.window > 0 ? max(0, pos1 - a.window + 1) : 0, all_hi = pos0 + 1;
+  const int base = lo & ~(kNTile - 1);
+  const int chunk = max(plan.chunk, ((hi - base + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
+  const int parts = max(1, (hi - base + chunk - 1) / chunk);
+  if (part >= parts) return;
+  const int begin = base + part * chunk, end = min(hi, begin + chunk);
+  const int steps = begin < end ? (end - begin + kNTile - 1) / kNTile : 0;
+  const int tiles = rows > kMTile ? 2 : 1;
+  const int32_t* table = a.table + (int64_t)max(0, min(slot, a.n_slots - 1)) * a.table_stride;
+  const int shift = 31 - __clz(a.page_tokens);
+  const uint32_t sq = smem_addr(smem), ring = sq + 2 * kTile;
+
+  // queries into shared memory, 128-byte swizzled lines; a negative scale turns their sign
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+  for (int x = threadIdx.x; x < tiles * kMTile * (D / 8); x += kChunkThreads) {
+    const int r = x / (D / 8), c = x % (D / 8);
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (r < rows) {
+      const int t = (tile.row0 + r) / group, h = tile.row0 + r - t * group;
+      w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(first + t) * a.q_token_stride +
+                                          (int64_t)(kvh * group + h) * a.q_head_stride + c * 8);
+      w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
+    }
+    const int row = r & (kMTile - 1);
+    *reinterpret_cast<uint4*>(smem + (r / kMTile) * kTile + (c / 8) * kLineTile + row * 128 +
+                              (((c & 7) ^ (row & 7)) * 16)) = w;
+  }
+  // is any page of these keys missing?
+  for (int64_t p = ((int64_t)begin >> shift) + threadIdx.x; p << shift < end; p += kChunkThreads)
+    if (table[p] < 0 || table[p] >= a.n_pages) s_bad = 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], 4);
+    bar_init(&o_full, 1);
+    bar_init(&care, 1);
+    bar_init_fence();
+  }
+  if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  fence_async();
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const bool bad = s_bad != 0;
+  volatile int* dead = &s_dead;
+
+  if (warp == 8) {
+    // ---- loads: K and V of a step take one ring stage each ----------------------
+    uint32_t care_phase = 0;
+    for (int j = 0; j < steps && !*dead; ++j) {
+      const int key = begin + j * kNTile;
+      const int pages = min(kNTile >> shift, (int)((end - key + a.page_tokens - 1) >> shift));
+      const int id = lane < pages ? table[(key >> shift) + lane] : -1;
+      const unsigned ok = __ballot_sync(~0u, id >= 0 && id < a.n_pages);
+      const uint32_t bytes = (uint32_t)__popc(ok) * a.page_tokens * D * 2;
+      // rows that no query of the pair sees, or that only some see
+      const bool partial = key < lo || key + kNTile > end || __popc(ok) != kNTile >> shift;
+      const bool mixed = key < all_lo || key + kNTile > all_hi;
+      for (int kind = 0; kind < 2; ++kind) {
+        const int use = 2 * j + kind, st = use % kStages;
+        if (use >= kStages && !bar_wait(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
+        __syncwarp();
+        if (*dead) break;
+        const uint32_t at = ring + st * kTile;
+        const bool careful = kind == 1 && (partial || mixed);
+        uint64_t* bar = careful ? &care : &full[st];
+        if (lane == 0) {
+          if (bytes)
+            bar_expect_tx(bar, bytes);
+          else
+            bar_arrive(bar);
+        }
+        __syncwarp();
+        if ((ok >> lane) & 1u) {
+#pragma unroll
+          for (int c = 0; c < kLines; ++c)
+            tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, kind ? &vmap : &kmap, c * 64, 0, kvh, id, bar);
+        }
+        if (!careful) continue;
+        // Values of keys that a row does not see meet a zero weight in its product, so they have to be finite:
+        // rows outside lo .. end (and of missing pages) become zeros, and infinities and NaNs are zeroed here and
+        // added at the end to the rows that do see them.
+        if (!bar_wait(&care, care_phase)) *dead = 1;
+        care_phase ^= 1;
+        unsigned char* v = smem + (at - sq);
+        bool odd = false;
+        for (int x = lane; x < kNTile * kLines * 8; x += 32) {
+          const int line = x / (kNTile * 8), r = (x / 8) % kNTile;
+          uint4* w = reinterpret_cast<uint4*>(v + line * kLineTile + r * 128 + (x & 7) * 16);
+          if (key + r < lo || key + r >= end || !((ok >> (r >> shift)) & 1u)) {
+            *w = make_uint4(0u, 0u, 0u, 0u);
+          } else {
+            const uint4 b = *w;
+            constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+            const uint32_t u[4] = {b.x, b.y, b.z, b.w};
+            uint32_t o[4];
+            bool some = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool l = (u[i] & kExp) == kExp, h = ((u[i] >> 16) & kExp) == kExp;
+              o[i] = (l ? 0u : u[i] & 0xffffu) | (h ? 0u : u[i] & 0xffff0000u);
+              some |= l || h;
+            }
+            if (some) *w = make_uint4(o[0], o[1], o[2], o[3]), odd = true;
+          }
+        }
+        if (odd) s_odd = 1;
+        fence_async();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&full[st]);
+      }
+    }
+  } else if (warp == 9) {
+    // ---- products, issued by one thread -----------------------------------------
+    if (lane == 0 && steps > 0) {
+      constexpr uint32_t qk = f16_idesc(kBf16, kMTile, kNTile, false), pv = f16_idesc(kBf16, kMTile, D, true);
+      auto stage_full = [&](int use) { return bar_wait(&full[use % kStages], (use / kStages) & 1); };
+      auto scores = [&](int t, int use) {
+        const uint32_t k = ring + (use % kStages) * kTile, q = sq + t * kTile;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+          mma_ss(tmem + kSCol + t * kNTile, sw128_desc(q + (i / 4) * kLineTile + (i & 3) * 32),
+                 sw128_desc(k + (i / 4) * kLineTile + (i & 3) * 32), qk, i > 0);
+        mma_commit(&s_full[t]);
+      };
+      bool live = stage_full(0);
+      if (live) {
+        fence_after_sync();
+        for (int t = 0; t < tiles; ++t) scores(t, 0);
+        mma_commit(&empty[0]);
+      }
+      for (int j = 0; j < steps && live; ++j) {
+        const int use = 2 * j + 1;
+        live = stage_full(use) && (j + 1 >= steps || stage_full(use + 1));
+        const uint32_t v = ring + (use % kStages) * kTile;
+        for (int t = 0; t < tiles && live; ++t) {
+          live = bar_wait(&p_full[t], j & 1);
+          if (!live) break;
+          fence_after_sync();
+#pragma unroll
+          for (int i = 0; i < kNTile / 16; ++i)
+            mma_ts(tmem + kOCol + t * D, tmem + kSCol + t * kNTile + i * 8, sw128_mn_desc(v + i * 2048, kLineTile), pv,
+                   j > 0 || i > 0);
+          if (j + 1 < steps) scores(t, use + 1);
+        }
+        mma_commit(&empty[use % kStages]);
+        if (j + 1 < steps) mma_commit(&empty[(use + 1) % kStages]);
+      }
+      if (!live) *dead = 1;
+      mma_commit(&o_full);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: one row a thread ------------------------------------------------
+    const int t = warp >> 2, r = t * kMTile + (threadIdx.x & (kMTile - 1));
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
+    const uint32_t ts = tmem + lanes + kSCol + t * kNTile, to = tmem + lanes + kOCol + t * D;
+    const bool mine = r < rows;
+    const int pos = mine ? len - n + (tile.row0 + r) / group : -1;
+    const float c2 = fabsf(a.scale) * 1.4426950408889634f;
+    float m = -INFINITY, sum = 0.f;
+    bool live = true;
+    if (t < tiles) {
+      for (int j = 0; j < steps; ++j) {
+        live = bar_wait(&s_full[t], j & 1) && !*dead;
+        if (!__all_sync(~0u, live)) break;
+        fence_after_sync();
+        const int key = begin + j * kNTile;
+        float s[kNTile];
+#pragma unroll
+        for (int c = 0; c < kNTile; c += 32) tm_ld32(ts + c, s + c);
+        tmem_ld_wait();
+        if (key < all_lo || key + kNTile > all_hi || bad) {
+          const int top = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : 0;
+#pragma unroll
+          for (int c = 0; c < kNTile; ++c)
+            if (c > top || c < low) s[c] = -INFINITY;
+          if (bad) {
+            unsigned ok = 0;
+            for (int p = 0; p < kNTile >> shift && key + (p << shift) < end; ++p) {
+              const int id = table[(key >> shift) + p];
+              ok |= (id >= 0 && id < a.n_pages ? 1u : 0u) << p;
+            }
+#pragma unroll
+            for (int c = 0; c < kNTile; ++c)
+              if (!((ok >> (c >> shift)) & 1u)) s[c] = -INFINITY;
+          }
+        }
+        float top = m;
+#pragma unroll
+        for (int c = 0; c < kNTile; ++c) top = fmaxf(top, s[c]);
+        // the first step sets the reference; later ones move it when it is left behind by more than 8
+        const bool move = j == 0 ? false : (top - m) * c2 > 8.f;
+        if (j == 0) m = top;
+        if (__any_sync(~0u, move)) {
+          const float f = move ? ex2((m - top) * c2) : 1.f;
+          if (move) m = top;
+          sum *= f;
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            tm_ld32(to + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            tm_st32(to + c, reinterpret_cast<const uint32_t*>(o));
+          }
+          tm_st_wait();
+        }
+        const float off = m == -INFINITY ? 0.f : -m * c2;
+        float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kNTile; c += 64) {
+          uint32_t p[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float x = ex2(fmaf(s[c + 2 * i], c2, off)), y = ex2(fmaf(s[c + 2 * i + 1], c2, off));
+            add[i & 3] += x + y;
+            p[i] = pack2<T>(x, y);  // weights in the cache's type for the tensor cores; their sum is not rounded
+          }
+          tm_st32(ts + c / 2, p);
+        }
+        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        tm_st_wait();
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&p_full[t]);
+      }
+      if (steps > 0) live = live && bar_wait(&o_full, 0);
+      live = __all_sync(~0u, live) && !*dead;
+      if (!live && lane == 0) {
+        *dead = 1;
+        if (a.err_flag) *a.err_flag = 2;
+      }
+      if (live) {
+        fence_after_sync();
+        const int q = (tile.row0 + r) / group, head = kvh * group + tile.row0 + r - q * group;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum, mm = m == -INFINITY ? 0.f : m * c2;
+        const int64_t item = (int64_t)tile.index * a.kv_heads + kvh;
+        const int64_t at = (item * plan.parts + part) * kPair + r;
+        const bool odd = s_odd != 0;
+        if (mine && parts == 1 && a.lse)
+          a.lse[(int64_t)(first + q) * a.q_heads + head] =
+              sum == 0.f ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
+        if (mine && parts > 1) plan.ml[at] = make_float2(m == -INFINITY ? m : mm, sum);
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          if (steps > 0) {
+            tm_ld32(to + c, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          }
+          if (odd && mine) {  // the infinities and NaNs that were kept out of the products
+            for (int k = begin; k < end; ++k) {
+              const int step = k & ~(kNTile - 1);
+              if (!bad && step >= all_lo && step + kNTile <= all_hi) continue;  // went through the products
+              if (k > pos || (a.window > 0 && k <= pos - a.window)) continue;
+              const int id = table[k >> shift];
+              if (id < 0 || id >= a.n_pages) continue;
+              const T* v = static_cast<const T*>(a.v_cache) + id * a.page_stride + kvh * a.head_stride +
+                           (k & (a.page_tokens - 1)) * a.row_stride + c;
+              for (int i = 0; i < 32; ++i) {
+                const float x = to_f32(v[i]);
+                if (!isfinite(x)) {
+#pragma unroll
+                  for (int e = 0; e < 32; ++e)
+                    if (e == i) o[e] += x;
+                }
+              }
+            }
+          }
+          if (!mine) continue;
+          if (parts > 1) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<float4*>(plan.o + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          } else {
+            T* out = static_cast<T*>(a.out) + (int64_t)(first + q) * a.out_token_stride +
+                     (int64_t)head * a.out_head_stride + c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= inv;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(out + i) = pack8<T>(o + i);
+          }
+        }
+      }
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of each row, in order: one warp a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, ChunkPlan plan) {
+  __shared__ ChunkTile s_tile;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
+  if (warp == 0) {
+    const ChunkTile t = find_tile(a, blockIdx.y);
+    if (lane == 0) s_tile = t;
+  }
+  __syncthreads();
+  const ChunkTile tile = s_tile;
+  if (tile.seq < 0) return;
+  const int group = a.q_heads / a.kv_heads;
+  const int first = max(0, min(a.cu_q[tile.seq], a.tokens));
+  const int n = min(a.cu_q[tile.seq + 1], a.tokens) - first;
+  const int slot = a.seq_ids ? a.seq_ids[tile.seq] : tile.seq;
+  const bool known = slot >= 0 && slot < a.n_slots;
+  const int len = known ? (int)max((int64_t)0, min((int64_t)a.lens[slot], a.table_stride * a.page_tokens)) : 0;
+  const int rows = (int)min((int64_t)kPair, (int64_t)n * group - tile.row0);
+  const int pos0 = len - n + tile.row0 / group, pos1 = len - n + (tile.row0 + rows - 1) / group;
+  const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1), base = lo & ~(kNTile - 1);
+  const int chunk = max(plan.chunk, ((hi - base + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
+  const int parts = max(1, (hi - base + chunk - 1) / chunk);
+  if (parts == 1) return;
+  const int r = blockIdx.z * 8 + warp;
+  if (r >= rows) return;
+  const int64_t at = ((int64_t)tile.index * a.kv_heads + kvh) * plan.parts * kPair + r;
+  float top = -INFINITY, sum = 0.f, o[D / 32];
+  for (int k = 0; k < parts; ++k) top = fmaxf(top, plan.ml[at + (int64_t)k * kPair].x);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) o[c] = 0.f;
+  for (int k = 0; k < parts; ++k) {
+    const float2 w = plan.ml[at + (int64_t)k * kPair];
+    const float f = ex2(w.x - ref);
+    sum = fmaf(w.y, f, sum);
+    const float* p = plan.o + (at + (int64_t)k * kPair) * D + lane;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = fmaf(p[c * 32], f, o[c]);
+  }
+  const int t = (tile.row0 + r) / group, head = kvh * group + tile.row0 + r - t * group;
+  T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) out[c * 32 + lane] = from_f32<T>(sum == 0.f ? 0.f : o[c] / sum);
+  if (a.lse && lane == 0)
+    a.lse[(int64_t)(first + t) * a.q_heads + head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+}
+
+}  // namespace paged
+}  // namespace q4

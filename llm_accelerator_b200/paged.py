@@ -125,8 +125,12 @@ class _Err:
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def check(self) -> None:
-        if int(self.err.item()):
+        what = int(self.err.item())
+        if what:
             self.err.zero_()
+        if what == 2:
+            raise _native.Q4GpuError(f"{type(self).__name__}: a wait inside a kernel ran out; its output is incomplete")
+        if what:
             raise _native.Q4GpuError(f"{type(self).__name__}: a position, row, page or slot was out of range; "
                                      "what it named was left untouched")
 
@@ -221,7 +225,7 @@ class RopeAppend(_Err):
         return t.data_ptr(), ts, hs
 
 
-class Attention:
+class Attention(_Err):
     """Attention of each sequence's newest tokens to its pages.
 
     ``k_cache`` / ``v_cache`` [pages, kv_heads, page_tokens, dim] (bf16 or f16, K and
@@ -247,13 +251,15 @@ class Attention:
         self.q_heads, self.dim, self.slots = q_heads, dim, table.shape[0]
         self.k_cache, self.v_cache, self.table, self.lens = k_cache, v_cache, table, lens
         self.workspace = None
+        self._new_err()
         # a row of the table is as long as its stride lets it name
         self.args = _native.AttnArgs(
             k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr(),
             page_stride=k_cache.stride(0), head_stride=k_cache.stride(1), row_stride=k_cache.stride(2),
             table_stride=table.stride(0) if self.slots > 1 else table.shape[1], n_slots=self.slots, q_heads=q_heads,
             kv_heads=kv_heads, dim=dim, page_tokens=page_tokens, n_pages=pages, window=window,
-            dtype=_DTYPES[self.dtype], scale=dim ** -0.5 if scale is None else scale)
+            dtype=_DTYPES[self.dtype], scale=dim ** -0.5 if scale is None else scale,
+            err_flag=self.err.data_ptr())
 
     def __call__(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
                  max_q: int = 1, max_ctx: int = 0, lse: Optional[torch.Tensor] = None,
