@@ -11,8 +11,9 @@ namespace paged {
 
 constexpr int kMTile = 128;             // query rows of one accumulator
 constexpr int kPair = 2 * kMTile;       // query rows of a CTA
-constexpr int kNTile = 128;             // keys of one step
-constexpr int kChunkThreads = 10 * 32;  // two softmax warpgroups, a TMA warp, an MMA warp
+constexpr int kNTile = 128;             // keys of one load
+constexpr int kStep = 64;               // keys of one step
+constexpr int kChunkThreads = 12 * 32;  // two softmax warpgroups; a TMA warp, two MMA warps, an idle one
 
 template <int D>
 __host__ __device__ constexpr int chunk_stages() { return D == 128 ? 5 : 10; }
@@ -77,6 +78,16 @@ __device__ __forceinline__ void tm_ld32(uint32_t at, float* r) {
         "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
       : "r"(at));
 }
+// Waits for the loads above; the values pass through, so no use moves before it.
+__device__ __forceinline__ void tm_ld_wait32(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+                 "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tm_st32(uint32_t at, const uint32_t* u) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -116,6 +127,28 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
       : "memory");
 }
+// Waits for a phase; false after about 0.3 s.  (bar_wait reads the global timer
+// after its first miss, which took longer than most waits here.)
+__device__ __forceinline__ bool wait_phase(uint64_t* b, unsigned parity) {
+  if (umma::bar_try_wait(b, parity)) return true;
+  long long since = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (umma::bar_try_wait(b, parity)) return true;
+    if ((it & 255u) == 0) {
+      const long long now = clock64();
+      if (!since)
+        since = now;
+      else if (now - since > 500000000ll)
+        return false;
+    }
+  }
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* m, int x, int y, int z, int w, uint64_t* b) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
@@ -123,17 +156,71 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* m, in
       "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(umma::smem_addr(b))
       : "memory");
 }
+
+// ---- pairs of float32 --------------------------------------------------------
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split_pair(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two values on the FMA pipe, for x <= 127.  Range reduction after Cody
+// and Waite: x = n + f with n = floor(x) from the low bits of x + 1.5 2^23
+// rounded down; 2^f on [0, 1] by the degree-4 polynomial with value 1 at 0 whose
+// largest relative error is least (3.0e-6, mean below 1e-8, against 2^-9 of a
+// bf16 weight; found by linear programming over 4001 points); n is added to the
+// exponent.  x below -127 (a masked score) gives exactly 0.
+__device__ __forceinline__ void ex2_pair(uint64_t x2, float& x, float& y) {
+  constexpr float kMagic = 12582912.f;
+  split_pair(x2, x, y);
+  const uint64_t v = pair_of(fmaxf(x, -127.f), fmaxf(y, -127.f));
+  uint64_t r, f;
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r) : "l"(v), "l"(pair_of(kMagic, kMagic)));
+  f = add_pair(r, pair_of(-kMagic, -kMagic));
+  f = fma_pair(f, pair_of(-1.f, -1.f), v);
+  uint64_t p = fma_pair(f, pair_of(0.013425154611468315f, 0.013425154611468315f),
+                        pair_of(0.0522453747689724f, 0.0522453747689724f));
+  p = fma_pair(p, f, pair_of(0.24127855896949768f, 0.24127855896949768f));
+  p = fma_pair(p, f, pair_of(0.6930451393127441f, 0.6930451393127441f));
+  p = fma_pair(p, f, pair_of(1.f, 1.f));
+  float a, b, n, m;
+  split_pair(p, a, b);
+  split_pair(r, n, m);
+  x = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n) << 23));
+  y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(m) << 23));
+}
+// The largest of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // One CTA: 256 query rows (row = token * group + head of the group) of one
 // sequence and key head against one part of its keys.  Two accumulators of 128
-// rows take turns: while one warpgroup works on the softmax of its 128 x 128
-// scores, the tensor cores multiply for the other.  Per step and tile
+// rows share the keys.  Per step of 64 keys and tile
 //   S = Q K^T (shared x shared -> TMEM);  P = exp2(S c - m) -> TMEM, over S;
 //   O += P V (TMEM x shared -> TMEM),
-// a thread holding one row of S.  O is rescaled only when a row's maximum grows
-// by more than 8 (in log2): until then P <= 2^8, which 16-bit weights and
-// 32-bit sums hold without loss.
+// a thread holding one row of S.  A tile has two score buffers, so the scores
+// of step i + 1 are there when the softmax of step i ends: from a product's
+// issue to its barrier's wake-up take about 400 clocks besides its own 64, and
+// with one buffer of 128 keys the softmax waited for them in every step (3300
+// clocks per 128 keys and both tiles, against 2048 of products).  O is rescaled
+// only when a row's maximum grows by more than 8 (in log2): until then P <= 2^8,
+// which 16-bit weights and 32-bit sums hold without loss.
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -147,7 +234,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr uint32_t kSCol = 0, kOCol = 2 * kNTile;  // TMEM columns: S0, S1, O0, O1
   extern __shared__ unsigned char raw[];
   unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kStages], empty[kStages], s_full[2], p_full[2], o_full, care;
+  __shared__ uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2], care;
   __shared__ uint32_t tmem_slot;
   __shared__ ChunkTile s_tile;
   __shared__ int s_bad, s_odd, s_dead;
@@ -179,6 +266,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (part >= parts) return;
   const int begin = base + part * chunk, end = min(hi, begin + chunk);
   const int steps = begin < end ? (end - begin + kNTile - 1) / kNTile : 0;
+  const int subs = begin < end ? (end - begin + kStep - 1) / kStep : 0;
   const int tiles = rows > kMTile ? 2 : 1;
   const int32_t* table = a.table + (int64_t)max(0, min(slot, a.n_slots - 1)) * a.table_stride;
   const int shift = 31 - __clz(a.page_tokens);
@@ -203,9 +291,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   for (int64_t p = ((int64_t)begin >> shift) + threadIdx.x; p << shift < end; p += kChunkThreads)
     if (table[p] < 0 || table[p] >= a.n_pages) s_bad = 1;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], 1);
-    for (int i = 0; i < 2; ++i) bar_init(&s_full[i], 1), bar_init(&p_full[i], 4);
-    bar_init(&o_full, 1);
+    for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], tiles);
+    for (int i = 0; i < 2; ++i) {
+      for (int k = 0; k < 2; ++k) bar_init(&s_full[i][k], 1), bar_init(&p_full[i][k], 4);
+      bar_init(&o_full[i], 1);
+    }
     bar_init(&care, 1);
     bar_init_fence();
   }
@@ -232,7 +322,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const bool mixed = key < all_lo || key + kNTile > all_hi;
       for (int kind = 0; kind < 2; ++kind) {
         const int use = 2 * j + kind, st = use % kStages;
-        if (use >= kStages && !bar_wait(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
+        if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
         __syncwarp();
         if (*dead) break;
         const uint32_t at = ring + st * kTile;
@@ -254,7 +344,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // Values of keys that a row does not see meet a zero weight in its product, so they have to be finite:
         // rows outside lo .. end (and of missing pages) become zeros, and infinities and NaNs are zeroed here and
         // added at the end to the rows that do see them.
-        if (!bar_wait(&care, care_phase)) *dead = 1;
+        if (!wait_phase(&care, care_phase)) *dead = 1;
         care_phase ^= 1;
         unsigned char* v = smem + (at - sq);
         bool odd = false;
@@ -284,123 +374,149 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (lane == 0) bar_arrive(&full[st]);
       }
     }
-  } else if (warp == 9) {
-    // ---- products, issued by one thread -----------------------------------------
-    if (lane == 0 && steps > 0) {
-      constexpr uint32_t qk = f16_idesc(kBf16, kMTile, kNTile, false), pv = f16_idesc(kBf16, kMTile, D, true);
-      auto stage_full = [&](int use) { return bar_wait(&full[use % kStages], (use / kStages) & 1); };
-      auto scores = [&](int t, int use) {
-        const uint32_t k = ring + (use % kStages) * kTile, q = sq + t * kTile;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          mma_ss(tmem + kSCol + t * kNTile, sw128_desc(q + (i / 4) * kLineTile + (i & 3) * 32),
-                 sw128_desc(k + (i / 4) * kLineTile + (i & 3) * 32), qk, i > 0);
-        mma_commit(&s_full[t]);
-      };
-      bool live = stage_full(0);
-      if (live) {
+  } else if (warp >= 9 && warp < 9 + tiles) {
+    // ---- products: one warp a tile, together; an elected thread issues ---------------
+    // Descriptors and addresses are the same in every lane and stay in uniform
+    // registers (issued from a divergent branch each product took twice as long).
+    // A warp's barrier tests queue up behind the products it has issued, so each
+    // tile has a warp of its own.
+    if (subs > 0) {
+      constexpr uint32_t qk = f16_idesc(kBf16, kMTile, kStep, false), pv = f16_idesc(kBf16, kMTile, D, true);
+      const int t = warp - 9;
+      const bool leader = elect_one();
+      const uint32_t sc = kSCol + t * 2 * kStep, oc = kOCol + t * D;
+      const uint64_t q = sw128_desc(sq) + t * (kTile / 16), k_desc = sw128_desc(ring),
+                     v_desc = sw128_mn_desc(ring, kLineTile);
+      auto stage_full = [&](int use) { return wait_phase(&full[use % kStages], (use / kStages) & 1); };
+      auto scores = [&](int i) {
+        const int use = i & ~1, st = use % kStages;
+        if (!stage_full(use)) return false;
         fence_after_sync();
-        for (int t = 0; t < tiles; ++t) scores(t, 0);
-        mma_commit(&empty[0]);
-      }
-      for (int j = 0; j < steps && live; ++j) {
-        const int use = 2 * j + 1;
-        live = stage_full(use) && (j + 1 >= steps || stage_full(use + 1));
-        const uint32_t v = ring + (use % kStages) * kTile;
-        for (int t = 0; t < tiles && live; ++t) {
-          live = bar_wait(&p_full[t], j & 1);
-          if (!live) break;
-          fence_after_sync();
+        const uint64_t k = k_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
+        if (leader) {
 #pragma unroll
-          for (int i = 0; i < kNTile / 16; ++i)
-            mma_ts(tmem + kOCol + t * D, tmem + kSCol + t * kNTile + i * 8, sw128_mn_desc(v + i * 2048, kLineTile), pv,
-                   j > 0 || i > 0);
-          if (j + 1 < steps) scores(t, use + 1);
+          for (int x = 0; x < D / 16; ++x) {
+            const int at = ((x / 4) * kLineTile + (x & 3) * 32) / 16;
+            mma_ss(sc + (i & 1) * kStep, q + at, k + at, qk, x > 0);
+          }
+          mma_commit(&s_full[t][i & 1]);
+          if ((i & 1) || i + 1 == subs) mma_commit(&empty[st]);
         }
-        mma_commit(&empty[use % kStages]);
-        if (j + 1 < steps) mma_commit(&empty[(use + 1) % kStages]);
+        return true;
+      };
+      // all 512 columns are this CTA's, so they start at 0
+      bool live = tmem == 0 && scores(0) && (subs == 1 || scores(1));
+      for (int i = 0; i < subs && live; ++i) {
+        const int use = i | 1, st = use % kStages;
+        live = stage_full(use) && wait_phase(&p_full[t][i & 1], (i >> 1) & 1);
+        if (!live) break;
+        fence_after_sync();
+        const uint64_t v = v_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
+        if (leader) {
+#pragma unroll
+          for (int x = 0; x < kStep / 16; ++x) mma_ts(oc, sc + (i & 1) * kStep + x * 8, v + x * 128, pv, i > 0 || x > 0);
+          if ((i & 1) || i + 1 == subs) mma_commit(&empty[st]);
+        }
+        if (i + 2 < subs)
+          live = scores(i + 2);
+        else if (leader)
+          mma_commit(&s_full[t][i & 1]);  // no scores: it tells that O is complete up to step i
       }
       if (!live) *dead = 1;
-      mma_commit(&o_full);
+      if (leader) mma_commit(&o_full[t]);
     }
     __syncwarp();
-  } else {
+  } else if (warp < 8) {
     // ---- softmax: one row a thread ------------------------------------------------
     const int t = warp >> 2, r = t * kMTile + (threadIdx.x & (kMTile - 1));
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
-    const uint32_t ts = tmem + lanes + kSCol + t * kNTile, to = tmem + lanes + kOCol + t * D;
+    const uint32_t ts = tmem + lanes + kSCol + t * 2 * kStep, to = tmem + lanes + kOCol + t * D;
     const bool mine = r < rows;
     const int pos = mine ? len - n + (tile.row0 + r) / group : -1;
     const float c2 = fabsf(a.scale) * 1.4426950408889634f;
+    const uint64_t c22 = pair_of(c2, c2);
     float m = -INFINITY, sum = 0.f;
     bool live = true;
     if (t < tiles) {
-      for (int j = 0; j < steps; ++j) {
-        live = bar_wait(&s_full[t], j & 1) && !*dead;
-        if (!__all_sync(~0u, live)) break;
+      for (int i = 0; i < subs; ++i) {
+        live = __all_sync(~0u, wait_phase(&s_full[t][i & 1], (i >> 1) & 1));
+        if (!live) break;
         fence_after_sync();
-        const int key = begin + j * kNTile;
-        float s[kNTile];
-#pragma unroll
-        for (int c = 0; c < kNTile; c += 32) tm_ld32(ts + c, s + c);
-        tmem_ld_wait();
-        if (key < all_lo || key + kNTile > all_hi || bad) {
-          const int top = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : 0;
-#pragma unroll
-          for (int c = 0; c < kNTile; ++c)
-            if (c > top || c < low) s[c] = -INFINITY;
+        const int key = begin + i * kStep;
+        const uint32_t at = ts + (i & 1) * kStep;
+        float s[kStep], tops[4] = {m, m, m, m};
+        tm_ld32(at, s);
+        tm_ld32(at + 32, s + 32);
+        tm_ld_wait32(s);
+        tm_ld_wait32(s + 32);
+        if (key < all_lo || key + kStep > all_hi || bad) {
+          const int last = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : 0;
+          unsigned ok = ~0u;  // pages that exist
+          const int in_page = key & (a.page_tokens - 1);  // 64 in the second half of a 128-token page
           if (bad) {
-            unsigned ok = 0;
-            for (int p = 0; p < kNTile >> shift && key + (p << shift) < end; ++p) {
-              const int id = table[(key >> shift) + p];
-              ok |= (id >= 0 && id < a.n_pages ? 1u : 0u) << p;
-            }
-#pragma unroll
-            for (int c = 0; c < kNTile; ++c)
-              if (!((ok >> (c >> shift)) & 1u)) s[c] = -INFINITY;
+            ok = 0;
+            for (int p = key >> shift; p << shift < min(key + kStep, end); ++p)
+              ok |= (table[p] >= 0 && table[p] < a.n_pages ? 1u : 0u) << (p - (key >> shift));
           }
-        }
-        float top = m;
 #pragma unroll
-        for (int c = 0; c < kNTile; ++c) top = fmaxf(top, s[c]);
-        // the first step sets the reference; later ones move it when it is left behind by more than 8
-        const bool move = j == 0 ? false : (top - m) * c2 > 8.f;
-        if (j == 0) m = top;
+          for (int c = 0; c < kStep; ++c)
+            if (c > last || c < low || !((ok >> ((in_page + c) >> shift)) & 1u)) s[c] = -INFINITY;
+        }
+#pragma unroll
+        for (int c = 0; c < kStep; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tops[k] = max3(tops[k], s[c + 2 * k], s[c + 2 * k + 1]);
+        const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+        // The first step sets the reference; later ones move it when a maximum
+        // leaves it behind by more than 8 (or is NaN).
+        const bool move = i > 0 && !(top <= m) && !((top - m) * c2 <= 8.f);
+        if (i == 0) m = top;
         if (__any_sync(~0u, move)) {
-          const float f = move ? ex2((m - top) * c2) : 1.f;
+          // O has to hold still: its products up to step i - 1 are done when the
+          // barrier of step i + 1's scores is through
+          live = __all_sync(~0u, wait_phase(&s_full[t][(i + 1) & 1], ((i + 1) >> 1) & 1));
+          if (!live) break;
+          fence_after_sync();
+          const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2((m - top) * c2);
           if (move) m = top;
           sum *= f;
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             float o[32];
             tm_ld32(to + c, o);
-            tmem_ld_wait();
+            tm_ld_wait32(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
+            for (int k = 0; k < 32; ++k) o[k] *= f;
             tm_st32(to + c, reinterpret_cast<const uint32_t*>(o));
           }
-          tm_st_wait();
         }
         const float off = m == -INFINITY ? 0.f : -m * c2;
-        float add[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t off2 = pair_of(off, off);
+        uint64_t add[2] = {0, 0};
+        uint32_t p[32];
 #pragma unroll
-        for (int c = 0; c < kNTile; c += 64) {
-          uint32_t p[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float x = ex2(fmaf(s[c + 2 * i], c2, off)), y = ex2(fmaf(s[c + 2 * i + 1], c2, off));
-            add[i & 3] += x + y;
-            p[i] = pack2<T>(x, y);  // weights in the cache's type for the tensor cores; their sum is not rounded
+        for (int k = 0; k < 32; ++k) {
+          float x, y;
+          const uint64_t e = fma_pair(pair_of(s[2 * k], s[2 * k + 1]), c22, off2);
+          if (k % 4 == 1) {  // a quarter on the FMA pipe: the exponential unit takes 8 clocks a warp
+            ex2_pair(e, x, y);
+          } else {
+            split_pair(e, x, y);
+            x = ex2(x), y = ex2(y);
           }
-          tm_st32(ts + c / 2, p);
+          add[k & 1] = add_pair(add[k & 1], pair_of(x, y));
+          p[k] = pack2<T>(x, y);  // weights in the cache's type for the tensor cores; their sum is not rounded
         }
-        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        tm_st32(at, p);
         tm_st_wait();
         fence_before_sync();
         __syncwarp();
-        if (lane == 0) bar_arrive(&p_full[t]);
+        if (lane == 0) bar_arrive(&p_full[t][i & 1]);
+        float x, y;
+        split_pair(add_pair(add[0], add[1]), x, y);
+        sum += x + y;
       }
-      if (steps > 0) live = live && bar_wait(&o_full, 0);
+      if (subs > 0) live = live && wait_phase(&o_full[t], 0);
       live = __all_sync(~0u, live) && !*dead;
       if (!live && lane == 0) {
         *dead = 1;
@@ -420,9 +536,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           float o[32];
-          if (steps > 0) {
+          if (subs > 0) {
             tm_ld32(to + c, o);
-            tmem_ld_wait();
+            tm_ld_wait32(o);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
