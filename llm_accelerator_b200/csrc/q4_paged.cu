@@ -22,22 +22,31 @@ inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uint
 // ---------------------------------------------------------------------------
 enum { kSame = 0, kE4m3 = 1, kS8 = 2 };
 
-// V consecutive values at p as floats, in as few accesses as V's bytes allow.
+// V consecutive values as they are stored, fetched in as few accesses as V's
+// bytes allow.
 template <typename T, int V>
-__device__ __forceinline__ void load_v(const T* p, float* f) {
-  if constexpr (sizeof(T) == 4 && V >= 4) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 w = *reinterpret_cast<const float4*>(p + i);
-      f[i] = w.x, f[i + 1] = w.y, f[i + 2] = w.z, f[i + 3] = w.w;
-    }
-  } else if constexpr (sizeof(T) == 2 && V == 8) {
-    unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = to_f32(p[i]);
+struct Raw {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void get(float* f) const { f[0] = to_f32(v); }
+};
+template <typename T>
+struct Raw<T, 8> {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float* f) const { unpack8<T>(v, f); }
+};
+template <>
+struct Raw<float, 8> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
   }
-}
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  }
+};
 template <typename T, int V>
 __device__ __forceinline__ void store_v(T* p, const float* f) {
   if constexpr (sizeof(T) == 4 && V >= 4) {
@@ -52,23 +61,28 @@ __device__ __forceinline__ void store_v(T* p, const float* f) {
 }
 template <int OUT, int V>
 __device__ __forceinline__ void store_8bit(uint8_t* p, const float* f, float inv) {
-  uint32_t w[(V + 3) / 4];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    uint32_t b;
-    if constexpr (OUT == kE4m3) {
-      b = __nv_cvt_float_to_fp8(f[i] * inv, __NV_SATFINITE, __NV_E4M3);
-    } else {
-      const int q = __float2int_rn(f[i] * inv);
-      b = (uint32_t)(q < -127 ? -127 : (q > 127 ? 127 : q)) & 0xffu;
-    }
-    w[i / 4] = (i % 4 ? w[i / 4] : 0u) | (b << (8 * (i % 4)));
-  }
+  auto s8 = [&](float v) {
+    const int q = __float2int_rn(v * inv);
+    return (uint32_t)(q < -127 ? -127 : (q > 127 ? 127 : q)) & 0xffu;
+  };
   if constexpr (V == 8) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      if constexpr (OUT == kE4m3)
+        w[i / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[i] * inv, f[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[i + 2] * inv, f[i + 3] * inv), __NV_SATFINITE,
+                                                      __NV_E4M3) << 16;
+      else
+        w[i / 4] = s8(f[i]) | s8(f[i + 1]) << 8 | s8(f[i + 2]) << 16 | s8(f[i + 3]) << 24;
+    }
     *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) p[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    static_assert(V == 1, "single values or eight");
+    if constexpr (OUT == kE4m3)
+      *p = __nv_cvt_float_to_fp8(f[0] * inv, __NV_SATFINITE, __NV_E4M3);
+    else
+      *p = (uint8_t)s8(f[0]);
   }
 }
 
@@ -86,143 +100,184 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
 }
-__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(~0u, v); }
+// NaN if a lane has one; over spans of `n` lanes (a power of two).
+__device__ __forceinline__ float span_max(float v, int n) {
+  for (int o = n >> 1; o; o >>= 1) {
+    const float u = __shfl_xor_sync(~0u, v, o);
+    v = max3(v, u, u);
+  }
+  return v;
+}
 
-// One row per blockDim.x threads (a power of two from 32), blockDim.y rows per
-// CTA (1 unless a row is one warp).  A thread holds E values of its row, V
-// consecutive ones at a time, so x and the residual are read once.  Magnitudes
-// are compared as the bits of |y|: a NaN is above everything and reaches the
-// scale.
+// Whether a thread's registers hold the next row's values and the weights too.
+template <typename T, int V, int E>
+__host__ __device__ constexpr bool norm_ahead() { return sizeof(T) == 2 && V == 8 && E <= 16; }
+
+// One row per blockDim.x threads (a power of two from 32), blockDim.y rows at a
+// time per CTA (1 unless a row is one warp).  A thread holds E values of its
+// row, V consecutive ones at a time, so x and the residual are read once.  Where
+// registers allow it (norm_ahead) CTAs stay and go from row to row: the next
+// row's values are on their way while this one is summed, scaled and stored.  Maxima pass NaNs on, so one reaches
+// the scale.  Bound by memory: 8192 x 4096 bf16 with a residual into e4m3 moves
+// 237 MB.
 template <typename T, int OUT, int V, int E>
 __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(NormParams p) {
   constexpr int N = E / V;
+  constexpr bool kAhead = norm_ahead<T, V, E>();
   const int tx = threadIdx.x, lanes = blockDim.x;
-  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  __shared__ float part[32];
-  __shared__ uint32_t partm[32];
-  if (row >= p.rows) return;  // only where a row is one warp
-  const T* x = static_cast<const T*>(p.x) + row * p.xs;
-  const T* res = p.residual ? static_cast<const T*>(p.residual) + row * p.rs : nullptr;
+  __shared__ float part[2][32];  // by turns, so that one barrier a row is enough
+  __shared__ float partm[32];
+  const T* x = static_cast<const T*>(p.x);
+  const T* res = static_cast<const T*>(p.residual);
   const T* w = static_cast<const T*>(p.weight);
-  float h[E];
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const int at = (c * lanes + tx) * V;
-#pragma unroll
-    for (int i = 0; i < V; ++i) h[c * V + i] = 0.f;
-    if (at < p.n) {
-      load_v<T, V>(x + at, h + c * V);
-      if (res) {
-        float r[V];
-        load_v<T, V>(res + at, r);
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[c * V + i] += r[i];
-      }
-    }
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) ss = fmaf(h[i], h[i], ss);
-  ss = warp_sum(ss);
-  if (lanes > 32) {
-    if ((tx & 31) == 0) part[tx >> 5] = ss;
-    __syncthreads();
-    ss = warp_sum((tx & 31) < (lanes >> 5) ? part[tx & 31] : 0.f);
-  }
-  const float inv = rsqrtf(ss / (float)p.n + p.eps);
-  if (p.residual_out) {
-    T* ro = static_cast<T*>(p.residual_out) + row * p.ros;
+  Raw<T, V> xr[N], rr[N], wr[N];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       const int at = (c * lanes + tx) * V;
-      if (at < p.n) store_v<T, V>(ro + at, h + c * V);
-    }
-  }
-  uint32_t most = 0;
-#pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const int at = (c * lanes + tx) * V;
-    if (at < p.n) {
-      float g[V];
-      load_v<T, V>(w + at, g);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        h[c * V + i] = h[c * V + i] * inv * g[i];
-        if constexpr (OUT != kSame) most = max(most, __float_as_uint(h[c * V + i]) & 0x7fffffffu);
+      if (at < p.n) {
+        xr[c].load(x + row * p.xs + at);
+        if (res) rr[c].load(res + row * p.rs + at);
       }
     }
+  };
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (kAhead && row < p.rows) fetch(row);
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if ((c * lanes + tx) * V < p.n) wr[c].load(w + (c * lanes + tx) * V);
   }
-  if constexpr (OUT == kSame) {
-    T* o = static_cast<T*>(p.out) + row * p.os;
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    float h[E], ss = 0.f;
+    if constexpr (!kAhead) fetch(row);
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int at = (c * lanes + tx) * V;
-      if (at < p.n) store_v<T, V>(o + at, h + c * V);
-    }
-  } else {
-    constexpr float kMost = OUT == kE4m3 ? 448.f : 127.f;
-    uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.os;
-    if (p.group == 0) {
-      most = warp_max(most);
-      if (lanes > 32) {
-        if ((tx & 31) == 0) partm[tx >> 5] = most;
-        __syncthreads();
-        most = warp_max((tx & 31) < (lanes >> 5) ? partm[tx & 31] : 0u);
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[c * V + i] = 0.f;
+      if ((c * lanes + tx) * V < p.n) {
+        xr[c].get(h + c * V);
+        if (res) {
+          float r[V];
+          rr[c].get(r);
+#pragma unroll
+          for (int i = 0; i < V; ++i) h[c * V + i] += r[i];
+        }
       }
-      const float top = __uint_as_float(most);
+    }
+    if (kAhead && row + step < p.rows) fetch(row + step);
+#pragma unroll
+    for (int i = 0; i < E; ++i) ss = fmaf(h[i], h[i], ss);
+    ss = warp_sum(ss);
+    if (lanes > 32) {
+      if ((tx & 31) == 0) part[turn][tx >> 5] = ss;
+      __syncthreads();
+      ss = warp_sum((tx & 31) < (lanes >> 5) ? part[turn][tx & 31] : 0.f);
+    }
+    const float inv = rsqrtf(ss / (float)p.n + p.eps);
+    if (p.residual_out) {
+      T* ro = static_cast<T*>(p.residual_out) + row * p.ros;
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const int at = (c * lanes + tx) * V;
+        if (at < p.n) store_v<T, V>(ro + at, h + c * V);
+      }
+    }
+    float most[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      most[c] = 0.f;
+      if ((c * lanes + tx) * V < p.n) {
+        float g[V];
+        if constexpr (!kAhead) wr[c].load(w + (c * lanes + tx) * V);
+        wr[c].get(g);
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[c * V + i] = h[c * V + i] * inv * g[i];
+        if constexpr (OUT != kSame && V > 1) {
+#pragma unroll
+          for (int i = 0; i < V; i += 2) most[c] = max3(most[c], fabsf(h[c * V + i]), fabsf(h[c * V + i + 1]));
+        } else if constexpr (OUT != kSame) {
+          most[c] = fabsf(h[c]);
+        }
+      }
+    }
+    if constexpr (OUT == kSame) {
+      T* o = static_cast<T*>(p.out) + row * p.os;
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const int at = (c * lanes + tx) * V;
+        if (at < p.n) store_v<T, V>(o + at, h + c * V);
+      }
+    } else {
+      constexpr float kMost = OUT == kE4m3 ? 448.f : 127.f;
+      uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.os;
       // a subnormal maximum would give an infinite factor
-      const float f = most ? fminf(__fdiv_rn(kMost, top), FLT_MAX) : 0.f;
-      if (tx == 0) p.scale[row] = __fdiv_rn(top, kMost);
+      auto factor = [&](float top) { return top == 0.f ? 0.f : fminf(__fdividef(kMost, top), FLT_MAX); };
+      if (p.group == 0) {
+        float top = 0.f;
 #pragma unroll
-      for (int c = 0; c < N; ++c) {
-        const int at = (c * lanes + tx) * V;
-        if (at < p.n) store_8bit<OUT, V>(o + at, h + c * V, f);
-      }
-    } else if constexpr (V == 8) {
-      // a group is group / 8 neighbouring lanes of one access
-      const int span = p.group / 8, groups = p.n / p.group;
-#pragma unroll
-      for (int c = 0; c < N; ++c) {
-        uint32_t m = 0;
-        const int at = (c * lanes + tx) * V;
-        if (at < p.n) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(h[c * V + i]) & 0x7fffffffu);
+        for (int c = 0; c < N; ++c) top = max3(top, most[c], most[c]);
+        top = span_max(top, 32);
+        if (lanes > 32) {
+          if ((tx & 31) == 0) partm[tx >> 5] = top;
+          __syncthreads();
+          top = span_max((tx & 31) < (lanes >> 5) ? partm[tx & 31] : 0.f, 32);
         }
-        for (int o2 = span >> 1; o2; o2 >>= 1) m = max(m, __shfl_xor_sync(~0u, m, o2));
-        if (at < p.n) {
-          const float top = __uint_as_float(m);
-          const float f = m ? fminf(__fdiv_rn(kMost, top), FLT_MAX) : 0.f;
-          if ((tx & (span - 1)) == 0) p.scale[row * groups + at / p.group] = __fdiv_rn(top, kMost);
-          store_8bit<OUT, V>(o + at, h + c * V, f);
+        const float f = factor(top);
+        if (tx == 0) p.scale[row] = top * (1.f / kMost);
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const int at = (c * lanes + tx) * V;
+          if (at < p.n) store_8bit<OUT, V>(o + at, h + c * V, f);
+        }
+      } else if constexpr (V == 8) {
+        // a group is group / 8 neighbouring lanes of one access
+        const int span = p.group / 8, groups = p.n / p.group;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const int at = (c * lanes + tx) * V;
+          const float top = span_max(most[c], span);
+          if (at < p.n) {
+            if ((tx & (span - 1)) == 0) p.scale[row * groups + at / p.group] = top * (1.f / kMost);
+            store_8bit<OUT, V>(o + at, h + c * V, factor(top));
+          }
         }
       }
     }
+    if constexpr (!kAhead) break;  // one row a CTA
   }
 }
 
-template <typename T, int OUT>
-void launch_norm(const NormParams& p, bool vec, cudaStream_t s) {
-  // A thread takes 8 values where that already gives a row enough threads
-  // and there are too few rows to fill the GPU, else 32.
-  const bool few = p.rows < 148 * 4 && p.n <= 8192;
-  const int per = few ? 8 : 32;
+template <typename T, int OUT, int V>
+void launch_norm_v(const NormParams& p, cudaStream_t s) {
+  // A thread takes 8 values of its row where there are too few rows to fill the
+  // GPU, else 16: two accesses of x and two of the residual in flight in each of
+  // 2048 threads cover the memory's latency (with 32 the loads were issued one
+  // after the other to stay within 64 registers: 70.8 us against 46.8 for 8192 x
+  // 4096 into e4m3).  32 only where a row is longer than 1024 threads x 16.
+  const int per = p.n > 16384 ? 32 : p.rows < 148 * 4 && p.n <= 8192 ? 8 : 16;
   int lanes = 32;
   while (lanes * per < p.n) lanes *= 2;
   const int ny = lanes == 32 ? 4 : 1;
   const dim3 block(lanes, ny);
-  const unsigned grid = (unsigned)((p.rows + ny - 1) / ny);
-  if (vec) {
-    if (few)
-      add_rmsnorm_kernel<T, OUT, 8, 8><<<grid, block, 0, s>>>(p);
-    else
-      add_rmsnorm_kernel<T, OUT, 8, 32><<<grid, block, 0, s>>>(p);
-  } else {
-    if (few)
-      add_rmsnorm_kernel<T, OUT, 1, 8><<<grid, block, 0, s>>>(p);
-    else
-      add_rmsnorm_kernel<T, OUT, 1, 32><<<grid, block, 0, s>>>(p);
-  }
+  // rows at a time; with 64 registers a thread 1024 threads stay on each SM
+  const int64_t all = (p.rows + ny - 1) / ny, some = 148 * (1024 / (lanes * ny));
+  const bool stay = per <= 16 && norm_ahead<T, V, 16>();
+  const unsigned grid = (unsigned)(stay ? std::min(all, some) : all);
+  if (per == 8)
+    add_rmsnorm_kernel<T, OUT, V, 8><<<grid, block, 0, s>>>(p);
+  else if (per == 16)
+    add_rmsnorm_kernel<T, OUT, V, 16><<<grid, block, 0, s>>>(p);
+  else
+    add_rmsnorm_kernel<T, OUT, V, 32><<<grid, block, 0, s>>>(p);
+}
+template <typename T, int OUT>
+void launch_norm(const NormParams& p, bool vec, cudaStream_t s) {
+  if (vec)
+    launch_norm_v<T, OUT, 8>(p, s);
+  else
+    launch_norm_v<T, OUT, 1>(p, s);
 }
 
 template <typename T>
@@ -241,43 +296,17 @@ void launch_norm_out(const NormParams& p, int out_dtype, bool vec, cudaStream_t 
 // A head vector is cut into units of 16 values: a rotated unit is 8 pairs (8
 // values and their 8 partners, or 16 neighbours where pairs are interleaved),
 // the rest are plain.  `lanes` threads (a power of two) share a head vector,
-// one unit each.
-template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rope_append_kernel(q4gpu_rope_args a, int lanes, int heads) {
-  const int64_t flat = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int u = (int)(flat & (lanes - 1));
-  const int64_t vec = flat / lanes;
-  const int64_t token = vec / heads;
-  int head = (int)(vec - token * heads);
-  const bool there = token < a.tokens;
+// one unit each, and a thread takes its unit of VECS head vectors of one token
+// (heads s, s + slots, ..), so the token's cosines and sines are fetched once
+// for all of them and 32 VECS bytes of data are in flight per thread.  Bound by
+// memory, and by the way from a token's position to its table row.
+template <typename T, bool INTERLEAVED, int VECS>
+__global__ void __launch_bounds__(256) rope_append_kernel(q4gpu_rope_args a, int lanes, int heads, int slots) {
+  const uint32_t flat = blockIdx.x * blockDim.x + threadIdx.x;
+  const int u = flat & (lanes - 1);
+  const uint32_t group = flat / lanes, token = group / (uint32_t)slots, slot = group - token * slots;
+  const bool there = token < (uint32_t)a.tokens;
   const int nq = a.q ? a.q_heads : 0, nk = a.k ? a.kv_heads : 0;
-  const T* src = nullptr;
-  T* dst = nullptr;
-  const T* gamma = nullptr;
-  bool rotate = true;
-  if (there) {
-    if (head < nq) {
-      src = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
-      dst = static_cast<T*>(a.q_out) + token * a.q_out_token_stride + head * a.q_out_head_stride;
-      gamma = static_cast<const T*>(a.q_gamma);
-    } else {
-      head -= nq;
-      const bool is_k = head < nk;
-      if (!is_k) head -= nk;
-      rotate = is_k;
-      src = is_k ? static_cast<const T*>(a.k) + token * a.k_token_stride + head * a.k_head_stride
-                 : static_cast<const T*>(a.v) + token * a.v_token_stride + head * a.v_head_stride;
-      gamma = is_k ? static_cast<const T*>(a.k_gamma) : nullptr;
-      const int64_t row = a.rows[token];
-      if (row >= a.n_rows) {
-        if (a.err_flag) *a.err_flag = 1;
-      } else if (row >= 0) {
-        const int64_t page = row / a.page_tokens;
-        dst = static_cast<T*>(is_k ? a.k_cache : a.v_cache) + page * a.page_stride + head * a.head_stride +
-              (row - page * a.page_tokens) * a.row_stride;
-      }
-    }
-  }
   const int turned = a.rot_dim / 16;
   int at0, at1;
   if (u < turned) {
@@ -287,54 +316,121 @@ __global__ void __launch_bounds__(256) rope_append_kernel(q4gpu_rope_args a, int
     at0 = 16 * u;
     at1 = at0 + 8;
   }
-  const bool has0 = src && at0 < a.dim, has1 = src && at1 < a.dim;
-  float f[16];
+  const bool has0 = there && at0 < a.dim, has1 = there && at1 < a.dim;
+
+  const int64_t row = there && a.rows ? a.rows[token] : -1;
+  const int pos = there && a.positions ? a.positions[token] : 0;
+  uint4 raw[VECS][2];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = 0.f;
-  if (has0) unpack8<T>(*reinterpret_cast<const uint4*>(src + at0), f);
-  if (has1) unpack8<T>(*reinterpret_cast<const uint4*>(src + at1), f + 8);
-  if (a.q_gamma || a.k_gamma) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) ss = fmaf(f[i], f[i], ss);
-    for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-    if (gamma) {
-      const float inv = rsqrtf(ss / (float)a.dim + a.eps);
-      float g[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) g[i] = 0.f;
-      if (has0) unpack8<T>(*reinterpret_cast<const uint4*>(gamma + at0), g);
-      if (has1) unpack8<T>(*reinterpret_cast<const uint4*>(gamma + at1), g + 8);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = f[i] * inv * g[i];
+  for (int i = 0; i < VECS; ++i) {
+    int head = slot + i * slots;
+    raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (head >= heads) continue;
+    const T* src;
+    if (head < nq)
+      src = static_cast<const T*>(a.q) + token * a.q_token_stride + head * a.q_head_stride;
+    else if ((head -= nq) < nk)
+      src = static_cast<const T*>(a.k) + token * a.k_token_stride + head * a.k_head_stride;
+    else
+      src = static_cast<const T*>(a.v) + token * a.v_token_stride + (head - nk) * a.v_head_stride;
+    if (has0) raw[i][0] = *reinterpret_cast<const uint4*>(src + at0);
+    if (has1) raw[i][1] = *reinterpret_cast<const uint4*>(src + at1);
+  }
+
+  bool known = true;  // the position has a table row
+  float cs[8], sn[8];
+  if (there && turned && nq + nk > 0) {
+    known = pos >= 0 && pos < a.table_positions;
+    if (known && u < turned) {
+      Raw<float, 8> w;
+      w.load(a.cos + (int64_t)pos * (a.rot_dim / 2) + 8 * u);
+      w.get(cs);
+      w.load(a.sin + (int64_t)pos * (a.rot_dim / 2) + 8 * u);
+      w.get(sn);
     }
   }
-  if (rotate && src && turned) {
-    const int pos = a.positions[token];
-    if (pos < 0 || pos >= a.table_positions) {
-      if (a.err_flag) *a.err_flag = 1;
-      dst = nullptr;
-    } else if (u < turned) {
-      const float* cs = a.cos + (int64_t)pos * (a.rot_dim / 2) + 8 * u;
-      const float* sn = a.sin + (int64_t)pos * (a.rot_dim / 2) + 8 * u;
+  const bool stored = row >= 0 && row < a.n_rows;
+  if (there && (!known || row >= a.n_rows) && a.err_flag) *a.err_flag = 1;
+  // (a 32-bit division where the row allows it)
+  const int64_t page = !stored ? 0 : row >> 32 ? row / a.page_tokens : (int64_t)((uint32_t)row / (uint32_t)a.page_tokens);
+  const int64_t cache = page * a.page_stride + (row - page * a.page_tokens) * a.row_stride;
+
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int x = INTERLEAVED ? 2 * i : i, y = INTERLEAVED ? 2 * i + 1 : i + 8;
-        const float c = cs[i], t = sn[i], p = f[x], q = f[y];
-        f[x] = p * c - q * t;
-        f[y] = q * c + p * t;
+  for (int i = 0; i < VECS; ++i) {
+    int head = slot + i * slots;
+    const bool is_q = head < nq, is_k = !is_q && head < nq + nk;
+    const T* gamma = static_cast<const T*>(is_q ? a.q_gamma : is_k ? a.k_gamma : nullptr);
+    float f[16];
+    unpack8<T>(raw[i][0], f);
+    unpack8<T>(raw[i][1], f + 8);
+    if (a.q_gamma || a.k_gamma) {
+      float ss = 0.f;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) ss = fmaf(f[x], f[x], ss);
+      for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+      if (gamma) {
+        const float inv = rsqrtf(ss / (float)a.dim + a.eps);
+        float g[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) g[x] = 0.f;
+        if (has0) unpack8<T>(*reinterpret_cast<const uint4*>(gamma + at0), g);
+        if (has1) unpack8<T>(*reinterpret_cast<const uint4*>(gamma + at1), g + 8);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) f[x] = f[x] * inv * g[x];
       }
     }
+    T* dst;
+    if (is_q) {
+      dst = static_cast<T*>(a.q_out) + token * a.q_out_token_stride + head * a.q_out_head_stride;
+    } else {
+      head -= nq + (is_k ? 0 : nk);
+      dst = static_cast<T*>(is_k ? a.k_cache : a.v_cache) + cache + head * a.head_stride;
+    }
+    if (slot + i * slots >= heads || (!is_q && !stored) || ((is_q || is_k) && !known)) continue;
+    if ((is_q || is_k) && u < turned) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const int x = INTERLEAVED ? 2 * p : p, y = INTERLEAVED ? 2 * p + 1 : p + 8;
+        const float v = f[x], w = f[y];
+        f[x] = v * cs[p] - w * sn[p];
+        f[y] = w * cs[p] + v * sn[p];
+      }
+    }
+    if (has0) *reinterpret_cast<uint4*>(dst + at0) = pack8<T>(f);
+    if (has1) *reinterpret_cast<uint4*>(dst + at1) = pack8<T>(f + 8);
   }
-  if (dst && has0) *reinterpret_cast<uint4*>(dst + at0) = pack8<T>(f);
-  if (dst && has1) *reinterpret_cast<uint4*>(dst + at1) = pack8<T>(f + 8);
+}
+
+template <typename T, bool INTERLEAVED>
+void launch_rope(const q4gpu_rope_args& a, int lanes, int heads, cudaStream_t s) {
+  // Four head vectors a thread once that still gives every SM 512 threads; one
+  // where latency counts.
+  const bool many = (int64_t)a.tokens * heads * lanes >= (int64_t)4 * 148 * 512;
+  const int slots = many ? (heads + 3) / 4 : heads;
+  const int64_t threads = (int64_t)a.tokens * slots * lanes;
+  const int block = (int)std::min<int64_t>(256, (threads + 31) / 32 * 32);
+  const unsigned grid = (unsigned)((threads + block - 1) / block);
+  if (many)
+    rope_append_kernel<T, INTERLEAVED, 4><<<grid, block, 0, s>>>(a, lanes, heads, slots);
+  else
+    rope_append_kernel<T, INTERLEAVED, 1><<<grid, block, 0, s>>>(a, lanes, heads, slots);
 }
 
 // ---------------------------------------------------------------------------
 // pages
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void copy16(uint4* d, const uint4* s, int64_t n, int64_t first, int64_t step) {
-  for (int64_t i = first; i < n; i += step) d[i] = s[i];
+// A CTA's copy of n 16-byte words, eight loads of a thread in flight.
+__device__ __forceinline__ void copy16(uint4* d, const uint4* s, int n) {
+  constexpr int kFlight = 8;
+  for (int i = threadIdx.x; i < n; i += kFlight * blockDim.x) {
+    uint4 v[kFlight];
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k)
+      if (i + k * (int)blockDim.x < n) v[k] = s[i + k * blockDim.x];
+#pragma unroll
+    for (int k = 0; k < kFlight; ++k)
+      if (i + k * (int)blockDim.x < n) d[i + k * blockDim.x] = v[k];
+  }
 }
 
 // Tokens that slot s holds, inside what its table row can name.
@@ -344,7 +440,7 @@ __device__ __forceinline__ int64_t held(const q4gpu_pages_args& a, int64_t s) {
 }
 
 // blockIdx.y = fork, blockIdx.x strides over the page's blocks.
-__global__ void __launch_bounds__(256) pages_fork_kernel(q4gpu_pages_args a, const int32_t* parents,
+__global__ void __launch_bounds__(128) pages_fork_kernel(q4gpu_pages_args a, const int32_t* parents,
                                                          const int32_t* children, const int32_t* fresh) {
   const int i = blockIdx.y;
   const int par = parents[i], chi = children[i];
@@ -375,24 +471,26 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(q4gpu_pages_args a, con
     if (threadIdx.x == 0) a.lens[chi] = (int32_t)n;
   }
   if (!part) return;
-  const int64_t vecs = a.block_bytes / a.page_tokens * part / 16;
+  const int vecs = (int)(a.block_bytes / a.page_tokens * part / 16);
   const char* s = static_cast<const char*>(a.pool) + source * a.page_bytes;
   char* d = static_cast<char*>(a.pool) + to * a.page_bytes;
   const int64_t blocks = a.page_bytes / a.block_bytes;
   for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x)
     copy16(reinterpret_cast<uint4*>(d + b * a.block_bytes), reinterpret_cast<const uint4*>(s + b * a.block_bytes),
-           vecs, threadIdx.x, blockDim.x);
+           vecs);
 }
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWords = 8192;  // bit words in shared memory: pools up to 262,144 pages
+constexpr int kPlanWords = 4096;  // bit words in shared memory: pools up to 131,072 pages
 
 // One CTA: marks the pages in use, counts them, and pairs each used page past
 // the packed end with an unused one below it (in order, so the result does not
 // depend on timing).  moves = {source, destination} pairs, *n_moves of them.
 __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(q4gpu_pages_args a, int32_t* remap, int32_t* n_live,
-                                                                  uint32_t* ws_bits, int32_t* n_moves, int2* moves) {
+                                                                  uint32_t* ws_bits, int32_t* ws_below,
+                                                                  int32_t* n_moves, int2* moves) {
   __shared__ uint32_t s_bits[kPlanWords];
+  __shared__ int32_t s_below[kPlanWords];  // used pages below a word
   __shared__ int s_warp[kPlanThreads / 32];
   __shared__ int s_before;
   const int t = threadIdx.x;
@@ -454,17 +552,20 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(q4gpu_pages_ar
     *n_live = total;
     *n_moves = total - low;
   }
-  int used = before;
+  int below = before;
   for (int w = lo; w < hi; ++w) {
+    (small ? s_below : ws_below)[w] = below;
+    below += __popc(word(w));
+  }
+  __syncthreads();
+  for (int page = t; page < a.n_pages; page += kPlanThreads) {
+    const int w = page >> 5, k = page & 31;
     const uint32_t b = word(w);
-    for (int k = 0; k < 32 && w * 32 + k < a.n_pages; ++k) {
-      const int page = w * 32 + k;
-      const bool live = (b >> k) & 1u;
-      remap[page] = live ? page : -1;
-      if (live && page >= total) moves[used - low].x = page;
-      if (!live && page < total) moves[page - used].y = page;
-      used += live;
-    }
+    const bool live = (b >> k) & 1u;
+    const int used = (small ? s_below[w] : __ldcg(ws_below + w)) + __popc(b & ((1u << k) - 1u));
+    remap[page] = live ? page : -1;
+    if (live && page >= total) moves[used - low].x = page;
+    if (!live && page < total) moves[page - used].y = page;
   }
   __syncthreads();
   for (int i = t; i < total - low; i += kPlanThreads) remap[moves[i].x] = moves[i].y;
@@ -489,8 +590,8 @@ __global__ void __launch_bounds__(512) pages_move_kernel(q4gpu_pages_args a, int
     const int2 mv = moves[m];
     const int64_t bytes = min(kMoveBytes, a.page_bytes - off);
     copy16(reinterpret_cast<uint4*>(static_cast<char*>(a.pool) + mv.y * a.page_bytes + off),
-           reinterpret_cast<const uint4*>(static_cast<const char*>(a.pool) + mv.x * a.page_bytes + off), bytes / 16,
-           threadIdx.x, blockDim.x);
+           reinterpret_cast<const uint4*>(static_cast<const char*>(a.pool) + mv.x * a.page_bytes + off),
+           (int)(bytes / 16));
   }
 }
 
@@ -501,6 +602,7 @@ int check_pages(const q4gpu_pages_args* a) {
     return q4gpu_fail(Q4GPU_ERR_ARG, "pages: n_pages, page_tokens, n_slots, table_stride and sizes must be positive");
   if (a->page_bytes % a->block_bytes || a->block_bytes % a->page_tokens)
     return q4gpu_fail(Q4GPU_ERR_SHAPE, "pages: a page is whole blocks and a block page_tokens equal rows");
+  if (a->block_bytes > INT32_MAX) return q4gpu_fail(Q4GPU_ERR_SHAPE, "pages: a block is at most 2 GiB");
   if (!aligned(a->pool, 16) || (a->block_bytes / a->page_tokens) % 16)
     return q4gpu_fail(Q4GPU_ERR_ALIGN, "pages: the pool and its rows are multiples of 16 bytes");
   return Q4GPU_OK;
@@ -548,6 +650,7 @@ int q4gpu_add_rmsnorm(const q4gpu_norm_args* a, void* stream) {
 int q4gpu_rope_append(const q4gpu_rope_args* a, void* stream) {
   if (!a) return q4gpu_fail(Q4GPU_ERR_ARG, "rope: null arguments");
   if (a->tokens < 0 || a->q_heads < 0 || a->kv_heads < 0) return q4gpu_fail(Q4GPU_ERR_ARG, "rope: negative size");
+  if (a->q_heads > 65535 || a->kv_heads > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "rope: too many heads");
   if (a->tokens == 0) return Q4GPU_OK;
   const bool turns = (a->q || a->k) && a->rot_dim > 0, stores = a->k || a->v;
   if ((!a->q && !stores) || (a->q && !a->q_out) || (a->k && !a->k_cache) || (a->v && !a->v_cache) ||
@@ -565,28 +668,25 @@ int q4gpu_rope_append(const q4gpu_rope_args* a, void* stream) {
       !ok(a->q ? a->q_out : nullptr, a->q_out_token_stride, a->q_out_head_stride) ||
       !ok(a->k ? a->k_cache : nullptr, a->page_stride, a->head_stride) ||
       !ok(a->v ? a->v_cache : nullptr, a->page_stride, a->head_stride) || (stores && a->row_stride % 8) ||
-      !ok(a->q_gamma, 0, 0) || !ok(a->k_gamma, 0, 0))
-    return q4gpu_fail(Q4GPU_ERR_ALIGN, "rope: head vectors start on 16-byte boundaries");
+      !ok(a->q_gamma, 0, 0) || !ok(a->k_gamma, 0, 0) || (turns && (!aligned(a->cos, 16) || !aligned(a->sin, 16))))
+    return q4gpu_fail(Q4GPU_ERR_ALIGN, "rope: head vectors and tables start on 16-byte boundaries");
   const int heads = (a->q ? a->q_heads : 0) + (a->k ? a->kv_heads : 0) + (a->v ? a->kv_heads : 0);
   if (heads == 0) return Q4GPU_OK;
   const int units = a->rot_dim / 16 + (a->dim - a->rot_dim + 15) / 16;
   int lanes = 1;
   while (lanes < units) lanes *= 2;
-  const int64_t threads = (int64_t)a->tokens * heads * lanes;
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > INT32_MAX) return q4gpu_fail(Q4GPU_ERR_SHAPE, "rope: too many tokens");
-  const unsigned grid = (unsigned)blocks;
+  if ((int64_t)a->tokens * heads * lanes > INT32_MAX) return q4gpu_fail(Q4GPU_ERR_SHAPE, "rope: too many tokens");
   cudaStream_t s = as_stream(stream);
   if (a->dtype == Q4GPU_F16) {
     if (a->interleaved)
-      rope_append_kernel<__half, true><<<grid, 256, 0, s>>>(*a, lanes, heads);
+      launch_rope<__half, true>(*a, lanes, heads, s);
     else
-      rope_append_kernel<__half, false><<<grid, 256, 0, s>>>(*a, lanes, heads);
+      launch_rope<__half, false>(*a, lanes, heads, s);
   } else {
     if (a->interleaved)
-      rope_append_kernel<__nv_bfloat16, true><<<grid, 256, 0, s>>>(*a, lanes, heads);
+      launch_rope<__nv_bfloat16, true>(*a, lanes, heads, s);
     else
-      rope_append_kernel<__nv_bfloat16, false><<<grid, 256, 0, s>>>(*a, lanes, heads);
+      launch_rope<__nv_bfloat16, false>(*a, lanes, heads, s);
   }
   return q4gpu_check_launch();
 }
@@ -599,16 +699,16 @@ int q4gpu_pages_fork(const q4gpu_pages_args* a, const int32_t* parents, const in
   if (n == 0) return Q4GPU_OK;
   if (!parents || !children || !fresh) return q4gpu_fail(Q4GPU_ERR_ARG, "pages: null pointer");
   const int64_t blocks = a->page_bytes / a->block_bytes;
-  const unsigned x = (unsigned)std::min<int64_t>(blocks, std::max(1, 148 * 16 / n));
-  pages_fork_kernel<<<dim3(x, n), 256, 0, as_stream(stream)>>>(*a, parents, children, fresh);
+  const unsigned x = (unsigned)std::min<int64_t>(blocks, std::max(1, 148 * 64 / n));
+  pages_fork_kernel<<<dim3(x, n), 128, 0, as_stream(stream)>>>(*a, parents, children, fresh);
   return q4gpu_check_launch();
 }
 
-// workspace: {count, padding}, moves, bit words
+// workspace: {count, padding}, moves, bit words, used pages below each word
 size_t q4gpu_pages_compact_workspace_bytes(int32_t n_pages) {
   if (n_pages < 1) return 0;
   const size_t moves = ((size_t)n_pages * sizeof(int2) + 15) / 16 * 16;
-  return 16 + moves + ((size_t)n_pages + 31) / 32 * 4;
+  return 16 + moves + ((size_t)n_pages + 31) / 32 * 8;
 }
 
 int q4gpu_pages_compact(const q4gpu_pages_args* a, int32_t* new_table, int32_t* remap, int32_t* n_live,
@@ -624,8 +724,9 @@ int q4gpu_pages_compact(const q4gpu_pages_args* a, int32_t* new_table, int32_t* 
   int32_t* count = reinterpret_cast<int32_t*>(ws);
   int2* moves = reinterpret_cast<int2*>(ws + 16);
   uint32_t* bits = reinterpret_cast<uint32_t*>(ws + 16 + moves_bytes);
+  int32_t* below = reinterpret_cast<int32_t*>(bits + ((size_t)a->n_pages + 31) / 32);
   cudaStream_t s = as_stream(stream);
-  pages_plan_kernel<<<1, kPlanThreads, 0, s>>>(*a, remap, n_live, bits, count, moves);
+  pages_plan_kernel<<<1, kPlanThreads, 0, s>>>(*a, remap, n_live, bits, below, count, moves);
   pages_move_kernel<<<148 * 4, 512, 0, s>>>(*a, new_table, remap, count, moves);
   return q4gpu_check_launch();
 }

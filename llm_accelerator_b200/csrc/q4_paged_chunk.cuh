@@ -201,12 +201,6 @@ __device__ __forceinline__ void ex2_pair(uint64_t x2, float& x, float& y) {
   x = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n) << 23));
   y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(m) << 23));
 }
-// The largest of three; NaN if one is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // One CTA: 256 query rows (row = token * group + head of the group) of one

@@ -33,8 +33,10 @@ _DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.b
            torch.float8_e4m3fn: _native.DT_E4M3, torch.int8: _native.DT_S8}
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+# torch's current stream of a device as a cudaStream_t.  The public accessor builds a Stream
+# object first (3 us on the host, as long as a small kernel); this is the call inside it.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                  lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _need(ok: bool, what: str) -> None:
@@ -84,27 +86,33 @@ class AddRmsNorm:
     def _rows(self, t: torch.Tensor, rows: int, name: str, dtype: torch.dtype) -> int:
         if t.dtype != dtype or t.device != self.device:
             raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {dtype} on {self.device}")
-        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != self.n or (t.stride(1) != 1 and self.n > 1):
-            raise ValueError(f"{name} must be [{rows}, {self.n}] with contiguous rows")
-        return t.stride(0)
+        if t.shape != (rows, self.n):
+            raise ValueError(f"{name} must be [{rows}, {self.n}], got {tuple(t.shape)}")
+        row, one = t.stride()
+        if one != 1 and self.n > 1:
+            raise ValueError(f"{name} must have contiguous rows")
+        return row
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                  residual_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
         """x, residual, residual_out, out: [rows, n]; returns out, or (out, scale) for 8 bits."""
-        _need(x.dim() == 2, "x must be [rows, n]")
-        rows = x.shape[0]
-        a = self.args
+        a, dtype = self.args, self.dtype
+        if x.dim() != 2:
+            raise ValueError("x must be [rows, n]")
+        a.rows = rows = len(x)
+        a.x_stride = self._rows(x, rows, "x", dtype)
+        a.x = x.data_ptr()
         if out is None:
             out = torch.empty(rows, self.n, dtype=self.out_dtype, device=self.device)
-        a.rows = rows
-        a.x, a.x_stride = x.data_ptr(), self._rows(x, rows, "x", self.dtype)
-        a.out, a.out_stride = out.data_ptr(), self._rows(out, rows, "out", self.out_dtype)
+        a.out_stride = self._rows(out, rows, "out", self.out_dtype)
+        a.out = out.data_ptr()
         a.residual = a.residual_out = a.scale = None
         if residual is not None:
-            a.residual, a.residual_stride = residual.data_ptr(), self._rows(residual, rows, "residual", self.dtype)
+            a.residual_stride = self._rows(residual, rows, "residual", dtype)
+            a.residual = residual.data_ptr()
         if residual_out is not None:
+            a.residual_out_stride = self._rows(residual_out, rows, "residual_out", dtype)
             a.residual_out = residual_out.data_ptr()
-            a.residual_out_stride = self._rows(residual_out, rows, "residual_out", self.dtype)
         if self.narrow:
             if scale is None:
                 scale = torch.empty(rows, self.groups, dtype=torch.float32, device=self.device)
@@ -112,7 +120,7 @@ class AddRmsNorm:
             _need(scale.shape == (rows, self.groups) and scale.is_contiguous(),
                   f"scale must be contiguous [{rows}, {self.groups}]")
             a.scale = scale.data_ptr()
-        rc = self.lib.q4gpu_add_rmsnorm(a, _stream())
+        rc = self.lib.q4gpu_add_rmsnorm(a, _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_add_rmsnorm")
         return (out, scale) if self.narrow else out
@@ -176,12 +184,14 @@ class RopeAppend(_Err):
         dtype, a = ref.dtype, self.args
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"head vectors are {dtype}, expected float16 or bfloat16")
-        _need(self.gamma_dim in (None, (dim, dtype)), f"gamma does not match head vectors of {dim} x {dtype}")
+        if self.gamma_dim is not None and self.gamma_dim != (dim, dtype):
+            raise ValueError(f"gamma does not match head vectors of {dim} x {dtype}")
         a.tokens, a.dim, a.dtype, a.q_heads, a.kv_heads = tokens, dim, _DTYPES[dtype], 0, 0
         a.q = a.k = a.v = a.q_out = a.k_cache = a.v_cache = a.positions = a.rows = None
         if q is not None or k is not None:
             _on(positions, self.device, "positions", torch.int32)
-            _need(positions.shape == (tokens,) and positions.is_contiguous(), f"positions must be [{tokens}]")
+            if positions.shape != (tokens,) or not positions.is_contiguous():
+                raise ValueError(f"positions must be a contiguous vector of {tokens}")
             a.positions = positions.data_ptr()
         if q is not None:
             q_out = q if q_out is None else q_out
@@ -191,27 +201,30 @@ class RopeAppend(_Err):
                                                                              "q_out")
         if k is not None or v is not None:
             _on(rows, self.device, "rows", torch.int64)
-            _need(rows.shape == (tokens,) and rows.is_contiguous(), f"rows must be [{tokens}]")
+            if rows.shape != (tokens,) or not rows.is_contiguous():
+                raise ValueError(f"rows must be a contiguous vector of {tokens}")
             a.rows = rows.data_ptr()
-            a.kv_heads = (k if k is not None else v).shape[1]
+            a.kv_heads = heads = (k if k is not None else v).shape[1]
             cache = k_cache if k is not None else v_cache
+            if cache is None:
+                raise ValueError("keys and values need their caches")
+            shape, strides = cache.shape, cache.stride()
             for t, c, name in ((k, k_cache, "k"), (v, v_cache, "v")):
                 if t is None:
                     continue
-                p, ts, hs = self._heads(t, tokens, a.kv_heads, dim, dtype, name)
-                setattr(a, name, p)
-                setattr(a, name + "_token_stride", ts)
-                setattr(a, name + "_head_stride", hs)
-                _on(c, self.device, name + "_cache", dtype)
-                st = c.stride()
-                if c.dim() != 4 or c.shape != cache.shape or st != cache.stride() or st[3] != 1 or \
-                        c.shape[1] != a.kv_heads or c.shape[3] != dim:
-                    raise ValueError(f"{name}_cache must be [pages, {a.kv_heads}, page_tokens, {dim}] with contiguous "
-                                     "head vectors, K and V laid out alike")
-                setattr(a, name + "_cache", c.data_ptr())
-            a.page_stride, a.head_stride, a.row_stride, _ = cache.stride()
-            a.page_tokens, a.n_rows = cache.shape[2], cache.shape[0] * cache.shape[2]
-        rc = self.lib.q4gpu_rope_append(a, _stream())
+                if c is None or c.dtype != dtype or c.device != self.device or c.shape != shape or c.stride() != strides:
+                    raise ValueError(f"{name}_cache must be {tuple(shape)} {dtype}, K and V laid out alike")
+            if len(shape) != 4 or strides[3] != 1 or shape[1] != heads or shape[3] != dim:
+                raise ValueError(f"the caches must be [pages, {heads}, page_tokens, {dim}] with contiguous head vectors")
+            if k is not None:
+                a.k, a.k_token_stride, a.k_head_stride = self._heads(k, tokens, heads, dim, dtype, "k")
+                a.k_cache = k_cache.data_ptr()
+            if v is not None:
+                a.v, a.v_token_stride, a.v_head_stride = self._heads(v, tokens, heads, dim, dtype, "v")
+                a.v_cache = v_cache.data_ptr()
+            a.page_stride, a.head_stride, a.row_stride, _ = strides
+            a.page_tokens, a.n_rows = shape[2], shape[0] * shape[2]
+        rc = self.lib.q4gpu_rope_append(a, _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_rope_append")
         return q_out
@@ -290,14 +303,15 @@ class Attention(_Err):
             raise ValueError(f"{n} sequences over {self.slots} slots")
         if lse is not None:
             _on(lse, self.device, "lse", torch.float32)
-            _need(lse.shape == (tokens, self.q_heads) and lse.is_contiguous(), f"lse must be [{tokens}, {self.q_heads}]")
+            if lse.shape != (tokens, self.q_heads) or not lse.is_contiguous():
+                raise ValueError(f"lse must be contiguous [{tokens}, {self.q_heads}]")
             a.lse = lse.data_ptr()
         need = self.lib.q4gpu_paged_attention_workspace_bytes(a)
         if need > a.workspace_bytes:
             # the old one stays alive until the work queued on this stream is done with it
             self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = self.workspace.data_ptr(), need
-        rc = self.lib.q4gpu_paged_attention(a, _stream())
+        rc = self.lib.q4gpu_paged_attention(a, _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_paged_attention")
         return out
@@ -345,7 +359,7 @@ class Pages(_Err):
         copied (its filled rows) to page fresh[i].  int32 [n] each."""
         n = parents.shape[0]
         rc = self.lib.q4gpu_pages_fork(self.args, self._ids(parents, n, "parents"), self._ids(children, n, "children"),
-                                       self._ids(fresh, n, "fresh"), n, _stream())
+                                       self._ids(fresh, n, "fresh"), n, _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_pages_fork")
 
@@ -354,13 +368,13 @@ class Pages(_Err):
         itself) int32 [slots, pages per slot], remap int32 [pages] (old -> new, -1 unused),
         n_live int32 [1]."""
         _on(new_table, self.device, "new_table", torch.int32)
-        _need(new_table.shape == self.table.shape and new_table.is_contiguous(),
-              f"new_table must be contiguous {tuple(self.table.shape)}")
+        if new_table.shape != self.table.shape or not new_table.is_contiguous():
+            raise ValueError(f"new_table must be contiguous {tuple(self.table.shape)}")
         if self.workspace is None:
             self.workspace = torch.empty(self.lib.q4gpu_pages_compact_workspace_bytes(self.args.n_pages),
                                          dtype=torch.uint8, device=self.device)
         rc = self.lib.q4gpu_pages_compact(self.args, new_table.data_ptr(), self._ids(remap, self.args.n_pages, "remap"),
                                           self._ids(n_live, 1, "n_live"), self.workspace.data_ptr(),
-                                          self.workspace.numel(), _stream())
+                                          self.workspace.numel(), _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_pages_compact")
