@@ -301,7 +301,7 @@ void launch_norm_out(const NormParams& p, int out_dtype, bool vec, cudaStream_t 
 // for all of them and 32 VECS bytes of data are in flight per thread.  Bound by
 // memory, and by the way from a token's position to its table row.
 template <typename T, bool INTERLEAVED, int VECS>
-__global__ void __launch_bounds__(256) rope_append_kernel(q4gpu_rope_args a, int lanes, int heads, int slots) {
+__global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4) rope_append_kernel(q4gpu_rope_args a, int lanes, int heads, int slots) {
   const uint32_t flat = blockIdx.x * blockDim.x + threadIdx.x;
   const int u = flat & (lanes - 1);
   const uint32_t group = flat / lanes, token = group / (uint32_t)slots, slot = group - token * slots;
@@ -406,12 +406,12 @@ void launch_rope(const q4gpu_rope_args& a, int lanes, int heads, cudaStream_t s)
   // Four head vectors a thread once that still gives every SM 512 threads; one
   // where latency counts.
   const bool many = (int64_t)a.tokens * heads * lanes >= (int64_t)4 * 148 * 512;
-  const int slots = many ? (heads + 3) / 4 : heads;
+  const int slots = many ? (heads + 1) / 2 : heads;
   const int64_t threads = (int64_t)a.tokens * slots * lanes;
   const int block = (int)std::min<int64_t>(256, (threads + 31) / 32 * 32);
   const unsigned grid = (unsigned)((threads + block - 1) / block);
   if (many)
-    rope_append_kernel<T, INTERLEAVED, 4><<<grid, block, 0, s>>>(a, lanes, heads, slots);
+    rope_append_kernel<T, INTERLEAVED, 2><<<grid, block, 0, s>>>(a, lanes, heads, slots);
   else
     rope_append_kernel<T, INTERLEAVED, 1><<<grid, block, 0, s>>>(a, lanes, heads, slots);
 }

@@ -78,254 +78,344 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// How the keys are split over CTAs, and where the parts of a row are joined.
-struct SplitPlan {
-  int chunk;      // keys of one part, a multiple of 64
-  int parts;      // most parts of a sequence
-  float* o;       // [item][part][kRows][D] unnormalised sums
-  float2* ml;     // [item][part][kRows] running maximum (log2 units) and sum
-  int32_t* done;  // [item] finished parts
+// Work is laid out on one axis: sequence by sequence, key head by key head, in
+// units of 64 keys, each (sequence, head) behind kPieceCost units that stand for
+// what starting it costs.  Every CTA takes an equal stretch of that axis, so the
+// longest sequence does not decide; a stretch's ends cut at most two (sequence,
+// head) items, whose pieces are joined by the CTA that finishes last, in the
+// order of the pieces.
+constexpr int kUnitKeys = kRowWarps * kTileKeys;
+constexpr int kPieceCost = 4;
+constexpr int kLeastStretch = 12;  // units: shorter pieces cost more to join than they save
+
+struct RowPlan {
+  int ctas;
+  float* o;       // [cta][2][kRows][D] unnormalised sums: of a piece begun earlier, of one that goes on
+  float2* ml;     // [cta][2][kRows] their running maximum (log2 units) and sum
+  int32_t* done;  // [sequence * kv_heads + head] finished pieces
 };
 
-// blockIdx = (part, key head, sequence).  Each warp runs over its own 16-key
-// steps of the part with its own running maximum and sum, so no barrier stands
-// in the loop; the four are joined at the end, and the parts of a long
-// sequence by the CTA that finishes last, in the order of the parts.
+// Keys that the kernel below walks for sequence i, from `lo` on; -1: not its
+// sequence (no queries, or more rows than a tile).
+__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const Seq& s, int group, int& lo) {
+  lo = 0;
+  if (s.n == 0 || s.n > kRows / group) return -1;
+  if (a.window > 0) lo = max(0, s.len - s.n - a.window + 1) & ~(kTileKeys - 1);
+  return max(0, s.len - lo);
+}
+__device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int group) {  // of one head
+  int lo;
+  const int keys = row_keys(a, sequence(a, i), group, lo);
+  return keys < 0 ? 0 : kPieceCost + (keys + kUnitKeys - 1) / kUnitKeys;
+}
+
+// Each warp runs over its own 16-key steps of a piece with its own running
+// maximum and sum, so no barrier stands in the loop; the four are joined at its
+// end.  Bound by memory: every key and value is read once, for all heads of its
+// group.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, SplitPlan plan) {
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, RowPlan plan, bool after_chunks) {
+  constexpr int kThreads = kRowWarps * 32;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float s_m[kRowWarps][kRows], s_l[kRowWarps][kRows];
-  __shared__ int s_last;
-  const int part = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  __shared__ int64_t s_sum[kRowWarps], s_start;
+  __shared__ int s_most[kRowWarps], s_seq, s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Seq s = sequence(a, seq);
   const int group = a.q_heads / a.kv_heads;
-  if (s.n == 0 || s.n > kRows / group) return;
-  const int rows = s.n * group;
-  const int pos0 = s.len - s.n, pos1 = s.len - 1;  // of the first and the last query
-  const int lo = (a.window > 0 ? max(0, pos0 - a.window + 1) : 0) & ~(kTileKeys - 1);
-  // a sequence longer than max_ctx said still gets no more than plan.parts parts
-  const int chunk = max(plan.chunk, ((s.len - lo + plan.parts - 1) / plan.parts + 63) & ~63);
-  const int parts = max(1, (s.len - lo + chunk - 1) / chunk);
-  if (part >= parts) return;
-  const int begin = lo + part * chunk, end = min(s.len, begin + chunk);
-
-  // the queries as A fragments: row g and g + 8, 16 values of a head per step
-  const int g = lane >> 2, tq = lane & 3;
-  uint32_t qf[D / 16][4];
-  int row_pos[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = g + 8 * h, t = r / group;
-    row_pos[h] = r < rows ? pos0 + t : -1;
-    const T* qp = static_cast<const T*>(a.q) + (int64_t)(s.first + t) * a.q_token_stride +
-                  (int64_t)(kvh * group + r - t * group) * a.q_head_stride + 2 * tq;
-#pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      qf[k][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
-      qf[k][h + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
-    }
+  // the axis: each thread adds up a run of sequences
+  const int per = (a.n_seqs + kThreads - 1) / kThreads;
+  const int run0 = min(a.n_seqs, (int)threadIdx.x * per), run1 = min(a.n_seqs, run0 + per);
+  int64_t mine_cost = 0;
+  int most = 0;
+  for (int i = run0; i < run1; ++i) {
+    const int c = row_cost(a, i, group);
+    mine_cost += (int64_t)c * a.kv_heads;
+    most = max(most, c);
   }
-
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kRowStages * 2 * kTileKeys * D * 2);
-  constexpr int kTileBytes = kTileKeys * D * 2;
-  const int32_t* table = a.table + (int64_t)max(0, min(s.slot, a.n_slots - 1)) * a.table_stride;
-  const int steps = begin < end ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
-  const int mine = steps > warp ? (steps - warp + kRowWarps - 1) / kRowWarps : 0;
-  const int shift = 31 - __clz(a.page_tokens);
-  auto page_of = [&](int i) {
-    if (i >= mine) return -1;
-    const int p = table[(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
-    return p < a.n_pages ? p : -1;
+  int64_t upto = mine_cost;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(~0u, upto, o);
+    if (lane >= o) upto += v;
+  }
+  most = __reduce_max_sync(~0u, most);
+  if (lane == 31) s_sum[warp] = upto;
+  if (lane == 0) s_most[warp] = most;
+  __syncthreads();
+  int64_t total = 0, before = upto - mine_cost;
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+    most = max(most, s_most[w]);
+  }
+  // (32-bit divisions where the numbers allow them)
+  auto quotient = [](int64_t x, int64_t y) {
+    return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
   };
-  int next_page = page_of(0);
-  uint32_t valid = 0;  // bit i % 32: step i's page exists
-  auto load = [&](int i) {
-    const int page = next_page;
-    next_page = page_of(i + 1);
-    if (i < mine) valid = (valid & ~(1u << (i & 31))) | ((page >= 0 ? 1u : 0u) << (i & 31));
-    if (i < mine && page >= 0) {
-      const int key = begin + kTileKeys * (warp + kRowWarps * i);
-      const int64_t off = page * a.page_stride + kvh * a.head_stride + (key & (a.page_tokens - 1)) * a.row_stride;
-      const uint32_t at = ring + (i % kRowStages) * 2 * kTileBytes;
-      constexpr int kPieces = D / 8, kPer = 32 / kPieces;  // lanes per row, rows per pass
-      const int c = lane % kPieces;
-#pragma unroll
-      for (int r0 = 0; r0 < kTileKeys; r0 += kPer) {
-        const int r = r0 + lane / kPieces;
-        // rows past the last key are zeros: whatever the page holds there meets a zero weight
-        const bool there = key + r < end;
-        const int64_t o = off + (there ? r : 0) * a.row_stride + c * 8;
-        cp16(at + piece<D>(r, c), static_cast<const T*>(a.k_cache) + o, there);
-        cp16(at + kTileBytes + piece<D>(r, c), static_cast<const T*>(a.v_cache) + o, there);
-      }
+  const int64_t stretch = max(quotient(total + plan.ctas - 1, plan.ctas), (int64_t)min(most, kLeastStretch));
+  const int64_t first_unit = blockIdx.x * stretch, last_unit = min(total, first_unit + stretch);
+  if (first_unit < last_unit) {
+    if (before <= first_unit && first_unit < before + mine_cost) {  // one thread's run holds it
+      int i = run0;
+      for (int64_t c; before + (c = (int64_t)row_cost(a, i, group) * a.kv_heads) <= first_unit; ++i) before += c;
+      s_seq = i, s_start = before;
     }
-    cp_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kRowStages - 1; ++i) load(i);
+    __syncthreads();
+    int seq = s_seq, lo;
+    int64_t start = s_start;  // where the sequence's first head begins
+    Seq s = sequence(a, seq);
+    int keys = row_keys(a, s, group, lo), cost = row_cost(a, seq, group), kvh = (int)quotient(first_unit - start, cost);
+    for (;;) {
+      const int64_t head_start = start + (int64_t)kvh * cost + kPieceCost;  // of its first real unit
+      if (head_start - kPieceCost >= last_unit) break;
+      const int units = cost - kPieceCost;
+      const int u0 = (int)max((int64_t)0, first_unit - head_start), u1 = (int)min((int64_t)units, last_unit - head_start);
+      // (a sequence without keys: its zeros are written by the CTA where its cost begins)
+      if (u1 > u0 || (units == 0 && head_start - kPieceCost >= first_unit)) {
+        const int rows = s.n * group;
+        const int64_t cta0 = quotient(head_start, stretch),
+                      cta1 = units == 0 ? cta0 : quotient(head_start + units - 1, stretch);
+        const int parts = (int)(cta1 - cta0) + 1, part = (int)(blockIdx.x - cta0);
+        const int pos0 = s.len - s.n, pos1 = s.len - 1;  // of the first and the last query
+        const int begin = lo + u0 * kUnitKeys, end = min(s.len, lo + u1 * kUnitKeys);
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
+        // the queries as A fragments: row g and g + 8, 16 values of a head per step
+        const int g = lane >> 2, tq = lane & 3;
+        uint32_t qf[D / 16][4];
+        int row_pos[2];
 #pragma unroll
-  for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  const float c2 = a.scale * kLog2e;
-  for (int i = 0; i < mine; ++i) {
-    cp_wait<kRowStages - 2>();
-    __syncwarp();
-    load(i + kRowStages - 1);
-    if (!((valid >> (i & 31)) & 1u)) continue;
-    const uint32_t kt = ring + (i % kRowStages) * 2 * kTileBytes, vt = kt + kTileBytes;
-    const int key = begin + kTileKeys * (warp + kRowWarps * i);
-    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int h = 0; h < 2; ++h) {
+          const int r = g + 8 * h, t = r / group;
+          row_pos[h] = r < rows ? pos0 + t : -1;
+          const T* qp = static_cast<const T*>(a.q) + (int64_t)(s.first + t) * a.q_token_stride +
+                        (int64_t)(kvh * group + r - t * group) * a.q_head_stride + 2 * tq;
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      uint32_t b[4];  // keys 0-7: b[0], b[1]; keys 8-15: b[2], b[3]
-      ldsm4(b, kt + piece<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
-      mma16816<T>(sc[0], qf[k], b[0], b[1]);
-      mma16816<T>(sc[1], qf[k], b[2], b[3]);
-    }
-    // element e of sc[n]: row g + 8 (e / 2), key 8 n + 2 tq + e % 2
-    const bool whole = key + kTileKeys <= pos0 + 1 && (a.window == 0 || key > pos1 - a.window);
-    float top[2] = {m[0], m[1]};
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float v = sc[n][e] * c2;
-        if (!whole) {
-          const int j = key + 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
-          if (j > p || (a.window > 0 && j <= p - a.window)) v = -INFINITY;
+          for (int k = 0; k < D / 16; ++k) {
+            qf[k][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
+            qf[k][h + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
+          }
         }
-        sc[n][e] = v;
-        top[e >> 1] = fmaxf(top[e >> 1], v);
-      }
-    float shrink[2], base[2];
+
+        const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kRowStages * 2 * kTileKeys * D * 2);
+        constexpr int kTileBytes = kTileKeys * D * 2;
+        const int32_t* table = a.table + (int64_t)max(0, min(s.slot, a.n_slots - 1)) * a.table_stride;
+        const int steps = units > 0 ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
+        const int mine = steps > warp ? (steps - warp + kRowWarps - 1) / kRowWarps : 0;
+        const int shift = 31 - __clz(a.page_tokens);
+        auto page_of = [&](int i) {
+          if (i >= mine) return -1;
+          const int p = table[(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
+          return p < a.n_pages ? p : -1;
+        };
+        int next_page = page_of(0);
+        uint32_t valid = 0;  // bit i % 32: step i's page exists
+        auto load = [&](int i) {
+          const int page = next_page;
+          next_page = page_of(i + 1);
+          if (i < mine) valid = (valid & ~(1u << (i & 31))) | ((page >= 0 ? 1u : 0u) << (i & 31));
+          if (i < mine && page >= 0) {
+            const int key = begin + kTileKeys * (warp + kRowWarps * i);
+            const int64_t off = page * a.page_stride + kvh * a.head_stride + (key & (a.page_tokens - 1)) * a.row_stride;
+            const uint32_t at = ring + (i % kRowStages) * 2 * kTileBytes;
+            constexpr int kPieces = D / 8, kPer = 32 / kPieces;  // lanes per row, rows per pass
+            const int c = lane % kPieces;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
-      base[h] = top[h] == -INFINITY ? 0.f : top[h];  // nothing seen yet
-      shrink[h] = ex2(m[h] - base[h]);
-      m[h] = top[h];
-      l[h] *= shrink[h];
-    }
+            for (int r0 = 0; r0 < kTileKeys; r0 += kPer) {
+              const int r = r0 + lane / kPieces;
+              // rows past the last key are zeros: whatever the page holds there meets a zero weight
+              const bool there = key + r < end;
+              const int64_t o = off + (there ? r : 0) * a.row_stride + c * 8;
+              cp16(at + piece<D>(r, c), static_cast<const T*>(a.k_cache) + o, there);
+              cp16(at + kTileBytes + piece<D>(r, c), static_cast<const T*>(a.v_cache) + o, there);
+            }
+          }
+          cp_commit();
+        };
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+        for (int i = 0; i < kRowStages - 1; ++i) load(i);
+
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[n][e] = ex2(sc[n][e] - base[e >> 1]);
-        l[e >> 1] += sc[n][e];  // this lane's keys; the four lanes of a row are added at the end
-      }
+        for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        const float c2 = a.scale * kLog2e;
+        for (int i = 0; i < mine; ++i) {
+          cp_wait<kRowStages - 2>();
+          __syncwarp();
+          load(i + kRowStages - 1);
+          if (!((valid >> (i & 31)) & 1u)) continue;
+          const uint32_t kt = ring + (i % kRowStages) * 2 * kTileBytes, vt = kt + kTileBytes;
+          const int key = begin + kTileKeys * (warp + kRowWarps * i);
+          float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t b[4];  // keys 0-7: b[0], b[1]; keys 8-15: b[2], b[3]
+            ldsm4(b, kt + piece<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+            mma16816<T>(sc[0], qf[k], b[0], b[1]);
+            mma16816<T>(sc[1], qf[k], b[2], b[3]);
+          }
+          // element e of sc[n]: row g + 8 (e / 2), key 8 n + 2 tq + e % 2
+          const bool whole = key + kTileKeys <= pos0 + 1 && (a.window == 0 || key > pos1 - a.window);
+          float top[2] = {m[0], m[1]};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] *= shrink[e >> 1];
-    // Some rows see a key of this step and some do not: an infinity or NaN in its value row may reach only the
-    // former, and a product would carry it to both (0 times infinity).  Such values are added by hand and zeroed.
-    if (key + kTileKeys > pos0 + 1 || (a.window > 0 && key <= pos1 - a.window)) {
-      unsigned char* v = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
-      bool odd = false;
-      for (int x = lane; x < kTileKeys * D; x += 32)
-        odd |= !isfinite(to_f32(*reinterpret_cast<const T*>(v + x * 2)));
-      if (__any_sync(~0u, odd)) {
-        for (int j = 0; j < kTileKeys; ++j)
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float v = sc[n][e] * c2;
+              if (!whole) {
+                const int j = key + 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
+                if (j > p || (a.window > 0 && j <= p - a.window)) v = -INFINITY;
+              }
+              sc[n][e] = v;
+              top[e >> 1] = fmaxf(top[e >> 1], v);
+            }
+          float shrink[2], base[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+            base[h] = top[h] == -INFINITY ? 0.f : top[h];  // nothing seen yet
+            shrink[h] = ex2(m[h] - base[h]);
+            m[h] = top[h];
+            l[h] *= shrink[h];
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sc[n][e] = ex2(sc[n][e] - base[e >> 1]);
+              l[e >> 1] += sc[n][e];  // this lane's keys; the four lanes of a row are added at the end
+            }
 #pragma unroll
           for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int col = 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
-              const float x = to_f32(*reinterpret_cast<const T*>(v + piece<D>(j, col / 8) + (col % 8) * 2));
-              if (!isfinite(x) && key + j <= p && (a.window == 0 || key + j > p - a.window)) o[n][e] += x;
+            for (int e = 0; e < 4; ++e) o[n][e] *= shrink[e >> 1];
+          // Some rows see a key of this step and some do not: an infinity or NaN in its value row may reach only the
+          // former, and a product would carry it to both (0 times infinity).  Such values are added by hand and zeroed.
+          if (key + kTileKeys > pos0 + 1 || (a.window > 0 && key <= pos1 - a.window)) {
+            unsigned char* v = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
+            bool odd = false;
+            for (int x = lane; x < kTileKeys * D; x += 32)
+              odd |= !isfinite(to_f32(*reinterpret_cast<const T*>(v + x * 2)));
+            if (__any_sync(~0u, odd)) {
+              for (int j = 0; j < kTileKeys; ++j)
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int col = 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
+                    const float x = to_f32(*reinterpret_cast<const T*>(v + piece<D>(j, col / 8) + (col % 8) * 2));
+                    if (!isfinite(x) && key + j <= p && (a.window == 0 || key + j > p - a.window)) o[n][e] += x;
+                  }
+              __syncwarp();
+              for (int x = lane; x < kTileKeys * D; x += 32) {
+                T* at = reinterpret_cast<T*>(v + x * 2);
+                if (!isfinite(to_f32(*at))) *at = from_f32<T>(0.f);
+              }
+              __syncwarp();
             }
-        __syncwarp();
-        for (int x = lane; x < kTileKeys * D; x += 32) {
-          T* at = reinterpret_cast<T*>(v + x * 2);
-          if (!isfinite(to_f32(*at))) *at = from_f32<T>(0.f);
+          }
+          // weights rounded to the cache's type for the tensor cores (their sum is not)
+          const uint32_t pf[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]), pack2<T>(sc[1][0], sc[1][1]),
+                                  pack2<T>(sc[1][2], sc[1][3])};
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) {
+            uint32_t b[4];  // 16 keys x 16 values
+            ldsm4_t(b, vt + piece<D>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
+            mma16816<T>(o[2 * n], pf, b[0], b[1]);
+            mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+          }
         }
-        __syncwarp();
+        cp_wait<0>();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[h] += __shfl_xor_sync(~0u, l[h], 1);
+          l[h] += __shfl_xor_sync(~0u, l[h], 2);
+          if (tq == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
+        }
+        __syncthreads();  // every warp is done with its ring
+        // the warps' sums, side by side in the ring's memory
+        float* so = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (g + 8 * h < rows)
+              *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
+                  make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        __syncthreads();
+        const int64_t item = (int64_t)seq * a.kv_heads + kvh;
+        auto put = [&](int r, int d, float m_all, float l_all, float v) {
+          const int t = r / group, head = kvh * group + r - t * group;
+          static_cast<T*>(a.out)[(int64_t)(s.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride + d] =
+              from_f32<T>(l_all == 0.f ? 0.f : v / l_all);
+          if (a.lse && d == 0)
+            a.lse[(int64_t)(s.first + t) * a.q_heads + head] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+        };
+        for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
+          const int r = x / D, d = x - r * D;
+          float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll
+          for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
+          const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int w = 0; w < kRowWarps; ++w) {
+            const float f = ex2(s_m[w][r] - base);
+            sum = fmaf(s_l[w][r], f, sum);
+            v = fmaf(so[(w * kRows + r) * D + d], f, v);
+          }
+          if (parts == 1) {
+            put(r, d, base, sum, v);
+          } else {
+            const int64_t at = (2 * (int64_t)blockIdx.x + (part == 0)) * kRows + r;
+            plan.o[at * D + d] = v;
+            if (d == 0) plan.ml[at] = make_float2(top, sum);
+          }
+        }
+        if (parts > 1) {
+          __threadfence();
+          __syncthreads();
+          if (threadIdx.x == 0) {
+            s_last = atomicAdd(plan.done + item, 1) == parts - 1;
+            if (s_last) plan.done[item] = 0;
+          }
+          __syncthreads();
+          if (s_last) __threadfence();
+        }
+        if (parts > 1 && s_last)
+        for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
+          const int r = x / D, d = x - r * D;
+          auto slot = [&](int k) { return (2 * (cta0 + k) + (k == 0)) * kRows + r; };
+          float top = -INFINITY, sum = 0.f, v = 0.f;
+#pragma unroll 8
+          for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
+          const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+          for (int k = 0; k < parts; ++k) {
+            const float2 w = __ldcg(&plan.ml[slot(k)]);
+            const float f = ex2(w.x - base);
+            sum = fmaf(w.y, f, sum);
+            v = fmaf(__ldcg(&plan.o[slot(k) * D + d]), f, v);
+          }
+          put(r, d, base, sum, v);
+        }
+        __syncthreads();  // the ring and the shared words are free for the next piece
+      }
+      if (++kvh == a.kv_heads) {
+        kvh = 0;
+        start += (int64_t)cost * a.kv_heads;
+        do {
+          if (++seq >= a.n_seqs) break;
+          s = sequence(a, seq);
+          keys = row_keys(a, s, group, lo);
+          cost = row_cost(a, seq, group);
+        } while (cost == 0);
+        if (seq >= a.n_seqs) break;
       }
     }
-    // weights rounded to the cache's type for the tensor cores (their sum is not)
-    const uint32_t pf[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]), pack2<T>(sc[1][0], sc[1][1]),
-                            pack2<T>(sc[1][2], sc[1][3])};
-#pragma unroll
-    for (int n = 0; n < D / 16; ++n) {
-      uint32_t b[4];  // 16 keys x 16 values
-      ldsm4_t(b, vt + piece<D>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * n + (lane >> 4)));
-      mma16816<T>(o[2 * n], pf, b[0], b[1]);
-      mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
-    }
   }
-  cp_wait<0>();
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(~0u, l[h], 1);
-    l[h] += __shfl_xor_sync(~0u, l[h], 2);
-    if (tq == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
-  }
-  __syncthreads();  // every warp is done with its ring
-  // the warps' sums, side by side in the ring's memory
-  float* so = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (g + 8 * h < rows)
-        *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
-            make_float2(o[n][2 * h], o[n][2 * h + 1]);
-  __syncthreads();
-  const int64_t item = (int64_t)seq * a.kv_heads + kvh;
-  auto put = [&](int r, int d, float m_all, float l_all, float v) {
-    const int t = r / group, head = kvh * group + r - t * group;
-    static_cast<T*>(a.out)[(int64_t)(s.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride + d] =
-        from_f32<T>(l_all == 0.f ? 0.f : v / l_all);
-    if (a.lse && d == 0)
-      a.lse[(int64_t)(s.first + t) * a.q_heads + head] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
-  };
-  for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
-    const int r = x / D, d = x - r * D;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
-    const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
-      const float f = ex2(s_m[w][r] - base);
-      sum = fmaf(s_l[w][r], f, sum);
-      v = fmaf(so[(w * kRows + r) * D + d], f, v);
-    }
-    if (parts == 1) {
-      put(r, d, base, sum, v);
-    } else {
-      const int64_t at = (item * plan.parts + part) * kRows + r;
-      plan.o[at * D + d] = v;
-      if (d == 0) plan.ml[at] = make_float2(top, sum);
-    }
-  }
-  if (parts == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s_last = atomicAdd(plan.done + item, 1) == parts - 1;
-    if (s_last) plan.done[item] = 0;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
-    const int r = x / D, d = x - r * D;
-    const int64_t at = item * plan.parts * kRows + r;
-    float top = -INFINITY, sum = 0.f, v = 0.f;
-    for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[at + k * kRows]).x);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int k = 0; k < parts; ++k) {
-      const float2 w = __ldcg(&plan.ml[at + k * kRows]);
-      const float f = ex2(w.x - base);
-      sum = fmaf(w.y, f, sum);
-      v = fmaf(__ldcg(&plan.o[(at + k * kRows) * D + d]), f, v);
-    }
-    put(r, d, base, sum, v);
-  }
+  // the kernel before is complete when this one is
+  if (after_chunks) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 int check_sizes(const q4gpu_attn_args* a) {
@@ -364,33 +454,26 @@ int check_attn(const q4gpu_attn_args* a) {
 // ---------------------------------------------------------------------------
 constexpr int kSms = 148;
 
-// Keys of one part of a split sequence.  Joining the parts costs about as much
-// as a CTA's pass over 400 keys, so a part is not shorter than that; beyond it
-// the parts are as short as gives every SM eight of them, and at most 2048
-// keys, so that sequences of different lengths even out.
-SplitPlan row_plan(const q4gpu_attn_args& a, size_t* bytes) {
-  SplitPlan p{};
-  const int64_t span = a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + a.max_q + kTileKeys) : a.max_ctx;
-  const int64_t items = (int64_t)a.n_seqs * a.kv_heads;
-  int64_t chunk = (span * items / (kSms * 8) + 63) / 64 * 64;
-  chunk = std::max<int64_t>(384, std::min<int64_t>(2048, chunk));
-  p.chunk = (int)chunk;
-  p.parts = (int)std::max<int64_t>(1, (span + chunk - 1) / chunk);
-  if (bytes) {
-    const size_t rows = p.parts > 1 ? (size_t)items * p.parts * kRows : 0;
-    *bytes = p.parts > 1 ? ((size_t)items * 4 + 15) / 16 * 16 + rows * (8 + (size_t)a.dim * 4) : 0;
-  }
+RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
+  RowPlan p{};
+  const size_t items = (size_t)a.n_seqs * a.kv_heads;
+  // no CTA without at least one (sequence, head) or kLeastStretch units of one
+  const int64_t units = (a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
+  const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + kLeastStretch - 1) / kLeastStretch + 1);
+  p.ctas = (int)std::min<int64_t>(most, kSms * (a.dim == 64 ? 4 : 2));
+  const size_t done = (items * 4 + 15) / 16 * 16, rows = (size_t)p.ctas * 2 * kRows;
+  if (bytes) *bytes = done + rows * (8 + (size_t)a.dim * 4);
+  p.done = reinterpret_cast<int32_t*>(ws);
+  p.ml = reinterpret_cast<float2*>(ws + done);
+  p.o = reinterpret_cast<float*>(p.ml + rows);
   return p;
 }
-void place(SplitPlan* p, const q4gpu_attn_args& a, char* ws) {
-  const size_t items = (size_t)a.n_seqs * a.kv_heads;
-  p->done = reinterpret_cast<int32_t*>(ws);
-  p->ml = reinterpret_cast<float2*>(ws + (items * 4 + 15) / 16 * 16);
-  p->o = reinterpret_cast<float*>(p->ml + items * p->parts * kRows);
-}
 
-// Parts of a chunk's keys: one where the row pairs alone fill the GPU, else as
-// many as fill it once, each of at least 512 keys.
+// Parts of a chunk's keys: one where the (row pair, key head) items fill the
+// GPU, else as many as fill it once, each of at least kMinPart keys.  (Cutting
+// the last wave of many items in two evens the SMs out, 348 steps on the longest
+// instead of 370 for 8192 tokens over 16384 keys, but the parts' traffic and the
+// join took more: 814 us against 771.)
 ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
   ChunkPlan p{};
   const int64_t group = a.q_heads / a.kv_heads;
@@ -402,10 +485,8 @@ ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
   p.tiles = (int)std::min<int64_t>(a.n_seqs == 1 ? (rows + kPair - 1) / kPair : rows / kPair + a.n_seqs, INT32_MAX);
   const int64_t items = (int64_t)p.tiles * a.kv_heads;
   const int64_t span = a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + kPair + kNTile) : a.max_ctx;
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(kSms / items, span / 512));
-  p.chunk = (int)std::max<int64_t>(kNTile, ((span + parts - 1) / parts + kNTile - 1) / kNTile * kNTile);
-  p.parts = (int)parts;
-  if (bytes) *bytes = parts > 1 ? (size_t)(items * parts * kPair) * (8 + (size_t)a.dim * 4) : 0;
+  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / items, span / kMinPart));
+  if (bytes) *bytes = p.parts > 1 ? (size_t)p.tiles * a.kv_heads * p.parts * kPair * (8 + (size_t)a.dim * 4) : 0;
   return p;
 }
 
@@ -445,33 +526,43 @@ int allow_smem(const void* kernel, int bytes, unsigned char* ready) {
 
 template <typename T, int D>
 int launch(const q4gpu_attn_args& a, cudaStream_t s) {
-  if (a.max_q > 0) {
-    SplitPlan plan = row_plan(a, nullptr);
-    place(&plan, a, static_cast<char*>(a.workspace));
-    static unsigned char ready[Q4GPU_MAX_DEVICES];
-    const int rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D>), row_smem<D>(), ready);
-    if (rc != Q4GPU_OK) return rc;
-    attn_rows_kernel<T, D>
-        <<<dim3(plan.parts, a.kv_heads, a.n_seqs), kRowWarps * 32, row_smem<D>(), s>>>(a, plan);
-  }
-  if ((int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows) {
-    size_t rows_bytes;
-    row_plan(a, &rows_bytes);
-    ChunkPlan plan = chunk_plan(a, nullptr);
+  if (a.max_q == 0) return Q4GPU_OK;
+  static unsigned char ready[2][Q4GPU_MAX_DEVICES];
+  size_t rows_bytes;
+  const RowPlan few = row_plan(a, static_cast<char*>(a.workspace), &rows_bytes);
+  int rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D>), row_smem<D>(), ready[0]);
+  const bool chunks = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows;
+  ChunkPlan plan{};
+  if (rc == Q4GPU_OK && chunks) {
+    plan = chunk_plan(a, nullptr);
     if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
     char* ws = static_cast<char*>(a.workspace) + (rows_bytes + 15) / 16 * 16;
     plan.ml = reinterpret_cast<float2*>(ws);
     plan.o = reinterpret_cast<float*>(plan.ml + (size_t)plan.tiles * a.kv_heads * plan.parts * kPair);
     CUtensorMap kmap, vmap;
-    int rc = encode_map(&kmap, a, a.k_cache);
+    rc = encode_map(&kmap, a, a.k_cache);
     if (rc == Q4GPU_OK) rc = encode_map(&vmap, a, a.v_cache);
-    static unsigned char ready[Q4GPU_MAX_DEVICES];
-    if (rc == Q4GPU_OK) rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D>), chunk_smem<D>(), ready);
-    if (rc != Q4GPU_OK) return rc;
-    attn_chunk_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, plan.parts), kChunkThreads, chunk_smem<D>(), s>>>(kmap, vmap,
-                                                                                                           a, plan);
-    if (plan.parts > 1) attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
+    if (rc == Q4GPU_OK)
+      rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D>), chunk_smem<D>(), ready[1]);
+    if (rc == Q4GPU_OK)
+      attn_chunk_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, plan.parts), kChunkThreads, chunk_smem<D>(), s>>>(
+          kmap, vmap, a, plan);
   }
+  if (rc != Q4GPU_OK) return rc;
+  // After chunks, the short sequences' CTAs start once the last chunk's CTA has, and fill the SMs that run dry.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(few.ctas);
+  cfg.blockDim = dim3(kRowWarps * 32);
+  cfg.dynamicSmemBytes = row_smem<D>();
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = chunks ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_rows_kernel<T, D>, a, few, chunks);
+  if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: launch: %s", cudaGetErrorString(e));
+  if (plan.parts > 1) attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
   return q4gpu_check_launch();
 }
 
@@ -482,9 +573,9 @@ extern "C" {
 size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args* a) {
   if (check_sizes(a) != Q4GPU_OK) return 0;
   size_t rows, chunks;
-  row_plan(*a, &rows);
+  row_plan(*a, nullptr, &rows);
   chunk_plan(*a, &chunks);
-  return chunks ? (rows + 15) / 16 * 16 + chunks : rows;
+  return (rows + 15) / 16 * 16 + chunks;
 }
 
 int q4gpu_paged_attention(const q4gpu_attn_args* a, void* stream) {

@@ -22,11 +22,15 @@ __host__ __device__ constexpr int chunk_smem() { return 1024 + (2 * kMTile + chu
 
 struct ChunkPlan {
   int tiles;  // grid of query row pairs over all sequences, an upper bound
-  int chunk;  // keys of one part, a multiple of kNTile
-  int parts;
-  float* o;    // [tile * kv_heads + head][part][kPair][D] unnormalised sums (parts > 1)
+  int parts;  // of a pair's keys, each of at least kMinPart
+  float* o;    // [pair * kv_heads + head][part][kPair][D] unnormalised sums (parts > 1)
   float2* ml;  // the same rows: running maximum (log2 units) and sum
 };
+constexpr int kMinPart = 512;
+// Keys of one part of `keys`, a multiple of kNTile.
+__device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
+  return max(kMinPart, ((keys + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
+}
 
 // Sequence and row pair of one grid index; sequences with few rows have none.
 // Later rows see more keys, so pairs are handed out from the last to the first.
@@ -37,13 +41,14 @@ __device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int gro
   const int n = max(0, min(a.cu_q[i + 1], a.tokens) - max(0, min(a.cu_q[i], a.tokens)));
   return n <= 16 / group ? 0 : (int)(((int64_t)n * group + kPair - 1) / kPair);
 }
-// By one full warp; seq = -1 where the index is past the last pair.
-__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int y) {
+// The y-th pair, or with `last_first` the y-th from the end; seq = -1 where
+// there are fewer.  By one full warp.
+__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int y, bool last_first) {
   const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
   int total = 0;
   for (int i = lane; i < a.n_seqs; i += 32) total += pairs_of(a, i, group);
   total = __reduce_add_sync(~0u, total);
-  ChunkTile t{-1, 0, total - 1 - y};
+  ChunkTile t{-1, 0, last_first ? total - 1 - y : y};
   if (y >= total) return t;
   int before = 0;
   for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
@@ -234,8 +239,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __shared__ int s_bad, s_odd, s_dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x, part = blockIdx.z;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // what follows reads nothing of this kernel
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, blockIdx.y);
+    const ChunkTile t = find_tile(a, blockIdx.y, true);
     if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
   }
   __syncthreads();
@@ -255,8 +261,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1);
   const int all_lo = a.window > 0 ? max(0, pos1 - a.window + 1) : 0, all_hi = pos0 + 1;
   const int base = lo & ~(kNTile - 1);
-  const int chunk = max(plan.chunk, ((hi - base + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
-  const int parts = max(1, (hi - base + chunk - 1) / chunk);
+  const int chunk = part_keys(plan, hi - base);
+  const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
   if (part >= parts) return;
   const int begin = base + part * chunk, end = min(hi, begin + chunk);
   const int steps = begin < end ? (end - begin + kNTile - 1) / kNTile : 0;
@@ -265,6 +271,41 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int32_t* table = a.table + (int64_t)max(0, min(slot, a.n_slots - 1)) * a.table_stride;
   const int shift = 31 - __clz(a.page_tokens);
   const uint32_t sq = smem_addr(smem), ring = sq + 2 * kTile;
+
+  if (threadIdx.x == 8 * 32) {
+    for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], tiles);
+    for (int i = 0; i < 2; ++i) {
+      for (int k = 0; k < 2; ++k) bar_init(&s_full[i][k], 1), bar_init(&p_full[i][k], 4);
+      bar_init(&o_full[i], 1);
+    }
+    bar_init(&care, 1);
+    bar_init_fence();
+  }
+  // the first keys are on their way before the queries are
+  auto pages_of = [&](int key, int& id) {  // which pages of the load at `key` exist; lane p gets page p's number
+    const int pages = min(kNTile >> shift, (int)((end - key + a.page_tokens - 1) >> shift));
+    id = lane < pages ? table[(key >> shift) + lane] : -1;
+    return __ballot_sync(~0u, id >= 0 && id < a.n_pages);
+  };
+  auto load = [&](const CUtensorMap* map, uint32_t at, int id, unsigned ok, uint64_t* bar) {
+    const uint32_t bytes = (uint32_t)__popc(ok) * a.page_tokens * D * 2;
+    if (lane == 0) {
+      if (bytes)
+        bar_expect_tx(bar, bytes);
+      else
+        bar_arrive(bar);
+    }
+    __syncwarp();
+    if ((ok >> lane) & 1u) {
+#pragma unroll
+      for (int c = 0; c < kLines; ++c) tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, map, c * 64, 0, kvh, id, bar);
+    }
+  };
+  if (warp == 8 && steps > 0) {
+    int id;
+    const unsigned ok = pages_of(begin, id);
+    load(&kmap, ring, id, ok, &full[0]);
+  }
 
   // queries into shared memory, 128-byte swizzled lines; a negative scale turns their sign
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
@@ -284,15 +325,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // is any page of these keys missing?
   for (int64_t p = ((int64_t)begin >> shift) + threadIdx.x; p << shift < end; p += kChunkThreads)
     if (table[p] < 0 || table[p] >= a.n_pages) s_bad = 1;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], tiles);
-    for (int i = 0; i < 2; ++i) {
-      for (int k = 0; k < 2; ++k) bar_init(&s_full[i][k], 1), bar_init(&p_full[i][k], 4);
-      bar_init(&o_full[i], 1);
-    }
-    bar_init(&care, 1);
-    bar_init_fence();
-  }
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
   fence_async();
   fence_before_sync();
@@ -307,10 +339,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint32_t care_phase = 0;
     for (int j = 0; j < steps && !*dead; ++j) {
       const int key = begin + j * kNTile;
-      const int pages = min(kNTile >> shift, (int)((end - key + a.page_tokens - 1) >> shift));
-      const int id = lane < pages ? table[(key >> shift) + lane] : -1;
-      const unsigned ok = __ballot_sync(~0u, id >= 0 && id < a.n_pages);
-      const uint32_t bytes = (uint32_t)__popc(ok) * a.page_tokens * D * 2;
+      int id;
+      const unsigned ok = pages_of(key, id);
       // rows that no query of the pair sees, or that only some see
       const bool partial = key < lo || key + kNTile > end || __popc(ok) != kNTile >> shift;
       const bool mixed = key < all_lo || key + kNTile > all_hi;
@@ -321,31 +351,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (*dead) break;
         const uint32_t at = ring + st * kTile;
         const bool careful = kind == 1 && (partial || mixed);
-        uint64_t* bar = careful ? &care : &full[st];
-        if (lane == 0) {
-          if (bytes)
-            bar_expect_tx(bar, bytes);
-          else
-            bar_arrive(bar);
-        }
-        __syncwarp();
-        if ((ok >> lane) & 1u) {
-#pragma unroll
-          for (int c = 0; c < kLines; ++c)
-            tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, kind ? &vmap : &kmap, c * 64, 0, kvh, id, bar);
-        }
+        if (use > 0) load(kind ? &vmap : &kmap, at, id, ok, careful ? &care : &full[st]);
         if (!careful) continue;
         // Values of keys that a row does not see meet a zero weight in its product, so they have to be finite:
-        // rows outside lo .. end (and of missing pages) become zeros, and infinities and NaNs are zeroed here and
-        // added at the end to the rows that do see them.
+        // rows outside lo .. end (and of missing pages) become zeros, and infinities and NaNs in rows that only
+        // some queries see are zeroed here and added at the end for the queries that do see them.
         if (!wait_phase(&care, care_phase)) *dead = 1;
         care_phase ^= 1;
         unsigned char* v = smem + (at - sq);
         bool odd = false;
         for (int x = lane; x < kNTile * kLines * 8; x += 32) {
-          const int line = x / (kNTile * 8), r = (x / 8) % kNTile;
-          uint4* w = reinterpret_cast<uint4*>(v + line * kLineTile + r * 128 + (x & 7) * 16);
-          if (key + r < lo || key + r >= end || !((ok >> (r >> shift)) & 1u)) {
+          const int r = x / (kLines * 8), c = x % (kLines * 8), k = key + r;
+          const bool there = (ok >> (r >> shift)) & 1u;
+          if (there && k >= all_lo && k < all_hi) continue;
+          uint4* w = reinterpret_cast<uint4*>(v + (c / 8) * kLineTile + r * 128 + (c & 7) * 16);
+          if (!there || k < lo || k >= end) {
             *w = make_uint4(0u, 0u, 0u, 0u);
           } else {
             const uint4 b = *w;
@@ -539,8 +559,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           if (odd && mine) {  // the infinities and NaNs that were kept out of the products
             for (int k = begin; k < end; ++k) {
-              const int step = k & ~(kNTile - 1);
-              if (!bad && step >= all_lo && step + kNTile <= all_hi) continue;  // went through the products
+              if (k >= all_lo && k < all_hi) continue;  // went through the products
               if (k > pos || (a.window > 0 && k <= pos - a.window)) continue;
               const int id = table[k >> shift];
               if (id < 0 || id >= a.n_pages) continue;
@@ -584,7 +603,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, Chunk
   __shared__ ChunkTile s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, blockIdx.y);
+    const ChunkTile t = find_tile(a, blockIdx.y, false);
     if (lane == 0) s_tile = t;
   }
   __syncthreads();
@@ -599,8 +618,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, Chunk
   const int rows = (int)min((int64_t)kPair, (int64_t)n * group - tile.row0);
   const int pos0 = len - n + tile.row0 / group, pos1 = len - n + (tile.row0 + rows - 1) / group;
   const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1), base = lo & ~(kNTile - 1);
-  const int chunk = max(plan.chunk, ((hi - base + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
-  const int parts = max(1, (hi - base + chunk - 1) / chunk);
+  const int chunk = part_keys(plan, hi - base);
+  const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
   if (parts == 1) return;
   const int r = blockIdx.z * 8 + warp;
   if (r >= rows) return;
