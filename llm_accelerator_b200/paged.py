@@ -22,9 +22,11 @@ library, both before any device work; there is no CPU fallback.
 """
 from __future__ import annotations
 
-import ctypes as C
-from typing import Optional
+import heapq
+from dataclasses import dataclass
+from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from . import _native
@@ -378,3 +380,138 @@ class Pages(_Err):
                                           self.workspace.numel(), _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_pages_compact")
+
+
+@dataclass
+class Step:
+    """One step's new tokens over a ``PagedCache``, as the operators take them (device tensors)."""
+    seq_ids: torch.Tensor    # int32 [sequences]
+    cu_q: torch.Tensor       # int32 [sequences + 1]
+    positions: torch.Tensor  # int32 [tokens]
+    rows: torch.Tensor       # int64 [tokens]
+    max_q: int
+    max_ctx: int
+
+
+class PagedCache:
+    """16-bit K/V pages of all layers for up to ``max_seqs`` sequences.
+
+    The pool is [pages, layers, K/V, kv_heads, page_tokens, head_dim]: a page holds
+    page_tokens positions of every layer, so a fork copies one run of memory.  Which
+    pages are free and whose they are is kept on the host; ``table`` and ``lens`` are the
+    device's view, updated in stream order.  Full pages can belong to several sequences
+    and are never written again; a partly filled last page belongs to one.
+    """
+
+    def __init__(self, n_layers: int, n_pages: int, page_tokens: int, kv_heads: int, head_dim: int, max_seqs: int,
+                 max_ctx: int, dtype: torch.dtype = torch.bfloat16, device: Optional[torch.device] = None):
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self.page_tokens, self.max_ctx, self.device = page_tokens, max_ctx, dev
+        self.pool = torch.empty(n_pages, n_layers, 2, kv_heads, page_tokens, head_dim, dtype=dtype, device=dev)
+        self.table = torch.full((max_seqs, -(-max_ctx // page_tokens)), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
+        self.pages = Pages(self.pool, self.table, self.lens, page_tokens)
+        self._held: list[list[int]] = [[] for _ in range(max_seqs)]
+        self._len = [0] * max_seqs
+        self._users = [0] * n_pages
+        self._free = list(range(n_pages))  # a heap: the lowest free page is taken first
+
+    def k(self, layer: int) -> torch.Tensor:
+        return self.pool[:, layer, 0]
+
+    def v(self, layer: int) -> torch.Tensor:
+        return self.pool[:, layer, 1]
+
+    def length(self, seq: int) -> int:
+        return self._len[seq]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self._free):
+            raise RuntimeError(f"the cache is full: {n} pages wanted, {len(self._free)} free")
+        got = [heapq.heappop(self._free) for _ in range(n)]
+        for p in got:
+            self._users[p] += 1
+        return got
+
+    def _drop(self, pages: Sequence[int]) -> None:
+        for p in pages:
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def _up(self, a: np.ndarray) -> torch.Tensor:
+        return torch.from_numpy(a).pin_memory().to(self.device, non_blocking=True)
+
+    def extend(self, seqs: Sequence[int], counts: Sequence[int]) -> Step:
+        """Room for counts[i] new tokens of sequence seqs[i]; returns the step's index tensors.
+        Nothing changes if the pages do not suffice."""
+        _need(len(seqs) == len(counts) and len(set(seqs)) == len(seqs) and len(seqs) > 0, "one count per sequence")
+        need = []
+        for s, n in zip(seqs, counts):
+            if n < 0 or self._len[s] + n > self.max_ctx:
+                raise ValueError(f"sequence {s}: {self._len[s]} + {n} tokens, at most {self.max_ctx}")
+            need.append(-(-(self._len[s] + n) // self.page_tokens) - len(self._held[s]))
+        got = self._take(sum(need))
+        pos, rows = [], []
+        table = np.full((len(seqs), self.table.shape[1]), -1, dtype=np.int32)
+        for i, (s, n) in enumerate(zip(seqs, counts)):
+            self._held[s] += got[:need[i]]
+            got = got[need[i]:]
+            held = np.asarray(self._held[s], dtype=np.int64)
+            table[i, :held.size] = held
+            p = np.arange(self._len[s], self._len[s] + n, dtype=np.int64)
+            pos.append(p)
+            rows.append(held[p // self.page_tokens] * self.page_tokens + p % self.page_tokens if n else p)
+            self._len[s] += n
+        ids = self._up(np.asarray(seqs, dtype=np.int32))
+        at = ids.long()
+        self.table.index_copy_(0, at, self._up(table))
+        lens = [self._len[s] for s in seqs]
+        self.lens.index_copy_(0, at, self._up(np.asarray(lens, dtype=np.int32)))
+        return Step(ids, self._up(np.concatenate(([0], np.cumsum(counts))).astype(np.int32)),
+                    self._up(np.concatenate(pos).astype(np.int32)), self._up(np.concatenate(rows)), max(counts),
+                    max(max(lens), 1))
+
+    def fork(self, parent: int, children: Sequence[int]) -> None:
+        """Empty sequences `children` continue `parent`: full pages are shared, its last one copied."""
+        _need(all(self._len[c] == 0 and c != parent for c in children) and len(set(children)) == len(children),
+              "children must be empty sequences")
+        n, held = self._len[parent], self._held[parent]
+        full = n // self.page_tokens
+        part = bool(n % self.page_tokens)
+        fresh = self._take(len(children) if part else 0)
+        for i, c in enumerate(children):
+            for p in held[:full]:
+                self._users[p] += 1
+            self._held[c] = held[:full] + ([fresh[i]] if part else [])
+            self._len[c] = n
+        if children:
+            self.pages.fork(self._up(np.full(len(children), parent, dtype=np.int32)),
+                            self._up(np.asarray(children, dtype=np.int32)),
+                            self._up(np.asarray(fresh or [-1] * len(children), dtype=np.int32)))
+
+    def free(self, seq: int) -> None:
+        """Ends a sequence; pages that nobody else uses become free."""
+        self._drop(self._held[seq])
+        self._held[seq], self._len[seq] = [], 0
+        self.lens[seq:seq + 1].zero_()
+        self.table[seq].fill_(-1)
+
+    def compact(self) -> int:
+        """Packs the pages in use into the first ones and returns their number (waits for the stream)."""
+        remap = torch.empty(self.pool.shape[0], dtype=torch.int32, device=self.device)
+        n_live = torch.empty(1, dtype=torch.int32, device=self.device)
+        self.pages.compact(self.table, remap, n_live)
+        to, live = remap.tolist(), int(n_live.item())
+        self._held = [[to[p] for p in held] for held in self._held]
+        users = [0] * len(to)
+        for p, n in enumerate(self._users):
+            if n:
+                users[to[p]] = n
+        self._users = users
+        self._free = [p for p, n in enumerate(users) if n == 0]
+        return live

@@ -13,6 +13,7 @@ builder (``q4gpu_build_tables``).
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -43,6 +44,29 @@ def rope_tables(n_positions: int, theta: float = ROPE_THETA) -> tuple[np.ndarray
         return np.clip(v, -32768, 32767).astype(np.int32)
 
     return q115(emb.cos()), q115(emb.sin())
+
+
+def rope_float_tables(n_positions: int, rot_dim: int = HEAD_DIM, theta: float = ROPE_THETA, factor: float = 1.0,
+                      original: int | None = None, device=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """float32 [n_positions, rot_dim / 2] cos and sin for ``paged.RopeAppend``, from float64 angles.
+
+    With ``factor`` above 1 the frequencies are stretched by parts (YaRN): pair i turns
+    ``original * inv_freq_i / 2 pi`` times over the ``original`` (trained) positions, by default
+    n_positions / factor; pairs that turn more than 32 times keep their frequency, those below
+    one turn are slowed by ``factor``, in between the two are mixed in proportion, and both
+    tables are scaled by 0.1 ln(factor) + 1.  (The reference has 256 positions and no scaling.)
+    """
+    if rot_dim < 2 or rot_dim % 2 or n_positions < 1 or factor < 1.0:
+        raise ValueError(f"no rotary table of {n_positions} positions x {rot_dim}, factor {factor}")
+    inv = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    scale = 1.0
+    if factor > 1.0:
+        turns = (original or n_positions / factor) * inv / (2.0 * math.pi)
+        keep = ((turns - 1.0) / 31.0).clamp(0.0, 1.0)
+        inv = inv * (keep + (1.0 - keep) / factor)
+        scale = 0.1 * math.log(factor) + 1.0
+    angle = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * inv
+    return (angle.cos() * scale).float(), (angle.sin() * scale).float()
 
 
 def luts() -> tuple[np.ndarray, np.ndarray]:
