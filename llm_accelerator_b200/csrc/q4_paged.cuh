@@ -81,5 +81,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 16 bytes to shared memory, or zeros where `there` is false.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 }  // namespace paged
 }  // namespace q4

@@ -70,14 +70,6 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 16 bytes to shared memory, or zeros where `there` is false.
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Work is laid out on one axis: sequence by sequence, key head by key head, in
 // units of 64 keys, each (sequence, head) behind kPieceCost units that stand for
 // what starting it costs.  Every CTA takes an equal stretch of that axis, so the
@@ -481,6 +473,8 @@ ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
     if (bytes) *bytes = 0;
     return p;
   }
+  // (a lone sequence of any length is the chunk kernel's: one launch)
+  p.least = a.n_seqs == 1 ? 1 : (int)(kRows / group) + 1;
   const int64_t rows = a.tokens * group;
   p.tiles = (int)std::min<int64_t>(a.n_seqs == 1 ? (rows + kPair - 1) / kPair : rows / kPair + a.n_seqs, INT32_MAX);
   const int64_t items = (int64_t)p.tiles * a.kv_heads;
@@ -549,6 +543,11 @@ int launch(const q4gpu_attn_args& a, cudaStream_t s) {
           kmap, vmap, a, plan);
   }
   if (rc != Q4GPU_OK) return rc;
+  if (chunks && plan.least == 1) {
+    if (plan.parts > 1)
+      attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
+    return q4gpu_check_launch();
+  }
   // After chunks, the short sequences' CTAs start once the last chunk's CTA has, and fill the SMs that run dry.
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -13,7 +13,8 @@ constexpr int kMTile = 128;             // query rows of one accumulator
 constexpr int kPair = 2 * kMTile;       // query rows of a CTA
 constexpr int kNTile = 128;             // keys of one load
 constexpr int kStep = 64;               // keys of one step
-constexpr int kChunkThreads = 12 * 32;  // two softmax warpgroups; a TMA warp, two MMA warps, an idle one
+constexpr int kChunkThreads = 12 * 32;  // two softmax warpgroups; a TMA warp, two MMA warps, one that cleans values
+constexpr int kCare = 8;                // barriers of value tiles to be cleaned, more than the ring holds
 
 template <int D>
 __host__ __device__ constexpr int chunk_stages() { return D == 128 ? 5 : 10; }
@@ -22,6 +23,7 @@ __host__ __device__ constexpr int chunk_smem() { return 1024 + (2 * kMTile + chu
 
 struct ChunkPlan {
   int tiles;  // grid of query row pairs over all sequences, an upper bound
+  int least;  // sequences with fewer queries are attn_rows_kernel's
   int parts;  // of a pair's keys, each of at least kMinPart
   float* o;    // [pair * kv_heads + head][part][kPair][D] unnormalised sums (parts > 1)
   float2* ml;  // the same rows: running maximum (log2 units) and sum
@@ -37,22 +39,22 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
 struct ChunkTile {
   int seq, row0, index;
 };
-__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int group) {
+__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int group, int least) {
   const int n = max(0, min(a.cu_q[i + 1], a.tokens) - max(0, min(a.cu_q[i], a.tokens)));
-  return n <= 16 / group ? 0 : (int)(((int64_t)n * group + kPair - 1) / kPair);
+  return n < least ? 0 : (int)(((int64_t)n * group + kPair - 1) / kPair);
 }
 // The y-th pair, or with `last_first` the y-th from the end; seq = -1 where
 // there are fewer.  By one full warp.
-__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int y, bool last_first) {
+__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int least, int y, bool last_first) {
   const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
   int total = 0;
-  for (int i = lane; i < a.n_seqs; i += 32) total += pairs_of(a, i, group);
+  for (int i = lane; i < a.n_seqs; i += 32) total += pairs_of(a, i, group, least);
   total = __reduce_add_sync(~0u, total);
   ChunkTile t{-1, 0, last_first ? total - 1 - y : y};
   if (y >= total) return t;
   int before = 0;
   for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
-    const int mine = i0 + lane < a.n_seqs ? pairs_of(a, i0 + lane, group) : 0;
+    const int mine = i0 + lane < a.n_seqs ? pairs_of(a, i0 + lane, group, least) : 0;
     int run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr uint32_t kSCol = 0, kOCol = 2 * kNTile;  // TMEM columns: S0, S1, O0, O1
   extern __shared__ unsigned char raw[];
   unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2], care;
+  __shared__ uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2], care[kCare];
   __shared__ uint32_t tmem_slot;
   __shared__ ChunkTile s_tile;
   __shared__ int s_bad, s_odd, s_dead;
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int kvh = blockIdx.x, part = blockIdx.z;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // what follows reads nothing of this kernel
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, blockIdx.y, true);
+    const ChunkTile t = find_tile(a, plan.least, blockIdx.y, true);
     if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
   }
   __syncthreads();
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       for (int k = 0; k < 2; ++k) bar_init(&s_full[i][k], 1), bar_init(&p_full[i][k], 4);
       bar_init(&o_full[i], 1);
     }
-    bar_init(&care, 1);
+    for (int i = 0; i < kCare; ++i) bar_init(&care[i], 1);
     bar_init_fence();
   }
   // the first keys are on their way before the queries are
@@ -307,25 +309,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     load(&kmap, ring, id, ok, &full[0]);
   }
 
-  // queries into shared memory, 128-byte swizzled lines; a negative scale turns their sign
-  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+  // queries into shared memory, 128-byte swizzled lines (rows past the last: zeros)
   for (int x = threadIdx.x; x < tiles * kMTile * (D / 8); x += kChunkThreads) {
-    const int r = x / (D / 8), c = x % (D / 8);
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (r < rows) {
-      const int t = (tile.row0 + r) / group, h = tile.row0 + r - t * group;
-      w = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(first + t) * a.q_token_stride +
-                                          (int64_t)(kvh * group + h) * a.q_head_stride + c * 8);
-      w.x ^= flip, w.y ^= flip, w.z ^= flip, w.w ^= flip;
-    }
-    const int row = r & (kMTile - 1);
-    *reinterpret_cast<uint4*>(smem + (r / kMTile) * kTile + (c / 8) * kLineTile + row * 128 +
-                              (((c & 7) ^ (row & 7)) * 16)) = w;
+    const int r = x / (D / 8), c = x % (D / 8), row = r & (kMTile - 1);
+    const bool there = r < rows;
+    const int t = there ? (tile.row0 + r) / group : t0, h = there ? tile.row0 + r - t * group : 0;
+    cp16(sq + (r / kMTile) * kTile + (c / 8) * kLineTile + row * 128 + (((c & 7) ^ (row & 7)) * 16),
+         static_cast<const T*>(a.q) + (int64_t)(first + t) * a.q_token_stride + (int64_t)(kvh * group + h) * a.q_head_stride +
+             c * 8,
+         there);
   }
   // is any page of these keys missing?
   for (int64_t p = ((int64_t)begin >> shift) + threadIdx.x; p << shift < end; p += kChunkThreads)
     if (table[p] < 0 || table[p] >= a.n_pages) s_bad = 1;
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  cp_commit();
+  cp_wait<0>();
+  if (a.scale < 0.f) {  // a negative scale turns the queries' sign (each thread its own words)
+    for (int x = threadIdx.x; x < tiles * kMTile * (D / 8); x += kChunkThreads) {
+      const int r = x / (D / 8), c = x % (D / 8), row = r & (kMTile - 1);
+      uint4* w = reinterpret_cast<uint4*>(smem + (r / kMTile) * kTile + (c / 8) * kLineTile + row * 128 +
+                                          (((c & 7) ^ (row & 7)) * 16));
+      w->x ^= 0x80008000u, w->y ^= 0x80008000u, w->z ^= 0x80008000u, w->w ^= 0x80008000u;
+    }
+  }
   fence_async();
   fence_before_sync();
   __syncthreads();
@@ -334,59 +341,73 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const bool bad = s_bad != 0;
   volatile int* dead = &s_dead;
 
+  // Values of keys that a row does not see meet a zero weight in its product, so
+  // they have to be finite.  A tile with rows that not every query of the pair
+  // sees, or that are not there, goes past the last warp before its product.
+  auto careful = [&](int key, unsigned ok) {
+    return key < all_lo || key + kNTile > all_hi || __popc(ok) != kNTile >> shift;
+  };
   if (warp == 8) {
     // ---- loads: K and V of a step take one ring stage each ----------------------
-    uint32_t care_phase = 0;
+    int id, next_id, cleaned = 0;
+    unsigned ok = pages_of(begin, id), next_ok = ok;
     for (int j = 0; j < steps && !*dead; ++j) {
       const int key = begin + j * kNTile;
-      int id;
-      const unsigned ok = pages_of(key, id);
-      // rows that no query of the pair sees, or that only some see
-      const bool partial = key < lo || key + kNTile > end || __popc(ok) != kNTile >> shift;
-      const bool mixed = key < all_lo || key + kNTile > all_hi;
+      if (j + 1 < steps) next_ok = pages_of(key + kNTile, next_id);
       for (int kind = 0; kind < 2; ++kind) {
         const int use = 2 * j + kind, st = use % kStages;
         if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
         __syncwarp();
         if (*dead) break;
-        const uint32_t at = ring + st * kTile;
-        const bool careful = kind == 1 && (partial || mixed);
-        if (use > 0) load(kind ? &vmap : &kmap, at, id, ok, careful ? &care : &full[st]);
-        if (!careful) continue;
-        // Values of keys that a row does not see meet a zero weight in its product, so they have to be finite:
-        // rows outside lo .. end (and of missing pages) become zeros, and infinities and NaNs in rows that only
-        // some queries see are zeroed here and added at the end for the queries that do see them.
-        if (!wait_phase(&care, care_phase)) *dead = 1;
-        care_phase ^= 1;
-        unsigned char* v = smem + (at - sq);
-        bool odd = false;
-        for (int x = lane; x < kNTile * kLines * 8; x += 32) {
-          const int r = x / (kLines * 8), c = x % (kLines * 8), k = key + r;
-          const bool there = (ok >> (r >> shift)) & 1u;
-          if (there && k >= all_lo && k < all_hi) continue;
-          uint4* w = reinterpret_cast<uint4*>(v + (c / 8) * kLineTile + r * 128 + (c & 7) * 16);
-          if (!there || k < lo || k >= end) {
-            *w = make_uint4(0u, 0u, 0u, 0u);
-          } else {
-            const uint4 b = *w;
-            constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
-            const uint32_t u[4] = {b.x, b.y, b.z, b.w};
-            uint32_t o[4];
-            bool some = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool l = (u[i] & kExp) == kExp, h = ((u[i] >> 16) & kExp) == kExp;
-              o[i] = (l ? 0u : u[i] & 0xffffu) | (h ? 0u : u[i] & 0xffff0000u);
-              some |= l || h;
-            }
-            if (some) *w = make_uint4(o[0], o[1], o[2], o[3]), odd = true;
-          }
-        }
-        if (odd) s_odd = 1;
-        fence_async();
-        __syncwarp();
-        if (lane == 0) bar_arrive(&full[st]);
+        uint64_t* bar = kind && careful(key, ok) ? &care[cleaned++ % kCare] : &full[st];
+        if (use > 0) load(kind ? &vmap : &kmap, ring + st * kTile, id, ok, bar);
       }
+      id = next_id, ok = next_ok;
+    }
+  } else if (warp == 11) {
+    // ---- cleaning: rows outside lo .. end and of missing pages become zeros;
+    // infinities and NaNs in rows that only some queries see become zeros too and
+    // are added at the end for the queries that do see them
+    int cleaned = 0;
+    for (int j = 0; j < steps && !*dead; ++j) {
+      const int key = begin + j * kNTile, st = (2 * j + 1) % kStages;
+      int id;
+      const unsigned ok = pages_of(key, id);
+      if (!careful(key, ok)) continue;
+      if (!wait_phase(&care[cleaned % kCare], (cleaned / kCare) & 1)) *dead = 1;
+      ++cleaned;
+      unsigned char* v = smem + (ring - sq) + st * kTile;
+      // rows 0 .. r0 - 1 and r1 .. 127 are not seen by all
+      const bool whole = __popc(ok) == kNTile >> shift;
+      const int r0 = whole ? max(0, min(kNTile, all_lo - key)) : kNTile;
+      const int r1 = whole ? max(r0, min(kNTile, all_hi - key)) : kNTile;
+      const int words = (r0 + kNTile - r1) * kLines * 8;
+      bool odd = false;
+#pragma unroll 4
+      for (int x = lane; x < words; x += 32) {
+        int r = x / (kLines * 8);
+        if (r >= r0) r += r1 - r0;
+        const int c = x % (kLines * 8), k = key + r;
+        uint4* w = reinterpret_cast<uint4*>(v + (c / 8) * kLineTile + r * 128 + (c & 7) * 16);
+        const uint4 b = *w;
+        const bool keep = k >= lo && k < end && ((ok >> (r >> shift)) & 1u), some_only = k < all_lo || k >= all_hi;
+        constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+        const uint32_t u[4] = {b.x, b.y, b.z, b.w};
+        uint32_t o[4];
+        bool found = !keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool l = (u[i] & kExp) == kExp && some_only, h = ((u[i] >> 16) & kExp) == kExp && some_only;
+          o[i] = !keep ? 0u : (l ? 0u : u[i] & 0xffffu) | (h ? 0u : u[i] & 0xffff0000u);
+          found |= l || h;
+        }
+        if (found) *w = make_uint4(o[0], o[1], o[2], o[3]);
+        odd |= found && keep;
+      }
+      if (odd) s_odd = 1;
+      fence_async();
+      __syncwarp();
+      if (lane == 0) bar_arrive(&full[st]);
     }
   } else if (warp >= 9 && warp < 9 + tiles) {
     // ---- products: one warp a tile, together; an elected thread issues ---------------
@@ -603,7 +624,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, Chunk
   __shared__ ChunkTile s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, blockIdx.y, false);
+    const ChunkTile t = find_tile(a, plan.least, blockIdx.y, false);
     if (lane == 0) s_tile = t;
   }
   __syncthreads();
