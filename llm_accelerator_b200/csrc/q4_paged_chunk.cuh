@@ -13,8 +13,7 @@ constexpr int kMTile = 128;             // query rows of one accumulator
 constexpr int kPair = 2 * kMTile;       // query rows of a CTA
 constexpr int kNTile = 128;             // keys of one load
 constexpr int kStep = 64;               // keys of one step
-constexpr int kChunkThreads = 12 * 32;  // two softmax warpgroups; a TMA warp, two MMA warps, one that cleans values
-constexpr int kCare = 8;                // barriers of value tiles to be cleaned, more than the ring holds
+constexpr int kChunkThreads = 12 * 32;  // two softmax warpgroups; a TMA warp, two MMA warps, an idle one
 
 template <int D>
 __host__ __device__ constexpr int chunk_stages() { return D == 128 ? 5 : 10; }
@@ -134,13 +133,16 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
       : "memory");
 }
-// Waits for a phase; false after about 0.3 s.  (bar_wait reads the global timer
-// after its first miss, which took longer than most waits here.)
+// Waits for a phase; false after about 0.3 s.  (umma::bar_wait reads the global
+// timer after its first miss, which took longer than most waits here.)  A wait
+// that lasts sleeps between its tests, which otherwise hold the shared-memory
+// pipe against the warp that has work to do.
 __device__ __forceinline__ bool wait_phase(uint64_t* b, unsigned parity) {
   if (umma::bar_try_wait(b, parity)) return true;
   long long since = 0;
   for (uint32_t it = 1;; ++it) {
     if (umma::bar_try_wait(b, parity)) return true;
+    if (it > 16) __nanosleep(40);
     if ((it & 255u) == 0) {
       const long long now = clock64();
       if (!since)
@@ -210,6 +212,43 @@ __device__ __forceinline__ void ex2_pair(uint64_t x2, float& x, float& y) {
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// A share of a value tile's cleaning by one thread of `threads`: 16-byte pieces of
+// the rows that not every query sees (keys outside all_lo .. all_hi - 1; all rows
+// where pages may be missing, then `table` is given).  Rows outside lo .. end and
+// of missing pages become zeros, and so do infinities and NaNs in the others;
+// true if there were any.  Out of line: few steps come here, and the registers it
+// takes cost the steps that do not.
+template <typename T, int D>
+__device__ __noinline__ bool clean_values(unsigned char* v, int key, int lo, int all_lo, int all_hi, int end,
+                                          const int32_t* table, int shift, int n_pages, int threads) {
+  constexpr int kPieces = D / 8;
+  // an all-ones exponent carries into the bit above it when one is added at its lowest bit
+  constexpr bool kBf16 = !__is_same(T, __half);
+  constexpr uint32_t kExp = kBf16 ? 0x7f807f80u : 0x7c007c00u, kOne = kBf16 ? 0x00800080u : 0x04000400u;
+  const int r0 = table ? kNTile : max(0, min(kNTile, all_lo - key));
+  const int r1 = table ? kNTile : max(r0, min(kNTile, all_hi - key));
+  bool any = false;
+#pragma unroll 4
+  for (int x = threadIdx.x; x < (r0 + kNTile - r1) * kPieces; x += threads) {
+    const int c = x % kPieces, y = x / kPieces, r = y < r0 ? y : y - r0 + r1, k = key + r;
+    uint4* w = reinterpret_cast<uint4*>(v + (c / 8) * (kNTile * 128) + r * 128 + (c & 7) * 16);
+    bool zero = k < lo || k >= end;
+    if (table && !zero) zero = table[k >> shift] < 0 || table[k >> shift] >= n_pages;
+    const uint4 b = *w;
+    const uint32_t u[4] = {b.x, b.y, b.z, b.w};
+    uint32_t o[4], found = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t high = ((u[i] & kExp) + kOne) & 0x80008000u;  // each half that is not finite
+      found |= high;
+      o[i] = zero ? 0u : u[i] & ~((high >> 15) * 0xffffu);
+    }
+    if (zero || (found && (k < all_lo || k >= all_hi))) *w = make_uint4(o[0], o[1], o[2], o[3]);
+    any |= found && !zero;
+  }
+  return any;
+}
+
 // One CTA: 256 query rows (row = token * group + head of the group) of one
 // sequence and key head against one part of its keys.  Two accumulators of 128
 // rows share the keys.  Per step of 64 keys and tile
@@ -235,7 +274,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr uint32_t kSCol = 0, kOCol = 2 * kNTile;  // TMEM columns: S0, S1, O0, O1
   extern __shared__ unsigned char raw[];
   unsigned char* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2], care[kCare];
+  __shared__ uint64_t full[kStages], empty[kStages], s_full[2][2], p_full[2][2], o_full[2], clean[2];
   __shared__ uint32_t tmem_slot;
   __shared__ ChunkTile s_tile;
   __shared__ int s_bad, s_odd, s_dead;
@@ -278,9 +317,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], tiles);
     for (int i = 0; i < 2; ++i) {
       for (int k = 0; k < 2; ++k) bar_init(&s_full[i][k], 1), bar_init(&p_full[i][k], 4);
-      bar_init(&o_full[i], 1);
+      bar_init(&o_full[i], 1), bar_init(&clean[i], 4 * tiles);
     }
-    for (int i = 0; i < kCare; ++i) bar_init(&care[i], 1);
     bar_init_fence();
   }
   // the first keys are on their way before the queries are
@@ -309,11 +347,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     load(&kmap, ring, id, ok, &full[0]);
   }
 
+  // Row r of the pair is query t0 + (rem0 + r) / group: a product with 2^20 / group, rounded
+  // up, is exact for these small numbers.
+  const int rem0 = tile.row0 - t0 * group;
+  const uint32_t per_group = ((1u << 20) + group - 1) / group;
   // queries into shared memory, 128-byte swizzled lines (rows past the last: zeros)
   for (int x = threadIdx.x; x < tiles * kMTile * (D / 8); x += kChunkThreads) {
     const int r = x / (D / 8), c = x % (D / 8), row = r & (kMTile - 1);
     const bool there = r < rows;
-    const int t = there ? (tile.row0 + r) / group : t0, h = there ? tile.row0 + r - t * group : 0;
+    const int q = there ? rem0 + r : 0, dt = (int)((q * per_group) >> 20), t = t0 + dt, h = q - dt * group;
     cp16(sq + (r / kMTile) * kTile + (c / 8) * kLineTile + row * 128 + (((c & 7) ^ (row & 7)) * 16),
          static_cast<const T*>(a.q) + (int64_t)(first + t) * a.q_token_stride + (int64_t)(kvh * group + h) * a.q_head_stride +
              c * 8,
@@ -343,13 +385,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
   // Values of keys that a row does not see meet a zero weight in its product, so
   // they have to be finite.  A tile with rows that not every query of the pair
-  // sees, or that are not there, goes past the last warp before its product.
-  auto careful = [&](int key, unsigned ok) {
-    return key < all_lo || key + kNTile > all_hi || __popc(ok) != kNTile >> shift;
-  };
+  // sees, or that are not there, is cleaned by the softmax warps before its
+  // product: rows outside lo .. end and of missing pages become zeros; infinities
+  // and NaNs in rows that only some queries see become zeros too and are added at
+  // the end for the queries that do see them.
+  auto careful = [&](int key) { return key < all_lo || key + kNTile > all_hi || bad; };
   if (warp == 8) {
     // ---- loads: K and V of a step take one ring stage each ----------------------
-    int id, next_id, cleaned = 0;
+    int id, next_id, issued = 0;
     unsigned ok = pages_of(begin, id), next_ok = ok;
     for (int j = 0; j < steps && !*dead; ++j) {
       const int key = begin + j * kNTile;
@@ -359,56 +402,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
         __syncwarp();
         if (*dead) break;
-        uint64_t* bar = kind && careful(key, ok) ? &care[cleaned++ % kCare] : &full[st];
-        if (use > 0) load(kind ? &vmap : &kmap, ring + st * kTile, id, ok, bar);
+        if (use > 0) load(kind ? &vmap : &kmap, ring + st * kTile, id, ok, &full[st]);
+        issued = use + 1;
       }
       id = next_id, ok = next_ok;
     }
-  } else if (warp == 11) {
-    // ---- cleaning: rows outside lo .. end and of missing pages become zeros;
-    // infinities and NaNs in rows that only some queries see become zeros too and
-    // are added at the end for the queries that do see them
-    int cleaned = 0;
-    for (int j = 0; j < steps && !*dead; ++j) {
-      const int key = begin + j * kNTile, st = (2 * j + 1) % kStages;
-      int id;
-      const unsigned ok = pages_of(key, id);
-      if (!careful(key, ok)) continue;
-      if (!wait_phase(&care[cleaned % kCare], (cleaned / kCare) & 1)) *dead = 1;
-      ++cleaned;
-      unsigned char* v = smem + (ring - sq) + st * kTile;
-      // rows 0 .. r0 - 1 and r1 .. 127 are not seen by all
-      const bool whole = __popc(ok) == kNTile >> shift;
-      const int r0 = whole ? max(0, min(kNTile, all_lo - key)) : kNTile;
-      const int r1 = whole ? max(r0, min(kNTile, all_hi - key)) : kNTile;
-      const int words = (r0 + kNTile - r1) * kLines * 8;
-      bool odd = false;
-#pragma unroll 4
-      for (int x = lane; x < words; x += 32) {
-        int r = x / (kLines * 8);
-        if (r >= r0) r += r1 - r0;
-        const int c = x % (kLines * 8), k = key + r;
-        uint4* w = reinterpret_cast<uint4*>(v + (c / 8) * kLineTile + r * 128 + (c & 7) * 16);
-        const uint4 b = *w;
-        const bool keep = k >= lo && k < end && ((ok >> (r >> shift)) & 1u), some_only = k < all_lo || k >= all_hi;
-        constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
-        const uint32_t u[4] = {b.x, b.y, b.z, b.w};
-        uint32_t o[4];
-        bool found = !keep;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool l = (u[i] & kExp) == kExp && some_only, h = ((u[i] >> 16) & kExp) == kExp && some_only;
-          o[i] = !keep ? 0u : (l ? 0u : u[i] & 0xffffu) | (h ? 0u : u[i] & 0xffff0000u);
-          found |= l || h;
-        }
-        if (found) *w = make_uint4(o[0], o[1], o[2], o[3]);
-        odd |= found && keep;
-      }
-      if (odd) s_odd = 1;
-      fence_async();
-      __syncwarp();
-      if (lane == 0) bar_arrive(&full[st]);
-    }
+    if (*dead)  // after a wait that ran out: copies in flight end first
+      for (int use = max(0, issued - kStages); use < issued; ++use) wait_phase(&full[use % kStages], (use / kStages) & 1);
   } else if (warp >= 9 && warp < 9 + tiles) {
     // ---- products: one warp a tile, together; an elected thread issues ---------------
     // Descriptors and addresses are the same in every lane and stay in uniform
@@ -441,9 +441,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       };
       // all 512 columns are this CTA's, so they start at 0
       bool live = tmem == 0 && scores(0) && (subs == 1 || scores(1));
+      int cleaned = 0;
       for (int i = 0; i < subs && live; ++i) {
         const int use = i | 1, st = use % kStages;
-        live = stage_full(use) && wait_phase(&p_full[t][i & 1], (i >> 1) & 1);
+        live = stage_full(use);
+        if (!(i & 1) && careful(begin + i * kStep)) {
+          live = live && wait_phase(&clean[cleaned & 1], (cleaned >> 1) & 1);
+          ++cleaned;
+        }
+        live = live && wait_phase(&p_full[t][i & 1], (i >> 1) & 1);
         if (!live) break;
         fence_after_sync();
         const uint64_t v = v_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
@@ -473,7 +479,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     float m = -INFINITY, sum = 0.f;
     bool live = true;
     if (t < tiles) {
+      int cleaned = 0;
       for (int i = 0; i < subs; ++i) {
+        if (!(i & 1) && careful(begin + i * kStep)) {
+          live = __all_sync(~0u, wait_phase(&full[(i | 1) % kStages], ((i | 1) / kStages) & 1));
+          if (!live) break;
+          if (clean_values<T, D>(smem + (ring - sq) + (i | 1) % kStages * kTile, begin + i * kStep, lo, all_lo, all_hi, end,
+                                 bad ? table : nullptr, shift, a.n_pages, tiles * 128))
+            s_odd = 1;
+          fence_async();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&clean[cleaned & 1]);
+          ++cleaned;
+        }
         live = __all_sync(~0u, wait_phase(&s_full[t][i & 1], (i >> 1) & 1));
         if (!live) break;
         fence_after_sync();
@@ -559,7 +577,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       if (live) {
         fence_after_sync();
-        const int q = (tile.row0 + r) / group, head = kvh * group + tile.row0 + r - q * group;
+        const int dt = (int)(((rem0 + r) * per_group) >> 20), q = t0 + dt, head = kvh * group + rem0 + r - dt * group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum, mm = m == -INFINITY ? 0.f : m * c2;
         const int64_t item = (int64_t)tile.index * a.kv_heads + kvh;
         const int64_t at = (item * plan.parts + part) * kPair + r;
@@ -568,6 +586,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           a.lse[(int64_t)(first + q) * a.q_heads + head] =
               sum == 0.f ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
         if (mine && parts > 1) plan.ml[at] = make_float2(m == -INFINITY ? m : mm, sum);
+        // The row goes through shared memory, where its queries were, so that whole rows are stored together.
+        unsigned char* stage = smem + t * kTile;
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           float o[32];
@@ -596,18 +616,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               }
             }
           }
-          if (!mine) continue;
           if (parts > 1) {
+            if (mine) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<float4*>(plan.o + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(plan.o + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
           } else {
-            T* out = static_cast<T*>(a.out) + (int64_t)(first + q) * a.out_token_stride +
-                     (int64_t)head * a.out_head_stride + c;
+            const int row = r & (kMTile - 1);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] *= inv;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(out + i) = pack8<T>(o + i);
+            for (int i = 0; i < 32; i += 8)
+              *reinterpret_cast<uint4*>(stage + (c / 64) * kLineTile + row * 128 +
+                                        ((((c + i) / 8 & 7) ^ (row & 7)) * 16)) = pack8<T>(o + i);
+          }
+        }
+        if (parts == 1) {
+          __syncwarp();
+          constexpr int kPieces = D / 8, kTogether = 32 / kPieces;  // 16-byte pieces of a row, rows at a time
+          const int c = lane % kPieces, row0 = (warp & 3) * 32;
+#pragma unroll 4
+          for (int i = 0; i < 32; i += kTogether) {
+            const int row = row0 + i + lane / kPieces, x = t * kMTile + row;
+            if (x >= rows) continue;
+            const int d = (int)(((rem0 + x) * per_group) >> 20), h = kvh * group + rem0 + x - d * group;
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t)(first + t0 + d) * a.out_token_stride +
+                                      (int64_t)h * a.out_head_stride + c * 8) =
+                *reinterpret_cast<const uint4*>(stage + (c / 8) * kLineTile + row * 128 + (((c & 7) ^ (row & 7)) * 16));
           }
         }
       }
@@ -615,6 +651,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
+  if (*dead && warp == 9 && subs > 0)  // after a wait that ran out: products in flight end first
+    for (int i = 0; i < tiles; ++i) wait_phase(&o_full[i], 0);
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
