@@ -390,6 +390,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // and NaNs in rows that only some queries see become zeros too and are added at
   // the end for the queries that do see them.
   auto careful = [&](int key) { return key < all_lo || key + kNTile > all_hi || bad; };
+  // 384 threads x 168 registers at launch = 64,512; a row of scores can use more: 256 x 208 + 128 x 80 = 63,488
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp == 8) {
     // ---- loads: K and V of a step take one ring stage each ----------------------
     int id, next_id, issued = 0;
@@ -467,7 +470,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (leader) mma_commit(&o_full[t]);
     }
     __syncwarp();
-  } else if (warp < 8) {
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: one row a thread ------------------------------------------------
     const int t = warp >> 2, r = t * kMTile + (threadIdx.x & (kMTile - 1));
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
