@@ -8,6 +8,8 @@ cache and a fused LM head + argmax, behind the reference's runner seam
 
 * ``llm_accelerator_b200.reference_api`` - the reference helper names on GPU.
 * ``llm_accelerator_b200.model.Q4Model`` - model context and decode APIs.
+* ``llm_accelerator_b200.paged`` / ``paged_decode`` - 16-bit operators over a paged
+  K/V cache, and the model's layers on them.
 * ``include/q4gpu.h`` / ``_lib/libq4gpu.so`` - the C ABI.
 """
 from ._native import load as load_library  # noqa: F401

@@ -61,9 +61,10 @@ __device__ __forceinline__ void ldsm4_t(uint32_t* r, uint32_t at) {
 template <typename T>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   if constexpr (sizeof(T) == 2 && __is_same(T, __half))
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -162,7 +163,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
       const int64_t head_start = start + (int64_t)kvh * cost + kPieceCost;  // of its first real unit
       if (head_start - kPieceCost >= last_unit) break;
       const int units = cost - kPieceCost;
-      const int u0 = (int)max((int64_t)0, first_unit - head_start), u1 = (int)min((int64_t)units, last_unit - head_start);
+      const int u0 = (int)max((int64_t)0, first_unit - head_start);
+      const int u1 = (int)min((int64_t)units, last_unit - head_start);
       // (a sequence without keys: its zeros are written by the CTA where its cost begins)
       if (u1 > u0 || (units == 0 && head_start - kPieceCost >= first_unit)) {
         const int rows = s.n * group;
@@ -308,7 +310,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
             }
           }
           // weights rounded to the cache's type for the tensor cores (their sum is not)
-          const uint32_t pf[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]), pack2<T>(sc[1][0], sc[1][1]),
+          const uint32_t pf[4] = {pack2<T>(sc[0][0], sc[0][1]), pack2<T>(sc[0][2], sc[0][3]),
+                                  pack2<T>(sc[1][0], sc[1][1]),
                                   pack2<T>(sc[1][2], sc[1][3])};
 #pragma unroll
           for (int n = 0; n < D / 16; ++n) {
@@ -499,8 +502,9 @@ int encode_map(CUtensorMap* map, const q4gpu_attn_args& a, const void* base) {
   const cuuint64_t strides[3] = {(cuuint64_t)a.row_stride * 2, (cuuint64_t)a.head_stride * 2,
                                  (cuuint64_t)a.page_stride * 2};
   const cuuint32_t box[4] = {64, (cuuint32_t)a.page_tokens, 1, 1}, one[4] = {1, 1, 1, 1};
-  const CUresult r = encode(map, a.dtype == Q4GPU_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                            4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUtensorMapDataType type =
+      a.dtype == Q4GPU_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = encode(map, type, 4, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed (%d)", (int)r);

@@ -135,8 +135,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
 }
 // Waits for a phase; false after about 0.3 s.  (umma::bar_wait reads the global
 // timer after its first miss, which took longer than most waits here.)  A wait
-// that lasts sleeps between its tests, which otherwise hold the shared-memory
-// pipe against the warp that has work to do.
+// that lasts sleeps between its tests.
 __device__ __forceinline__ bool wait_phase(uint64_t* b, unsigned parity) {
   if (umma::bar_try_wait(b, parity)) return true;
   long long since = 0;
@@ -338,7 +337,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     __syncwarp();
     if ((ok >> lane) & 1u) {
 #pragma unroll
-      for (int c = 0; c < kLines; ++c) tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, map, c * 64, 0, kvh, id, bar);
+      for (int c = 0; c < kLines; ++c)
+        tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, map, c * 64, 0, kvh, id, bar);
     }
   };
   if (warp == 8 && steps > 0) {
@@ -357,8 +357,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const bool there = r < rows;
     const int q = there ? rem0 + r : 0, dt = (int)((q * per_group) >> 20), t = t0 + dt, h = q - dt * group;
     cp16(sq + (r / kMTile) * kTile + (c / 8) * kLineTile + row * 128 + (((c & 7) ^ (row & 7)) * 16),
-         static_cast<const T*>(a.q) + (int64_t)(first + t) * a.q_token_stride + (int64_t)(kvh * group + h) * a.q_head_stride +
-             c * 8,
+         static_cast<const T*>(a.q) + (int64_t)(first + t) * a.q_token_stride +
+             (int64_t)(kvh * group + h) * a.q_head_stride + c * 8,
          there);
   }
   // is any page of these keys missing?
@@ -393,84 +393,86 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // 384 threads x 168 registers at launch = 64,512; a row of scores can use more: 256 x 208 + 128 x 80 = 63,488
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  if (warp == 8) {
-    // ---- loads: K and V of a step take one ring stage each ----------------------
-    int id, next_id, issued = 0;
-    unsigned ok = pages_of(begin, id), next_ok = ok;
-    for (int j = 0; j < steps && !*dead; ++j) {
-      const int key = begin + j * kNTile;
-      if (j + 1 < steps) next_ok = pages_of(key + kNTile, next_id);
-      for (int kind = 0; kind < 2; ++kind) {
-        const int use = 2 * j + kind, st = use % kStages;
-        if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
-        __syncwarp();
-        if (*dead) break;
-        if (use > 0) load(kind ? &vmap : &kmap, ring + st * kTile, id, ok, &full[st]);
-        issued = use + 1;
+    if (warp == 8) {
+      // ---- loads: K and V of a step take one ring stage each ----------------------
+      int id, next_id, issued = 0;
+      unsigned ok = pages_of(begin, id), next_ok = ok;
+      for (int j = 0; j < steps && !*dead; ++j) {
+        const int key = begin + j * kNTile;
+        if (j + 1 < steps) next_ok = pages_of(key + kNTile, next_id);
+        for (int kind = 0; kind < 2; ++kind) {
+          const int use = 2 * j + kind, st = use % kStages;
+          if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
+          __syncwarp();
+          if (*dead) break;
+          if (use > 0) load(kind ? &vmap : &kmap, ring + st * kTile, id, ok, &full[st]);
+          issued = use + 1;
+        }
+        id = next_id, ok = next_ok;
       }
-      id = next_id, ok = next_ok;
-    }
-    if (*dead)  // after a wait that ran out: copies in flight end first
-      for (int use = max(0, issued - kStages); use < issued; ++use) wait_phase(&full[use % kStages], (use / kStages) & 1);
-  } else if (warp >= 9 && warp < 9 + tiles) {
-    // ---- products: one warp a tile, together; an elected thread issues ---------------
-    // Descriptors and addresses are the same in every lane and stay in uniform
-    // registers (issued from a divergent branch each product took twice as long).
-    // A warp's barrier tests queue up behind the products it has issued, so each
-    // tile has a warp of its own.
-    if (subs > 0) {
-      constexpr uint32_t qk = f16_idesc(kBf16, kMTile, kStep, false), pv = f16_idesc(kBf16, kMTile, D, true);
-      const int t = warp - 9;
-      const bool leader = elect_one();
-      const uint32_t sc = kSCol + t * 2 * kStep, oc = kOCol + t * D;
-      const uint64_t q = sw128_desc(sq) + t * (kTile / 16), k_desc = sw128_desc(ring),
-                     v_desc = sw128_mn_desc(ring, kLineTile);
-      auto stage_full = [&](int use) { return wait_phase(&full[use % kStages], (use / kStages) & 1); };
-      auto scores = [&](int i) {
-        const int use = i & ~1, st = use % kStages;
-        if (!stage_full(use)) return false;
-        fence_after_sync();
-        const uint64_t k = k_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
-        if (leader) {
+      if (*dead)  // after a wait that ran out: copies in flight end first
+        for (int use = max(0, issued - kStages); use < issued; ++use)
+          wait_phase(&full[use % kStages], (use / kStages) & 1);
+    } else if (warp >= 9 && warp < 9 + tiles) {
+      // ---- products: one warp a tile, together; an elected thread issues ---------------
+      // Descriptors and addresses are the same in every lane and stay in uniform
+      // registers (issued from a divergent branch each product took twice as long).
+      // A warp's barrier tests queue up behind the products it has issued, so each
+      // tile has a warp of its own.
+      if (subs > 0) {
+        constexpr uint32_t qk = f16_idesc(kBf16, kMTile, kStep, false), pv = f16_idesc(kBf16, kMTile, D, true);
+        const int t = warp - 9;
+        const bool leader = elect_one();
+        const uint32_t sc = kSCol + t * 2 * kStep, oc = kOCol + t * D;
+        const uint64_t q = sw128_desc(sq) + t * (kTile / 16), k_desc = sw128_desc(ring),
+                       v_desc = sw128_mn_desc(ring, kLineTile);
+        auto stage_full = [&](int use) { return wait_phase(&full[use % kStages], (use / kStages) & 1); };
+        auto scores = [&](int i) {
+          const int use = i & ~1, st = use % kStages;
+          if (!stage_full(use)) return false;
+          fence_after_sync();
+          const uint64_t k = k_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
+          if (leader) {
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            const int at = ((x / 4) * kLineTile + (x & 3) * 32) / 16;
-            mma_ss(sc + (i & 1) * kStep, q + at, k + at, qk, x > 0);
+            for (int x = 0; x < D / 16; ++x) {
+              const int at = ((x / 4) * kLineTile + (x & 3) * 32) / 16;
+              mma_ss(sc + (i & 1) * kStep, q + at, k + at, qk, x > 0);
+            }
+            mma_commit(&s_full[t][i & 1]);
+            if ((i & 1) || i + 1 == subs) mma_commit(&empty[st]);
           }
-          mma_commit(&s_full[t][i & 1]);
-          if ((i & 1) || i + 1 == subs) mma_commit(&empty[st]);
-        }
-        return true;
-      };
-      // all 512 columns are this CTA's, so they start at 0
-      bool live = tmem == 0 && scores(0) && (subs == 1 || scores(1));
-      int cleaned = 0;
-      for (int i = 0; i < subs && live; ++i) {
-        const int use = i | 1, st = use % kStages;
-        live = stage_full(use);
-        if (!(i & 1) && careful(begin + i * kStep)) {
-          live = live && wait_phase(&clean[cleaned & 1], (cleaned >> 1) & 1);
-          ++cleaned;
-        }
-        live = live && wait_phase(&p_full[t][i & 1], (i >> 1) & 1);
-        if (!live) break;
-        fence_after_sync();
-        const uint64_t v = v_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
-        if (leader) {
+          return true;
+        };
+        // all 512 columns are this CTA's, so they start at 0
+        bool live = tmem == 0 && scores(0) && (subs == 1 || scores(1));
+        int cleaned = 0;
+        for (int i = 0; i < subs && live; ++i) {
+          const int use = i | 1, st = use % kStages;
+          live = stage_full(use);
+          if (!(i & 1) && careful(begin + i * kStep)) {
+            live = live && wait_phase(&clean[cleaned & 1], (cleaned >> 1) & 1);
+            ++cleaned;
+          }
+          live = live && wait_phase(&p_full[t][i & 1], (i >> 1) & 1);
+          if (!live) break;
+          fence_after_sync();
+          const uint64_t v = v_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
+          if (leader) {
 #pragma unroll
-          for (int x = 0; x < kStep / 16; ++x) mma_ts(oc, sc + (i & 1) * kStep + x * 8, v + x * 128, pv, i > 0 || x > 0);
-          if ((i & 1) || i + 1 == subs) mma_commit(&empty[st]);
+            for (int x = 0; x < kStep / 16; ++x)
+              mma_ts(oc, sc + (i & 1) * kStep + x * 8, v + x * 128, pv, i > 0 || x > 0);
+            if ((i & 1) || i + 1 == subs) mma_commit(&empty[st]);
+          }
+          if (i + 2 < subs)
+            live = scores(i + 2);
+          else if (leader)
+            mma_commit(&s_full[t][i & 1]);  // no scores: it tells that O is complete up to step i
         }
-        if (i + 2 < subs)
-          live = scores(i + 2);
-        else if (leader)
-          mma_commit(&s_full[t][i & 1]);  // no scores: it tells that O is complete up to step i
+        if (!live) *dead = 1;
+        if (leader) mma_commit(&o_full[t]);
       }
-      if (!live) *dead = 1;
-      if (leader) mma_commit(&o_full[t]);
+      __syncwarp();
     }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: one row a thread ------------------------------------------------
@@ -489,8 +491,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (!(i & 1) && careful(begin + i * kStep)) {
           live = __all_sync(~0u, wait_phase(&full[(i | 1) % kStages], ((i | 1) / kStages) & 1));
           if (!live) break;
-          if (clean_values<T, D>(smem + (ring - sq) + (i | 1) % kStages * kTile, begin + i * kStep, lo, all_lo, all_hi, end,
-                                 bad ? table : nullptr, shift, a.n_pages, tiles * 128))
+          if (clean_values<T, D>(smem + (ring - sq) + (i | 1) % kStages * kTile, begin + i * kStep, lo, all_lo, all_hi,
+                                 end, bad ? table : nullptr, shift, a.n_pages, tiles * kMTile))
             s_odd = 1;
           fence_async();
           __syncwarp();
@@ -548,7 +550,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             tm_st32(to + c, reinterpret_cast<const uint32_t*>(o));
           }
         }
-        const float off = m == -INFINITY ? 0.f : -m * c2;
+        // (m - m is 0, or NaN where a score was infinite or NaN: the whole row becomes NaN, as it should)
+        const float off = m == -INFINITY ? 0.f : fmaf(-m, c2, m - m);
         const uint64_t off2 = pair_of(off, off);
         uint64_t add[2] = {0, 0};
         uint32_t p[32];

@@ -214,10 +214,12 @@ class RopeAppend(_Err):
             for t, c, name in ((k, k_cache, "k"), (v, v_cache, "v")):
                 if t is None:
                     continue
-                if c is None or c.dtype != dtype or c.device != self.device or c.shape != shape or c.stride() != strides:
+                if c is None or c.dtype != dtype or c.device != self.device or c.shape != shape or \
+                        c.stride() != strides:
                     raise ValueError(f"{name}_cache must be {tuple(shape)} {dtype}, K and V laid out alike")
             if len(shape) != 4 or strides[3] != 1 or shape[1] != heads or shape[3] != dim:
-                raise ValueError(f"the caches must be [pages, {heads}, page_tokens, {dim}] with contiguous head vectors")
+                raise ValueError(f"the caches must be [pages, {heads}, page_tokens, {dim}] with contiguous head "
+                                 "vectors")
             if k is not None:
                 a.k, a.k_token_stride, a.k_head_stride = self._heads(k, tokens, heads, dim, dtype, "k")
                 a.k_cache = k_cache.data_ptr()

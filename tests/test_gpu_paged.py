@@ -376,6 +376,23 @@ def test_attention_masked_infinities_in_queries():
     assert torch.equal(out, clean)
 
 
+@pytest.mark.parametrize("new,old", [(1, 300), (50, 300), (400, 300)])
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("at", [0, 1, 2, 130])
+def test_attention_seen_infinities_and_nans(new, old, what, at):
+    """A key that is not finite makes every query that sees it NaN, wherever it stands in a step; the others keep
+    their results."""
+    args = make([new], [old], 4, 2, 128, 64, BF, 13)
+    pool, table = args[:2]
+    at += old if new > 200 else 0
+    clean, _ = attend(*args)
+    pool[table[0, at // 64], 0, 1, at % 64] = what  # key head 1: query heads 2 and 3
+    out, lse = attend(*args)
+    sees = torch.arange(old, old + new, device="cuda") >= at
+    assert out[sees][:, 2:].isnan().all() and lse[sees][:, 2:].isnan().all()
+    assert torch.equal(out[:, :2], clean[:, :2]) and torch.equal(out[~sees], clean[~sees])
+
+
 @pytest.mark.parametrize("new,old", [([1, 1], [100, 900]), ([70, 3], [100, 900])])
 def test_attention_strides_and_stream(new, old):
     """Queries inside a fused projection, an output with its own strides, another stream, and max_ctx left open."""
