@@ -107,7 +107,7 @@ __device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int gro
 // end.  Bound by memory: every key and value is read once, for all heads of its
 // group.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, RowPlan plan, bool after_chunks) {
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, RowPlan plan) {
   constexpr int kThreads = kRowWarps * 32;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float s_m[kRowWarps][kRows], s_l[kRowWarps][kRows];
@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   __shared__ int s_most[kRowWarps], s_seq, s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.q_heads / a.kv_heads;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the chunk kernel reads nothing of this one
   // the axis: each thread adds up a run of sequences
   const int per = (a.n_seqs + kThreads - 1) / kThreads;
   const int run0 = min(a.n_seqs, (int)threadIdx.x * per), run1 = min(a.n_seqs, run0 + per);
@@ -409,8 +410,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
       }
     }
   }
-  // the kernel before is complete when this one is
-  if (after_chunks) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 int check_sizes(const q4gpu_attn_args* a) {
@@ -528,44 +527,43 @@ int launch(const q4gpu_attn_args& a, cudaStream_t s) {
   static unsigned char ready[2][Q4GPU_MAX_DEVICES];
   size_t rows_bytes;
   const RowPlan few = row_plan(a, static_cast<char*>(a.workspace), &rows_bytes);
-  int rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D>), row_smem<D>(), ready[0]);
   const bool chunks = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows;
-  ChunkPlan plan{};
-  if (rc == Q4GPU_OK && chunks) {
-    plan = chunk_plan(a, nullptr);
-    if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
+  ChunkPlan plan = chunk_plan(a, nullptr);
+  if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
+  const bool short_ones = !chunks || plan.least > 1;  // sequences for attn_rows_kernel
+  int rc = Q4GPU_OK;
+  if (short_ones) {
+    rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D>), row_smem<D>(), ready[0]);
+    if (rc != Q4GPU_OK) return rc;
+  }
+  CUtensorMap kmap, vmap;
+  if (chunks) {
     char* ws = static_cast<char*>(a.workspace) + (rows_bytes + 15) / 16 * 16;
     plan.ml = reinterpret_cast<float2*>(ws);
     plan.o = reinterpret_cast<float*>(plan.ml + (size_t)plan.tiles * a.kv_heads * plan.parts * kPair);
-    CUtensorMap kmap, vmap;
     rc = encode_map(&kmap, a, a.k_cache);
     if (rc == Q4GPU_OK) rc = encode_map(&vmap, a, a.v_cache);
     if (rc == Q4GPU_OK)
       rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D>), chunk_smem<D>(), ready[1]);
-    if (rc == Q4GPU_OK)
-      attn_chunk_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, plan.parts), kChunkThreads, chunk_smem<D>(), s>>>(
-          kmap, vmap, a, plan);
+    if (rc != Q4GPU_OK) return rc;
   }
-  if (rc != Q4GPU_OK) return rc;
-  if (chunks && plan.least == 1) {
-    if (plan.parts > 1)
-      attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
-    return q4gpu_check_launch();
+  if (short_ones) attn_rows_kernel<T, D><<<few.ctas, kRowWarps * 32, row_smem<D>(), s>>>(a, few);
+  if (chunks) {
+    // starts beside the short sequences' kernel, on the SMs that it leaves free
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.kv_heads, plan.tiles, plan.parts);
+    cfg.blockDim = dim3(kChunkThreads);
+    cfg.dynamicSmemBytes = chunk_smem<D>();
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = short_ones ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_chunk_kernel<T, D>, kmap, vmap, a, plan);
+    if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: launch: %s", cudaGetErrorString(e));
+    if (plan.parts > 1) attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
   }
-  // After chunks, the short sequences' CTAs start once the last chunk's CTA has, and fill the SMs that run dry.
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(few.ctas);
-  cfg.blockDim = dim3(kRowWarps * 32);
-  cfg.dynamicSmemBytes = row_smem<D>();
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = chunks ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_rows_kernel<T, D>, a, few, chunks);
-  if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: launch: %s", cudaGetErrorString(e));
-  if (plan.parts > 1) attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
   return q4gpu_check_launch();
 }
 

@@ -33,38 +33,73 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
   return max(kMinPart, ((keys + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
 }
 
-// Sequence and row pair of one grid index; sequences with few rows have none.
-// Later rows see more keys, so pairs are handed out from the last to the first.
+// Sequence and row pair of one grid index, and what its CTA needs to know of the
+// sequence: first query token, query tokens, cache slot, stored keys.
 struct ChunkTile {
-  int seq, row0, index;
+  int seq, row0, index, first, n, slot, len;
 };
-__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int group, int least) {
-  const int n = max(0, min(a.cu_q[i + 1], a.tokens) - max(0, min(a.cu_q[i], a.tokens)));
-  return n < least ? 0 : (int)(((int64_t)n * group + kPair - 1) / kPair);
+// Row pairs of sequence i (none where it has few rows); keys: about how many one walks.
+__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int group, int least, ChunkTile& t, int& keys) {
+  keys = 0;
+  if (i >= a.n_seqs) return 0;
+  t.first = max(0, min(a.cu_q[i], a.tokens));
+  t.n = max(0, min(a.cu_q[i + 1], a.tokens) - t.first);
+  t.slot = a.seq_ids ? a.seq_ids[i] : i;
+  const bool known = t.slot >= 0 && t.slot < a.n_slots;
+  t.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[t.slot], a.table_stride * a.page_tokens)) : 0;
+  if (t.n < least) return 0;
+  keys = a.window > 0 ? min(t.len, a.window) : t.len;
+  return (int)(((int64_t)t.n * group + kPair - 1) / kPair);
 }
-// The y-th pair, or with `last_first` the y-th from the end; seq = -1 where
-// there are fewer.  By one full warp.
-__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int least, int y, bool last_first) {
+// The pair of grid row y; seq = -1 where there are fewer.  By one full warp.
+// Pairs with many keys come first, so that they do not start when the others
+// end: sequences in four classes (at least half, a quarter, an eighth of the most
+// keys, the rest), and within a class from its last row pair to its first, as
+// later rows see more keys.
+__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int least, int y) {
   const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
-  int total = 0;
-  for (int i = lane; i < a.n_seqs; i += 32) total += pairs_of(a, i, group, least);
-  total = __reduce_add_sync(~0u, total);
-  ChunkTile t{-1, 0, last_first ? total - 1 - y : y};
-  if (y >= total) return t;
+  ChunkTile t{-1, 0, y, 0, 0, 0, 0}, own;
+  int most = 0, keys;
+  for (int i = lane; i < a.n_seqs; i += 32) {
+    pairs_of(a, i, group, least, own, keys);
+    most = max(most, keys);
+  }
+  most = __reduce_max_sync(~0u, most);
+  auto rank = [&](int k) { return k >= most / 2 ? 0 : k >= most / 4 ? 1 : k >= most / 8 ? 2 : 3; };
+  int count[4] = {0, 0, 0, 0};
+  for (int i = lane; i < a.n_seqs; i += 32) {
+    const int n = pairs_of(a, i, group, least, own, keys);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) count[c] += rank(keys) == c ? n : 0;
+  }
+  int wanted = -1;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int n = __reduce_add_sync(~0u, count[c]);
+    if (wanted >= 0) continue;
+    if (y < n)
+      wanted = c, y = n - 1 - y;
+    else
+      y -= n;
+  }
+  if (wanted < 0) return t;
   int before = 0;
   for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
-    const int mine = i0 + lane < a.n_seqs ? pairs_of(a, i0 + lane, group, least) : 0;
+    int mine = pairs_of(a, i0 + lane, group, least, own, keys);
+    if (rank(keys) != wanted) mine = 0;
     int run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(~0u, run, o);
       if (lane >= o) run += v;
     }
-    const unsigned hit = __ballot_sync(~0u, before + run > t.index);
+    const unsigned hit = __ballot_sync(~0u, before + run > y);
     if (hit) {
       const int k = __ffs(hit) - 1;
       t.seq = i0 + k;
-      t.row0 = (t.index - before - __shfl_sync(~0u, run - mine, k)) * kPair;
+      t.row0 = (y - before - __shfl_sync(~0u, run - mine, k)) * kPair;
+      t.first = __shfl_sync(~0u, own.first, k), t.n = __shfl_sync(~0u, own.n, k);
+      t.slot = __shfl_sync(~0u, own.slot, k), t.len = __shfl_sync(~0u, own.len, k);
       return t;
     }
     before += __shfl_sync(~0u, run, 31);
@@ -279,20 +314,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __shared__ int s_bad, s_odd, s_dead;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.x, part = blockIdx.z;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // what follows reads nothing of this kernel
+  // One CTA waits for the kernel before (the short sequences') at its end, so that this one is not complete earlier.
+  const bool waits = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
+  auto wait_before = [&] {
+    if (waits) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, plan.least, blockIdx.y, true);
+    const ChunkTile t = find_tile(a, plan.least, blockIdx.y);
     if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
   }
   __syncthreads();
   const ChunkTile tile = s_tile;
-  if (tile.seq < 0) return;
+  if (tile.seq < 0) return wait_before();
   const int group = a.q_heads / a.kv_heads;
-  const int first = max(0, min(a.cu_q[tile.seq], a.tokens));
-  const int n = min(a.cu_q[tile.seq + 1], a.tokens) - first;
-  const int slot = a.seq_ids ? a.seq_ids[tile.seq] : tile.seq;
-  const bool known = slot >= 0 && slot < a.n_slots;
-  const int len = known ? (int)max((int64_t)0, min((int64_t)a.lens[slot], a.table_stride * a.page_tokens)) : 0;
+  const int first = tile.first, n = tile.n, slot = tile.slot, len = tile.len;
   const int64_t all_rows = (int64_t)n * group;
   const int rows = (int)min((int64_t)kPair, all_rows - tile.row0);
   const int t0 = tile.row0 / group, t1 = (tile.row0 + rows - 1) / group;  // first and last query of the pair
@@ -303,7 +338,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int base = lo & ~(kNTile - 1);
   const int chunk = part_keys(plan, hi - base);
   const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
-  if (part >= parts) return;
+  if (part >= parts) return wait_before();
   const int begin = base + part * chunk, end = min(hi, begin + chunk);
   const int steps = begin < end ? (end - begin + kNTile - 1) / kNTile : 0;
   const int subs = begin < end ? (end - begin + kStep - 1) / kStep : 0;
@@ -662,6 +697,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (*dead && warp == 9 && subs > 0)  // after a wait that ran out: products in flight end first
     for (int i = 0; i < tiles; ++i) wait_phase(&o_full[i], 0);
   if (warp == 9) tmem_dealloc(tmem, 512);
+  wait_before();
 }
 
 // Joins the parts of each row, in order: one warp a row.
@@ -670,18 +706,14 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, Chunk
   __shared__ ChunkTile s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, plan.least, blockIdx.y, false);
+    const ChunkTile t = find_tile(a, plan.least, blockIdx.y);
     if (lane == 0) s_tile = t;
   }
   __syncthreads();
   const ChunkTile tile = s_tile;
   if (tile.seq < 0) return;
   const int group = a.q_heads / a.kv_heads;
-  const int first = max(0, min(a.cu_q[tile.seq], a.tokens));
-  const int n = min(a.cu_q[tile.seq + 1], a.tokens) - first;
-  const int slot = a.seq_ids ? a.seq_ids[tile.seq] : tile.seq;
-  const bool known = slot >= 0 && slot < a.n_slots;
-  const int len = known ? (int)max((int64_t)0, min((int64_t)a.lens[slot], a.table_stride * a.page_tokens)) : 0;
+  const int first = tile.first, n = tile.n, len = tile.len;
   const int rows = (int)min((int64_t)kPair, (int64_t)n * group - tile.row0);
   const int pos0 = len - n + tile.row0 / group, pos1 = len - n + (tile.row0 + rows - 1) / group;
   const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1), base = lo & ~(kNTile - 1);
