@@ -322,7 +322,7 @@ int q4gpu_pages_fork(const q4gpu_pages_args *a, const int32_t *parents, const in
 /* Packs the pages in use (named in any slot's first ceil(lens / page_tokens)
  * entries; shared pages once) into pages 0 .. n_live - 1: the i-th used page
  * from n_live on, in ascending order, moves to the i-th unused page below it.
- * new_table (may be a->table) gets the renumbered entries, -1 past each
+ * new_table (a->table itself or other memory) gets the renumbered entries, -1 past each
  * slot's last; remap[old page] (int32 [n_pages]) the new number or -1; *n_live
  * the number of pages in use.  All arrays are device memory; workspace:
  * q4gpu_pages_compact_workspace_bytes(n_pages) bytes, 16-byte aligned. */

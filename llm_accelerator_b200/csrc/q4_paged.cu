@@ -583,6 +583,20 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(q4gpu_pages_ar
 
 constexpr int64_t kMoveBytes = 1 << 16;  // a work item of the page copy
 
+// Copies `count` moved pages, kMoveBytes at a time, all CTAs together.
+template <typename Move>
+__device__ __forceinline__ void move_pages(const q4gpu_pages_args& a, int count, Move move) {
+  const int64_t per = (a.page_bytes + kMoveBytes - 1) / kMoveBytes, items = (int64_t)count * per;
+  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const int64_t m = i / per, off = (i - m * per) * kMoveBytes;
+    const int2 mv = move((int)m);
+    const int64_t bytes = min(kMoveBytes, a.page_bytes - off);
+    copy16(reinterpret_cast<uint4*>(static_cast<char*>(a.pool) + mv.y * a.page_bytes + off),
+           reinterpret_cast<const uint4*>(static_cast<const char*>(a.pool) + mv.x * a.page_bytes + off),
+           (int)(bytes / 16));
+  }
+}
+
 // Renumbers the tables and copies the moved pages, kMoveBytes at a time.
 // Sources lie at or past the packed end and destinations below it, so no copy
 // reads what another writes.  Bound by memory: 0.55 GB of pages move in 178 us, 6.2
@@ -595,15 +609,70 @@ __global__ void __launch_bounds__(512) pages_move_kernel(q4gpu_pages_args a, int
     const int id = a.table[e];
     new_table[e] = c * a.page_tokens < held(a, s) && id >= 0 && id < a.n_pages ? remap[id] : -1;
   }
-  const int64_t per = (a.page_bytes + kMoveBytes - 1) / kMoveBytes, items = (int64_t)*n_moves * per;
-  for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const int64_t m = i / per, off = (i - m * per) * kMoveBytes;
-    const int2 mv = moves[m];
-    const int64_t bytes = min(kMoveBytes, a.page_bytes - off);
-    copy16(reinterpret_cast<uint4*>(static_cast<char*>(a.pool) + mv.y * a.page_bytes + off),
-           reinterpret_cast<const uint4*>(static_cast<const char*>(a.pool) + mv.x * a.page_bytes + off),
-           (int)(bytes / 16));
+  move_pages(a, *n_moves, [&](int m) { return moves[m]; });
+}
+
+constexpr int kOnePages = 2048;     // pools of one launch
+constexpr int kOneEntries = 32768;  // and their tables
+
+// The same plan and moves in one launch for a small pool whose tables go to new
+// memory: every CTA makes the plan for itself, so none waits for another.
+__global__ void __launch_bounds__(512) pages_compact_kernel(q4gpu_pages_args a, int32_t* new_table, int32_t* remap,
+                                                            int32_t* n_live) {
+  __shared__ uint32_t s_bits[kOnePages / 32];
+  __shared__ int s_below[kOnePages / 32], s_total, s_src[kOnePages / 2], s_dst[kOnePages / 2];
+  const int t = threadIdx.x, lane = t & 31;
+  if (t < kOnePages / 32) s_bits[t] = 0u;
+  __syncthreads();
+  for (int s = t >> 5; s < a.n_slots; s += blockDim.x / 32) {
+    const int64_t used = (held(a, s) + a.page_tokens - 1) / a.page_tokens;
+    for (int64_t c = lane; c < used; c += 32) {
+      const int id = a.table[s * a.table_stride + c];
+      if (id >= 0 && id < a.n_pages)
+        atomicOr(&s_bits[id >> 5], 1u << (id & 31));
+      else if (a.err_flag)
+        *a.err_flag = 1;
+    }
   }
+  __syncthreads();
+  if (t < 32) {
+    int before = 0;
+    for (int w = lane; w < kOnePages / 32; w += 32) {
+      const int n = __popc(s_bits[w]);
+      int run = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, run, o);
+        if (lane >= o) run += v;
+      }
+      s_below[w] = before + run - n;
+      before += __shfl_sync(~0u, run, 31);
+    }
+    if (lane == 0) s_total = before;
+  }
+  __syncthreads();
+  const int total = s_total;
+  auto live = [&](int page) { return (s_bits[page >> 5] >> (page & 31)) & 1u; };
+  auto used_below = [&](int page) {
+    return s_below[page >> 5] + __popc(s_bits[page >> 5] & ((1u << (page & 31)) - 1u));
+  };
+  const int low = total < a.n_pages ? used_below(total) : total, moves = total - low;
+  for (int page = t; page < a.n_pages; page += blockDim.x) {
+    if (live(page) && page >= total) s_src[used_below(page) - low] = page;
+    if (!live(page) && page < total) s_dst[page - used_below(page)] = page;
+  }
+  __syncthreads();
+  auto renumbered = [&](int page) { return page < total ? page : s_dst[used_below(page) - low]; };
+  const int64_t first = (int64_t)blockIdx.x * blockDim.x + t, step = (int64_t)gridDim.x * blockDim.x;
+  if (first == 0) *n_live = total;
+  for (int64_t page = first; page < a.n_pages; page += step)
+    remap[page] = live((int)page) ? renumbered((int)page) : -1;
+  for (int64_t e = first; e < (int64_t)a.n_slots * a.table_stride; e += step) {
+    const int64_t s = e / a.table_stride, c = e - s * a.table_stride;
+    const int id = a.table[e];
+    new_table[e] = c * a.page_tokens < held(a, s) && id >= 0 && id < a.n_pages ? renumbered(id) : -1;
+  }
+  move_pages(a, moves, [&](int m) { return make_int2(s_src[m], s_dst[m]); });
 }
 
 int check_pages(const q4gpu_pages_args* a) {
@@ -737,6 +806,13 @@ int q4gpu_pages_compact(const q4gpu_pages_args* a, int32_t* new_table, int32_t* 
   uint32_t* bits = reinterpret_cast<uint32_t*>(ws + 16 + moves_bytes);
   int32_t* below = reinterpret_cast<int32_t*>(bits + ((size_t)a->n_pages + 31) / 32);
   cudaStream_t s = as_stream(stream);
+  // One launch where each CTA's own plan is short and nothing is read that another CTA changes: 96 small pages
+  // take 5.5 us on the device and 8.8 us a call in two launches, 5.7 us a call in one.
+  if (new_table != a->table && a->n_pages <= kOnePages && (int64_t)a->n_slots * a->table_stride <= kOneEntries) {
+    const int64_t items = (a->page_bytes + kMoveBytes - 1) / kMoveBytes * ((a->n_pages + 1) / 2);
+    pages_compact_kernel<<<(unsigned)std::min<int64_t>(148 * 4, items), 512, 0, s>>>(*a, new_table, remap, n_live);
+    return q4gpu_check_launch();
+  }
   pages_plan_kernel<<<1, kPlanThreads, 0, s>>>(*a, remap, n_live, bits, below, count, moves);
   pages_move_kernel<<<148 * 4, 512, 0, s>>>(*a, new_table, remap, count, moves);
   return q4gpu_check_launch();

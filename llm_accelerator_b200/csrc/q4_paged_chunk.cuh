@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int shift = 31 - __clz(a.page_tokens);
   const uint32_t sq = smem_addr(smem), ring = sq + 2 * kTile;
 
+  if (warp == 9) tmem_alloc(&tmem_slot, 512);
   if (threadIdx.x == 8 * 32) {
     for (int i = 0; i < kStages; ++i) bar_init(&full[i], 1), bar_init(&empty[i], tiles);
     for (int i = 0; i < 2; ++i) {
@@ -382,6 +383,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     load(&kmap, ring, id, ok, &full[0]);
   }
 
+  // is any page of these keys missing? (looked up here, needed after the queries are on their way)
+  const int64_t page0 = ((int64_t)begin >> shift) + threadIdx.x;
+  const int id0 = page0 << shift < end ? table[page0] : 0;
+  const bool missing = id0 < 0 || id0 >= a.n_pages;
   // Row r of the pair is query t0 + (rem0 + r) / group: a product with 2^20 / group, rounded
   // up, is exact for these small numbers.
   const int rem0 = tile.row0 - t0 * group;
@@ -396,10 +401,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
              (int64_t)(kvh * group + h) * a.q_head_stride + c * 8,
          there);
   }
-  // is any page of these keys missing?
-  for (int64_t p = ((int64_t)begin >> shift) + threadIdx.x; p << shift < end; p += kChunkThreads)
+  if (missing) s_bad = 1;
+  for (int64_t p = page0 + kChunkThreads; p << shift < end; p += kChunkThreads)
     if (table[p] < 0 || table[p] >= a.n_pages) s_bad = 1;
-  if (warp == 9) tmem_alloc(&tmem_slot, 512);
   cp_commit();
   cp_wait<0>();
   if (a.scale < 0.f) {  // a negative scale turns the queries' sign (each thread its own words)

@@ -160,6 +160,7 @@ class RopeAppend(_Err):
             _on(t, self.device, name, torch.float32)
             _need(t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape, f"{name} must be [positions, rot / 2]")
         self.cos, self.sin, self.q_gamma, self.k_gamma = cos, sin, q_gamma, k_gamma
+        self.layout = None
         self._new_err()
         a = self.args = _native.RopeArgs(cos=cos.data_ptr(), sin=sin.data_ptr(), table_positions=cos.shape[0],
                                          rot_dim=2 * cos.shape[1], interleaved=int(interleaved), eps=eps,
@@ -180,6 +181,22 @@ class RopeAppend(_Err):
         positions int32 [tokens]; rows int64 [tokens], the cache row of each token
         (page * page_tokens + offset, negative: not stored); k_cache / v_cache
         [pages, kv_heads, page_tokens, dim].  Returns q_out (default: q in place)."""
+        layout = None
+        if q is not None and k is not None and v is not None and q_out is not None:
+            # what the checks below look at: tensors laid out like the last call's need only their addresses
+            layout = (q.shape, q.stride(), q.dtype, q.device, q_out.shape, q_out.stride(), q_out.dtype, q_out.device,
+                      k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+                      positions.shape, positions.stride(), positions.dtype, positions.device,
+                      rows.shape, rows.stride(), rows.dtype, rows.device,
+                      k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+                      v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device)
+            if layout == self.layout:
+                a = self.args
+                a.q, a.q_out, a.k, a.v = q.data_ptr(), q_out.data_ptr(), k.data_ptr(), v.data_ptr()
+                a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+                a.positions, a.rows = positions.data_ptr(), rows.data_ptr()
+                return self._launch(q_out)
+        self.layout = None
         ref = q if q is not None else k if k is not None else v
         _need(ref is not None, "one of q, k, v is needed")
         tokens, _, dim = ref.shape
@@ -228,7 +245,11 @@ class RopeAppend(_Err):
                 a.v_cache = v_cache.data_ptr()
             a.page_stride, a.head_stride, a.row_stride, _ = strides
             a.page_tokens, a.n_rows = shape[2], shape[0] * shape[2]
-        rc = self.lib.q4gpu_rope_append(a, _stream(self.device.index))
+        self.layout = layout
+        return self._launch(q_out)
+
+    def _launch(self, q_out: Optional[torch.Tensor]):
+        rc = self.lib.q4gpu_rope_append(self.args, _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_rope_append")
         return q_out
