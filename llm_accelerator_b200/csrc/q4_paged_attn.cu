@@ -79,13 +79,14 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 // order of the pieces.
 constexpr int kUnitKeys = kRowWarps * kTileKeys;
 constexpr int kPieceCost = 4;
+constexpr int kMostCtas = 1024;   // counters, always at the workspace's start: no other call's data gets there
 constexpr int kLeastStretch = 12;  // units: shorter pieces cost more to join than they save
 
 struct RowPlan {
   int ctas;
   float* o;       // [cta][2][kRows][D] unnormalised sums: of a piece begun earlier, of one that goes on
   float2* ml;     // [cta][2][kRows] their running maximum (log2 units) and sum
-  int32_t* done;  // [sequence * kv_heads + head] finished pieces
+  int32_t* done;  // [cta] finished pieces of the item whose first piece goes on from this CTA
 };
 
 // Keys that the kernel below walks for sequence i, from `lo` on; -1: not its
@@ -340,7 +341,6 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
               *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
                   make_float2(o[n][2 * h], o[n][2 * h + 1]);
         __syncthreads();
-        const int64_t item = (int64_t)seq * a.kv_heads + kvh;
         auto put = [&](int r, int d, float m_all, float l_all, float v) {
           const int t = r / group, head = kvh * group + r - t * group;
           static_cast<T*>(a.out)[(int64_t)(s.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride + d] =
@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           __threadfence();
           __syncthreads();
           if (threadIdx.x == 0) {
-            s_last = atomicAdd(plan.done + item, 1) == parts - 1;
-            if (s_last) plan.done[item] = 0;
+            s_last = atomicAdd(plan.done + cta0, 1) == parts - 1;
+            if (s_last) plan.done[cta0] = 0;
           }
           __syncthreads();
           if (s_last) __threadfence();
@@ -455,7 +455,8 @@ RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
   const int64_t units = (a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
   const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + kLeastStretch - 1) / kLeastStretch + 1);
   p.ctas = (int)std::min<int64_t>(most, kSms * (a.dim == 64 ? 4 : 2));
-  const size_t done = (items * 4 + 15) / 16 * 16, rows = (size_t)p.ctas * 2 * kRows;
+  static_assert(kSms * 4 <= kMostCtas, "a counter a CTA");
+  const size_t done = kMostCtas * sizeof(int32_t), rows = (size_t)p.ctas * 2 * kRows;
   if (bytes) *bytes = done + rows * (8 + (size_t)a.dim * 4);
   p.done = reinterpret_cast<int32_t*>(ws);
   p.ml = reinterpret_cast<float2*>(ws + done);

@@ -354,6 +354,37 @@ def test_attention_unseen_rows_do_not_reach_results(new, old, what):
     assert torch.equal(attend(*args, window=20)[0], want)
 
 
+@pytest.mark.parametrize("hq,hk,dim,page", [(32, 1, 128, 64), (17, 1, 64, 16), (40, 2, 64, 32), (48, 1, 128, 128)])
+def test_attention_many_heads_a_key_head(hq, hk, dim, page):
+    check_attn(*make([1, 2, 40, 0, 1], [0, 700, 100, 5, 64], hq, hk, dim, page, HF, 14))
+
+
+@pytest.mark.parametrize("most", [1, 3, 40])
+def test_attention_many_sequences(most):
+    g = torch.Generator().manual_seed(most)
+    new = torch.randint(0 if most > 1 else 1, most + 1, (300,), generator=g).tolist()
+    old = torch.randint(0, 90, (300,), generator=g).tolist()
+    old[7], old[250] = 1500, 900
+    check_attn(*make(new, old, 4, 2, 64, 16, BF, 15))
+
+
+def test_attention_workspace_serves_calls_of_all_shapes():
+    """One operator, one workspace: splits, joins and chunks of different batches one after the other."""
+    pool, table, lens, cu, q = make([1] * 40 + [70, 130], [3000] * 3 + [200] * 39, 8, 4, 128, 64, BF, 16)
+    op = paged.Attention(pool[:, 0], pool[:, 1], table, lens, q_heads=8)
+    batches = [[0], list(range(40)), [40], [0, 1, 2], list(range(42)), [2], list(range(3, 40)), [1, 41], [0]]
+    first = cu.tolist()
+    for _ in range(2):
+        for ids in batches:
+            rows = torch.cat([torch.arange(first[i], first[i + 1], device="cuda") for i in ids])
+            new = [first[i + 1] - first[i] for i in ids]
+            c = i32([0] + torch.tensor(new).cumsum(0).tolist())
+            got = op(q[rows], None, c, max_q=max(new), max_ctx=3200, seq_ids=i32(ids))
+            ref, mag, _ = attn_ref(pool, table, lens, c, q[rows], 128 ** -0.5, 0, ids)
+            within(got, ref, U[BF] * ref.abs() + (U[BF] + 3e-4) * mag)
+    op.check()
+
+
 def test_attention_extreme_scores():
     """Scores of +-1e4: weights are 0 or 1, nothing overflows."""
     pool, table, lens, cu, q = make([1, 150], [300, 200], 4, 2, 64, 64, BF, 8)
