@@ -35,7 +35,7 @@ __device__ __forceinline__ Seq sequence(const q4gpu_attn_args& a, int i) {
 // ---------------------------------------------------------------------------
 constexpr int kRows = 16;        // rows of one mma.sync tile
 constexpr int kTileKeys = 16;    // keys of a warp's step; a page holds whole steps
-constexpr int kRowWarps = 4;
+constexpr int kRowWarps = 8;
 constexpr int kRowStages = 3;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -72,15 +72,16 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Work is laid out on one axis: sequence by sequence, key head by key head, in
-// units of 64 keys, each (sequence, head) behind kPieceCost units that stand for
-// what starting it costs.  Every CTA takes an equal stretch of that axis, so the
+// units of 128 keys, each (sequence, head) behind kPieceCost units that stand for
+// what starting it costs (64 decodes at 1 to 8704 keys: 59.3 us with 2, 56.7 with
+// 3, 60.2 with 4).  Every CTA takes an equal stretch of that axis, so the
 // longest sequence does not decide; a stretch's ends cut at most two (sequence,
 // head) items, whose pieces are joined by the CTA that finishes last, in the
 // order of the pieces.
 constexpr int kUnitKeys = kRowWarps * kTileKeys;
-constexpr int kPieceCost = 4;
+constexpr int kPieceCost = 3;
 constexpr int kMostCtas = 1024;   // counters, always at the workspace's start: no other call's data gets there
-constexpr int kLeastStretch = 12;  // units: shorter pieces cost more to join than they save
+constexpr int kLeastStretch = 6;  // units: shorter pieces cost more to join than they save
 
 struct RowPlan {
   int ctas;
@@ -104,9 +105,12 @@ __device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int gro
 }
 
 // Each warp runs over its own 16-key steps of a piece with its own running
-// maximum and sum, so no barrier stands in the loop; the four are joined at its
-// end.  Bound by memory: every key and value is read once, for all heads of its
-// group.
+// maximum and sum, so no barrier stands in the loop; the eight are joined at its
+// end.  (Eight warps and one CTA per SM for heads of 128, two for 64; four warps
+// and twice the CTAs start short pieces a little faster, 64 decodes at 1 to 8704
+// keys 55.6 us against 56.8, but take 33.0 against 24.0 for one at 16384 and 122
+// against 94 for 16 of 64-value heads.)  Bound by memory: every key and value is
+// read once, for all heads of its group; 16 decodes at 16384 keys stream 6.1 TB/s.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, RowPlan plan) {
   constexpr int kThreads = kRowWarps * 32;
@@ -454,7 +458,7 @@ RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
   // no CTA without at least one (sequence, head) or kLeastStretch units of one
   const int64_t units = (a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
   const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + kLeastStretch - 1) / kLeastStretch + 1);
-  p.ctas = (int)std::min<int64_t>(most, kSms * (a.dim == 64 ? 4 : 2));
+  p.ctas = (int)std::min<int64_t>(most, kSms * (a.dim == 64 ? 2 : 1));
   static_assert(kSms * 4 <= kMostCtas, "a counter a CTA");
   const size_t done = kMostCtas * sizeof(int32_t), rows = (size_t)p.ctas * 2 * kRows;
   if (bytes) *bytes = done + rows * (8 + (size_t)a.dim * 4);

@@ -48,6 +48,8 @@ def _need(ok: bool, what: str) -> None:
 
 def _on(t: torch.Tensor, device: torch.device, name: str, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """`t`, if it is a CUDA tensor of this device (and type)."""
+    if t is None:
+        raise ValueError(f"{name} is needed")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     if dtype is not None and t.dtype != dtype:
@@ -182,7 +184,7 @@ class RopeAppend(_Err):
         (page * page_tokens + offset, negative: not stored); k_cache / v_cache
         [pages, kv_heads, page_tokens, dim].  Returns q_out (default: q in place)."""
         layout = None
-        if q is not None and k is not None and v is not None and q_out is not None:
+        if not any(t is None for t in (q, k, v, q_out, positions, rows, k_cache, v_cache)):
             # what the checks below look at: tensors laid out like the last call's need only their addresses
             layout = (q.shape, q.stride(), q.dtype, q.device, q_out.shape, q_out.stride(), q_out.dtype, q_out.device,
                       k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
@@ -288,7 +290,7 @@ class Attention(_Err):
         pages, kv_heads, page_tokens, dim = k_cache.shape
         self.q_heads, self.dim, self.slots = q_heads, dim, table.shape[0]
         self.k_cache, self.v_cache, self.table, self.lens = k_cache, v_cache, table, lens
-        self.workspace = None
+        self.workspace = self.layout = None
         self._new_err()
         # a row of the table is as long as its stride lets it name
         self.args = _native.AttnArgs(
@@ -306,11 +308,25 @@ class Attention(_Err):
         tokens cu_q[i] .. cu_q[i + 1] - 1, at most max_q; seq_ids int32 [sequences]: their
         slots (default: 0, 1, ..); max_ctx: no lens is larger (0: the table's width).
         lse (optional) float32 [tokens, q_heads] receives log sum exp of the scores."""
-        a, tokens = self.args, q.shape[0]
+        a = self.args
         if cu_q is None:
             raise ValueError("cu_q is needed")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        # what the checks below look at: tensors laid out like the last call's need only their addresses
+        layout = (q.shape, q.stride(), q.dtype, q.device, out.shape, out.stride(), out.dtype, out.device, cu_q.shape,
+                  cu_q.stride(), cu_q.dtype, cu_q.device, max_q, max_ctx,
+                  None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device),
+                  None if seq_ids is None else (seq_ids.shape, seq_ids.stride(), seq_ids.dtype, seq_ids.device))
+        if layout == self.layout:
+            a.q, a.out, a.cu_q = q.data_ptr(), out.data_ptr(), cu_q.data_ptr()
+            if lse is not None:
+                a.lse = lse.data_ptr()
+            if seq_ids is not None:
+                a.seq_ids = seq_ids.data_ptr()
+            return self._launch(out)
+        self.layout = None
+        tokens = q.shape[0]
         a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, "q")
         a.out, a.out_token_stride, a.out_head_stride = self._heads(out, tokens, "out")
         if cu_q.dtype != torch.int32 or cu_q.device != self.device or cu_q.dim() != 1 or cu_q.shape[0] < 1 or \
@@ -336,7 +352,11 @@ class Attention(_Err):
             # the old one stays alive until the work queued on this stream is done with it
             self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
             a.workspace, a.workspace_bytes = self.workspace.data_ptr(), need
-        rc = self.lib.q4gpu_paged_attention(a, _stream(self.device.index))
+        self.layout = layout
+        return self._launch(out)
+
+    def _launch(self, out: torch.Tensor) -> torch.Tensor:
+        rc = self.lib.q4gpu_paged_attention(self.args, _stream(self.device.index))
         if rc:
             _native.check(rc, "q4gpu_paged_attention")
         return out

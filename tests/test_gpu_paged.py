@@ -592,7 +592,8 @@ def test_refusals():
     for bad in (lambda: op(q.float(), None, None, pos, None, None, None),
                 lambda: op(q, None, None, pos.long(), None, None, None),
                 lambda: op(q, q, q, pos, rows.int(), kc, kc), lambda: op(q, q, q, pos, rows, kc, kc[:, :2]),
-                lambda: op(None, None, None, pos, rows, kc, kc),
+                lambda: op(None, None, None, pos, rows, kc, kc), lambda: op(q, q, q, None, rows, kc, kc, q),
+                lambda: op(q, q, q, pos, None, kc, kc, q), lambda: op(q, q, q, pos, rows, kc, None, q),
                 lambda: paged.RopeAppend(cos, sin, q_gamma=w.float())(q, None, None, pos, None, None, None)):
         with pytest.raises(ValueError):
             bad()
