@@ -71,6 +71,7 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+
 // Work is laid out on one axis: sequence by sequence, key head by key head, in
 // units of 128 keys, each (sequence, head) behind kPieceCost units that stand for
 // what starting it costs (64 decodes at 1 to 8704 keys: 59.3 us with 2, 56.7 with
