@@ -477,7 +477,7 @@ RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
 ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
   ChunkPlan p{};
   const int64_t group = a.q_heads / a.kv_heads;
-  if (a.max_q * group <= kRows) {
+  if (a.max_q * group <= kRows || a.n_seqs == 0 || a.tokens == 0) {  // nothing for the chunk kernel
     if (bytes) *bytes = 0;
     return p;
   }
