@@ -524,7 +524,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t ts = tmem + lanes + kSCol + t * 2 * kStep, to = tmem + lanes + kOCol + t * D;
     const bool mine = r < rows;
     const int pos = mine ? len - n + (tile.row0 + r) / group : -1;
-    const float c2 = fabsf(a.scale) * 1.4426950408889634f;
+    // (not 0: masked scores are -infinity before the factor; with the least number above 0 the exponents of finite
+    // scores still vanish, and the weights are equal as a scale of 0 asks)
+    const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
     const uint64_t c22 = pair_of(c2, c2);
     float m = -INFINITY, sum = 0.f;
     bool live = true;

@@ -48,3 +48,21 @@ def test_attention_of_an_empty_step(hq, hk, max_q):
     assert op(q[:0], None, i32([0, 0]), max_q=max_q).shape == (0, hq, 64)
     assert op(q[:0], None, i32([0]), max_q=max_q).shape == (0, hq, 64)
     check(op, pool, table, lens, cu, q, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,old", [([1, 2], [300, 0]), ([200], [300]), ([3, 40, 300, 1], [500, 0, 20, 70]),
+                                     ([70], [4000])])
+@pytest.mark.parametrize("window", [0, 70])
+def test_attention_scale_zero_is_the_mean(dtype, dim, new, old, window):
+    args = make(new, old, 4, 2, dim, 32, dtype, 21)
+    for scale in (0.0, -0.0, 1e-44):
+        check(operator(*args[:3], 4, scale=scale, window=window), *args, scale, window)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,old", [([1, 2], [300, 0]), ([3, 40, 300, 1], [500, 0, 20, 70])])
+def test_attention_negative_scale(dim, new, old):
+    args = make(new, old, 4, 2, dim, 32, BF, 22)
+    check(operator(*args[:3], 4, scale=-dim ** -0.5), *args, -dim ** -0.5)
