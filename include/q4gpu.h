@@ -272,6 +272,10 @@ int q4gpu_rope_append(const q4gpu_rope_args *a, void *stream);
  * out [tokens, q_heads, dim]; lse (optional) float32 [tokens, q_heads]
  * contiguous.  A query that sees no key (p < 0, or pages whose table entry is
  * outside 0 .. n_pages - 1, which hold no keys) gets zeros and -infinity.
+ * *err_flag (optional) becomes 1 where a page of a seen key, the slot of a
+ * sequence with queries (it holds no keys then), its lens (cut off at what its
+ * row of the table can name) or cu_q (cut off at 0 .. tokens) is out of range,
+ * and where a sequence has more than max_q queries.
  * What stands in a key or value row that a query does not see does not reach
  * its result.  dim is 64 or 128; F16 or BF16; query and cache head vectors
  * start on 16-byte boundaries.

@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   int64_t mine_cost = 0;
   int most = 0;
   for (int i = run0; i < run1; ++i) {
+    if (blockIdx.x == 0 && a.err_flag && !sequence_ok(a, i)) *a.err_flag = 1;
     const int c = row_cost(a, i, group);
     mine_cost += (int64_t)c * a.kv_heads;
     most = max(most, c);
@@ -207,7 +208,9 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         auto page_of = [&](int i) {
           if (i >= mine) return -1;
           const int p = table[(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
-          return p < a.n_pages ? p : -1;
+          if (p >= 0 && p < a.n_pages) return p;
+          if (a.err_flag) *a.err_flag = 1;
+          return -1;
         };
         int next_page = page_of(0);
         uint32_t valid = 0;  // bit i % 32: step i's page exists

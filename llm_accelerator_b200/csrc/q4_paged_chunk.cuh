@@ -33,6 +33,16 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
   return max(kMinPart, ((keys + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
 }
 
+// Whether what only the device sees of sequence i is in range: its query tokens, and if it has any its slot and that
+// slot's length.  (What is not is cut off or taken as empty; one kernel of a call reports it.)
+__device__ __forceinline__ bool sequence_ok(const q4gpu_attn_args& a, int i) {
+  const int c0 = a.cu_q[i], c1 = a.cu_q[i + 1];
+  if (c0 < 0 || c1 < c0 || c1 > a.tokens || c1 - c0 > a.max_q) return false;
+  if (c0 == c1) return true;
+  const int s = a.seq_ids ? a.seq_ids[i] : i;
+  return s >= 0 && s < a.n_slots && a.lens[s] >= 0 && a.lens[s] <= a.table_stride * a.page_tokens;
+}
+
 // Sequence and row pair of one grid index, and what its CTA needs to know of the
 // sequence: first query token, query tokens, cache slot, stored keys.
 struct ChunkTile {
@@ -327,6 +337,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const ChunkTile t = find_tile(a, plan.least, blockIdx.y);
     if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
   }
+  if (waits && warp == 11 && plan.least == 1 && a.err_flag)  // no other kernel in this call looks at the sequences
+    for (int i = lane; i < a.n_seqs; i += 32)
+      if (!sequence_ok(a, i)) *a.err_flag = 1;
   __syncthreads();
   const ChunkTile tile = s_tile;
   if (tile.seq < 0) return wait_before();
@@ -387,8 +400,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     load(&kmap, ring, id, ok, &full[0]);
   }
 
-  // is any page of these keys missing? (looked up here, needed after the queries are on their way)
-  const int64_t page0 = ((int64_t)begin >> shift) + threadIdx.x;
+  // is any page of the seen keys missing? (looked up here, needed after the queries are on their way; `begin` may lie
+  // before the first seen key, whose pages a window has left behind may be gone)
+  const int64_t page0 = ((int64_t)max(begin, lo) >> shift) + threadIdx.x;
   const int id0 = page0 << shift < end ? table[page0] : 0;
   const bool missing = id0 < 0 || id0 >= a.n_pages;
   // Row r of the pair is query t0 + (rem0 + r) / group: a product with 2^20 / group, rounded
@@ -405,9 +419,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
              (int64_t)(kvh * group + h) * a.q_head_stride + c * 8,
          there);
   }
-  if (missing) s_bad = 1;
+  auto gone = [&] {
+    s_bad = 1;
+    if (a.err_flag) *a.err_flag = 1;
+  };
+  if (missing) gone();
   for (int64_t p = page0 + kChunkThreads; p << shift < end; p += kChunkThreads)
-    if (table[p] < 0 || table[p] >= a.n_pages) s_bad = 1;
+    if (table[p] < 0 || table[p] >= a.n_pages) gone();
   cp_commit();
   cp_wait<0>();
   if (a.scale < 0.f) {  // a negative scale turns the queries' sign (each thread its own words)

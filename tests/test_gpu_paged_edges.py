@@ -66,3 +66,64 @@ def test_attention_scale_zero_is_the_mean(dtype, dim, new, old, window):
 def test_attention_negative_scale(dim, new, old):
     args = make(new, old, 4, 2, dim, 32, BF, 22)
     check(operator(*args[:3], 4, scale=-dim ** -0.5), *args, -dim ** -0.5)
+
+
+def reported(op):
+    try:
+        op.check()
+    except _native.Q4GpuError as e:
+        assert "out of range" in str(e)
+        return True
+    return False
+
+
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_attention_reports_what_is_out_of_range(new):
+    pool, table, lens, cu, q = make([new] * 4, [130, 100, 0, 200], 4, 2, 64, 32, BF, 23)
+    op = operator(pool, table, lens, 4)
+    room = table.shape[1] * 32
+
+    def run(ids=None, c=cu):
+        out = op(q, torch.zeros_like(q), c, max_q=new, max_ctx=512, seq_ids=ids)
+        return out, reported(op)
+
+    def rest(out, rows):  # the other sequences (whose work may be split in other places) keep their results
+        within(out[rows], ref[rows], U[BF] * ref[rows].abs() + (U[BF] + 3e-4) * mag[rows])
+
+    ref, mag, _ = attn_ref(pool, table, lens, cu, q, 64 ** -0.5)
+    good, said = run()
+    assert not said
+    for bad in (-1, 4, 2 ** 31 - 1, -2 ** 31):
+        out, said = run(i32([0, bad, 2, 3]))
+        assert said and not out[new:2 * new].any()
+        rest(out, slice(2 * new, None))
+    for s, n in ((1, room + 1), (0, -1), (3, 2 ** 31 - 1)):
+        kept = int(lens[s])
+        lens[s] = n
+        assert run()[1]
+        lens[s] = kept
+    for page in (pool.shape[0], -1, 2 ** 31 - 1):
+        kept = int(table[3, 1])
+        table[3, 1] = page
+        out, said = run()
+        assert said
+        rest(out, slice(0, 3 * new))
+        table[3, 1] = kept
+    for c in ([0, new, 2 * new, 3 * new, 4 * new + 1], [-1, new, 2 * new, 3 * new, 4 * new],
+              [0, new, new - 1, 3 * new, 4 * new]):
+        assert run(c=i32(c))[1]
+    out, said = run()
+    assert not said and torch.equal(out, good)
+
+
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_attention_does_not_report_what_nothing_reads(new):
+    """Sequences without queries may name any slot (padding); pages before every query's window may be gone."""
+    pool, table, lens, cu, q = make([new] * 2, [700, 300], 4, 2, 64, 32, BF, 24)
+    op = operator(pool, table, lens, 4, window=100)
+    want = op(q, None, cu, max_q=new)
+    assert not reported(op)
+    table[0, :(700 - 100 + 1) // 32] = -1  # the first query sees the keys from 601 on
+    assert torch.equal(op(q, None, cu, max_q=new), want) and not reported(op)
+    padded = torch.cat((cu, cu[-1:], cu[-1:]))
+    assert torch.equal(op(q, None, padded, max_q=new, seq_ids=i32([0, 1, -1, 99])), want) and not reported(op)
