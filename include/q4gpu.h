@@ -275,7 +275,8 @@ int q4gpu_rope_append(const q4gpu_rope_args *a, void *stream);
  * *err_flag (optional) becomes 1 where a page of a seen key, the slot of a
  * sequence with queries (it holds no keys then), its lens (cut off at what its
  * row of the table can name) or cu_q (cut off at 0 .. tokens) is out of range,
- * and where a sequence has more than max_q queries.
+ * and where a sequence has more than max_q queries (its rows are then complete
+ * or zeros and -infinity).
  * What stands in a key or value row that a query does not see does not reach
  * its result.  dim is 64 or 128; F16 or BF16; query and cache head vectors
  * start on 16-byte boundaries.

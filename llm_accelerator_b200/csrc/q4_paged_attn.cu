@@ -127,7 +127,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   const int run0 = min(a.n_seqs, (int)threadIdx.x * per), run1 = min(a.n_seqs, run0 + per);
   int64_t mine_cost = 0;
   int most = 0;
+  // without a chunk kernel beside this one nobody computes a sequence longer than max_q and a tile: its rows become zeros
+  const bool alone = (int64_t)a.max_q * group <= kRows;
+  bool over = false;
   for (int i = run0; i < run1; ++i) {
+    over |= alone && sequence(a, i).n > kRows / group;
     if (blockIdx.x == 0 && a.err_flag && !sequence_ok(a, i)) *a.err_flag = 1;
     const int c = row_cost(a, i, group);
     mine_cost += (int64_t)c * a.kv_heads;
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   most = __reduce_max_sync(~0u, most);
   if (lane == 31) s_sum[warp] = upto;
   if (lane == 0) s_most[warp] = most;
-  __syncthreads();
+  over = __syncthreads_or(over);
   int64_t total = 0, before = upto - mine_cost;
 #pragma unroll
   for (int w = 0; w < kRowWarps; ++w) {
@@ -418,6 +422,16 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
       }
     }
   }
+  if (over)
+    for (int i = blockIdx.x; i < a.n_seqs; i += gridDim.x) {
+      const Seq s = sequence(a, i);
+      if (s.n <= kRows / group) continue;
+      for (int64_t x = threadIdx.x; x < (int64_t)s.n * a.q_heads * D; x += kThreads) {
+        const int64_t row = x / D, t = s.first + row / a.q_heads, head = row % a.q_heads;
+        static_cast<T*>(a.out)[t * a.out_token_stride + head * a.out_head_stride + x % D] = from_f32<T>(0.f);
+        if (a.lse && x % D == 0) a.lse[t * a.q_heads + head] = -INFINITY;
+      }
+    }
 }
 
 int check_sizes(const q4gpu_attn_args* a) {
@@ -532,7 +546,6 @@ int allow_smem(const void* kernel, int bytes, unsigned char* ready) {
 
 template <typename T, int D>
 int launch(const q4gpu_attn_args& a, cudaStream_t s) {
-  if (a.max_q == 0) return Q4GPU_OK;
   static unsigned char ready[2][Q4GPU_MAX_DEVICES];
   size_t rows_bytes;
   const RowPlan few = row_plan(a, static_cast<char*>(a.workspace), &rows_bytes);

@@ -127,3 +127,24 @@ def test_attention_does_not_report_what_nothing_reads(new):
     assert torch.equal(op(q, None, cu, max_q=new), want) and not reported(op)
     padded = torch.cat((cu, cu[-1:], cu[-1:]))
     assert torch.equal(op(q, None, padded, max_q=new, seq_ids=i32([0, 1, -1, 99])), want) and not reported(op)
+
+
+@pytest.mark.parametrize("hq,hk,max_q", [(4, 2, 1), (4, 2, 8), (7, 1, 2), (16, 1, 1), (32, 1, 0), (4, 2, 0)])
+def test_attention_of_a_sequence_longer_than_max_q(hq, hk, max_q):
+    """A sequence with more queries than promised is reported and its rows are zeros or complete, never left over."""
+    new = [1, 40, max_q, 0, 300]
+    args = make(new, [30, 200, 500, 10, 0], hq, hk, 64, 32, BF, 25)
+    pool, table, lens, cu, q = args
+    op = operator(pool, table, lens, hq)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    op(q, out, cu, max_q=max_q, lse=lse)
+    assert reported(op)
+    ref, mag, rl = attn_ref(pool, table, lens, cu, q, 64 ** -0.5)
+    for i, n in enumerate(new):
+        rows = slice(int(cu[i]), int(cu[i + 1]))
+        if n > max_q and not out[rows].any():
+            assert (lse[rows] == -math.inf).all()
+        else:
+            close(out[rows], lse[rows], ref[rows], mag[rows], rl[rows], BF)
+    check(op, *args, 64 ** -0.5)  # and the next call is as ever
+    assert not reported(op)
