@@ -240,7 +240,8 @@ int q4gpu_add_rmsnorm(const q4gpu_norm_args *a, void *stream);
  * Rotated queries go to q_out (may be q); rotated keys and unchanged values
  * go to cache row rows[token] = page * page_tokens + offset, at
  *   cache + page * page_stride + head * head_stride + offset * row_stride;
- * a negative row stores nothing.  q, k or v may be NULL (with its outputs).
+ * a negative row stores nothing, and nothing is written of a token whose
+ * position has no table row.  q, k or v may be NULL (with its outputs).
  * rot_dim is a multiple of 16, dim a multiple of 8 up to 512; every head
  * vector starts on a 16-byte boundary. */
 typedef struct q4gpu_rope_args {

@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4)
       head -= nq + (is_k ? 0 : nk);
       dst = static_cast<T*>(is_k ? a.k_cache : a.v_cache) + cache + head * a.head_stride;
     }
-    if (slot + i * slots >= heads || (!is_q && !stored) || ((is_q || is_k) && !known)) continue;
+    if (slot + i * slots >= heads || (!is_q && !stored) || !known) continue;  // (values alone: always known)
     if ((is_q || is_k) && u < turned) {
 #pragma unroll
       for (int p = 0; p < 8; ++p) {

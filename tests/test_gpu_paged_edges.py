@@ -148,3 +148,21 @@ def test_attention_of_a_sequence_longer_than_max_q(hq, hk, max_q):
             close(out[rows], lse[rows], ref[rows], mag[rows], rl[rows], BF)
     check(op, *args, 64 ** -0.5)  # and the next call is as ever
     assert not reported(op)
+
+
+def test_rope_stores_nothing_of_a_token_without_a_position():
+    cos, sin = angles(64, 128)
+    k, v = rnd((4, 2, 128), BF, 1), rnd((4, 2, 128), BF, 2)
+    rows = torch.tensor([3, 2, 1, 0], device="cuda")
+    for bad in (-1, 64, 2 ** 31 - 1):
+        op = paged.RopeAppend(cos, sin)
+        kc, vc = (torch.full((1, 2, 16, 128), 3.0, dtype=BF, device="cuda") for _ in range(2))
+        op(None, k, v, i32([0, bad, 5, 63]), rows, kc, vc)
+        with pytest.raises(_native.Q4GpuError):
+            op.check()
+        assert (kc[0, :, 2] == 3).all() and (vc[0, :, 2] == 3).all()
+        assert torch.equal(vc[0][:, [3, 1, 0]].transpose(0, 1), v[[0, 2, 3]])
+    op = paged.RopeAppend(cos, sin)
+    op(None, None, v, None, rows, None, vc)  # values alone have no position
+    op.check()
+    assert torch.equal(vc[0][:, rows].transpose(0, 1), v)
