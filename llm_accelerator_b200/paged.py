@@ -13,9 +13,10 @@ K/V cache, and what happens to the cache's pages between steps.
 Each operator is an object that holds what a serving loop keeps (weights,
 tables, cache, workspace) and is called with the step's tensors.  Calls
 enqueue on torch's current stream and do not synchronise; a workspace belongs
-to its object, so one object's calls run on one stream at a time.  Nothing has
-a reference counterpart (the reference decodes one token at a time in fixed
-point with a flat cache of 256 positions,
+to its object, so one object's calls run on one stream at a time.  Threads may
+share an object: a lock keeps the arguments of a call together until the library
+has taken them.  Nothing has a reference counterpart (the reference decodes one
+token at a time in fixed point with a flat cache of 256 positions,
 ``FPGA_Project/software/qmap_one_token_runtime/qmap_one_token_runtime.h:369-500``).
 Wrong arguments raise ``ValueError`` here or ``_native.Q4GpuError`` from the
 library, both before any device work; there is no CPU fallback.
@@ -23,6 +24,7 @@ library, both before any device work; there is no CPU fallback.
 from __future__ import annotations
 
 import heapq
+import threading
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -80,6 +82,7 @@ class AddRmsNorm:
         _need(weight.dim() == 1 and weight.is_contiguous(), "weight must be a contiguous vector")
         _need(weight.dtype in (torch.float32, torch.float16, torch.bfloat16), f"weight is {weight.dtype}")
         self.weight, self.n, self.dtype = weight, weight.shape[0], weight.dtype
+        self.lock = threading.Lock()
         self.out_dtype = out_dtype or weight.dtype
         _need(self.out_dtype in _DTYPES, f"unsupported output type {self.out_dtype}")
         self.narrow = self.out_dtype in (torch.float8_e4m3fn, torch.int8)
@@ -100,34 +103,35 @@ class AddRmsNorm:
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                  residual_out: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None):
         """x, residual, residual_out, out: [rows, n]; returns out, or (out, scale) for 8 bits."""
-        a, dtype = self.args, self.dtype
-        if x.dim() != 2:
-            raise ValueError("x must be [rows, n]")
-        a.rows = rows = len(x)
-        a.x_stride = self._rows(x, rows, "x", dtype)
-        a.x = x.data_ptr()
-        if out is None:
-            out = torch.empty(rows, self.n, dtype=self.out_dtype, device=self.device)
-        a.out_stride = self._rows(out, rows, "out", self.out_dtype)
-        a.out = out.data_ptr()
-        a.residual = a.residual_out = a.scale = None
-        if residual is not None:
-            a.residual_stride = self._rows(residual, rows, "residual", dtype)
-            a.residual = residual.data_ptr()
-        if residual_out is not None:
-            a.residual_out_stride = self._rows(residual_out, rows, "residual_out", dtype)
-            a.residual_out = residual_out.data_ptr()
-        if self.narrow:
-            if scale is None:
-                scale = torch.empty(rows, self.groups, dtype=torch.float32, device=self.device)
-            _on(scale, self.device, "scale", torch.float32)
-            _need(scale.shape == (rows, self.groups) and scale.is_contiguous(),
-                  f"scale must be contiguous [{rows}, {self.groups}]")
-            a.scale = scale.data_ptr()
-        rc = self.lib.q4gpu_add_rmsnorm(a, _stream(self.device.index))
-        if rc:
-            _native.check(rc, "q4gpu_add_rmsnorm")
-        return (out, scale) if self.narrow else out
+        with self.lock:
+            a, dtype = self.args, self.dtype
+            if x.dim() != 2:
+                raise ValueError("x must be [rows, n]")
+            a.rows = rows = len(x)
+            a.x_stride = self._rows(x, rows, "x", dtype)
+            a.x = x.data_ptr()
+            if out is None:
+                out = torch.empty(rows, self.n, dtype=self.out_dtype, device=self.device)
+            a.out_stride = self._rows(out, rows, "out", self.out_dtype)
+            a.out = out.data_ptr()
+            a.residual = a.residual_out = a.scale = None
+            if residual is not None:
+                a.residual_stride = self._rows(residual, rows, "residual", dtype)
+                a.residual = residual.data_ptr()
+            if residual_out is not None:
+                a.residual_out_stride = self._rows(residual_out, rows, "residual_out", dtype)
+                a.residual_out = residual_out.data_ptr()
+            if self.narrow:
+                if scale is None:
+                    scale = torch.empty(rows, self.groups, dtype=torch.float32, device=self.device)
+                _on(scale, self.device, "scale", torch.float32)
+                _need(scale.shape == (rows, self.groups) and scale.is_contiguous(),
+                      f"scale must be contiguous [{rows}, {self.groups}]")
+                a.scale = scale.data_ptr()
+            rc = self.lib.q4gpu_add_rmsnorm(a, _stream(self.device.index))
+            if rc:
+                _native.check(rc, "q4gpu_add_rmsnorm")
+            return (out, scale) if self.narrow else out
 
 
 class _Err:
@@ -162,7 +166,7 @@ class RopeAppend(_Err):
             _on(t, self.device, name, torch.float32)
             _need(t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape, f"{name} must be [positions, rot / 2]")
         self.cos, self.sin, self.q_gamma, self.k_gamma = cos, sin, q_gamma, k_gamma
-        self.layout = None
+        self.layout, self.lock = None, threading.Lock()
         self._new_err()
         a = self.args = _native.RopeArgs(cos=cos.data_ptr(), sin=sin.data_ptr(), table_positions=cos.shape[0],
                                          rot_dim=2 * cos.shape[1], interleaved=int(interleaved), eps=eps,
@@ -183,72 +187,74 @@ class RopeAppend(_Err):
         positions int32 [tokens]; rows int64 [tokens], the cache row of each token
         (page * page_tokens + offset, negative: not stored); k_cache / v_cache
         [pages, kv_heads, page_tokens, dim].  Returns q_out (default: q in place)."""
-        layout = None
-        if not any(t is None for t in (q, k, v, q_out, positions, rows, k_cache, v_cache)):
-            # what the checks below look at: tensors laid out like the last call's need only their addresses
-            layout = (q.shape, q.stride(), q.dtype, q.device, q_out.shape, q_out.stride(), q_out.dtype, q_out.device,
-                      k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
-                      positions.shape, positions.stride(), positions.dtype, positions.device,
-                      rows.shape, rows.stride(), rows.dtype, rows.device,
-                      k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
-                      v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device)
-            if layout == self.layout:
-                a = self.args
-                a.q, a.q_out, a.k, a.v = q.data_ptr(), q_out.data_ptr(), k.data_ptr(), v.data_ptr()
-                a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-                a.positions, a.rows = positions.data_ptr(), rows.data_ptr()
-                return self._launch(q_out)
-        self.layout = None
-        ref = q if q is not None else k if k is not None else v
-        _need(ref is not None, "one of q, k, v is needed")
-        tokens, _, dim = ref.shape
-        dtype, a = ref.dtype, self.args
-        if dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"head vectors are {dtype}, expected float16 or bfloat16")
-        if self.gamma_dim is not None and self.gamma_dim != (dim, dtype):
-            raise ValueError(f"gamma does not match head vectors of {dim} x {dtype}")
-        a.tokens, a.dim, a.dtype, a.q_heads, a.kv_heads = tokens, dim, _DTYPES[dtype], 0, 0
-        a.q = a.k = a.v = a.q_out = a.k_cache = a.v_cache = a.positions = a.rows = None
-        if q is not None or k is not None:
-            _on(positions, self.device, "positions", torch.int32)
-            if positions.shape != (tokens,) or not positions.is_contiguous():
-                raise ValueError(f"positions must be a contiguous vector of {tokens}")
-            a.positions = positions.data_ptr()
-        if q is not None:
-            q_out = q if q_out is None else q_out
-            a.q_heads = q.shape[1]
-            a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, a.q_heads, dim, dtype, "q")
-            a.q_out, a.q_out_token_stride, a.q_out_head_stride = self._heads(q_out, tokens, a.q_heads, dim, dtype,
-                                                                             "q_out")
-        if k is not None or v is not None:
-            _on(rows, self.device, "rows", torch.int64)
-            if rows.shape != (tokens,) or not rows.is_contiguous():
-                raise ValueError(f"rows must be a contiguous vector of {tokens}")
-            a.rows = rows.data_ptr()
-            a.kv_heads = heads = (k if k is not None else v).shape[1]
-            cache = k_cache if k is not None else v_cache
-            if cache is None:
-                raise ValueError("keys and values need their caches")
-            shape, strides = cache.shape, cache.stride()
-            for t, c, name in ((k, k_cache, "k"), (v, v_cache, "v")):
-                if t is None:
-                    continue
-                if c is None or c.dtype != dtype or c.device != self.device or c.shape != shape or \
-                        c.stride() != strides:
-                    raise ValueError(f"{name}_cache must be {tuple(shape)} {dtype}, K and V laid out alike")
-            if len(shape) != 4 or strides[3] != 1 or shape[1] != heads or shape[3] != dim:
-                raise ValueError(f"the caches must be [pages, {heads}, page_tokens, {dim}] with contiguous head "
-                                 "vectors")
-            if k is not None:
-                a.k, a.k_token_stride, a.k_head_stride = self._heads(k, tokens, heads, dim, dtype, "k")
-                a.k_cache = k_cache.data_ptr()
-            if v is not None:
-                a.v, a.v_token_stride, a.v_head_stride = self._heads(v, tokens, heads, dim, dtype, "v")
-                a.v_cache = v_cache.data_ptr()
-            a.page_stride, a.head_stride, a.row_stride, _ = strides
-            a.page_tokens, a.n_rows = shape[2], shape[0] * shape[2]
-        self.layout = layout
-        return self._launch(q_out)
+        with self.lock:
+            layout = None
+            if not any(t is None for t in (q, k, v, q_out, positions, rows, k_cache, v_cache)):
+                # what the checks below look at: tensors laid out like the last call's need only their addresses
+                layout = (q.shape, q.stride(), q.dtype, q.device,
+                          q_out.shape, q_out.stride(), q_out.dtype, q_out.device,
+                          k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device,
+                          positions.shape, positions.stride(), positions.dtype, positions.device,
+                          rows.shape, rows.stride(), rows.dtype, rows.device,
+                          k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+                          v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device)
+                if layout == self.layout:
+                    a = self.args
+                    a.q, a.q_out, a.k, a.v = q.data_ptr(), q_out.data_ptr(), k.data_ptr(), v.data_ptr()
+                    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+                    a.positions, a.rows = positions.data_ptr(), rows.data_ptr()
+                    return self._launch(q_out)
+            self.layout = None
+            ref = q if q is not None else k if k is not None else v
+            _need(ref is not None, "one of q, k, v is needed")
+            tokens, _, dim = ref.shape
+            dtype, a = ref.dtype, self.args
+            if dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"head vectors are {dtype}, expected float16 or bfloat16")
+            if self.gamma_dim is not None and self.gamma_dim != (dim, dtype):
+                raise ValueError(f"gamma does not match head vectors of {dim} x {dtype}")
+            a.tokens, a.dim, a.dtype, a.q_heads, a.kv_heads = tokens, dim, _DTYPES[dtype], 0, 0
+            a.q = a.k = a.v = a.q_out = a.k_cache = a.v_cache = a.positions = a.rows = None
+            if q is not None or k is not None:
+                _on(positions, self.device, "positions", torch.int32)
+                if positions.shape != (tokens,) or not positions.is_contiguous():
+                    raise ValueError(f"positions must be a contiguous vector of {tokens}")
+                a.positions = positions.data_ptr()
+            if q is not None:
+                q_out = q if q_out is None else q_out
+                a.q_heads = q.shape[1]
+                a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, a.q_heads, dim, dtype, "q")
+                a.q_out, a.q_out_token_stride, a.q_out_head_stride = self._heads(q_out, tokens, a.q_heads, dim, dtype,
+                                                                                 "q_out")
+            if k is not None or v is not None:
+                _on(rows, self.device, "rows", torch.int64)
+                if rows.shape != (tokens,) or not rows.is_contiguous():
+                    raise ValueError(f"rows must be a contiguous vector of {tokens}")
+                a.rows = rows.data_ptr()
+                a.kv_heads = heads = (k if k is not None else v).shape[1]
+                cache = k_cache if k is not None else v_cache
+                if cache is None:
+                    raise ValueError("keys and values need their caches")
+                shape, strides = cache.shape, cache.stride()
+                for t, c, name in ((k, k_cache, "k"), (v, v_cache, "v")):
+                    if t is None:
+                        continue
+                    if c is None or c.dtype != dtype or c.device != self.device or c.shape != shape or \
+                            c.stride() != strides:
+                        raise ValueError(f"{name}_cache must be {tuple(shape)} {dtype}, K and V laid out alike")
+                if len(shape) != 4 or strides[3] != 1 or shape[1] != heads or shape[3] != dim:
+                    raise ValueError(f"the caches must be [pages, {heads}, page_tokens, {dim}] with contiguous head "
+                                     "vectors")
+                if k is not None:
+                    a.k, a.k_token_stride, a.k_head_stride = self._heads(k, tokens, heads, dim, dtype, "k")
+                    a.k_cache = k_cache.data_ptr()
+                if v is not None:
+                    a.v, a.v_token_stride, a.v_head_stride = self._heads(v, tokens, heads, dim, dtype, "v")
+                    a.v_cache = v_cache.data_ptr()
+                a.page_stride, a.head_stride, a.row_stride, _ = strides
+                a.page_tokens, a.n_rows = shape[2], shape[0] * shape[2]
+            self.layout = layout
+            return self._launch(q_out)
 
     def _launch(self, q_out: Optional[torch.Tensor]):
         rc = self.lib.q4gpu_rope_append(self.args, _stream(self.device.index))
@@ -291,6 +297,7 @@ class Attention(_Err):
         self.q_heads, self.dim, self.slots = q_heads, dim, table.shape[0]
         self.k_cache, self.v_cache, self.table, self.lens = k_cache, v_cache, table, lens
         self.workspace = self.layout = None
+        self.lock = threading.Lock()
         self._new_err()
         # a row of the table is as long as its stride lets it name
         self.args = _native.AttnArgs(
@@ -308,52 +315,53 @@ class Attention(_Err):
         tokens cu_q[i] .. cu_q[i + 1] - 1, at most max_q; seq_ids int32 [sequences]: their
         slots (default: 0, 1, ..); max_ctx: no lens is larger (0: the table's width).
         lse (optional) float32 [tokens, q_heads] receives log sum exp of the scores."""
-        a = self.args
-        if cu_q is None:
-            raise ValueError("cu_q is needed")
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        # what the checks below look at: tensors laid out like the last call's need only their addresses
-        layout = (q.shape, q.stride(), q.dtype, q.device, out.shape, out.stride(), out.dtype, out.device, cu_q.shape,
-                  cu_q.stride(), cu_q.dtype, cu_q.device, max_q, max_ctx,
-                  None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device),
-                  None if seq_ids is None else (seq_ids.shape, seq_ids.stride(), seq_ids.dtype, seq_ids.device))
-        if layout == self.layout:
-            a.q, a.out, a.cu_q = q.data_ptr(), out.data_ptr(), cu_q.data_ptr()
-            if lse is not None:
-                a.lse = lse.data_ptr()
+        with self.lock:
+            a = self.args
+            if cu_q is None:
+                raise ValueError("cu_q is needed")
+            if out is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            # what the checks below look at: tensors laid out like the last call's need only their addresses
+            layout = (q.shape, q.stride(), q.dtype, q.device, out.shape, out.stride(), out.dtype, out.device,
+                      cu_q.shape, cu_q.stride(), cu_q.dtype, cu_q.device, max_q, max_ctx,
+                      None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device),
+                      None if seq_ids is None else (seq_ids.shape, seq_ids.stride(), seq_ids.dtype, seq_ids.device))
+            if layout == self.layout:
+                a.q, a.out, a.cu_q = q.data_ptr(), out.data_ptr(), cu_q.data_ptr()
+                if lse is not None:
+                    a.lse = lse.data_ptr()
+                if seq_ids is not None:
+                    a.seq_ids = seq_ids.data_ptr()
+                return self._launch(out)
+            self.layout = None
+            tokens = q.shape[0]
+            a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, "q")
+            a.out, a.out_token_stride, a.out_head_stride = self._heads(out, tokens, "out")
+            if cu_q.dtype != torch.int32 or cu_q.device != self.device or cu_q.dim() != 1 or cu_q.shape[0] < 1 or \
+                    not cu_q.is_contiguous():
+                raise ValueError(f"cu_q must be a contiguous int32 vector on {self.device}")
+            n = cu_q.shape[0] - 1
+            a.cu_q, a.n_seqs, a.tokens, a.max_q = cu_q.data_ptr(), n, tokens, max_q
+            a.max_ctx = max_ctx or int(min(a.table_stride * a.page_tokens, 2 ** 31 - 1))
+            a.seq_ids = a.lse = None
             if seq_ids is not None:
+                _on(seq_ids, self.device, "seq_ids", torch.int32)
+                _need(seq_ids.shape == (n,) and seq_ids.is_contiguous(), f"seq_ids must be [{n}]")
                 a.seq_ids = seq_ids.data_ptr()
+            elif n > self.slots:
+                raise ValueError(f"{n} sequences over {self.slots} slots")
+            if lse is not None:
+                _on(lse, self.device, "lse", torch.float32)
+                if lse.shape != (tokens, self.q_heads) or not lse.is_contiguous():
+                    raise ValueError(f"lse must be contiguous [{tokens}, {self.q_heads}]")
+                a.lse = lse.data_ptr()
+            need = self.lib.q4gpu_paged_attention_workspace_bytes(a)
+            if need > a.workspace_bytes:
+                # the old one stays alive until the work queued on this stream is done with it
+                self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
+                a.workspace, a.workspace_bytes = self.workspace.data_ptr(), need
+            self.layout = layout
             return self._launch(out)
-        self.layout = None
-        tokens = q.shape[0]
-        a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, "q")
-        a.out, a.out_token_stride, a.out_head_stride = self._heads(out, tokens, "out")
-        if cu_q.dtype != torch.int32 or cu_q.device != self.device or cu_q.dim() != 1 or cu_q.shape[0] < 1 or \
-                not cu_q.is_contiguous():
-            raise ValueError(f"cu_q must be a contiguous int32 vector on {self.device}")
-        n = cu_q.shape[0] - 1
-        a.cu_q, a.n_seqs, a.tokens, a.max_q = cu_q.data_ptr(), n, tokens, max_q
-        a.max_ctx = max_ctx or int(min(a.table_stride * a.page_tokens, 2 ** 31 - 1))
-        a.seq_ids = a.lse = None
-        if seq_ids is not None:
-            _on(seq_ids, self.device, "seq_ids", torch.int32)
-            _need(seq_ids.shape == (n,) and seq_ids.is_contiguous(), f"seq_ids must be [{n}]")
-            a.seq_ids = seq_ids.data_ptr()
-        elif n > self.slots:
-            raise ValueError(f"{n} sequences over {self.slots} slots")
-        if lse is not None:
-            _on(lse, self.device, "lse", torch.float32)
-            if lse.shape != (tokens, self.q_heads) or not lse.is_contiguous():
-                raise ValueError(f"lse must be contiguous [{tokens}, {self.q_heads}]")
-            a.lse = lse.data_ptr()
-        need = self.lib.q4gpu_paged_attention_workspace_bytes(a)
-        if need > a.workspace_bytes:
-            # the old one stays alive until the work queued on this stream is done with it
-            self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
-            a.workspace, a.workspace_bytes = self.workspace.data_ptr(), need
-        self.layout = layout
-        return self._launch(out)
 
     def _launch(self, out: torch.Tensor) -> torch.Tensor:
         rc = self.lib.q4gpu_paged_attention(self.args, _stream(self.device.index))

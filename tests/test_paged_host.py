@@ -1,6 +1,7 @@
 """The host side of the 16-bit paged operators, without a GPU."""
 import subprocess
 import sys
+import threading
 
 import pytest
 
@@ -40,3 +41,99 @@ n = size(**kw)
 assert 0 < n < 1 << 26, n
 assert lib.q4gpu_paged_attention(attn(**kw), None) == 0  # no work
 """)
+
+
+# ---------------------------------------------------------------------------
+# operators on CPU tensors with a stand-in for the library
+# ---------------------------------------------------------------------------
+torch = pytest.importorskip("torch")
+
+from llm_accelerator_b200 import _native, paged  # noqa: E402
+
+CPU = torch.device("cpu")
+
+
+class Lib:
+    """Records what each call was given; `during` runs inside a call, where the library has let other threads run."""
+
+    def __init__(self):
+        self.calls, self.during, self.need = [], lambda: None, 0
+
+    def _call(self, a, *fields):
+        before = [getattr(a, f) for f in fields]
+        self.during()
+        self.calls.append(before)
+        assert before == [getattr(a, f) for f in fields], "another thread's call changed this one's arguments"
+        return 0
+
+    def q4gpu_add_rmsnorm(self, a, stream):
+        return self._call(a, "x", "out", "rows")
+
+    def q4gpu_rope_append(self, a, stream):
+        return self._call(a, "q", "q_out", "positions", "tokens")
+
+    def q4gpu_paged_attention_workspace_bytes(self, a):
+        return self.need
+
+    def q4gpu_paged_attention(self, a, stream):
+        return self._call(a, "q", "out", "cu_q", "tokens", "workspace", "workspace_bytes")
+
+    def q4gpu_pages_compact_workspace_bytes(self, n):
+        return 64
+
+    def q4gpu_pages_fork(self, *a):
+        return 0
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    fake = Lib()
+    monkeypatch.setattr(_native, "load", lambda: fake)
+    monkeypatch.setattr(paged, "_cuda", lambda t, name: CPU)
+    monkeypatch.setattr(paged, "_stream", lambda index: 7)
+    return fake
+
+
+def make_norm():
+    op = paged.AddRmsNorm(torch.ones(8))
+    return op, lambda n: op(torch.zeros(n, 8))
+
+
+def make_rope():
+    op = paged.RopeAppend(torch.ones(4, 8), torch.ones(4, 8))
+    return op, lambda n: op(torch.zeros(n, 2, 16, dtype=torch.half), None, None, torch.zeros(n, dtype=torch.int32), None,
+                            None, None)
+
+
+def make_attn():
+    c = torch.zeros(2, 1, 16, 64, dtype=torch.half)
+    op = paged.Attention(c, c, torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), q_heads=2)
+    return op, lambda n: op(torch.zeros(n, 2, 64, dtype=torch.half), None, torch.tensor([0, n], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("make", [make_norm, make_rope, make_attn])
+def test_two_threads_with_one_operator(lib, make):
+    """A second thread calls the operator while the first is inside the library."""
+    op, call = make()
+    inside, errors, others = threading.Event(), [], []
+
+    def other():
+        inside.wait(5)
+        try:
+            call(5)
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    second = threading.Thread(target=other)
+
+    def during():
+        if not inside.is_set():
+            inside.set()
+            second.join(0.3)  # long enough for the other call, if nothing holds it up
+
+    lib.during = during
+    second.start()
+    call(3)
+    second.join()
+    assert not errors
+    assert len(lib.calls) == 2 and [c[2] if len(c) == 3 else c[3] for c in lib.calls] == [3, 5]
