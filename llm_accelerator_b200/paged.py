@@ -13,7 +13,8 @@ K/V cache, and what happens to the cache's pages between steps.
 Each operator is an object that holds what a serving loop keeps (weights,
 tables, cache, workspace) and is called with the step's tensors.  Calls
 enqueue on torch's current stream and do not synchronise; a workspace belongs
-to its object, so one object's calls run on one stream at a time.  Threads may
+to its object, so one object's calls run on one stream at a time (and a captured
+graph that holds them needs the object as long as it is replayed).  Threads may
 share an object: a lock keeps the arguments of a call together until the library
 has taken them.  Nothing has a reference counterpart (the reference decodes one
 token at a time in fixed point with a flat cache of 256 positions,
@@ -135,10 +136,24 @@ class AddRmsNorm:
 
 
 class _Err:
-    """The device error word of an operator: `check` waits for the stream and raises once."""
+    """The device error word of an operator: `check` waits for the stream and raises once.
+
+    ``own`` is the memory that the operator itself allocated.  torch keeps freed memory back for work queued on the
+    stream it came from only, so a call on another stream is made known to it.
+    """
 
     def _new_err(self) -> None:
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self.own, self.stream = [self.err], _stream(self.device.index)
+
+    def _here(self) -> int:
+        """The current stream, which may use what the operator owns."""
+        now = _stream(self.device.index)
+        if now != self.stream:
+            self.stream = now
+            for t in self.own:
+                t.record_stream(torch.cuda.current_stream(self.device))
+        return now
 
     def check(self) -> None:
         what = int(self.err.item())
@@ -257,7 +272,7 @@ class RopeAppend(_Err):
             return self._launch(q_out)
 
     def _launch(self, q_out: Optional[torch.Tensor]):
-        rc = self.lib.q4gpu_rope_append(self.args, _stream(self.device.index))
+        rc = self.lib.q4gpu_rope_append(self.args, self._here())
         if rc:
             _native.check(rc, "q4gpu_rope_append")
         return q_out
@@ -357,14 +372,29 @@ class Attention(_Err):
                 a.lse = lse.data_ptr()
             need = self.lib.q4gpu_paged_attention_workspace_bytes(a)
             if need > a.workspace_bytes:
-                # the old one stays alive until the work queued on this stream is done with it
-                self.workspace = torch.zeros(need, dtype=torch.uint8, device=self.device)
-                a.workspace, a.workspace_bytes = self.workspace.data_ptr(), need
+                if torch.cuda.is_current_stream_capturing():
+                    return self._launch_captured(out, need)
+                # the old ones stay: captured graphs know their addresses (each at least twice the last, so all
+                # together are less than two of the newest)
+                self.workspace = torch.zeros(max(need, 2 * a.workspace_bytes), dtype=torch.uint8, device=self.device)
+                self.own.append(self.workspace)
+                a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
             self.layout = layout
             return self._launch(out)
 
+    def _launch_captured(self, out: torch.Tensor, need: int) -> torch.Tensor:
+        """A captured call that wants more workspace than there is: what is allocated now is zeroed by the graph's
+        replays only, so it serves this call and no other."""
+        a, once = self.args, torch.zeros(need, dtype=torch.uint8, device=self.device)
+        kept = a.workspace, a.workspace_bytes
+        a.workspace, a.workspace_bytes = once.data_ptr(), need
+        try:
+            return self._launch(out)
+        finally:
+            a.workspace, a.workspace_bytes = kept
+
     def _launch(self, out: torch.Tensor) -> torch.Tensor:
-        rc = self.lib.q4gpu_paged_attention(self.args, _stream(self.device.index))
+        rc = self.lib.q4gpu_paged_attention(self.args, self._here())
         if rc:
             _native.check(rc, "q4gpu_paged_attention")
         return out
@@ -400,7 +430,9 @@ class Pages(_Err):
                                       err_flag=self.err.data_ptr(), page_bytes=pool.stride(0) * es,
                                       block_bytes=page_tokens * pool.shape[-1] * es, table_stride=table.shape[1],
                                       n_pages=pool.shape[0], page_tokens=page_tokens, n_slots=table.shape[0])
-        self.workspace = None
+        self.workspace = torch.empty(self.lib.q4gpu_pages_compact_workspace_bytes(pool.shape[0]), dtype=torch.uint8,
+                                     device=self.device)
+        self.own.append(self.workspace)
 
     def _ids(self, t: torch.Tensor, n: int, name: str) -> int:
         if t.dtype != torch.int32 or t.device != self.device or t.shape != (n,) or not t.is_contiguous():
@@ -412,7 +444,7 @@ class Pages(_Err):
         copied (its filled rows) to page fresh[i].  int32 [n] each."""
         n = parents.shape[0]
         rc = self.lib.q4gpu_pages_fork(self.args, self._ids(parents, n, "parents"), self._ids(children, n, "children"),
-                                       self._ids(fresh, n, "fresh"), n, _stream(self.device.index))
+                                       self._ids(fresh, n, "fresh"), n, self._here())
         if rc:
             _native.check(rc, "q4gpu_pages_fork")
 
@@ -423,12 +455,9 @@ class Pages(_Err):
         _on(new_table, self.device, "new_table", torch.int32)
         if new_table.shape != self.table.shape or not new_table.is_contiguous():
             raise ValueError(f"new_table must be contiguous {tuple(self.table.shape)}")
-        if self.workspace is None:
-            self.workspace = torch.empty(self.lib.q4gpu_pages_compact_workspace_bytes(self.args.n_pages),
-                                         dtype=torch.uint8, device=self.device)
         rc = self.lib.q4gpu_pages_compact(self.args, new_table.data_ptr(), self._ids(remap, self.args.n_pages, "remap"),
                                           self._ids(n_live, 1, "n_live"), self.workspace.data_ptr(),
-                                          self.workspace.numel(), _stream(self.device.index))
+                                          self.workspace.numel(), self._here())
         if rc:
             _native.check(rc, "q4gpu_pages_compact")
 

@@ -166,3 +166,96 @@ def test_rope_stores_nothing_of_a_token_without_a_position():
     op(None, None, v, None, rows, None, vc)  # values alone have no position
     op.check()
     assert torch.equal(vc[0][:, rows].transpose(0, 1), v)
+
+
+def grown_args():
+    """Forty decodes, a short chunk and a longer one; the split of long decodes and of chunks both need workspace."""
+    return make([1] * 40 + [70, 130], [3000] * 3 + [200] * 39, 8, 4, 128, 64, BF, 27)
+
+
+def part_of(args, ids):
+    cu, q = args[3].tolist(), args[4]
+    new = [cu[i + 1] - cu[i] for i in ids]
+    rows = torch.cat([q[cu[i]:cu[i + 1]] for i in ids])
+    return rows, i32([0] + torch.tensor(new).cumsum(0).tolist()), max(new), i32(ids)
+
+
+def test_attention_captured_decodes_survive_larger_calls():
+    """A decode step captured in a graph, then calls that need more workspace, then replays over new inputs; and a
+    graph captured by an operator that had no workspace yet."""
+    args = grown_args()
+    pool, table, lens, cu, q = args
+    few, c, most, ids = part_of(args, [0, 1, 7])
+    big = part_of(args, list(range(42)))
+    fresh = rnd(few.shape, BF, 77)
+    for warm in (True, False):
+        op = operator(pool, table, lens, 8)
+        x, out, lse = few.clone(), torch.empty_like(few), torch.empty(few.shape[:2], device="cuda")
+        if warm:
+            op(x, out, c, max_q=most, max_ctx=3200, lse=lse, seq_ids=ids)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            op(x, out, c, max_q=most, max_ctx=3200, lse=lse, seq_ids=ids)
+        for step in (few, fresh):
+            x.copy_(step)
+            got = op(big[0], None, big[1], max_q=big[2], max_ctx=3200, seq_ids=big[3])
+            filler = [torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda") for _ in range(8)]
+            graph.replay()
+            close(out, lse, *attn_ref(pool, table, lens, c, step, 128 ** -0.5, 0, ids.tolist()), BF)
+            ref, mag, _ = attn_ref(pool, table, lens, big[1], big[0], 128 ** -0.5, 0, big[3].tolist())
+            within(got, ref, U[BF] * ref.abs() + (U[BF] + 3e-4) * mag)
+            assert all((f == 255).all() for f in filler)
+        assert not reported(op)
+
+
+def test_operators_captured_together():
+    """A decode step of all operators as one graph."""
+    heads, kv, dim, page = 8, 4, 128, 16
+    cache = paged.PagedCache(1, 40, page, kv, dim, max_seqs=3, max_ctx=200)
+    cos, sin = angles(200, dim)
+    rope, attn = paged.RopeAppend(cos, sin), paged.Attention(cache.k(0), cache.v(0), cache.table, cache.lens, heads)
+    norm = paged.AddRmsNorm(torch.ones(heads * dim, dtype=BF, device="cuda"))
+    cache.pool.normal_()
+    cache.extend([0, 1, 2], [100, 17, 1])
+    step = cache.extend([0, 1, 2], [1, 1, 1])
+    qkv = rnd((3, heads + 2 * kv, dim), BF, 5)
+    y, out = torch.empty(3, heads * dim, dtype=BF, device="cuda"), torch.empty(3, heads, dim, dtype=BF, device="cuda")
+    turned = torch.empty(3, heads, dim, dtype=BF, device="cuda")
+
+    def run():
+        q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv], qkv[:, heads + kv:]
+        rope(q, k, v, step.positions, step.rows, cache.k(0), cache.v(0), turned)
+        attn(turned, out, step.cu_q, max_q=1, max_ctx=200, seq_ids=step.seq_ids)
+        norm(out.view(3, -1), out=y)
+
+    run()
+    want = y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    y.zero_()
+    graph.replay()
+    assert torch.equal(y, want)
+    qkv.mul_(-0.5)
+    graph.replay()
+    replayed = y.clone()
+    run()
+    assert torch.equal(y, replayed) and not torch.equal(y, want)
+
+
+def test_attention_moves_to_another_stream_and_grows_there():
+    args = grown_args()
+    pool, table, lens, cu, q = args
+    op = operator(pool, table, lens, 8)
+    small, big = part_of(args, [0, 1]), part_of(args, list(range(42)))
+    op(small[0], None, small[1], max_q=small[2], max_ctx=3200, seq_ids=small[3])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            got = op(big[0], None, big[1], max_q=big[2], max_ctx=3200, seq_ids=big[3])
+            op(small[0], None, small[1], max_q=small[2], max_ctx=3200, seq_ids=small[3])
+    torch.cuda.current_stream().wait_stream(s)
+    ref, mag, _ = attn_ref(pool, table, lens, big[1], big[0], 128 ** -0.5, 0, big[3].tolist())
+    within(got, ref, U[BF] * ref.abs() + (U[BF] + 3e-4) * mag)
+    assert not reported(op)

@@ -2,6 +2,7 @@
 import subprocess
 import sys
 import threading
+import weakref
 
 import pytest
 
@@ -91,6 +92,7 @@ def lib(monkeypatch):
     monkeypatch.setattr(_native, "load", lambda: fake)
     monkeypatch.setattr(paged, "_cuda", lambda t, name: CPU)
     monkeypatch.setattr(paged, "_stream", lambda index: 7)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return fake
 
 
@@ -137,3 +139,73 @@ def test_two_threads_with_one_operator(lib, make):
     second.join()
     assert not errors
     assert len(lib.calls) == 2 and [c[2] if len(c) == 3 else c[3] for c in lib.calls] == [3, 5]
+
+
+def test_workspaces_outlive_the_calls_that_used_them(lib):
+    """A captured graph and queued work keep the address of a workspace that has become too small."""
+    op, call = make_attn()
+    held = []
+    for need in (100, 101, 5000, 90000, 90001):
+        lib.need = need
+        call(len(held) + 1)
+        assert op.workspace.numel() >= need and op.args.workspace == op.workspace.data_ptr()
+        assert op.args.workspace_bytes == op.workspace.numel() and not op.workspace.any()
+        if not held or held[-1]() is not op.workspace:
+            held.append(weakref.ref(op.workspace))
+    assert all(w() is not None for w in held)
+    assert sum(w().numel() for w in held) <= 2 * held[-1]().numel() and len(held) == 5
+    ws = held[-1]
+    del op, call
+    assert ws() is None
+
+
+def test_workspaces_know_the_streams_that_use_them(lib, monkeypatch):
+    """A workspace comes from the pool of the stream of its first call: its memory must not go back there while a
+    later stream's work is queued."""
+    told = []
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: told.append((t.data_ptr(), s)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "other")
+    raw = {"stream": 7}
+    monkeypatch.setattr(paged, "_stream", lambda index: raw["stream"])
+    op, call = make_attn()
+    lib.need = 100
+    call(1)
+    call(1)
+    assert not told
+    raw["stream"] = 9
+    call(1)  # laid out like the last call
+    call(2)
+    assert {(op.workspace.data_ptr(), "other"), (op.err.data_ptr(), "other")} <= set(told)
+
+    lib.q4gpu_pages_compact = lambda *a: 0
+    pool = torch.zeros(4, 16, 8, dtype=torch.int16)
+    table, lens = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    raw["stream"] = 7
+    pages = paged.Pages(pool, table, lens, 16)
+    del told[:]
+    remap, n = torch.zeros(4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    pages.compact(table, remap, n)
+    pages.fork(n, n, n)
+    assert not told
+    raw["stream"] = 9
+    pages.compact(table, remap, n)
+    assert (pages.workspace.data_ptr(), "other") in told
+
+
+def test_a_call_under_capture_leaves_the_workspace_alone(lib, monkeypatch):
+    """What is allocated under capture is zeroed by the graph's replays only, so it serves that call and no other."""
+    op, call = make_attn()
+    lib.need = 100
+    call(1)
+    own = op.workspace.data_ptr()
+    capturing = {"now": True}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing["now"])
+    lib.need = 5000
+    call(2)
+    assert lib.calls[-1][4] not in (None, own) and lib.calls[-1][5] >= 5000
+    assert op.workspace.data_ptr() == own and op.args.workspace == own
+    call(2)  # the same layout: the small workspace must not serve it
+    assert lib.calls[-1][4] != own and lib.calls[-1][5] >= 5000
+    capturing["now"] = False
+    call(2)
+    assert lib.calls[-1][4] == op.workspace.data_ptr() and op.workspace.numel() >= 5000
