@@ -502,7 +502,13 @@ class PagedCache:
     def v(self, layer: int) -> torch.Tensor:
         return self.pool[:, layer, 1]
 
+    def _known(self, seqs: Sequence[int]) -> None:
+        for s in seqs:  # a negative number would mean another sequence on the host and none on the device
+            if not 0 <= s < len(self._len):
+                raise ValueError(f"sequence {s} is not one of {len(self._len)}")
+
     def length(self, seq: int) -> int:
+        self._known((seq,))
         return self._len[seq]
 
     @property
@@ -530,6 +536,7 @@ class PagedCache:
         """Room for counts[i] new tokens of sequence seqs[i]; returns the step's index tensors.
         Nothing changes if the pages do not suffice."""
         _need(len(seqs) == len(counts) and len(set(seqs)) == len(seqs) and len(seqs) > 0, "one count per sequence")
+        self._known(seqs)
         need = []
         for s, n in zip(seqs, counts):
             if n < 0 or self._len[s] + n > self.max_ctx:
@@ -558,6 +565,7 @@ class PagedCache:
 
     def fork(self, parent: int, children: Sequence[int]) -> None:
         """Empty sequences `children` continue `parent`: full pages are shared, its last one copied."""
+        self._known((parent, *children))
         _need(all(self._len[c] == 0 and c != parent for c in children) and len(set(children)) == len(children),
               "children must be empty sequences")
         n, held = self._len[parent], self._held[parent]
@@ -576,6 +584,7 @@ class PagedCache:
 
     def free(self, seq: int) -> None:
         """Ends a sequence; pages that nobody else uses become free."""
+        self._known((seq,))
         self._drop(self._held[seq])
         self._held[seq], self._len[seq] = [], 0
         self.lens[seq:seq + 1].zero_()

@@ -209,3 +209,32 @@ def test_a_call_under_capture_leaves_the_workspace_alone(lib, monkeypatch):
     capturing["now"] = False
     call(2)
     assert lib.calls[-1][4] == op.workspace.data_ptr() and op.workspace.numel() >= 5000
+
+
+# ---------------------------------------------------------------------------
+# the cache's bookkeeping
+# ---------------------------------------------------------------------------
+def make_cache(lib, monkeypatch):
+    monkeypatch.setattr(paged.PagedCache, "_up", lambda self, a: torch.from_numpy(a))
+    return paged.PagedCache(1, 8, 16, 1, 8, max_seqs=3, max_ctx=64, device=CPU)
+
+
+def state(c):
+    return (c._held.copy(), [list(h) for h in c._held], list(c._len), list(c._users), sorted(c._free), c.table.tolist(),
+            c.lens.tolist())
+
+
+@pytest.mark.parametrize("bad", [-1, 3, -3, 2 ** 31])
+def test_cache_refuses_unknown_sequences(lib, monkeypatch, bad):
+    c = make_cache(lib, monkeypatch)
+    c.extend([0, 2], [20, 5])
+    before = state(c)
+    for call in (lambda: c.extend([bad], [1]), lambda: c.extend([0, bad], [1, 1]), lambda: c.extend([bad, 2], [1, 1]),
+                 lambda: c.fork(bad, [1]), lambda: c.fork(0, [bad]), lambda: c.fork(0, [1, bad]), lambda: c.free(bad),
+                 lambda: c.length(bad)):
+        with pytest.raises(ValueError):
+            call()
+        assert state(c) == before
+    c.extend([1], [1])
+    c.free(2)
+    assert c.lens.tolist() == [20, 1, 0] and c.length(0) == 20 and c.free_pages == 5
