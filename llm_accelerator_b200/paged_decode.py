@@ -73,6 +73,9 @@ class PagedDecoder:
         counts = [len(t) for t in tokens]
         if min(counts, default=0) < 1:
             raise ValueError("every sequence of a step needs a token")
+        vocab = self.embed.shape[0]
+        if not all(0 <= t < vocab for one in tokens for t in one):
+            raise ValueError(f"a token is outside the vocabulary of {vocab}")
         flat = torch.tensor([t for one in tokens for t in one], dtype=torch.long).pin_memory()
         step = self.cache.extend(seqs, counts)
         h = self.embed[flat.to(self.embed.device, non_blocking=True)]
@@ -98,7 +101,8 @@ class PagedDecoder:
 
     def prefill(self, seq: int, prompt: Sequence[int], chunk: int = 512) -> torch.Tensor:
         """A prompt in chunks; the logits after its last token."""
-        logits = None
+        if not len(prompt) or chunk < 1:
+            raise ValueError("a prompt has a token and a chunk at least one")
         for at in range(0, len(prompt), chunk):
             logits = self.forward([seq], [prompt[at:at + chunk]])
         return logits

@@ -238,3 +238,36 @@ def test_cache_refuses_unknown_sequences(lib, monkeypatch, bad):
     c.extend([1], [1])
     c.free(2)
     assert c.lens.tolist() == [20, 1, 0] and c.length(0) == 20 and c.free_pages == 5
+
+
+def make_decoder(lib, monkeypatch, vocab=10):
+    from llm_accelerator_b200 import fp32_diag as F
+    from llm_accelerator_b200 import paged_decode
+    T, h = _native, 64
+    monkeypatch.setattr(paged.PagedCache, "_up", lambda self, a: torch.from_numpy(a))
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    z = torch.zeros
+    layer = {T.T_Q: z(F.HEADS * F.HEAD_DIM, h), T.T_K: z(F.KV_HEADS * F.HEAD_DIM, h),
+             T.T_V: z(F.KV_HEADS * F.HEAD_DIM, h), T.T_O: z(h, F.HEADS * F.HEAD_DIM), T.T_GATE: z(F.INTER, h),
+             T.T_UP: z(F.INTER, h), T.T_DOWN: z(h, F.INTER), T.T_INPUT_GAMMA: z(h), T.T_POST_GAMMA: z(h),
+             T.T_Q_GAMMA: z(F.HEAD_DIM), T.T_K_GAMMA: z(F.HEAD_DIM)}
+    return paged_decode.PagedDecoder({"embed": z(vocab, h), "final": z(h), "layers": [layer]}, max_seqs=2, max_ctx=64,
+                                     page_tokens=16, dtype=torch.half)
+
+
+@pytest.mark.parametrize("tokens", [[[3, 10]], [[-1]], [[1], [2 ** 40]]])
+def test_decoder_refuses_tokens_outside_the_vocabulary(lib, monkeypatch, tokens):
+    d = make_decoder(lib, monkeypatch)
+    before = state(d.cache)
+    with pytest.raises(ValueError, match="token"):
+        d.forward(list(range(len(tokens))), tokens)
+    assert state(d.cache) == before
+
+
+def test_decoder_refuses_empty_prompts(lib, monkeypatch):
+    d = make_decoder(lib, monkeypatch)
+    for call in (lambda: d.prefill(0, []), lambda: d.prefill(0, [1, 2], -1), lambda: d.forward([0], [[]]),
+                 lambda: d.forward([], []), lambda: d.forward([0, 1], [[1]])):
+        with pytest.raises(ValueError):
+            call()
+    assert d.cache.free_pages == 8 and d.cache.length(0) == 0
