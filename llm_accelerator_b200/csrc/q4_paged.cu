@@ -4,7 +4,6 @@
 // in q4_paged_attn.cu.
 #include <cuda_fp8.h>
 
-#include <cfloat>
 #include <cstdint>
 
 #include "q4_paged.cuh"
@@ -213,8 +212,15 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(NormParams p) {
     } else {
       constexpr float kMost = OUT == kE4m3 ? 448.f : 127.f;
       uint8_t* o = static_cast<uint8_t*>(p.out) + row * p.os;
-      // a subnormal maximum would give an infinite factor
-      auto factor = [&](float top) { return top == 0.f ? 0.f : fminf(__fdividef(kMost, top), FLT_MAX); };
+      // The factor of values v[0 .. n) whose largest is `top`.  A quarter of each side of the quotient: __fdividef gives
+      // 0 for divisors above 2^126.  Tiny values are made larger first, or the factor would be infinite.
+      auto factor = [&](float top, float* v, int n) {
+        if (top < 0x1p-96f) {
+          top *= 0x1p64f;
+          for (int i = 0; i < n; ++i) v[i] *= 0x1p64f;
+        }
+        return top == 0.f ? 0.f : __fdividef(kMost * 0.25f, top * 0.25f);
+      };
       if (p.group == 0) {
         float top = 0.f;
 #pragma unroll
@@ -225,8 +231,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(NormParams p) {
           __syncthreads();
           top = span_max((tx & 31) < (lanes >> 5) ? partm[tx & 31] : 0.f, 32);
         }
-        const float f = factor(top);
         if (tx == 0) p.scale[row] = top * (1.f / kMost);
+        const float f = factor(top, h, E);
 #pragma unroll
         for (int c = 0; c < N; ++c) {
           const int at = (c * lanes + tx) * V;
@@ -241,7 +247,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(NormParams p) {
           const float top = span_max(most[c], span);
           if (at < p.n) {
             if ((tx & (span - 1)) == 0) p.scale[row * groups + at / p.group] = top * (1.f / kMost);
-            store_8bit<OUT, V>(o + at, h + c * V, factor(top));
+            const float f = factor(top, h + c * V, V);
+            store_8bit<OUT, V>(o + at, h + c * V, f);
           }
         }
       }

@@ -259,3 +259,23 @@ def test_attention_moves_to_another_stream_and_grows_there():
     ref, mag, _ = attn_ref(pool, table, lens, big[1], big[0], 128 ** -0.5, 0, big[3].tolist())
     within(got, ref, U[BF] * ref.abs() + (U[BF] + 3e-4) * mag)
     assert not reported(op)
+
+
+@pytest.mark.parametrize("out", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("group,n", [(0, 512), (64, 512), (0, 333)])
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("size", [3e38, 1e38, 5e-35, 1e-36, 3e-37])
+def test_norm_8bit_of_any_magnitude(out, group, n, dtype, size):
+    """Groups whose largest value lies near either end of float32.  A scale below 2^-126 is a subnormal number, off by
+    up to 2^-150: the tolerance has that times the largest factor."""
+    w = (torch.linspace(-1, 1, n, device="cuda", dtype=torch.float64) * size).to(dtype)
+    x = torch.ones(3, n, device="cuda", dtype=dtype)
+    q, s = paged.AddRmsNorm(w, eps=0.0, out_dtype=out, group=group)(x)
+    _, ref = norm_ref(x, None, w, 0.0)
+    g = ref.unflatten(-1, (-1, group or n))
+    most = 448.0 if out == torch.float8_e4m3fn else 127.0
+    want = g.abs().amax(-1) / most
+    within(s, want, 2e-5 * want + 2.0 ** -149)
+    value = q.double().unflatten(-1, (-1, group or n)) * s.double()[..., None]
+    step = 2.0 ** -4 * g.abs() + 2.0 ** -10 * want[..., None] if out == torch.float8_e4m3fn else 0.5 * want[..., None]
+    within(value, g, step * (1 + 1e-4) + 3e-5 * g.abs() + most * 2.0 ** -149)
