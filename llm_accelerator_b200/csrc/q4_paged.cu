@@ -309,7 +309,7 @@ void launch_norm_out(const NormParams& p, int out_dtype, bool vec, cudaStream_t 
 // (heads s, s + slots, ..), so the token's cosines and sines are fetched once
 // for all of them and 32 VECS bytes of data are in flight per thread.  Bound by
 // memory, and by the way from a token's position to its table row: 8192 tokens of
-// 16 + 8 + 8 heads of 128, normed, take 34.8 us (4.0 TB/s; a plain copy of the same
+// 16 + 8 + 8 heads of 128, normed, take 34.4 us (4.1 TB/s; a plain copy of the same
 // bytes 24.8).
 template <typename T, bool INTERLEAVED, int VECS>
 __global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4)
@@ -361,8 +361,12 @@ __global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4)
       w.get(sn);
     }
   }
-  const bool stored = row >= 0 && row < a.n_rows;
-  if (there && (!known || row >= a.n_rows) && a.err_flag) *a.err_flag = 1;
+  // (tested at each store instead, an unknown position costs 8192 tokens 38.8 us, not 34.4)
+  bool stored = row >= 0 && row < a.n_rows;
+  if (there && (!known || row >= a.n_rows)) {
+    stored = false;
+    if (a.err_flag) *a.err_flag = 1;
+  }
   // (a 32-bit division where the row allows it)
   const int64_t page = !stored     ? 0
                        : row >> 32 ? row / a.page_tokens
@@ -400,7 +404,7 @@ __global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4)
       head -= nq + (is_k ? 0 : nk);
       dst = static_cast<T*>(is_k ? a.k_cache : a.v_cache) + cache + head * a.head_stride;
     }
-    if (slot + i * slots >= heads || (!is_q && !stored) || !known) continue;  // (values alone: always known)
+    if (slot + i * slots >= heads || (!is_q && !stored) || ((is_q || is_k) && !known)) continue;
     if ((is_q || is_k) && u < turned) {
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
