@@ -263,7 +263,8 @@ int q4gpu_rope_append(const q4gpu_rope_args *a, void *stream);
 /* Attention of each sequence's newest tokens to its pages.  Sequence i owns
  * query tokens [cu_q[i], cu_q[i + 1]) (int32 [n_seqs + 1], at most max_q
  * each) and slot s = seq_ids[i] (NULL: i): keys 0 .. lens[s] - 1 stand in the
- * pages table[s][0 ..] (int32, table_stride entries a slot), page_tokens each
+ * pages table[s][0 ..] (int32, table_pages entries a slot, the slots
+ * table_stride apart), page_tokens each
  * (16, 32, 64 or 128), at cache + page * page_stride + kv_head * head_stride +
  * offset * row_stride.  The new tokens are the last of those keys: query t of
  * n stands at position p = lens[s] - n + t and sees keys j <= p, with
@@ -299,7 +300,7 @@ typedef struct q4gpu_attn_args {
     int64_t page_stride, head_stride, row_stride, table_stride;
     int32_t n_seqs, n_slots, tokens, max_q, max_ctx, q_heads, kv_heads, dim, page_tokens, n_pages, window, dtype;
     float scale;
-    int32_t reserved;
+    int32_t table_pages; /* entries of a slot's row (0: table_stride) */
 } q4gpu_attn_args;
 size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args *a);
 int q4gpu_paged_attention(const q4gpu_attn_args *a, void *stream);

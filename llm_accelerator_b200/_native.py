@@ -116,7 +116,7 @@ class AttnArgs(C.Structure):
                                          "page_stride", "head_stride", "row_stride", "table_stride")] + \
                [(n, C.c_int32) for n in ("n_seqs", "n_slots", "tokens", "max_q", "max_ctx", "q_heads", "kv_heads",
                                          "dim", "page_tokens", "n_pages", "window", "dtype")] + \
-               [("scale", C.c_float), ("reserved", C.c_int32)]
+               [("scale", C.c_float), ("table_pages", C.c_int32)]
 
 
 class PagesArgs(C.Structure):

@@ -309,7 +309,7 @@ void launch_norm_out(const NormParams& p, int out_dtype, bool vec, cudaStream_t 
 // (heads s, s + slots, ..), so the token's cosines and sines are fetched once
 // for all of them and 32 VECS bytes of data are in flight per thread.  Bound by
 // memory, and by the way from a token's position to its table row: 8192 tokens of
-// 16 + 8 + 8 heads of 128, normed, take 34.4 us (4.1 TB/s; a plain copy of the same
+// 16 + 8 + 8 heads of 128, normed, take 34.4 us (4.0 TB/s; a plain copy of the same
 // bytes 24.8).
 template <typename T, bool INTERLEAVED, int VECS>
 __global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4)
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(256, VECS == 1 ? 5 : 4)
 template <typename T, bool INTERLEAVED>
 void launch_rope(const q4gpu_rope_args& a, int lanes, int heads, cudaStream_t s) {
   // Two head vectors a thread once that still gives every SM 1024 threads; one
-  // where latency counts (8192 tokens: 36.3 us with one, 34.8 with two at 64
+  // where latency counts (8192 tokens: 36.3 us with one, 34.4 with two at 64
   // registers, 38.0 with four at 99).
   const bool many = (int64_t)a.tokens * heads * lanes >= (int64_t)2 * 148 * 1024;
   const int slots = many ? (heads + 1) / 2 : heads;

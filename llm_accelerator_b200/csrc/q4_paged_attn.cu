@@ -26,7 +26,7 @@ __device__ __forceinline__ Seq sequence(const q4gpu_attn_args& a, int i) {
   s.n = max(0, min(a.cu_q[i + 1], a.tokens) - s.first);
   s.slot = a.seq_ids ? a.seq_ids[i] : i;
   const bool known = s.slot >= 0 && s.slot < a.n_slots;
-  s.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[s.slot], a.table_stride * a.page_tokens)) : 0;
+  s.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[s.slot], most_keys(a))) : 0;
   return s;
 }
 
@@ -446,7 +446,7 @@ int check_sizes(const q4gpu_attn_args* a) {
   if (a->q_heads > 256 || a->kv_heads > 256)
     return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: at most 256 heads");
   if (a->n_seqs < 0 || a->n_seqs > 65535 || a->tokens < 0 || a->max_q < 0 || a->max_ctx < 0 || a->window < 0 ||
-      a->n_slots < 1 || a->n_pages < 1 || a->table_stride < 1)
+      a->n_slots < 1 || a->n_pages < 1 || a->table_stride < 1 || a->table_pages < 0)
     return q4gpu_fail(Q4GPU_ERR_ARG, "attention: negative or empty size");
   return Q4GPU_OK;
 }
@@ -469,6 +469,13 @@ int check_attn(const q4gpu_attn_args* a) {
 // host
 // ---------------------------------------------------------------------------
 constexpr int kSms = 148;
+
+// The arguments as the kernels take them.
+q4gpu_attn_args settled(const q4gpu_attn_args& a) {
+  q4gpu_attn_args b = a;
+  if (b.table_pages == 0) b.table_pages = (int32_t)std::min<int64_t>(b.table_stride, INT32_MAX);
+  return b;
+}
 
 RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
   RowPlan p{};
@@ -595,9 +602,10 @@ extern "C" {
 
 size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args* a) {
   if (check_sizes(a) != Q4GPU_OK) return 0;
+  const q4gpu_attn_args b = settled(*a);
   size_t rows, chunks;
-  row_plan(*a, nullptr, &rows);
-  chunk_plan(*a, &chunks);
+  row_plan(b, nullptr, &rows);
+  chunk_plan(b, &chunks);
   return (rows + 15) / 16 * 16 + chunks;
 }
 
@@ -609,9 +617,10 @@ int q4gpu_paged_attention(const q4gpu_attn_args* a, void* stream) {
   if (a->workspace_bytes < need || (need && !a->workspace))
     return q4gpu_fail(Q4GPU_ERR_WORKSPACE, "attention: needs a workspace of %zu bytes", need);
   if (!aligned(a->workspace, 16)) return q4gpu_fail(Q4GPU_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
+  const q4gpu_attn_args b = settled(*a);
   cudaStream_t s = as_stream(stream);
-  if (a->dtype == Q4GPU_F16) return a->dim == 64 ? launch<__half, 64>(*a, s) : launch<__half, 128>(*a, s);
-  return a->dim == 64 ? launch<__nv_bfloat16, 64>(*a, s) : launch<__nv_bfloat16, 128>(*a, s);
+  if (b.dtype == Q4GPU_F16) return b.dim == 64 ? launch<__half, 64>(b, s) : launch<__half, 128>(b, s);
+  return b.dim == 64 ? launch<__nv_bfloat16, 64>(b, s) : launch<__nv_bfloat16, 128>(b, s);
 }
 
 }  // extern "C"

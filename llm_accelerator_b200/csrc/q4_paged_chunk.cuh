@@ -33,6 +33,9 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
   return max(kMinPart, ((keys + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
 }
 
+// Keys that a slot's row of the table can name.
+__device__ __forceinline__ int64_t most_keys(const q4gpu_attn_args& a) { return (int64_t)a.table_pages * a.page_tokens; }
+
 // Whether what only the device sees of sequence i is in range: its query tokens, and if it has any its slot and that
 // slot's length.  (What is not is cut off or taken as empty; one kernel of a call reports it.)
 __device__ __forceinline__ bool sequence_ok(const q4gpu_attn_args& a, int i) {
@@ -40,7 +43,7 @@ __device__ __forceinline__ bool sequence_ok(const q4gpu_attn_args& a, int i) {
   if (c0 < 0 || c1 < c0 || c1 > a.tokens || c1 - c0 > a.max_q) return false;
   if (c0 == c1) return true;
   const int s = a.seq_ids ? a.seq_ids[i] : i;
-  return s >= 0 && s < a.n_slots && a.lens[s] >= 0 && a.lens[s] <= a.table_stride * a.page_tokens;
+  return s >= 0 && s < a.n_slots && a.lens[s] >= 0 && a.lens[s] <= most_keys(a);
 }
 
 // Sequence and row pair of one grid index, and what its CTA needs to know of the
@@ -56,7 +59,7 @@ __device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int gro
   t.n = max(0, min(a.cu_q[i + 1], a.tokens) - t.first);
   t.slot = a.seq_ids ? a.seq_ids[i] : i;
   const bool known = t.slot >= 0 && t.slot < a.n_slots;
-  t.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[t.slot], a.table_stride * a.page_tokens)) : 0;
+  t.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[t.slot], most_keys(a))) : 0;
   if (t.n < least) return 0;
   keys = a.window > 0 ? min(t.len, a.window) : t.len;
   return (int)(((int64_t)t.n * group + kPair - 1) / kPair);

@@ -314,11 +314,11 @@ class Attention(_Err):
         self.workspace = self.layout = None
         self.lock = threading.Lock()
         self._new_err()
-        # a row of the table is as long as its stride lets it name
         self.args = _native.AttnArgs(
             k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr(),
             page_stride=k_cache.stride(0), head_stride=k_cache.stride(1), row_stride=k_cache.stride(2),
-            table_stride=table.stride(0) if self.slots > 1 else table.shape[1], n_slots=self.slots, q_heads=q_heads,
+            table_stride=table.stride(0) if self.slots > 1 else table.shape[1], table_pages=table.shape[1],
+            n_slots=self.slots, q_heads=q_heads,
             kv_heads=kv_heads, dim=dim, page_tokens=page_tokens, n_pages=pages, window=window,
             dtype=_DTYPES[self.dtype], scale=dim ** -0.5 if scale is None else scale,
             err_flag=self.err.data_ptr())
@@ -357,7 +357,7 @@ class Attention(_Err):
                 raise ValueError(f"cu_q must be a contiguous int32 vector on {self.device}")
             n = cu_q.shape[0] - 1
             a.cu_q, a.n_seqs, a.tokens, a.max_q = cu_q.data_ptr(), n, tokens, max_q
-            a.max_ctx = max_ctx or int(min(a.table_stride * a.page_tokens, 2 ** 31 - 1))
+            a.max_ctx = max_ctx or min(a.table_pages * a.page_tokens, 2 ** 31 - 1)
             a.seq_ids = a.lse = None
             if seq_ids is not None:
                 _on(seq_ids, self.device, "seq_ids", torch.int32)

@@ -279,3 +279,26 @@ def test_norm_8bit_of_any_magnitude(out, group, n, dtype, size):
     value = q.double().unflatten(-1, (-1, group or n)) * s.double()[..., None]
     step = 2.0 ** -4 * g.abs() + 2.0 ** -10 * want[..., None] if out == torch.float8_e4m3fn else 0.5 * want[..., None]
     within(value, g, step * (1 + 1e-4) + 3e-5 * g.abs() + most * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 300])
+def test_attention_over_columns_of_a_wider_table(new):
+    """A slot's row is as long as the table is wide, whatever lies between the rows."""
+    pool, table, lens, cu, q = make([new] * 3, [100, 300, 40], 4, 2, 64, 32, BF, 26)
+    pool.nan_to_num_(0.5)  # the unfilled rows of last pages are seen below
+    w = table.shape[1]
+    wide = torch.zeros(4, 2 * w + 1, dtype=torch.int32, device="cuda")  # its other entries name page 0
+    wide[:3, w - 2:2 * w - 2] = table
+    part = wide[:3, w - 2:2 * w - 2]
+    op = operator(pool, part, lens, 4)
+    check(op, pool, table, lens, cu, q, 64 ** -0.5)
+    assert not reported(op)
+    for s in range(3):
+        kept = lens.clone()
+        lens[s] = 32 * w + 50  # more than the slot's entries can name: cut off there
+        cut = lens.clamp(max=32 * w)
+        out, lse = torch.full_like(q, 5.0), torch.full(q.shape[:2], 5.0, device="cuda")
+        op(q, out, cu, max_q=new, lse=lse)
+        close(out, lse, *attn_ref(pool, table, cut, cu, q, 64 ** -0.5), BF)
+        assert reported(op)
+        lens.copy_(kept)
