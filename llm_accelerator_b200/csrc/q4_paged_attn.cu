@@ -96,7 +96,7 @@ struct RowPlan {
 __device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const Seq& s, int group, int& lo) {
   lo = 0;
   if (s.n == 0 || s.n > kRows / group) return -1;
-  if (a.window > 0) lo = max(0, s.len - s.n - a.window + 1) & ~(kTileKeys - 1);
+  if (a.window > 0) lo = first_seen(s.len - s.n, a.window) & ~(kTileKeys - 1);
   return max(0, s.len - lo);
 }
 __device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int group) {  // of one head
@@ -474,6 +474,8 @@ constexpr int kSms = 148;
 q4gpu_attn_args settled(const q4gpu_attn_args& a) {
   q4gpu_attn_args b = a;
   if (b.table_pages == 0) b.table_pages = (int32_t)std::min<int64_t>(b.table_stride, INT32_MAX);
+  // a window that no slot's keys fill is none (position - window would pass 31 bits for queries before the first key)
+  if (b.window >= std::min<int64_t>((int64_t)b.table_pages * b.page_tokens, INT32_MAX)) b.window = 0;
   return b;
 }
 

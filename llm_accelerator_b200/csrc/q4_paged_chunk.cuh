@@ -36,6 +36,9 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
 // Keys that a slot's row of the table can name.
 __device__ __forceinline__ int64_t most_keys(const q4gpu_attn_args& a) { return (int64_t)a.table_pages * a.page_tokens; }
 
+// First key that a query at position pos (negative: before all keys) sees through a window.
+__device__ __forceinline__ int first_seen(int pos, int window) { return (int)max((int64_t)0, (int64_t)pos - window + 1); }
+
 // Whether what only the device sees of sequence i is in range: its query tokens, and if it has any its slot and that
 // slot's length.  (What is not is cut off or taken as empty; one kernel of a call reports it.)
 __device__ __forceinline__ bool sequence_ok(const q4gpu_attn_args& a, int i) {
@@ -353,8 +356,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int t0 = tile.row0 / group, t1 = (tile.row0 + rows - 1) / group;  // first and last query of the pair
   const int pos0 = len - n + t0, pos1 = len - n + t1;
   // keys that some row sees, and those that every row sees
-  const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1);
-  const int all_lo = a.window > 0 ? max(0, pos1 - a.window + 1) : 0, all_hi = pos0 + 1;
+  const int lo = a.window > 0 ? first_seen(pos0, a.window) : 0, hi = max(0, pos1 + 1);
+  const int all_lo = a.window > 0 ? first_seen(pos1, a.window) : 0, all_hi = pos0 + 1;
   const int base = lo & ~(kNTile - 1);
   const int chunk = part_keys(plan, hi - base);
   const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
@@ -747,7 +750,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, Chunk
   const int first = tile.first, n = tile.n, len = tile.len;
   const int rows = (int)min((int64_t)kPair, (int64_t)n * group - tile.row0);
   const int pos0 = len - n + tile.row0 / group, pos1 = len - n + (tile.row0 + rows - 1) / group;
-  const int lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0, hi = max(0, pos1 + 1), base = lo & ~(kNTile - 1);
+  const int lo = a.window > 0 ? first_seen(pos0, a.window) : 0, hi = max(0, pos1 + 1), base = lo & ~(kNTile - 1);
   const int chunk = part_keys(plan, hi - base);
   const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
   if (parts == 1) return;

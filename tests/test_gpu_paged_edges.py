@@ -302,3 +302,14 @@ def test_attention_over_columns_of_a_wider_table(new):
         close(out, lse, *attn_ref(pool, table, cut, cu, q, 64 ** -0.5), BF)
         assert reported(op)
         lens.copy_(kept)
+
+
+@pytest.mark.parametrize("new,held", [(3, 1), (3, 0), (40, 30), (300, 100), (300, 1), (1, 200), (40, 300)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 100000])
+def test_attention_windows_wider_than_any_context(new, held, window):
+    """Also where a slot holds fewer keys than it has queries: differences of positions pass 31 bits."""
+    pool, table, lens, cu, q = make([new] * 2, [held, 50], 4, 2, 64, 32, BF, 28)
+    lens[0] = held
+    out, lse = check(operator(pool, table, lens, 4, window=window), pool, table, lens, cu, q, 64 ** -0.5)
+    want = check(operator(pool, table, lens, 4), pool, table, lens, cu, q, 64 ** -0.5)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
