@@ -483,7 +483,7 @@ RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
   RowPlan p{};
   const size_t items = (size_t)a.n_seqs * a.kv_heads;
   // no CTA without at least one (sequence, head) or kLeastStretch units of one
-  const int64_t units = (a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
+  const int64_t units = ((int64_t)a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
   const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + kLeastStretch - 1) / kLeastStretch + 1);
   p.ctas = (int)std::min<int64_t>(most, kSms * (a.dim == 64 ? 2 : 1));
   static_assert(kSms * 4 <= kMostCtas, "a counter a CTA");

@@ -271,3 +271,13 @@ def test_decoder_refuses_empty_prompts(lib, monkeypatch):
         with pytest.raises(ValueError):
             call()
     assert d.cache.free_pages == 8 and d.cache.length(0) == 0
+
+
+@pytest.mark.parametrize("max_ctx", [2 ** 31 - 1, 2 ** 31 - 100])
+@pytest.mark.parametrize("kw", [dict(), dict(dim=128), dict(n_seqs=3, tokens=3, q_heads=4, kv_heads=2)])
+def test_contexts_near_the_largest_are_split_like_long_ones(max_ctx, kw):
+    """One decode over a context of unknown length is spread over the GPU, whatever bound stands for 'unknown'."""
+    child(f"""
+kw = dict({kw!r}, table_stride=1 << 27)
+assert size(max_ctx={max_ctx}, **kw) == size(max_ctx=1 << 26, **kw) > size(max_ctx=16, **kw)
+""")
