@@ -464,22 +464,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // ---- loads: K and V of a step take one ring stage each ----------------------
       int id, next_id, issued = 0;
       unsigned ok = pages_of(begin, id), next_ok = ok;
-      for (int j = 0; j < steps && !*dead; ++j) {
+      bool stop = false;  // the same in every lane: the loads below are by full warps
+      for (int j = 0; j < steps && !stop; ++j) {
         const int key = begin + j * kNTile;
         if (j + 1 < steps) next_ok = pages_of(key + kNTile, next_id);
         for (int kind = 0; kind < 2; ++kind) {
           const int use = 2 * j + kind, st = use % kStages;
           if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
-          __syncwarp();
-          if (*dead) break;
+          stop = __any_sync(~0u, *dead);
+          if (stop) break;
           if (use > 0) load(kind ? &vmap : &kmap, ring + st * kTile, id, ok, &full[st]);
           issued = use + 1;
         }
         id = next_id, ok = next_ok;
       }
-      if (*dead)  // after a wait that ran out: copies in flight end first
-        for (int use = max(0, issued - kStages); use < issued; ++use)
-          wait_phase(&full[use % kStages], (use / kStages) & 1);
+      // copies in flight end first (they have, unless a wait ran out)
+      for (int use = max(0, issued - kStages); use < issued; ++use)
+        wait_phase(&full[use % kStages], (use / kStages) & 1);
     } else if (warp >= 9 && warp < 9 + tiles) {
       // ---- products: one warp a tile, together; an elected thread issues ---------------
       // Descriptors and addresses are the same in every lane and stay in uniform
@@ -513,14 +514,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // all 512 columns are this CTA's, so they start at 0
         bool live = tmem == 0 && scores(0) && (subs == 1 || scores(1));
         int cleaned = 0;
-        for (int i = 0; i < subs && live; ++i) {
+        for (int i = 0; i < subs; ++i) {
           const int use = i | 1, st = use % kStages;
-          live = stage_full(use);
+          live = live && stage_full(use);
           if (!(i & 1) && careful(begin + i * kStep)) {
             live = live && wait_phase(&clean[cleaned & 1], (cleaned >> 1) & 1);
             ++cleaned;
           }
-          live = live && wait_phase(&p_full[t][i & 1], (i >> 1) & 1);
+          // no lane is a step ahead of another: one that fell behind would wait for a barrier's next phase
+          live = __all_sync(~0u, live && wait_phase(&p_full[t][i & 1], (i >> 1) & 1));
           if (!live) break;
           fence_after_sync();
           const uint64_t v = v_desc + st * (kTile / 16) + (i & 1) * (kStep * 128 / 16);
@@ -669,6 +671,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int c = 0; c < D; c += 32) {
           float o[32];
           if (subs > 0) {
+            __syncwarp();  // rows took their own ways below
             tm_ld32(to + c, o);
             tm_ld_wait32(o);
           } else {
@@ -730,7 +733,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __syncthreads();
   if (*dead && warp == 9 && subs > 0)  // after a wait that ran out: products in flight end first
     for (int i = 0; i < tiles; ++i) wait_phase(&o_full[i], 0);
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 9) {
+    __syncwarp();
+    fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
   wait_before();
 }
 
