@@ -527,11 +527,14 @@ int encode_map(CUtensorMap* map, const q4gpu_attn_args& a, const void* base) {
         q != cudaDriverEntryPointSuccess || !encode)
       return q4gpu_fail(Q4GPU_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   }
-  // one 128-byte line of every row of a page per box
-  const cuuint64_t dims[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.page_tokens, (cuuint64_t)a.kv_heads,
+  // one 128-byte line of every row of a page per box; a stride that nothing takes (one head, heads that share their
+  // keys, one page) is given as the least that the map allows
+  const cuuint64_t unused = (cuuint64_t)a.dim * 2;
+  const bool heads = a.kv_heads > 1 && a.head_stride != 0;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.page_tokens, heads ? (cuuint64_t)a.kv_heads : 1,
                               (cuuint64_t)a.n_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)a.row_stride * 2, (cuuint64_t)a.head_stride * 2,
-                                 (cuuint64_t)a.page_stride * 2};
+  const cuuint64_t strides[3] = {(cuuint64_t)a.row_stride * 2, heads ? (cuuint64_t)a.head_stride * 2 : unused,
+                                 a.n_pages > 1 ? (cuuint64_t)a.page_stride * 2 : unused};
   const cuuint32_t box[4] = {64, (cuuint32_t)a.page_tokens, 1, 1}, one[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type =
       a.dtype == Q4GPU_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if ((ok >> lane) & 1u) {
 #pragma unroll
       for (int c = 0; c < kLines; ++c)
-        tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, map, c * 64, 0, kvh, id, bar);
+        tma_load4(at + c * kLineTile + lane * a.page_tokens * 128, map, c * 64, 0, a.head_stride ? kvh : 0, id, bar);
     }
   };
   if (warp == 8 && steps > 0) {

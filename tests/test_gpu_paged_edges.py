@@ -313,3 +313,38 @@ def test_attention_windows_wider_than_any_context(new, held, window):
     out, lse = check(operator(pool, table, lens, 4, window=window), pool, table, lens, cu, q, 64 ** -0.5)
     want = check(operator(pool, table, lens, 4), pool, table, lens, cu, q, 64 ** -0.5)
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("hq,hk,dim,page", [(16, 8, 128, 64), (7, 1, 64, 16), (8, 4, 64, 128)])
+@pytest.mark.parametrize("order", ["page", "split", "one page"])
+def test_attention_cache_orders(hq, hk, dim, page, order):
+    """Positions before heads in memory ([pages, page_tokens, kv_heads, dim]), K and V in rows of one wider tensor, and
+    a pool of one page."""
+    one = order == "one page"
+    new, old = ([1, 5], [0, 0]) if one else ([1, 3, 40, 300], [300, 17, 5, 200])
+    pool, table, lens, cu, q = make(new[:1] if one else new, old[:1] if one else old, hq, hk, dim, page, BF, 29)
+    if order == "page":
+        kv = [pool[:, i].permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for i in (0, 1)]
+    elif order == "split":
+        wide = torch.empty(pool.shape[0], page, hk, 2, dim, dtype=BF, device="cuda")
+        kv = [wide[:, :, :, i].permute(0, 2, 1, 3) for i in (0, 1)]
+        for i in (0, 1):
+            kv[i].copy_(pool[:, i])
+    else:
+        page_at = int(table[0, 0])
+        table.zero_()
+        pool = pool[page_at:page_at + 1].clone()
+        kv = [pool[:, 0], pool[:, 1]]
+    op = paged.Attention(kv[0], kv[1], table, lens, q_heads=hq)
+    check(op, pool, table, lens, cu, q, dim ** -0.5)
+    assert not reported(op)
+
+
+@pytest.mark.parametrize("new", [1, 5, 40, 300])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_heads_that_share_their_keys(new, dim):
+    """One key head expanded to four (a head stride of 0)."""
+    pool, table, lens, cu, q = make([new] * 2, [300, 20], 8, 1, dim, 32, BF, 30)
+    k, v = (pool[:, i].expand(-1, 4, -1, -1) for i in (0, 1))
+    op = paged.Attention(k, v, table, lens, q_heads=8)
+    check(op, pool, table, lens, cu, q, dim ** -0.5)
