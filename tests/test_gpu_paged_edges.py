@@ -15,7 +15,7 @@ if not torch.cuda.is_available():
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
 from llm_accelerator_b200 import _native, paged  # noqa: E402
-from test_gpu_paged import BF, HF, SF, TINY, U, angles, attn_ref, i32, make, norm_ref, rnd, within  # noqa: E402
+from test_gpu_paged import BF, HF, SF, TINY, U, angles, attn_ref, i32, make, norm_ref, rnd, rope_ref, within  # noqa: E402
 
 
 def operator(pool, table, lens, hq, **kw):
@@ -348,3 +348,63 @@ def test_attention_heads_that_share_their_keys(new, dim):
     k, v = (pool[:, i].expand(-1, 4, -1, -1) for i in (0, 1))
     op = paged.Attention(k, v, table, lens, q_heads=8)
     check(op, pool, table, lens, cu, q, dim ** -0.5)
+
+
+@pytest.mark.parametrize("new,old", [(1, 300), (3, 300), (50, 300), (400, 300), (40, 3000)])
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("window", [0, 90])
+def test_attention_infinite_values_reach_the_queries_that_see_them(new, old, what, window):
+    """Keys stay finite; one value of one key is not.  The queries that see it have it in that column (its weight is far
+    above the least bf16 number), and nothing else changes."""
+    args = make([new], [old], 4, 2, 128, 64, BF, 31)
+    pool, table, lens, cu, q = args
+    op = operator(pool, table, lens, 4, window=window)
+    clean, base = check(op, *args, 128 ** -0.5, window)
+    for at in sorted({old + new // 2, old, max(0, old - 60), old + new - 1}):
+        kept = pool[table[0, at // 64], 1, 1, at % 64, 5].item()
+        pool[table[0, at // 64], 1, 1, at % 64, 5] = what  # key head 1: query heads 2 and 3
+        lse = torch.empty_like(base)
+        out = op(q, None, cu, max_q=new, max_ctx=old + new, lse=lse)
+        pos = torch.arange(old, old + new, device="cuda")
+        sees = (pos >= at) & ((pos - window < at) if window else (pos >= 0))
+        hit = out[sees][:, 2:, 5]
+        assert hit.isnan().all() if math.isnan(what) else (hit == what).all()
+        out[:, 2:, 5] = torch.where(sees[:, None], clean[:, 2:, 5], out[:, 2:, 5])
+        assert torch.equal(out, clean) and torch.equal(lse, base)
+        pool[table[0, at // 64], 1, 1, at % 64, 5] = kept
+
+
+def test_rope_remembers_a_layout_not_its_tensors():
+    """One object called again and again: the same layout at other addresses, other layouts between, errors between."""
+    cos, sin = angles(300, 128)
+    g = rnd((128,), BF, 3) + 1
+    op = paged.RopeAppend(cos, sin, q_gamma=g, k_gamma=g)
+
+    def one(tokens, hq, hk, page, seed, wide=0, q_out=True):
+        qkv = rnd((tokens, hq + 2 * hk + wide, 128), BF, seed)
+        q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:hq + 2 * hk]
+        kc, vc = (torch.zeros(8, hk, page, 128, dtype=BF, device="cuda") for _ in range(2))
+        pos = torch.randint(0, 300, (tokens,), device="cuda", dtype=torch.int32)
+        rows = torch.randperm(8 * page, device="cuda")[:tokens].contiguous()
+        want = [rope(t.clone(), pos) for t in (q, k)] + [v.clone()]
+        got = op(q, k, v, pos, rows, kc, vc, torch.empty_like(q) if q_out else None)
+        turned(got, *want[0])
+        turned(kc[rows // page, :, rows % page], *want[1])
+        assert torch.equal(vc[rows // page, :, rows % page], want[2])
+
+    def rope(x, pos):
+        return rope_ref(x, g, cos, sin, pos.long(), False, 1e-6)
+
+    def turned(got, want, m):
+        within(got, want, U[BF] * want.abs() + 1e-5 * m + TINY[BF])
+
+    for seed in range(3):
+        one(5, 4, 2, 16, seed)
+        one(5, 4, 2, 16, 10 + seed)
+        one(5, 4, 2, 16, 20 + seed, wide=1)  # other strides
+        one(5, 4, 2, 16, 30 + seed, q_out=False)
+        with pytest.raises(ValueError):
+            op(rnd((5, 4, 128), BF, 1), rnd((5, 2, 128), HF, 1), None, None, None, None, None)
+        one(5, 4, 2, 16, 40 + seed)
+        one(6, 2, 4, 32, 50 + seed)
+    op.check()
