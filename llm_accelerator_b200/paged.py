@@ -42,6 +42,15 @@ _DTYPES = {torch.float32: _native.DT_F32, torch.float16: _native.DT_F16, torch.b
 # object first (3 us on the host, as long as a small kernel); this is the call inside it.
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                   lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _at(index: int) -> int:
+    """The current stream of device `index`, which has to be the current device: a launch goes to that one, and the
+    default stream's handle is the same on all."""
+    if _current() != index:
+        raise ValueError(f"the operator is on cuda:{index}, the current device is cuda:{_current()}")
+    return _stream(index)
 
 
 def _need(ok: bool, what: str) -> None:
@@ -80,6 +89,7 @@ class AddRmsNorm:
                  group: int = 0):
         self.lib = _native.load()
         self.device = _cuda(weight, "weight")
+        self.index = self.device.index
         _need(weight.dim() == 1 and weight.is_contiguous(), "weight must be a contiguous vector")
         _need(weight.dtype in (torch.float32, torch.float16, torch.bfloat16), f"weight is {weight.dtype}")
         self.weight, self.n, self.dtype = weight, weight.shape[0], weight.dtype
@@ -129,7 +139,7 @@ class AddRmsNorm:
                 _need(scale.shape == (rows, self.groups) and scale.is_contiguous(),
                       f"scale must be contiguous [{rows}, {self.groups}]")
                 a.scale = scale.data_ptr()
-            rc = self.lib.q4gpu_add_rmsnorm(a, _stream(self.device.index))
+            rc = self.lib.q4gpu_add_rmsnorm(a, _at(self.index))
             if rc:
                 _native.check(rc, "q4gpu_add_rmsnorm")
             return (out, scale) if self.narrow else out
@@ -144,11 +154,12 @@ class _Err:
 
     def _new_err(self) -> None:
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self.own, self.stream = [self.err], _stream(self.device.index)
+        self.index = self.device.index
+        self.own, self.stream = [self.err], _stream(self.index)
 
     def _here(self) -> int:
         """The current stream, which may use what the operator owns."""
-        now = _stream(self.device.index)
+        now = _at(self.index)
         if now != self.stream:
             self.stream = now
             for t in self.own:

@@ -408,3 +408,23 @@ def test_rope_remembers_a_layout_not_its_tensors():
         one(5, 4, 2, 16, 40 + seed)
         one(6, 2, 4, 32, 50 + seed)
     op.check()
+
+
+def test_attention_mixed_step_captured():
+    """Decodes, a short chunk and a split chunk in one call: both kernels and the join, replayed over new queries."""
+    args = grown_args()
+    pool, table, lens, cu, q = args
+    for ids in (list(range(42)), [0, 41], [41], [2]):
+        x, c, most, slots = part_of(args, ids)
+        op = operator(pool, table, lens, 8)
+        out, lse = torch.empty_like(x), torch.empty(x.shape[:2], device="cuda")
+        op(x, out, c, max_q=most, max_ctx=3200, lse=lse, seq_ids=slots)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            op(x, out, c, max_q=most, max_ctx=3200, lse=lse, seq_ids=slots)
+        for seed in (61, 62):
+            x.copy_(rnd(x.shape, BF, seed))
+            out.zero_()
+            graph.replay()
+            close(out, lse, *attn_ref(pool, table, lens, c, x, 128 ** -0.5, 0, ids), BF)
+        assert not reported(op)

@@ -92,6 +92,7 @@ def lib(monkeypatch):
     monkeypatch.setattr(_native, "load", lambda: fake)
     monkeypatch.setattr(paged, "_cuda", lambda t, name: CPU)
     monkeypatch.setattr(paged, "_stream", lambda index: 7)
+    monkeypatch.setattr(paged, "_current", lambda: CPU.index)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     return fake
 
@@ -281,3 +282,26 @@ def test_contexts_near_the_largest_are_split_like_long_ones(max_ctx, kw):
 kw = dict({kw!r}, table_stride=1 << 27)
 assert size(max_ctx={max_ctx}, **kw) == size(max_ctx=1 << 26, **kw) > size(max_ctx=16, **kw)
 """)
+
+
+@pytest.mark.parametrize("make", [make_norm, make_rope, make_attn])
+def test_calls_while_another_device_is_current_are_refused(lib, monkeypatch, make):
+    """The default stream's handle is the same on every device: a launch would go to the current one."""
+    op, call = make()
+    call(2)
+    monkeypatch.setattr(paged, "_current", lambda: 1)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="current device"):
+            call(2)
+    assert len(lib.calls) == 1
+
+
+def test_page_calls_while_another_device_is_current_are_refused(lib, monkeypatch):
+    table, lens, remap = (torch.zeros(n, dtype=torch.int32) for n in (2, 1, 4))
+    pages = paged.Pages(torch.zeros(4, 16, 8, dtype=torch.int16), table[None], lens, 16)
+    lib.q4gpu_pages_fork = lib.q4gpu_pages_compact = lambda *a: pytest.fail("launched")
+    monkeypatch.setattr(paged, "_current", lambda: 1)
+    with pytest.raises(ValueError, match="current device"):
+        pages.fork(lens, lens, lens)
+    with pytest.raises(ValueError, match="current device"):
+        pages.compact(table[None], remap, lens)
