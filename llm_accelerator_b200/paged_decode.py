@@ -64,6 +64,7 @@ class PagedDecoder:
                    "attn": Attention(k, v, self.cache.table, self.cache.lens, q_heads=HEADS), "k": k, "v": v}
             if eight_bit:
                 top = lay["gu"].float().abs().amax(1, keepdim=True) / 448.0
+                top[top == 0] = 1.0  # a row of zeros stays zeros
                 lay["gu8"] = (lay["gu"].float() / top).to(torch.float8_e4m3fn)
                 lay["gu8_scale"] = top.t().contiguous()
             self.layers.append(lay)

@@ -241,7 +241,7 @@ def test_cache_refuses_unknown_sequences(lib, monkeypatch, bad):
     assert c.lens.tolist() == [20, 1, 0] and c.length(0) == 20 and c.free_pages == 5
 
 
-def make_decoder(lib, monkeypatch, vocab=10):
+def make_decoder(lib, monkeypatch, vocab=10, **kw):
     from llm_accelerator_b200 import fp32_diag as F
     from llm_accelerator_b200 import paged_decode
     T, h = _native, 64
@@ -253,7 +253,7 @@ def make_decoder(lib, monkeypatch, vocab=10):
              T.T_UP: z(F.INTER, h), T.T_DOWN: z(h, F.INTER), T.T_INPUT_GAMMA: z(h), T.T_POST_GAMMA: z(h),
              T.T_Q_GAMMA: z(F.HEAD_DIM), T.T_K_GAMMA: z(F.HEAD_DIM)}
     return paged_decode.PagedDecoder({"embed": z(vocab, h), "final": z(h), "layers": [layer]}, max_seqs=2, max_ctx=64,
-                                     page_tokens=16, dtype=torch.half)
+                                     page_tokens=16, dtype=torch.half, **kw)
 
 
 @pytest.mark.parametrize("tokens", [[[3, 10]], [[-1]], [[1], [2 ** 40]]])
@@ -305,3 +305,10 @@ def test_page_calls_while_another_device_is_current_are_refused(lib, monkeypatch
         pages.fork(lens, lens, lens)
     with pytest.raises(ValueError, match="current device"):
         pages.compact(table[None], remap, lens)
+
+
+def test_decoder_8bit_weights_with_rows_of_zeros(lib, monkeypatch):
+    d = make_decoder(lib, monkeypatch, eight_bit=True)
+    lay = d.layers[0]
+    assert lay["gu8_scale"].isfinite().all()
+    assert not (lay["gu8"].float() * lay["gu8_scale"].t()).isnan().any()
