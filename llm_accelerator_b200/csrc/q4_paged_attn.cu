@@ -391,22 +391,22 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           if (s_last) __threadfence();
         }
         if (parts > 1 && s_last)
-        for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
-          const int r = x / D, d = x - r * D;
-          auto slot = [&](int k) { return (2 * (cta0 + k) + (k == 0)) * kRows + r; };
-          float top = -INFINITY, sum = 0.f, v = 0.f;
+          for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
+            const int r = x / D, d = x - r * D;
+            auto slot = [&](int k) { return (2 * (cta0 + k) + (k == 0)) * kRows + r; };
+            float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll 8
-          for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
-          const float base = top == -INFINITY ? 0.f : top;
+            for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
+            const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll 8
-          for (int k = 0; k < parts; ++k) {
-            const float2 w = __ldcg(&plan.ml[slot(k)]);
-            const float f = ex2(w.x - base);
-            sum = fmaf(w.y, f, sum);
-            v = fmaf(__ldcg(&plan.o[slot(k) * D + d]), f, v);
+            for (int k = 0; k < parts; ++k) {
+              const float2 w = __ldcg(&plan.ml[slot(k)]);
+              const float f = ex2(w.x - base);
+              sum = fmaf(w.y, f, sum);
+              v = fmaf(__ldcg(&plan.o[slot(k) * D + d]), f, v);
+            }
+            put(r, d, base, sum, v);
           }
-          put(r, d, base, sum, v);
-        }
         __syncthreads();  // the ring and the shared words are free for the next piece
       }
       if (++kvh == a.kv_heads) {
