@@ -200,7 +200,7 @@ int q4gpu_lm_head_argmax_noalloc(const int32_t *act, const uint8_t *packed, cons
  * enqueues on `stream` and returns without synchronising.  Strides count
  * elements.  Sums, softmax statistics and rotations are held in 32 bits and
  * each result is rounded once.  What only the device can check (a position, a
- * row, a page or a slot named in device memory) is checked there: the access
+ * row, a page, a slot or a length in device memory) is checked there: the access
  * is skipped and *err_flag (an optional device int that the caller zeroes) is
  * set to 1.
  * ======================================================================= */
@@ -308,6 +308,8 @@ int q4gpu_paged_attention(const q4gpu_attn_args *a, void *stream);
 /* A pool of pages and the tables that name them.  A page is page_bytes long:
  * blocks of block_bytes (one per layer, K/V and head), each page_tokens rows.
  * Slot s holds lens[s] tokens in pages table[s][0 .. ceil(lens[s] / page_tokens)).
+ * (A lens that its row of the table cannot hold sets *err_flag to 1; a fork of
+ * such a slot does nothing, compaction takes it as cut off.)
  * Pages, blocks and rows are multiples of 16 bytes. */
 typedef struct q4gpu_pages_args {
     void *pool;

@@ -457,6 +457,7 @@ __device__ __forceinline__ int64_t held(const q4gpu_pages_args& a, int64_t s) {
   const int64_t most = a.table_stride * a.page_tokens, n = a.lens[s];
   return n < 0 ? 0 : (n < most ? n : most);
 }
+__device__ __forceinline__ bool fits(const q4gpu_pages_args& a, int64_t s) { return a.lens[s] == held(a, s); }
 
 // blockIdx.y = fork, blockIdx.x strides over the page's blocks.  Only filled rows
 // are copied; forks of one parent read it from L2.  Bound by memory: 48 forks of
@@ -470,6 +471,7 @@ __global__ void __launch_bounds__(128) pages_fork_kernel(q4gpu_pages_args a, con
   int64_t n = 0;
   int part = 0, source = 0, to = 0;
   int64_t last = -1;
+  ok = ok && fits(a, par);
   if (ok) {
     n = held(a, par);
     part = (int)(n % a.page_tokens);
@@ -524,6 +526,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(q4gpu_pages_ar
   __syncthreads();
   for (int s = t >> 5; s < a.n_slots; s += kPlanThreads / 32) {
     const int64_t used = (held(a, s) + a.page_tokens - 1) / a.page_tokens;
+    if (a.err_flag && !fits(a, s)) *a.err_flag = 1;
     for (int64_t c = t & 31; c < used; c += 32) {
       const int id = a.table[s * a.table_stride + c];
       if (id >= 0 && id < a.n_pages)
@@ -637,6 +640,7 @@ __global__ void __launch_bounds__(512) pages_compact_kernel(q4gpu_pages_args a, 
   __syncthreads();
   for (int s = t >> 5; s < a.n_slots; s += blockDim.x / 32) {
     const int64_t used = (held(a, s) + a.page_tokens - 1) / a.page_tokens;
+    if (a.err_flag && !fits(a, s)) *a.err_flag = 1;
     for (int64_t c = lane; c < used; c += 32) {
       const int id = a.table[s * a.table_stride + c];
       if (id >= 0 && id < a.n_pages)

@@ -15,7 +15,8 @@ if not torch.cuda.is_available():
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
 from llm_accelerator_b200 import _native, paged  # noqa: E402
-from test_gpu_paged import BF, HF, SF, TINY, U, angles, attn_ref, i32, make, norm_ref, rnd, rope_ref, within  # noqa: E402
+from test_gpu_paged import (BF, HF, SF, TINY, U, angles, attn_ref, i32, make, norm_ref, pages_of, rnd,  # noqa: E402
+                            rope_ref, within)
 
 
 def operator(pool, table, lens, hq, **kw):
@@ -428,3 +429,24 @@ def test_attention_mixed_step_captured():
             graph.replay()
             close(out, lse, *attn_ref(pool, table, lens, c, x, 128 ** -0.5, 0, ids), BF)
         assert not reported(op)
+
+
+@pytest.mark.parametrize("n", [-1, 3 * 16 + 1, 2 ** 31 - 1])
+def test_pages_report_lengths_that_no_row_of_the_table_holds(n):
+    pool, table, lens = pages_of(8, 2, 16, 8, 4, 3)
+    table[0, 0], lens[0] = 5, 7
+    table[1] = i32([1, 2, 3])
+    lens[1] = n
+    before, tb, kept = pool.clone(), table.clone(), lens.clone()
+    op = paged.Pages(pool, table, lens, 16)
+    op.fork(i32([1]), i32([2]), i32([4]))
+    assert reported(op)
+    assert torch.equal(pool, before) and torch.equal(table, tb) and torch.equal(lens, kept)
+    op.fork(i32([0]), i32([2]), i32([4]))
+    assert not reported(op) and int(lens[2]) == 7
+    for new in (torch.empty_like(table), table):
+        op.compact(new, torch.empty(8, dtype=torch.int32, device="cuda"), i32([0]))
+        assert reported(op)
+    lens[1] = 0
+    op.compact(torch.empty_like(table), torch.empty(8, dtype=torch.int32, device="cuda"), i32([0]))
+    assert not reported(op)
