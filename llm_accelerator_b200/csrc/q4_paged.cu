@@ -117,9 +117,11 @@ __host__ __device__ constexpr bool norm_ahead() { return sizeof(T) == 2 && V == 
 // time per CTA (1 unless a row is one warp).  A thread holds E values of its
 // row, V consecutive ones at a time, so x and the residual are read once.  Where
 // registers allow it (norm_ahead) CTAs stay and go from row to row: the next
-// row's values are on their way while this one is summed, scaled and stored.  Maxima pass NaNs on, so one reaches
-// the scale.  Bound by memory: 8192 x 4096 bf16 with a residual into e4m3 moves
-// 237 MB in 49 us, 4.8 TB/s.
+// row's values are on their way while this one is summed, scaled and stored.
+// Maxima pass NaNs on, so one reaches the scale.  8192 x 4096 bf16 with a
+// residual into e4m3 moves 237 MB in 49.5 us, 4.8 TB/s; the SMs' busiest pipe is
+// at 65 % and 27 of 64 warps are resident, so a row's chain of steps shows beside
+// the memory.
 template <typename T, int OUT, int V, int E>
 __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(NormParams p) {
   constexpr int N = E / V;
@@ -460,8 +462,9 @@ __device__ __forceinline__ int64_t held(const q4gpu_pages_args& a, int64_t s) {
 __device__ __forceinline__ bool fits(const q4gpu_pages_args& a, int64_t s) { return a.lens[s] == held(a, s); }
 
 // blockIdx.y = fork, blockIdx.x strides over the page's blocks.  Only filled rows
-// are copied; forks of one parent read it from L2.  Bound by memory: 48 forks of
-// 12 prompts write 111 MB in 28 us.
+// are copied; forks of one parent read it from L2.  48 forks of 12 prompts
+// write 111 MB in 30 us; half of a warp's time between instructions is the wait for
+// its loads.
 __global__ void __launch_bounds__(128) pages_fork_kernel(q4gpu_pages_args a, const int32_t* parents,
                                                          const int32_t* children, const int32_t* fresh) {
   const int i = blockIdx.y;
@@ -613,8 +616,8 @@ __device__ __forceinline__ void move_pages(const q4gpu_pages_args& a, int count,
 
 // Renumbers the tables and copies the moved pages, kMoveBytes at a time.
 // Sources lie at or past the packed end and destinations below it, so no copy
-// reads what another writes.  Bound by memory: 0.55 GB of pages move in 178 us, 6.2
-// TB/s read and written.
+// reads what another writes.  Bound by memory: 0.55 GB of pages move in 176 to
+// 192 us, 6.2 to 5.7 TB/s read and written.
 __global__ void __launch_bounds__(512) pages_move_kernel(q4gpu_pages_args a, int32_t* new_table, const int32_t* remap,
                                                          const int32_t* n_moves, const int2* moves) {
   const int64_t entries = (int64_t)a.n_slots * a.table_stride;

@@ -109,7 +109,7 @@ __device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int gro
 // maximum and sum, so no barrier stands in the loop; the eight are joined at its
 // end.  (Eight warps and one CTA per SM for heads of 128, two for 64; four warps
 // and twice the CTAs start short pieces a little faster, 64 decodes at 1 to 8704
-// keys 55.6 us against 56.8, but take 33.0 against 24.0 for one at 16384 and 122
+// keys 55.6 us against 57.0, but take 33.0 against 24.0 for one at 16384 and 122
 // against 94 for 16 of 64-value heads.)  Bound by memory: every key and value is
 // read once, for all heads of its group; 16 decodes at 16384 keys stream 6.1 TB/s.
 template <typename T, int D>

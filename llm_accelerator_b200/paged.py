@@ -339,7 +339,8 @@ class Attention(_Err):
                  seq_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q [tokens, q_heads, dim]; cu_q int32 [sequences + 1]: sequence i has the query
         tokens cu_q[i] .. cu_q[i + 1] - 1, at most max_q; seq_ids int32 [sequences]: their
-        slots (default: 0, 1, ..); max_ctx: no lens is larger (0: the table's width).
+        slots (default: 0, 1, ..); max_ctx: no lens is larger (0: the table's width).  A
+        sequence with more than max_q tokens is an error that `check` reports.
         lse (optional) float32 [tokens, q_heads] receives log sum exp of the scores."""
         with self.lock:
             a = self.args

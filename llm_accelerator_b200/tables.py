@@ -54,7 +54,11 @@ def rope_float_tables(n_positions: int, rot_dim: int = HEAD_DIM, theta: float = 
     ``original * inv_freq_i / 2 pi`` times over the ``original`` (trained) positions, by default
     n_positions / factor; pairs that turn more than 32 times keep their frequency, those below
     one turn are slowed by ``factor``, in between the two are mixed in proportion, and both
-    tables are scaled by 0.1 ln(factor) + 1.  (The reference has 256 positions and no scaling.)
+    tables are scaled by 0.1 ln(factor) + 1.  That is the published formula, a mix in proportion to
+    the number of turns; a checkpoint that was stretched by a mix in proportion to the pair's index
+    between the two limits has other frequencies in between (16 of 64, by up to 42 %, for 128
+    values, theta 1e6, 32768 trained positions, factor 4) and needs tables of its own, which ``paged.RopeAppend`` takes as
+    they are.  (The reference has 256 positions and no scaling.)
     """
     if rot_dim < 2 or rot_dim % 2 or n_positions < 1 or factor < 1.0:
         raise ValueError(f"no rotary table of {n_positions} positions x {rot_dim}, factor {factor}")
