@@ -312,3 +312,10 @@ def test_decoder_8bit_weights_with_rows_of_zeros(lib, monkeypatch):
     lay = d.layers[0]
     assert lay["gu8_scale"].isfinite().all()
     assert not (lay["gu8"].float() * lay["gu8_scale"].t()).isnan().any()
+
+
+def test_table_pages_refusals_and_default():
+    child("""
+assert lib.q4gpu_paged_attention(attn(table_pages=-1), None) == -1001 and size(table_pages=-1) == 0
+assert size(table_pages=5) == size() > 0
+""")
