@@ -305,6 +305,14 @@ typedef struct q4gpu_attn_args {
 size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args *a);
 int q4gpu_paged_attention(const q4gpu_attn_args *a, void *stream);
 
+/* The same through a window whose sequences' first `sinks` keys stay visible:
+ * query t at position p sees keys j <= p with j > p - window or j < sinks.
+ * Pages that hold neither a sink nor a key of some query's window are not read
+ * (their table entries may be -1).  window = 0 or sinks = 0:
+ * q4gpu_paged_attention. */
+size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args *a, int32_t sinks);
+int q4gpu_sink_attention(const q4gpu_attn_args *a, int32_t sinks, void *stream);
+
 /* A pool of pages and the tables that name them.  A page is page_bytes long:
  * blocks of block_bytes (one per layer, K/V and head), each page_tokens rows.
  * Slot s holds lens[s] tokens in pages table[s][0 .. ceil(lens[s] / page_tokens)).

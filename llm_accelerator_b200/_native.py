@@ -158,6 +158,8 @@ SIGNATURES = {
     "q4gpu_rope_append": (C.c_int, [C.POINTER(RopeArgs), P]),
     "q4gpu_paged_attention_workspace_bytes": (SZ, [C.POINTER(AttnArgs)]),
     "q4gpu_paged_attention": (C.c_int, [C.POINTER(AttnArgs), P]),
+    "q4gpu_sink_attention_workspace_bytes": (SZ, [C.POINTER(AttnArgs), I32]),
+    "q4gpu_sink_attention": (C.c_int, [C.POINTER(AttnArgs), I32, P]),
     "q4gpu_pages_fork": (C.c_int, [C.POINTER(PagesArgs), P, P, P, I32, P]),
     "q4gpu_pages_compact_workspace_bytes": (SZ, [I32]),
     "q4gpu_pages_compact": (C.c_int, [C.POINTER(PagesArgs), P, P, P, P, SZ, P]),

@@ -1,5 +1,5 @@
 // Attention of each sequence's newest tokens to its pages (16-bit paged
-// serving operators, include/q4gpu.h: q4gpu_paged_attention).
+// serving operators, include/q4gpu.h: q4gpu_paged_attention, q4gpu_sink_attention).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -92,16 +92,26 @@ struct RowPlan {
 };
 
 // Keys that the kernel below walks for sequence i, from `lo` on; -1: not its
-// sequence (no queries, or more rows than a tile).
-__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const Seq& s, int group, int& lo) {
+// sequence (no queries, or more rows than a tile).  With sinks the walk starts
+// at key 0 and leaves out `gap.skip` keys from key gap.from on.
+template <int MODE>
+__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const More& x, const Seq& s, int group, int& lo,
+                                        Gap& gap) {
   lo = 0;
+  gap = Gap{0, 0};
   if (s.n == 0 || s.n > kRows / group) return -1;
   if (a.window > 0) lo = first_seen(s.len - s.n, a.window) & ~(kTileKeys - 1);
-  return max(0, s.len - lo);
+  if constexpr (MODE == kSinks) {
+    gap = gap_before(lo, x.sinks, kTileKeys);
+    lo = 0;
+  }
+  return max(0, s.len - gap.skip - lo);
 }
-__device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int group) {  // of one head
+template <int MODE>
+__device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, const More& x, int i, int group) {  // of one head
   int lo;
-  const int keys = row_keys(a, sequence(a, i), group, lo);
+  Gap gap;
+  const int keys = row_keys<MODE>(a, x, sequence(a, i), group, lo, gap);
   return keys < 0 ? 0 : kPieceCost + (keys + kUnitKeys - 1) / kUnitKeys;
 }
 
@@ -112,8 +122,8 @@ __device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, int i, int gro
 // keys 55.6 us against 57.0, but take 33.0 against 24.0 for one at 16384 and 122
 // against 94 for 16 of 64-value heads.)  Bound by memory: every key and value is
 // read once, for all heads of its group; 16 decodes at 16384 keys stream 6.1 TB/s.
-template <typename T, int D>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, RowPlan plan) {
+template <typename T, int D, int MODE>
+__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, More x, RowPlan plan) {
   constexpr int kThreads = kRowWarps * 32;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float s_m[kRowWarps][kRows], s_l[kRowWarps][kRows];
@@ -133,7 +143,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   for (int i = run0; i < run1; ++i) {
     over |= alone && sequence(a, i).n > kRows / group;
     if (blockIdx.x == 0 && a.err_flag && !sequence_ok(a, i)) *a.err_flag = 1;
-    const int c = row_cost(a, i, group);
+    const int c = row_cost<MODE>(a, x, i, group);
     mine_cost += (int64_t)c * a.kv_heads;
     most = max(most, c);
   }
@@ -163,14 +173,15 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   if (first_unit < last_unit) {
     if (before <= first_unit && first_unit < before + mine_cost) {  // one thread's run holds it
       int i = run0;
-      for (int64_t c; before + (c = (int64_t)row_cost(a, i, group) * a.kv_heads) <= first_unit; ++i) before += c;
+      for (int64_t c; before + (c = (int64_t)row_cost<MODE>(a, x, i, group) * a.kv_heads) <= first_unit; ++i) before += c;
       s_seq = i, s_start = before;
     }
     __syncthreads();
     int seq = s_seq, lo;
+    Gap gap;
     int64_t start = s_start;  // where the sequence's first head begins
     Seq s = sequence(a, seq);
-    int keys = row_keys(a, s, group, lo), cost = row_cost(a, seq, group), kvh = (int)quotient(first_unit - start, cost);
+    int keys = row_keys<MODE>(a, x, s, group, lo, gap), cost = row_cost<MODE>(a, x, seq, group), kvh = (int)quotient(first_unit - start, cost);
     for (;;) {
       const int64_t head_start = start + (int64_t)kvh * cost + kPieceCost;  // of its first real unit
       if (head_start - kPieceCost >= last_unit) break;
@@ -184,7 +195,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
                       cta1 = units == 0 ? cta0 : quotient(head_start + units - 1, stretch);
         const int parts = (int)(cta1 - cta0) + 1, part = (int)(blockIdx.x - cta0);
         const int pos0 = s.len - s.n, pos1 = s.len - 1;  // of the first and the last query
-        const int begin = lo + u0 * kUnitKeys, end = min(s.len, lo + u1 * kUnitKeys);
+        // along the walk; key_at gives the key
+        const int begin = lo + u0 * kUnitKeys, end = min(s.len - gap.skip, lo + u1 * kUnitKeys);
+        auto key_at = [&](int walk) { return MODE == kSinks && walk >= gap.from ? walk + gap.skip : walk; };
+        auto unseen = [&](int j, int p) {
+          return j > p || (a.window > 0 && j <= p - a.window && (MODE != kSinks || j >= x.sinks));
+        };
 
         // the queries as A fragments: row g and g + 8, 16 values of a head per step
         const int g = lane >> 2, tq = lane & 3;
@@ -211,7 +227,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         const int shift = 31 - __clz(a.page_tokens);
         auto page_of = [&](int i) {
           if (i >= mine) return -1;
-          const int p = table[(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
+          const int p = table[key_at(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
           if (p >= 0 && p < a.n_pages) return p;
           if (a.err_flag) *a.err_flag = 1;
           return -1;
@@ -223,7 +239,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           next_page = page_of(i + 1);
           if (i < mine) valid = (valid & ~(1u << (i & 31))) | ((page >= 0 ? 1u : 0u) << (i & 31));
           if (i < mine && page >= 0) {
-            const int key = begin + kTileKeys * (warp + kRowWarps * i);
+            const int walk = begin + kTileKeys * (warp + kRowWarps * i), key = key_at(walk);
             const int64_t off = page * a.page_stride + kvh * a.head_stride + (key & (a.page_tokens - 1)) * a.row_stride;
             const uint32_t at = ring + (i % kRowStages) * 2 * kTileBytes;
             constexpr int kPieces = D / 8, kPer = 32 / kPieces;  // lanes per row, rows per pass
@@ -232,7 +248,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
             for (int r0 = 0; r0 < kTileKeys; r0 += kPer) {
               const int r = r0 + lane / kPieces;
               // rows past the last key are zeros: whatever the page holds there meets a zero weight
-              const bool there = key + r < end;
+              const bool there = walk + r < end;
               const int64_t o = off + (there ? r : 0) * a.row_stride + c * 8;
               cp16(at + piece<D>(r, c), static_cast<const T*>(a.k_cache) + o, there);
               cp16(at + kTileBytes + piece<D>(r, c), static_cast<const T*>(a.v_cache) + o, there);
@@ -253,7 +269,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           load(i + kRowStages - 1);
           if (!((valid >> (i & 31)) & 1u)) continue;
           const uint32_t kt = ring + (i % kRowStages) * 2 * kTileBytes, vt = kt + kTileBytes;
-          const int key = begin + kTileKeys * (warp + kRowWarps * i);
+          const int key = key_at(begin + kTileKeys * (warp + kRowWarps * i));
           float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -263,7 +279,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
             mma16816<T>(sc[1], qf[k], b[2], b[3]);
           }
           // element e of sc[n]: row g + 8 (e / 2), key 8 n + 2 tq + e % 2
-          const bool whole = key + kTileKeys <= pos0 + 1 && (a.window == 0 || key > pos1 - a.window);
+          const bool whole = key + kTileKeys <= pos0 + 1 &&
+                             (a.window == 0 || key > pos1 - a.window || (MODE == kSinks && key + kTileKeys <= x.sinks));
           float top[2] = {m[0], m[1]};
 #pragma unroll
           for (int n = 0; n < 2; ++n)
@@ -272,7 +289,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
               float v = sc[n][e] * c2;
               if (!whole) {
                 const int j = key + 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
-                if (j > p || (a.window > 0 && j <= p - a.window)) v = -INFINITY;
+                if (unseen(j, p)) v = -INFINITY;
               }
               sc[n][e] = v;
               top[e >> 1] = fmaxf(top[e >> 1], v);
@@ -300,11 +317,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
             for (int e = 0; e < 4; ++e) o[n][e] *= shrink[e >> 1];
           // Some rows see a key of this step and some do not: an infinity or NaN in its value row may reach only the
           // former, and a product would carry it to both (0 times infinity).  Such values are added by hand and zeroed.
-          if (key + kTileKeys > pos0 + 1 || (a.window > 0 && key <= pos1 - a.window)) {
+          if (!whole) {
             unsigned char* v = smem + (vt - (uint32_t)__cvta_generic_to_shared(smem));
             bool odd = false;
-            for (int x = lane; x < kTileKeys * D; x += 32)
-              odd |= !isfinite(to_f32(*reinterpret_cast<const T*>(v + x * 2)));
+            for (int i = lane; i < kTileKeys * D; i += 32)
+              odd |= !isfinite(to_f32(*reinterpret_cast<const T*>(v + i * 2)));
             if (__any_sync(~0u, odd)) {
               for (int j = 0; j < kTileKeys; ++j)
 #pragma unroll
@@ -312,12 +329,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
                     const int col = 8 * n + 2 * tq + (e & 1), p = row_pos[e >> 1];
-                    const float x = to_f32(*reinterpret_cast<const T*>(v + piece<D>(j, col / 8) + (col % 8) * 2));
-                    if (!isfinite(x) && key + j <= p && (a.window == 0 || key + j > p - a.window)) o[n][e] += x;
+                    const float f = to_f32(*reinterpret_cast<const T*>(v + piece<D>(j, col / 8) + (col % 8) * 2));
+                    if (!isfinite(f) && !unseen(key + j, p)) o[n][e] += f;
                   }
               __syncwarp();
-              for (int x = lane; x < kTileKeys * D; x += 32) {
-                T* at = reinterpret_cast<T*>(v + x * 2);
+              for (int i = lane; i < kTileKeys * D; i += 32) {
+                T* at = reinterpret_cast<T*>(v + i * 2);
                 if (!isfinite(to_f32(*at))) *at = from_f32<T>(0.f);
               }
               __syncwarp();
@@ -360,8 +377,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           if (a.lse && d == 0)
             a.lse[(int64_t)(s.first + t) * a.q_heads + head] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
         };
-        for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
-          const int r = x / D, d = x - r * D;
+        for (int i = threadIdx.x; i < rows * D; i += kRowWarps * 32) {
+          const int r = i / D, d = i - r * D;
           float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll
           for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
@@ -391,8 +408,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           if (s_last) __threadfence();
         }
         if (parts > 1 && s_last)
-          for (int x = threadIdx.x; x < rows * D; x += kRowWarps * 32) {
-            const int r = x / D, d = x - r * D;
+          for (int i = threadIdx.x; i < rows * D; i += kRowWarps * 32) {
+            const int r = i / D, d = i - r * D;
             auto slot = [&](int k) { return (2 * (cta0 + k) + (k == 0)) * kRows + r; };
             float top = -INFINITY, sum = 0.f, v = 0.f;
 #pragma unroll 8
@@ -415,8 +432,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         do {
           if (++seq >= a.n_seqs) break;
           s = sequence(a, seq);
-          keys = row_keys(a, s, group, lo);
-          cost = row_cost(a, seq, group);
+          keys = row_keys<MODE>(a, x, s, group, lo, gap);
+          cost = row_cost<MODE>(a, x, seq, group);
         } while (cost == 0);
         if (seq >= a.n_seqs) break;
       }
@@ -426,10 +443,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
     for (int i = blockIdx.x; i < a.n_seqs; i += gridDim.x) {
       const Seq s = sequence(a, i);
       if (s.n <= kRows / group) continue;
-      for (int64_t x = threadIdx.x; x < (int64_t)s.n * a.q_heads * D; x += kThreads) {
-        const int64_t row = x / D, t = s.first + row / a.q_heads, head = row % a.q_heads;
-        static_cast<T*>(a.out)[t * a.out_token_stride + head * a.out_head_stride + x % D] = from_f32<T>(0.f);
-        if (a.lse && x % D == 0) a.lse[t * a.q_heads + head] = -INFINITY;
+      for (int64_t e = threadIdx.x; e < (int64_t)s.n * a.q_heads * D; e += kThreads) {
+        const int64_t row = e / D, t = s.first + row / a.q_heads, head = row % a.q_heads;
+        static_cast<T*>(a.out)[t * a.out_token_stride + head * a.out_head_stride + e % D] = from_f32<T>(0.f);
+        if (a.lse && e % D == 0) a.lse[t * a.q_heads + head] = -INFINITY;
       }
     }
 }
@@ -500,7 +517,7 @@ RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
 // the last wave of many items in two evens the SMs out, 348 steps on the longest
 // instead of 370 for 8192 tokens over 16384 keys, but the parts' traffic and the
 // join took more: 814 us against 771.)
-ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
+ChunkPlan chunk_plan(const q4gpu_attn_args& a, const More& x, size_t* bytes) {
   ChunkPlan p{};
   const int64_t group = a.q_heads / a.kv_heads;
   if (a.max_q * group <= kRows || a.n_seqs == 0 || a.tokens == 0) {  // nothing for the chunk kernel
@@ -512,7 +529,8 @@ ChunkPlan chunk_plan(const q4gpu_attn_args& a, size_t* bytes) {
   const int64_t rows = a.tokens * group;
   p.tiles = (int)std::min<int64_t>(a.n_seqs == 1 ? (rows + kPair - 1) / kPair : rows / kPair + a.n_seqs, INT32_MAX);
   const int64_t items = (int64_t)p.tiles * a.kv_heads;
-  const int64_t span = a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + kPair + kNTile) : a.max_ctx;
+  const int64_t span =
+      a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + kPair + kNTile + x.sinks) : a.max_ctx;
   p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / items, span / kMinPart));
   if (bytes) *bytes = p.parts > 1 ? (size_t)p.tiles * a.kv_heads * p.parts * kPair * (8 + (size_t)a.dim * 4) : 0;
   return p;
@@ -556,18 +574,18 @@ int allow_smem(const void* kernel, int bytes, unsigned char* ready) {
   return Q4GPU_OK;
 }
 
-template <typename T, int D>
-int launch(const q4gpu_attn_args& a, cudaStream_t s) {
+template <typename T, int D, int MODE>
+int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
   static unsigned char ready[2][Q4GPU_MAX_DEVICES];
   size_t rows_bytes;
   const RowPlan few = row_plan(a, static_cast<char*>(a.workspace), &rows_bytes);
   const bool chunks = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows;
-  ChunkPlan plan = chunk_plan(a, nullptr);
+  ChunkPlan plan = chunk_plan(a, x, nullptr);
   if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
   const bool short_ones = !chunks || plan.least > 1;  // sequences for attn_rows_kernel
   int rc = Q4GPU_OK;
   if (short_ones) {
-    rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D>), row_smem<D>(), ready[0]);
+    rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D, MODE>), row_smem<D>(), ready[0]);
     if (rc != Q4GPU_OK) return rc;
   }
   CUtensorMap kmap, vmap;
@@ -578,10 +596,10 @@ int launch(const q4gpu_attn_args& a, cudaStream_t s) {
     rc = encode_map(&kmap, a, a.k_cache);
     if (rc == Q4GPU_OK) rc = encode_map(&vmap, a, a.v_cache);
     if (rc == Q4GPU_OK)
-      rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D>), chunk_smem<D>(), ready[1]);
+      rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D, MODE>), chunk_smem<D>(), ready[1]);
     if (rc != Q4GPU_OK) return rc;
   }
-  if (short_ones) attn_rows_kernel<T, D><<<few.ctas, kRowWarps * 32, row_smem<D>(), s>>>(a, few);
+  if (short_ones) attn_rows_kernel<T, D, MODE><<<few.ctas, kRowWarps * 32, row_smem<D>(), s>>>(a, x, few);
   if (chunks) {
     // starts beside the short sequences' kernel, on the SMs that it leaves free
     cudaLaunchAttribute attr[1];
@@ -594,38 +612,56 @@ int launch(const q4gpu_attn_args& a, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = short_ones ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_chunk_kernel<T, D>, kmap, vmap, a, plan);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_chunk_kernel<T, D, MODE>, kmap, vmap, a, x, plan);
     if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: launch: %s", cudaGetErrorString(e));
-    if (plan.parts > 1) attn_join_kernel<T, D><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, plan);
+    if (plan.parts > 1) attn_join_kernel<T, D, MODE><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, x, plan);
   }
   return q4gpu_check_launch();
+}
+
+template <int MODE>
+int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
+  if (a.dtype == Q4GPU_F16) return a.dim == 64 ? launch<__half, 64, MODE>(a, x, s) : launch<__half, 128, MODE>(a, x, s);
+  return a.dim == 64 ? launch<__nv_bfloat16, 64, MODE>(a, x, s) : launch<__nv_bfloat16, 128, MODE>(a, x, s);
+}
+
+// Sinks as the kernels take them: without a window every key is seen anyway.
+More settled_sinks(const q4gpu_attn_args& settled, int32_t sinks) {
+  More x{};
+  x.sinks = settled.window > 0 ? sinks : 0;
+  return x;
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args* a) {
-  if (check_sizes(a) != Q4GPU_OK) return 0;
+size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args* a, int32_t sinks) {
+  if (check_sizes(a) != Q4GPU_OK || sinks < 0) return 0;
   const q4gpu_attn_args b = settled(*a);
   size_t rows, chunks;
   row_plan(b, nullptr, &rows);
-  chunk_plan(b, &chunks);
+  chunk_plan(b, settled_sinks(b, sinks), &chunks);
   return (rows + 15) / 16 * 16 + chunks;
 }
 
-int q4gpu_paged_attention(const q4gpu_attn_args* a, void* stream) {
+int q4gpu_sink_attention(const q4gpu_attn_args* a, int32_t sinks, void* stream) {
   const int rc = check_attn(a);
   if (rc != Q4GPU_OK) return rc;
+  if (sinks < 0) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: %d sinks", sinks);
   if (a->n_seqs == 0 || a->tokens == 0) return Q4GPU_OK;
-  const size_t need = q4gpu_paged_attention_workspace_bytes(a);
+  const size_t need = q4gpu_sink_attention_workspace_bytes(a, sinks);
   if (a->workspace_bytes < need || (need && !a->workspace))
     return q4gpu_fail(Q4GPU_ERR_WORKSPACE, "attention: needs a workspace of %zu bytes", need);
   if (!aligned(a->workspace, 16)) return q4gpu_fail(Q4GPU_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
   const q4gpu_attn_args b = settled(*a);
-  cudaStream_t s = as_stream(stream);
-  if (b.dtype == Q4GPU_F16) return b.dim == 64 ? launch<__half, 64>(b, s) : launch<__half, 128>(b, s);
-  return b.dim == 64 ? launch<__nv_bfloat16, 64>(b, s) : launch<__nv_bfloat16, 128>(b, s);
+  const More x = settled_sinks(b, sinks);
+  return x.sinks ? launch<kSinks>(b, x, as_stream(stream)) : launch<kPlain>(b, x, as_stream(stream));
 }
+
+size_t q4gpu_paged_attention_workspace_bytes(const q4gpu_attn_args* a) {
+  return q4gpu_sink_attention_workspace_bytes(a, 0);
+}
+int q4gpu_paged_attention(const q4gpu_attn_args* a, void* stream) { return q4gpu_sink_attention(a, 0, stream); }
 
 }  // extern "C"

@@ -36,6 +36,24 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
 // Keys that a slot's row of the table can name.
 __device__ __forceinline__ int64_t most_keys(const q4gpu_attn_args& a) { return (int64_t)a.table_pages * a.page_tokens; }
 
+// Which keys a query sees: those up to its own (through a window the last of them), or those and the first few keys of
+// the sequence as well.
+enum Mode { kPlain, kSinks };
+struct More {  // what the modes need besides the arguments they share
+  int sinks;   // kSinks: the first keys that every query sees
+};
+// A walk over a sequence's keys that leaves out `skip` keys from key `from` on.
+struct Gap {
+  int from, skip;
+};
+// Between the sinks, rounded up to whole steps of the walk, and the first key `lo` (a multiple of the step) of a window.
+__device__ __forceinline__ Gap gap_before(int lo, int sinks, int step) {
+  Gap g;
+  g.from = (int)min((int64_t)lo, ((int64_t)sinks + step - 1) & ~(int64_t)(step - 1));
+  g.skip = lo - g.from;
+  return g;
+}
+
 // First key that a query at position pos (negative: before all keys) sees through a window.
 __device__ __forceinline__ int first_seen(int pos, int window) { return (int)max((int64_t)0, (int64_t)pos - window + 1); }
 
@@ -64,7 +82,7 @@ __device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int gro
   const bool known = t.slot >= 0 && t.slot < a.n_slots;
   t.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[t.slot], most_keys(a))) : 0;
   if (t.n < least) return 0;
-  keys = a.window > 0 ? min(t.len, a.window) : t.len;
+  keys = a.window > 0 ? min(t.len, a.window) : t.len;  // (of sinks there are few)
   return (int)(((int64_t)t.n * group + kPair - 1) / kPair);
 }
 // The pair of grid row y; seq = -1 where there are fewer.  By one full warp.
@@ -121,6 +139,21 @@ __device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int lea
     before += __shfl_sync(~0u, run, 31);
   }
   return t;
+}
+
+// The walk of a row pair whose rows see keys lo .. hi - 1, and the sinks before those.
+struct Span {
+  int begin, end;
+  Gap gap;
+};
+template <int MODE>
+__device__ __forceinline__ Span span_of(int lo, int hi, const More& more) {
+  const int base = lo & ~(kNTile - 1);
+  if constexpr (MODE == kSinks) {
+    const Gap gap = gap_before(base, more.sinks, kNTile);
+    return Span{0, hi - gap.skip, gap};
+  }
+  return Span{base, hi, Gap{0, 0}};
 }
 
 // ---- tensor memory, 32 columns at a time ---------------------------------------
@@ -264,13 +297,13 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 
 // A share of a value tile's cleaning by one thread of `threads`: 16-byte pieces of
 // the rows that not every query sees (keys outside all_lo .. all_hi - 1; all rows
-// where pages may be missing, then `table` is given).  Rows outside lo .. end and
-// of missing pages become zeros, and so do infinities and NaNs in the others;
+// where pages may be missing, then `table` is given).  Rows outside lo .. end
+// (but for the first `sinks`) and of missing pages become zeros, and so do infinities and NaNs in the others;
 // true if there were any.  Out of line: few steps come here, and the registers it
 // takes cost the steps that do not.
 template <typename T, int D>
 __device__ __noinline__ bool clean_values(unsigned char* v, int key, int lo, int all_lo, int all_hi, int end,
-                                          const int32_t* table, int shift, int n_pages, int threads) {
+                                          int sinks, const int32_t* table, int shift, int n_pages, int threads) {
   constexpr int kPieces = D / 8;
   // an all-ones exponent carries into the bit above it when one is added at its lowest bit
   constexpr bool kBf16 = !__is_same(T, __half);
@@ -282,7 +315,7 @@ __device__ __noinline__ bool clean_values(unsigned char* v, int key, int lo, int
   for (int x = threadIdx.x; x < (r0 + kNTile - r1) * kPieces; x += threads) {
     const int c = x % kPieces, y = x / kPieces, r = y < r0 ? y : y - r0 + r1, k = key + r;
     uint4* w = reinterpret_cast<uint4*>(v + (c / 8) * (kNTile * 128) + r * 128 + (c & 7) * 16);
-    bool zero = k < lo || k >= end;
+    bool zero = (k < lo && k >= sinks) || k >= end;
     if (table && !zero) zero = table[k >> shift] < 0 || table[k >> shift] >= n_pages;
     const uint4 b = *w;
     const uint32_t u[4] = {b.x, b.y, b.z, b.w};
@@ -315,10 +348,11 @@ __device__ __noinline__ bool clean_values(unsigned char* v, int key, int lo, int
 // against 726.  O is rescaled only when a row's maximum grows by more than 8 (in
 // log2): until then P <= 2^8, which 16-bit weights and 32-bit sums hold without
 // loss.
-template <typename T, int D>
+template <typename T, int D, int MODE>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attn_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                      const __grid_constant__ q4gpu_attn_args a, const __grid_constant__ ChunkPlan plan) {
+                      const __grid_constant__ q4gpu_attn_args a, const __grid_constant__ More more,
+                      const __grid_constant__ ChunkPlan plan) {
   using namespace umma;
   constexpr int kStages = chunk_stages<D>();
   constexpr int kLines = D / 64;                  // 128-byte lines of a head vector
@@ -358,11 +392,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // keys that some row sees, and those that every row sees
   const int lo = a.window > 0 ? first_seen(pos0, a.window) : 0, hi = max(0, pos1 + 1);
   const int all_lo = a.window > 0 ? first_seen(pos1, a.window) : 0, all_hi = pos0 + 1;
-  const int base = lo & ~(kNTile - 1);
-  const int chunk = part_keys(plan, hi - base);
-  const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
+  const Span span = span_of<MODE>(lo, hi, more);
+  const int chunk = part_keys(plan, span.end - span.begin);
+  const int parts = span.end > span.begin ? (span.end - span.begin + chunk - 1) / chunk : 1;
   if (part >= parts) return wait_before();
-  const int begin = base + part * chunk, end = min(hi, begin + chunk);
+  const int begin = span.begin + part * chunk, end = min(span.end, begin + chunk);
+  // `begin`, `end` and what lies between are places of the walk; the key that stands there:
+  auto key_at = [&](int walk) { return MODE == kSinks && walk >= span.gap.from ? walk + span.gap.skip : walk; };
   const int steps = begin < end ? (end - begin + kNTile - 1) / kNTile : 0;
   const int subs = begin < end ? (end - begin + kStep - 1) / kStep : 0;
   const int tiles = rows > kMTile ? 2 : 1;
@@ -380,9 +416,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     bar_init_fence();
   }
   // the first keys are on their way before the queries are
-  auto pages_of = [&](int key, int& id) {  // which pages of the load at `key` exist; lane p gets page p's number
-    const int pages = min(kNTile >> shift, (int)((end - key + a.page_tokens - 1) >> shift));
-    id = lane < pages ? table[(key >> shift) + lane] : -1;
+  auto pages_of = [&](int walk, int& id) {  // which pages of the load at `walk` exist; lane p gets page p's number
+    const int pages = min(kNTile >> shift, (int)((end - walk + a.page_tokens - 1) >> shift));
+    id = lane < pages ? table[(key_at(walk) >> shift) + lane] : -1;
     return __ballot_sync(~0u, id >= 0 && id < a.n_pages);
   };
   auto load = [&](const CUtensorMap* map, uint32_t at, int id, unsigned ok, uint64_t* bar) {
@@ -408,9 +444,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
   // is any page of the seen keys missing? (looked up here, needed after the queries are on their way; `begin` may lie
   // before the first seen key, whose pages a window has left behind may be gone)
-  const int64_t page0 = ((int64_t)max(begin, lo) >> shift) + threadIdx.x;
-  const int id0 = page0 << shift < end ? table[page0] : 0;
-  const bool missing = id0 < 0 || id0 >= a.n_pages;
+  const int64_t walk0 = (int64_t)(MODE == kSinks ? begin : max(begin, lo) & ~(a.page_tokens - 1)) +
+                        ((int64_t)threadIdx.x << shift);
+  auto page_missing = [&](int64_t walk) {
+    if (walk >= end) return false;
+    const int key = key_at((int)walk);
+    if (MODE == kSinks && key >= more.sinks && key + a.page_tokens <= lo) return false;  // between the sinks and a window
+    const int id = table[key >> shift];
+    return id < 0 || id >= a.n_pages;
+  };
+  const bool missing = page_missing(walk0);
   // Row r of the pair is query t0 + (rem0 + r) / group: a product with 2^20 / group, rounded
   // up, is exact for these small numbers.
   const int rem0 = tile.row0 - t0 * group;
@@ -430,8 +473,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (a.err_flag) *a.err_flag = 1;
   };
   if (missing) gone();
-  for (int64_t p = page0 + kChunkThreads; p << shift < end; p += kChunkThreads)
-    if (table[p] < 0 || table[p] >= a.n_pages) gone();
+  for (int64_t w = walk0 + ((int64_t)kChunkThreads << shift); w < end; w += (int64_t)kChunkThreads << shift)
+    if (page_missing(w)) gone();
   cp_commit();
   cp_wait<0>();
   if (a.scale < 0.f) {  // a negative scale turns the queries' sign (each thread its own words)
@@ -466,8 +509,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       unsigned ok = pages_of(begin, id), next_ok = ok;
       bool stop = false;  // the same in every lane: the loads below are by full warps
       for (int j = 0; j < steps && !stop; ++j) {
-        const int key = begin + j * kNTile;
-        if (j + 1 < steps) next_ok = pages_of(key + kNTile, next_id);
+        if (j + 1 < steps) next_ok = pages_of(begin + (j + 1) * kNTile, next_id);
         for (int kind = 0; kind < 2; ++kind) {
           const int use = 2 * j + kind, st = use % kStages;
           if (use >= kStages && !wait_phase(&empty[st], ((use / kStages) - 1) & 1)) *dead = 1;
@@ -517,7 +559,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int i = 0; i < subs; ++i) {
           const int use = i | 1, st = use % kStages;
           live = live && stage_full(use);
-          if (!(i & 1) && careful(begin + i * kStep)) {
+          if (!(i & 1) && careful(key_at(begin + i * kStep))) {
             live = live && wait_phase(&clean[cleaned & 1], (cleaned >> 1) & 1);
             ++cleaned;
           }
@@ -559,11 +601,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (t < tiles) {
       int cleaned = 0;
       for (int i = 0; i < subs; ++i) {
-        if (!(i & 1) && careful(begin + i * kStep)) {
+        const int key = key_at(begin + i * kStep), key_end = key + end - (begin + i * kStep);
+        if (!(i & 1) && careful(key)) {
           live = __all_sync(~0u, wait_phase(&full[(i | 1) % kStages], ((i | 1) / kStages) & 1));
           if (!live) break;
-          if (clean_values<T, D>(smem + (ring - sq) + (i | 1) % kStages * kTile, begin + i * kStep, lo, all_lo, all_hi,
-                                 end, bad ? table : nullptr, shift, a.n_pages, tiles * kMTile))
+          if (clean_values<T, D>(smem + (ring - sq) + (i | 1) % kStages * kTile, key, lo, all_lo, all_hi, key_end,
+                                 MODE == kSinks ? more.sinks : 0, bad ? table : nullptr, shift, a.n_pages, tiles * kMTile))
             s_odd = 1;
           fence_async();
           __syncwarp();
@@ -573,7 +616,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         live = __all_sync(~0u, wait_phase(&s_full[t][i & 1], (i >> 1) & 1));
         if (!live) break;
         fence_after_sync();
-        const int key = begin + i * kStep;
         const uint32_t at = ts + (i & 1) * kStep;
         float s[kStep], tops[4] = {m, m, m, m};
         tm_ld32(at, s);
@@ -582,16 +624,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tm_ld_wait32(s + 32);
         if (key < all_lo || key + kStep > all_hi || bad) {
           const int last = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : 0;
+          const int sunk = MODE == kSinks ? more.sinks - key : 0;
           unsigned ok = ~0u;  // pages that exist
           const int in_page = key & (a.page_tokens - 1);  // 64 in the second half of a 128-token page
           if (bad) {
             ok = 0;
-            for (int p = key >> shift; p << shift < min(key + kStep, end); ++p)
+            for (int p = key >> shift; p << shift < min(key + kStep, key_end); ++p)
               ok |= (table[p] >= 0 && table[p] < a.n_pages ? 1u : 0u) << (p - (key >> shift));
           }
 #pragma unroll
           for (int c = 0; c < kStep; ++c)
-            if (c > last || c < low || !((ok >> ((in_page + c) >> shift)) & 1u)) s[c] = -INFINITY;
+            if (c > last || (c < low && (MODE != kSinks || c >= sunk)) || !((ok >> ((in_page + c) >> shift)) & 1u)) s[c] = -INFINITY;
         }
 #pragma unroll
         for (int c = 0; c < kStep; c += 8)
@@ -679,9 +722,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
           if (odd && mine) {  // the infinities and NaNs that were kept out of the products
-            for (int k = begin; k < end; ++k) {
+            for (int w = begin; w < end; ++w) {
+              const int k = key_at(w);
               if (k >= all_lo && k < all_hi) continue;  // went through the products
-              if (k > pos || (a.window > 0 && k <= pos - a.window)) continue;
+              if (k > pos || (a.window > 0 && k <= pos - a.window && (MODE != kSinks || k >= more.sinks))) continue;
               const int id = table[k >> shift];
               if (id < 0 || id >= a.n_pages) continue;
               const T* v = static_cast<const T*>(a.v_cache) + id * a.page_stride + kvh * a.head_stride +
@@ -742,8 +786,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 }
 
 // Joins the parts of each row, in order: one warp a row.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, ChunkPlan plan) {
+template <typename T, int D, int MODE>
+__global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, More more, ChunkPlan plan) {
   __shared__ ChunkTile s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
   if (warp == 0) {
@@ -757,9 +801,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, Chunk
   const int first = tile.first, n = tile.n, len = tile.len;
   const int rows = (int)min((int64_t)kPair, (int64_t)n * group - tile.row0);
   const int pos0 = len - n + tile.row0 / group, pos1 = len - n + (tile.row0 + rows - 1) / group;
-  const int lo = a.window > 0 ? first_seen(pos0, a.window) : 0, hi = max(0, pos1 + 1), base = lo & ~(kNTile - 1);
-  const int chunk = part_keys(plan, hi - base);
-  const int parts = hi > base ? (hi - base + chunk - 1) / chunk : 1;
+  const Span span = span_of<MODE>(a.window > 0 ? first_seen(pos0, a.window) : 0, max(0, pos1 + 1), more);
+  const int chunk = part_keys(plan, span.end - span.begin);
+  const int parts = span.end > span.begin ? (span.end - span.begin + chunk - 1) / chunk : 1;
   if (parts == 1) return;
   const int r = blockIdx.z * 8 + warp;
   if (r >= rows) return;

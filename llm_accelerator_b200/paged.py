@@ -303,11 +303,13 @@ class Attention(_Err):
     ``k_cache`` / ``v_cache`` [pages, kv_heads, page_tokens, dim] (bf16 or f16, K and
     V laid out alike), ``table`` int32 [slots, pages per slot], ``lens`` int32 [slots]:
     the keys a slot holds, the new ones included.  ``scale`` defaults to
-    dim ** -0.5; with ``window`` a query sees the last ``window`` keys up to its own.
+    dim ** -0.5; with ``window`` a query sees the last ``window`` keys up to its own, and
+    the first ``sinks`` keys of its sequence up to its own (pages that hold neither are
+    not read).
     """
 
     def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
-                 q_heads: int, scale: Optional[float] = None, window: int = 0):
+                 q_heads: int, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
         self.lib = _native.load()
         self.device = _cuda(k_cache, "k_cache")
         self.dtype = k_cache.dtype
@@ -320,7 +322,9 @@ class Attention(_Err):
         _need(table.dim() == 2 and table.stride(1) == 1 and lens.dim() == 1 and lens.is_contiguous() and
               lens.shape[0] == table.shape[0], "table must be [slots, pages] and lens [slots]")
         pages, kv_heads, page_tokens, dim = k_cache.shape
-        self.q_heads, self.dim, self.slots = q_heads, dim, table.shape[0]
+        _need(0 <= sinks < 2 ** 31, f"{sinks} sinks")
+        _need(window > 0 or sinks == 0, "sinks need a window")
+        self.q_heads, self.dim, self.slots, self.sinks = q_heads, dim, table.shape[0], sinks
         self.k_cache, self.v_cache, self.table, self.lens = k_cache, v_cache, table, lens
         self.workspace = self.layout = None
         self.lock = threading.Lock()
@@ -382,7 +386,7 @@ class Attention(_Err):
                 if lse.shape != (tokens, self.q_heads) or not lse.is_contiguous():
                     raise ValueError(f"lse must be contiguous [{tokens}, {self.q_heads}]")
                 a.lse = lse.data_ptr()
-            need = self.lib.q4gpu_paged_attention_workspace_bytes(a)
+            need = self._workspace_bytes(a)
             if need > a.workspace_bytes:
                 if torch.cuda.is_current_stream_capturing():
                     return self._launch_captured(out, need)
@@ -406,10 +410,18 @@ class Attention(_Err):
             a.workspace, a.workspace_bytes = kept
 
     def _launch(self, out: torch.Tensor) -> torch.Tensor:
-        rc = self.lib.q4gpu_paged_attention(self.args, self._here())
+        if self.sinks:
+            rc = self.lib.q4gpu_sink_attention(self.args, self.sinks, self._here())
+        else:
+            rc = self.lib.q4gpu_paged_attention(self.args, self._here())
         if rc:
-            _native.check(rc, "q4gpu_paged_attention")
+            _native.check(rc, "q4gpu_sink_attention" if self.sinks else "q4gpu_paged_attention")
         return out
+
+    def _workspace_bytes(self, a: _native.AttnArgs) -> int:
+        if self.sinks:
+            return self.lib.q4gpu_sink_attention_workspace_bytes(a, self.sinks)
+        return self.lib.q4gpu_paged_attention_workspace_bytes(a)
 
     def _heads(self, t: torch.Tensor, tokens: int, name: str):
         if t.device != self.device or t.dtype != self.dtype:
