@@ -313,6 +313,33 @@ int q4gpu_paged_attention(const q4gpu_attn_args *a, void *stream);
 size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args *a, int32_t sinks);
 int q4gpu_sink_attention(const q4gpu_attn_args *a, int32_t sinks, void *stream);
 
+/* Log probabilities of given tokens, the entropy and the likeliest tokens of
+ * rows of logits x [rows, vocab] (F32, F16 or BF16, rows `stride` elements
+ * apart, any alignment of the type).  For each row, with p = softmax(x):
+ *   logprob = log p_t of token t = targets[row] (int64, or NULL: none),
+ *   rank    = 1 + the tokens before t in the order of falling logits, equal ones
+ *             by rising index,
+ *   entropy = - sum p log p,
+ *   top_logprob, top_index [rows, top]: the first `top` (at most
+ *             Q4GPU_TOP_MAX and vocab; 0: none) of that order.
+ * A row without a target (targets[row] < 0, or at least vocab, which sets
+ * *err_flag to 1) has logprob 0 and rank 0.  A logit of -infinity has
+ * probability 0.  Where all are, every log probability is -infinity and the entropy 0;
+ * where one is +infinity or NaN, log probabilities and the entropy are NaN
+ * (and NaN comes first in the order).  Results have 32 bits and
+ * are contiguous; they may not overlap the inputs. */
+#define Q4GPU_TOP_MAX 32
+typedef struct q4gpu_logprob_args {
+    const void *logits;
+    const int64_t *targets;
+    float *logprob, *entropy, *top_logprob;
+    int32_t *rank, *top_index;
+    int32_t *err_flag; /* optional */
+    int64_t rows, stride;
+    int32_t vocab, top, dtype, reserved;
+} q4gpu_logprob_args;
+int q4gpu_token_logprobs(const q4gpu_logprob_args *a, void *stream);
+
 /* A pool of pages and the tables that name them.  A page is page_bytes long:
  * blocks of block_bytes (one per layer, K/V and head), each page_tokens rows.
  * Slot s holds lens[s] tokens in pages table[s][0 .. ceil(lens[s] / page_tokens)).

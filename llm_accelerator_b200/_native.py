@@ -125,6 +125,13 @@ class PagesArgs(C.Structure):
                [(n, C.c_int32) for n in ("n_pages", "page_tokens", "n_slots", "reserved")]
 
 
+class LogprobArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "targets", "logprob", "entropy", "top_logprob", "rank", "top_index",
+                                          "err_flag")] + \
+               [(n, C.c_int64) for n in ("rows", "stride")] + \
+               [(n, C.c_int32) for n in ("vocab", "top", "dtype", "reserved")]
+
+
 # element types of the 16-bit paged operators (Q4GPU_F32 ..)
 DT_F32, DT_F16, DT_BF16, DT_E4M3, DT_S8 = range(5)
 
@@ -160,6 +167,7 @@ SIGNATURES = {
     "q4gpu_paged_attention": (C.c_int, [C.POINTER(AttnArgs), P]),
     "q4gpu_sink_attention_workspace_bytes": (SZ, [C.POINTER(AttnArgs), I32]),
     "q4gpu_sink_attention": (C.c_int, [C.POINTER(AttnArgs), I32, P]),
+    "q4gpu_token_logprobs": (C.c_int, [C.POINTER(LogprobArgs), P]),
     "q4gpu_pages_fork": (C.c_int, [C.POINTER(PagesArgs), P, P, P, I32, P]),
     "q4gpu_pages_compact_workspace_bytes": (SZ, [I32]),
     "q4gpu_pages_compact": (C.c_int, [C.POINTER(PagesArgs), P, P, P, P, SZ, P]),

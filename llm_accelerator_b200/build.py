@@ -19,7 +19,7 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "libq4gpu.so"
 SOURCES = ["q4_modules.cu", "q4_decode.cu", "q4_persistent.cu", "q4_batch.cu", "q4_qmap.cu", "q4_paged.cu",
-           "q4_paged_attn.cu"]
+           "q4_paged_attn.cu", "q4_logprob.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

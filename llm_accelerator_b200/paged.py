@@ -7,6 +7,7 @@ K/V cache, and what happens to the cache's pages between steps.
 * ``AddRmsNorm``  residual addition + RMS norm, 16-bit or 8-bit output with scales
 * ``RopeAppend``  q/k head norm, rotary positions, K/V stored in their pages
 * ``Attention``   a chunk of new tokens per sequence (or one) over the pages
+* ``TokenLogprobs``  log probabilities of given tokens, entropy, likeliest tokens
 * ``Pages``       forking sequences, packing the pages in use
 * ``PagedCache``  a pool with its tables, and which pages are free
 
@@ -429,6 +430,84 @@ class Attention(_Err):
         if t.shape != (tokens, self.q_heads, self.dim) or t.stride(2) != 1:
             raise ValueError(f"{name} must be [{tokens}, {self.q_heads}, {self.dim}] with contiguous head vectors")
         return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+class TokenScores:
+    """What ``TokenLogprobs`` gives for each row, as contiguous device tensors.
+
+    ``logprob`` / ``entropy`` float32 [rows], ``rank`` int32 [rows], ``top_logprob`` float32 and
+    ``top_index`` int32 [rows, top].  Made by ``TokenLogprobs.empty``.
+    """
+
+    __slots__ = ("logprob", "entropy", "rank", "top_logprob", "top_index", "_made", "_room", "_at")
+
+    def __init__(self, rows: int, top: int, device: torch.device):
+        def room(dtype, *shape):
+            return torch.empty(*shape, dtype=dtype, device=device)
+        self.logprob, self.entropy = room(torch.float32, rows), room(torch.float32, rows)
+        self.rank = room(torch.int32, rows)
+        self.top_logprob, self.top_index = room(torch.float32, rows, top), room(torch.int32, rows, top)
+        self._made = rows, top, device
+        # (kept, so that the addresses hold whatever becomes of the names above)
+        self._room = self.logprob, self.entropy, self.rank, self.top_logprob, self.top_index
+        self._at = tuple(t.data_ptr() for t in self._room)
+
+
+class TokenLogprobs(_Err):
+    """Log probabilities of given tokens, the entropy and the ``top`` likeliest tokens of rows of logits.
+
+    logprob = log softmax(x)[t]; rank: 1 + the tokens before t by falling logit (equal ones by
+    rising index), the order of top_logprob / top_index; entropy in nats.
+    """
+
+    MOST = 32  # of the likeliest tokens
+
+    def __init__(self, top: int = 0, device: Optional[torch.device] = None):
+        self.lib = _native.load()
+        _need(0 <= top <= self.MOST, f"top = {top}, at most {self.MOST}")
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        _need(self.device.type == "cuda" and self.device.index is not None, f"{self.device} is not a CUDA device")
+        self.top, self.layout, self.lock = top, None, threading.Lock()
+        self._new_err()
+        self.args = _native.LogprobArgs(top=top, err_flag=self.err.data_ptr())
+
+    def empty(self, rows: int) -> TokenScores:
+        """Room for the results of ``rows`` rows."""
+        return TokenScores(rows, self.top, self.device)
+
+    def __call__(self, logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
+                 out: Optional[TokenScores] = None) -> TokenScores:
+        """logits [rows, vocab] float32, float16 or bfloat16 with contiguous rows; targets int64 [rows],
+        negative: no token (logprob 0, rank 0; without targets they are not written).  A target past the
+        vocabulary counts as none and is an error that ``check`` reports."""
+        with self.lock:
+            a = self.args
+            layout = (logits.shape, logits.stride(), logits.dtype, logits.device,
+                      None if targets is None else (targets.shape, targets.stride(), targets.dtype, targets.device))
+            if layout != self.layout:
+                self.layout = None
+                if logits.dim() != 2 or logits.device != self.device or \
+                        logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+                    raise ValueError(f"logits must be [rows, vocab] float32, float16 or bfloat16 on {self.device}")
+                rows, vocab = logits.shape
+                _need(vocab > 0 and (logits.stride(1) == 1 or vocab == 1), "logits must have contiguous rows")
+                _need(vocab < 2 ** 31, f"a vocabulary of {vocab}")
+                if targets is not None:
+                    _on(targets, self.device, "targets", torch.int64)
+                    _need(targets.shape == (rows,) and targets.is_contiguous(),
+                          f"targets must be a contiguous vector of {rows}")
+                a.rows, a.vocab, a.stride, a.dtype = rows, vocab, logits.stride(0), _DTYPES[logits.dtype]
+                self.layout = layout
+            if out is None:
+                out = TokenScores(a.rows, self.top, self.device)
+            elif out._made != (a.rows, self.top, self.device):
+                raise ValueError(f"out must be what empty({a.rows}) of this operator makes")
+            a.logits, a.targets = logits.data_ptr(), None if targets is None else targets.data_ptr()
+            a.logprob, a.entropy, a.rank, a.top_logprob, a.top_index = out._at
+            rc = self.lib.q4gpu_token_logprobs(a, self._here())
+            if rc:
+                _native.check(rc, "q4gpu_token_logprobs")
+            return out
 
 
 class Pages(_Err):

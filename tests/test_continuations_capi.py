@@ -31,3 +31,44 @@ def test_sink_sizes(lib):
     assert lib.q4gpu_sink_attention_workspace_bytes(attn(**big), -1) == 0
     assert lib.q4gpu_sink_attention(None, 4, None) == ARG
     assert lib.q4gpu_sink_attention(attn(window=4, tokens=0), 4, None) == 0
+
+
+def logprob(**kw):
+    a = _native.LogprobArgs(logits=256, targets=256, logprob=256, entropy=256, top_logprob=256, rank=256, top_index=256,
+                            rows=1, stride=64, vocab=64, top=5, dtype=2)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(logits=None), ARG), (dict(entropy=None), ARG), (dict(logprob=None), ARG), (dict(rank=None), ARG),
+    (dict(top_logprob=None), ARG), (dict(top_index=None), ARG), (dict(dtype=3), ARG), (dict(rows=-1), SHAPE),
+    (dict(rows=2 ** 31), SHAPE), (dict(vocab=0), SHAPE), (dict(top=-1), SHAPE), (dict(top=33), SHAPE),
+    (dict(top=5, vocab=4), SHAPE), (dict(logits=257), ALIGN), (dict(logits=258, dtype=0), ALIGN)])
+def test_logprob_refusals(lib, kw, rc):
+    assert lib.q4gpu_token_logprobs(logprob(**kw), None) == rc
+    assert lib.q4gpu_last_error().startswith(b"logprobs")
+
+
+def test_logprobs_of_no_rows(lib):
+    assert lib.q4gpu_token_logprobs(logprob(rows=0, logits=None), None) == 0
+    assert lib.q4gpu_token_logprobs(None, None) == ARG
+
+
+def test_logprob_structure(tmp_path):
+    """ctypes and the header agree on the arguments' layout."""
+    import subprocess
+
+    from conftest import REPO
+    src = "#include <stddef.h>\n#include <stdio.h>\n#include \"q4gpu.h\"\nint main(void) {\n"
+    for name, _ in _native.LogprobArgs._fields_:
+        src += f'  printf("{name} %zu\\n", offsetof(q4gpu_logprob_args, {name}));\n'
+    src += '  printf("size %zu\\n", sizeof(q4gpu_logprob_args));\n  return 0;\n}\n'
+    (tmp_path / "t.c").write_text(src)
+    subprocess.run(["gcc", "-I", str(REPO / "include"), "-o", str(tmp_path / "t"), str(tmp_path / "t.c")], check=True)
+    out = dict(line.split() for line in subprocess.run([str(tmp_path / "t")], capture_output=True, text=True,
+                                                       check=True).stdout.splitlines())
+    assert int(out.pop("size")) == C.sizeof(_native.LogprobArgs)
+    assert {k: int(v) for k, v in out.items()} == {n: getattr(_native.LogprobArgs, n).offset
+                                                   for n, _ in _native.LogprobArgs._fields_}
