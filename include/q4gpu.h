@@ -313,6 +313,28 @@ int q4gpu_paged_attention(const q4gpu_attn_args *a, void *stream);
 size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args *a, int32_t sinks);
 int q4gpu_sink_attention(const q4gpu_attn_args *a, int32_t sinks, void *stream);
 
+/* Attention of sequences that share their first keys, which are read once for
+ * all of them.  Group g is the sequences cu_group[g] .. cu_group[g + 1] - 1 of the
+ * call (device int32 [n_groups + 1], ascending; a sequence may stand in no group)
+ * and shares the keys 0 .. prefix_lens[g] - 1 (device int32 [n_groups], any number,
+ * 0: none): they are read from the pages of the group's first sequence, the others'
+ * table entries of pages that hold shared keys only are not looked at.  Every query of the group
+ * stands behind them (prefix_lens[g] <= lens[s] - n of each sequence with queries).
+ * Results are those of q4gpu_paged_attention (window = 0) over tables that name
+ * the same keys.  What only the device sees is checked as there; besides, *err_flag becomes 1
+ * where cu_group or prefix_lens is out of range (where cu_group or cu_q does not
+ * ascend, all rows become zeros and -infinity), where the first sequence's slot
+ * holds fewer keys than are shared (those that are there count), and where a sequence's
+ * queries do not stand behind the shared keys (its rows become zeros and
+ * -infinity, as do those of a sequence with more than max_q queries).
+ * max_prefix bounds prefix_lens; like max_ctx it only decides how the work is split. */
+typedef struct q4gpu_shared_args {
+    const int32_t *cu_group, *prefix_lens;
+    int32_t n_groups, max_prefix;
+} q4gpu_shared_args;
+size_t q4gpu_shared_attention_workspace_bytes(const q4gpu_attn_args *a, const q4gpu_shared_args *shared);
+int q4gpu_shared_attention(const q4gpu_attn_args *a, const q4gpu_shared_args *shared, void *stream);
+
 /* Log probabilities of given tokens, the entropy and the likeliest tokens of
  * rows of logits x [rows, vocab] (F32, F16 or BF16, rows `stride` elements
  * apart, any alignment of the type).  For each row, with p = softmax(x):

@@ -125,6 +125,11 @@ class PagesArgs(C.Structure):
                [(n, C.c_int32) for n in ("n_pages", "page_tokens", "n_slots", "reserved")]
 
 
+class SharedArgs(C.Structure):
+    _fields_ = [("cu_group", C.c_void_p), ("prefix_lens", C.c_void_p), ("n_groups", C.c_int32),
+                ("max_prefix", C.c_int32)]
+
+
 class LogprobArgs(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("logits", "targets", "logprob", "entropy", "top_logprob", "rank", "top_index",
                                           "err_flag")] + \
@@ -167,6 +172,8 @@ SIGNATURES = {
     "q4gpu_paged_attention": (C.c_int, [C.POINTER(AttnArgs), P]),
     "q4gpu_sink_attention_workspace_bytes": (SZ, [C.POINTER(AttnArgs), I32]),
     "q4gpu_sink_attention": (C.c_int, [C.POINTER(AttnArgs), I32, P]),
+    "q4gpu_shared_attention_workspace_bytes": (SZ, [C.POINTER(AttnArgs), C.POINTER(SharedArgs)]),
+    "q4gpu_shared_attention": (C.c_int, [C.POINTER(AttnArgs), C.POINTER(SharedArgs), P]),
     "q4gpu_token_logprobs": (C.c_int, [C.POINTER(LogprobArgs), P]),
     "q4gpu_pages_fork": (C.c_int, [C.POINTER(PagesArgs), P, P, P, I32, P]),
     "q4gpu_pages_compact_workspace_bytes": (SZ, [I32]),

@@ -1,5 +1,6 @@
 // Attention of each sequence's newest tokens to its pages (16-bit paged
-// serving operators, include/q4gpu.h: q4gpu_paged_attention, q4gpu_sink_attention).
+// serving operators, include/q4gpu.h: q4gpu_paged_attention, q4gpu_sink_attention,
+// q4gpu_shared_attention).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -15,20 +16,6 @@ namespace {
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-
-// What a CTA needs to know of sequence i.
-struct Seq {
-  int slot, len, first, n;  // cache slot, stored keys, first query token, query tokens
-};
-__device__ __forceinline__ Seq sequence(const q4gpu_attn_args& a, int i) {
-  Seq s;
-  s.first = max(0, min(a.cu_q[i], a.tokens));
-  s.n = max(0, min(a.cu_q[i + 1], a.tokens) - s.first);
-  s.slot = a.seq_ids ? a.seq_ids[i] : i;
-  const bool known = s.slot >= 0 && s.slot < a.n_slots;
-  s.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[s.slot], most_keys(a))) : 0;
-  return s;
-}
 
 // ---------------------------------------------------------------------------
 // few query rows (decode): at most 16 (token, head) pairs share a key head
@@ -91,11 +78,11 @@ struct RowPlan {
   int32_t* done;  // [cta] finished pieces of the item whose first piece goes on from this CTA
 };
 
-// Keys that the kernel below walks for sequence i, from `lo` on; -1: not its
-// sequence (no queries, or more rows than a tile).  With sinks the walk starts
+// Keys that the kernel below walks for item s, from `lo` on; -1: not its
+// item (no queries, or more rows than a tile).  With sinks the walk starts
 // at key 0 and leaves out `gap.skip` keys from key gap.from on.
 template <int MODE>
-__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const More& x, const Seq& s, int group, int& lo,
+__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const More& x, const Item& s, int group, int& lo,
                                         Gap& gap) {
   lo = 0;
   gap = Gap{0, 0};
@@ -104,6 +91,8 @@ __device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const More& x,
   if constexpr (MODE == kSinks) {
     gap = gap_before(lo, x.sinks, kTileKeys);
     lo = 0;
+  } else if constexpr (MODE == kShared) {
+    lo = s.lo & ~(kTileKeys - 1);
   }
   return max(0, s.len - gap.skip - lo);
 }
@@ -111,8 +100,33 @@ template <int MODE>
 __device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, const More& x, int i, int group) {  // of one head
   int lo;
   Gap gap;
-  const int keys = row_keys<MODE>(a, x, sequence(a, i), group, lo, gap);
+  const int keys = row_keys<MODE>(a, x, item_of<MODE>(a, x, i), group, lo, gap);
   return keys < 0 ? 0 : kPieceCost + (keys + kUnitKeys - 1) / kUnitKeys;
+}
+
+// With kShared: whether cu_q and cu_group ascend at item i, within what they index.
+__device__ __forceinline__ bool ascends(const q4gpu_attn_args& a, const More& x, int i) {
+  const bool group = i >= a.n_seqs;
+  const int32_t* cu = group ? x.cu_group + (i - a.n_seqs) : a.cu_q + i;
+  return cu[0] >= 0 && cu[1] >= cu[0] && cu[1] <= (group ? a.n_seqs : a.tokens);
+}
+// Whether what only the device sees of item i is in range.
+template <int MODE>
+__device__ __forceinline__ bool item_ok(const q4gpu_attn_args& a, const More& x, int i) {
+  if (i < a.n_seqs) {
+    if (!sequence_ok(a, i)) return false;
+    if constexpr (MODE == kShared) {
+      const int n = a.cu_q[i + 1] - a.cu_q[i], g = group_of(x, i);
+      if (n > 0 && g >= 0 && x.prefix_lens[g] > 0 && x.prefix_lens[g] > a.lens[a.seq_ids ? a.seq_ids[i] : i] - n)
+        return false;
+    }
+    return true;
+  }
+  const int g = i - a.n_seqs, c = x.cu_group[g];
+  if (!ascends(a, x, i) || x.prefix_lens[g] < 0) return false;
+  if (c == x.cu_group[g + 1] || x.prefix_lens[g] == 0) return true;
+  const int s = a.seq_ids ? a.seq_ids[c] : c;  // whose pages hold the shared keys
+  return s >= 0 && s < a.n_slots && x.prefix_lens[g] <= keys_of(a, s);
 }
 
 // Each warp runs over its own 16-key steps of a piece with its own running
@@ -133,16 +147,21 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   const int group = a.q_heads / a.kv_heads;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the chunk kernel reads nothing of this one
   // the axis: each thread adds up a run of sequences
-  const int per = (a.n_seqs + kThreads - 1) / kThreads;
-  const int run0 = min(a.n_seqs, (int)threadIdx.x * per), run1 = min(a.n_seqs, run0 + per);
+  const int items = item_count<MODE>(a, x), per = (items + kThreads - 1) / kThreads;
+  const int run0 = min(items, (int)threadIdx.x * per), run1 = min(items, run0 + per);
   int64_t mine_cost = 0;
   int most = 0;
+  bool malformed = false;
   // without a chunk kernel beside this one nobody computes a sequence longer than max_q and a tile: its rows become zeros
-  const bool alone = (int64_t)a.max_q * group <= kRows;
+  // (with kShared, attn_shared_join_kernel writes the zeros)
+  const bool alone = MODE != kShared && (int64_t)a.max_q * group <= kRows;
   bool over = false;
   for (int i = run0; i < run1; ++i) {
-    over |= alone && sequence(a, i).n > kRows / group;
-    if (blockIdx.x == 0 && a.err_flag && !sequence_ok(a, i)) *a.err_flag = 1;
+    over |= alone && item_of<MODE>(a, x, i).n > kRows / group;
+    if (blockIdx.x == 0) {
+      if (MODE == kShared && !ascends(a, x, i)) malformed = true;
+      if (a.err_flag && !item_ok<MODE>(a, x, i)) *a.err_flag = 1;
+    }
     const int c = row_cost<MODE>(a, x, i, group);
     mine_cost += (int64_t)c * a.kv_heads;
     most = max(most, c);
@@ -156,7 +175,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   most = __reduce_max_sync(~0u, most);
   if (lane == 31) s_sum[warp] = upto;
   if (lane == 0) s_most[warp] = most;
-  over = __syncthreads_or(over);
+  if constexpr (MODE == kShared) {
+    malformed = __syncthreads_or(malformed);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *x.malformed = malformed;
+  } else {
+    over = __syncthreads_or(over);
+  }
   int64_t total = 0, before = upto - mine_cost;
 #pragma unroll
   for (int w = 0; w < kRowWarps; ++w) {
@@ -180,7 +204,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
     int seq = s_seq, lo;
     Gap gap;
     int64_t start = s_start;  // where the sequence's first head begins
-    Seq s = sequence(a, seq);
+    Item s = item_of<MODE>(a, x, seq);
     int keys = row_keys<MODE>(a, x, s, group, lo, gap), cost = row_cost<MODE>(a, x, seq, group), kvh = (int)quotient(first_unit - start, cost);
     for (;;) {
       const int64_t head_start = start + (int64_t)kvh * cost + kPieceCost;  // of its first real unit
@@ -194,11 +218,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         const int64_t cta0 = quotient(head_start, stretch),
                       cta1 = units == 0 ? cta0 : quotient(head_start + units - 1, stretch);
         const int parts = (int)(cta1 - cta0) + 1, part = (int)(blockIdx.x - cta0);
-        const int pos0 = s.len - s.n, pos1 = s.len - 1;  // of the first and the last query
+        const int pos0 = MODE == kShared && s.flat ? s.len - 1 : s.len - s.n, pos1 = s.len - 1;  // first, last query
         // along the walk; key_at gives the key
         const int begin = lo + u0 * kUnitKeys, end = min(s.len - gap.skip, lo + u1 * kUnitKeys);
         auto key_at = [&](int walk) { return MODE == kSinks && walk >= gap.from ? walk + gap.skip : walk; };
         auto unseen = [&](int j, int p) {
+          if (MODE == kShared && j < s.lo) return true;
           return j > p || (a.window > 0 && j <= p - a.window && (MODE != kSinks || j >= x.sinks));
         };
 
@@ -209,7 +234,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = g + 8 * h, t = r / group;
-          row_pos[h] = r < rows ? pos0 + t : -1;
+          row_pos[h] = r >= rows ? -1 : MODE == kShared && s.flat ? pos0 : pos0 + t;
           const T* qp = static_cast<const T*>(a.q) + (int64_t)(s.first + t) * a.q_token_stride +
                         (int64_t)(kvh * group + r - t * group) * a.q_head_stride + 2 * tq;
 #pragma unroll
@@ -280,7 +305,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           }
           // element e of sc[n]: row g + 8 (e / 2), key 8 n + 2 tq + e % 2
           const bool whole = key + kTileKeys <= pos0 + 1 &&
-                             (a.window == 0 || key > pos1 - a.window || (MODE == kSinks && key + kTileKeys <= x.sinks));
+                             (a.window == 0 || key > pos1 - a.window || (MODE == kSinks && key + kTileKeys <= x.sinks)) &&
+                             (MODE != kShared || key >= s.lo);
           float top[2] = {m[0], m[1]};
 #pragma unroll
           for (int n = 0; n < 2; ++n)
@@ -372,6 +398,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         __syncthreads();
         auto put = [&](int r, int d, float m_all, float l_all, float v) {
           const int t = r / group, head = kvh * group + r - t * group;
+          if constexpr (MODE == kShared) {
+            const int64_t at = ((int64_t)(s.flat ? x.own_parts : 0) * a.tokens + s.first + t) * a.q_heads + head;
+            x.o[at * D + d] = v;
+            if (d == 0) x.ml[at] = make_float2(l_all == 0.f ? -INFINITY : m_all, l_all);
+            return;
+          }
           static_cast<T*>(a.out)[(int64_t)(s.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride + d] =
               from_f32<T>(l_all == 0.f ? 0.f : v / l_all);
           if (a.lse && d == 0)
@@ -430,18 +462,18 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         kvh = 0;
         start += (int64_t)cost * a.kv_heads;
         do {
-          if (++seq >= a.n_seqs) break;
-          s = sequence(a, seq);
+          if (++seq >= items) break;
+          s = item_of<MODE>(a, x, seq);
           keys = row_keys<MODE>(a, x, s, group, lo, gap);
           cost = row_cost<MODE>(a, x, seq, group);
         } while (cost == 0);
-        if (seq >= a.n_seqs) break;
+        if (seq >= items) break;
       }
     }
   }
   if (over)
     for (int i = blockIdx.x; i < a.n_seqs; i += gridDim.x) {
-      const Seq s = sequence(a, i);
+      const Item s = item_of<MODE>(a, x, i);
       if (s.n <= kRows / group) continue;
       for (int64_t e = threadIdx.x; e < (int64_t)s.n * a.q_heads * D; e += kThreads) {
         const int64_t row = e / D, t = s.first + row / a.q_heads, head = row % a.q_heads;
@@ -496,9 +528,9 @@ q4gpu_attn_args settled(const q4gpu_attn_args& a) {
   return b;
 }
 
-RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
+RowPlan row_plan(const q4gpu_attn_args& a, const More& x, char* ws, size_t* bytes) {
   RowPlan p{};
-  const size_t items = (size_t)a.n_seqs * a.kv_heads;
+  const size_t items = (size_t)(a.n_seqs + x.n_groups) * a.kv_heads;
   // no CTA without at least one (sequence, head) or kLeastStretch units of one
   const int64_t units = ((int64_t)a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
   const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + kLeastStretch - 1) / kLeastStretch + 1);
@@ -517,16 +549,28 @@ RowPlan row_plan(const q4gpu_attn_args& a, char* ws, size_t* bytes) {
 // the last wave of many items in two evens the SMs out, 348 steps on the longest
 // instead of 370 for 8192 tokens over 16384 keys, but the parts' traffic and the
 // join took more: 814 us against 771.)
+template <int MODE>
 ChunkPlan chunk_plan(const q4gpu_attn_args& a, const More& x, size_t* bytes) {
   ChunkPlan p{};
-  const int64_t group = a.q_heads / a.kv_heads;
+  const int64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
+  if constexpr (MODE == kShared) {
+    // a group's queries count together: tiles for its shared keys, and for own keys of long chunks
+    p.least = (int)(kRows / group) + 1, p.parts = 1;
+    const int64_t most = a.tokens / p.least;  // items of so many queries
+    int64_t tiles = 0;
+    if (rows > kRows) tiles = rows / kPair + std::min<int64_t>(x.n_groups, most);
+    if (a.max_q * group > kRows) tiles += rows / kPair + std::min<int64_t>(a.n_seqs, most);
+    p.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+    if (tiles)
+      p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / (tiles * a.kv_heads), a.max_ctx / kMinPart));
+    return p;
+  }
   if (a.max_q * group <= kRows || a.n_seqs == 0 || a.tokens == 0) {  // nothing for the chunk kernel
     if (bytes) *bytes = 0;
     return p;
   }
   // (a lone sequence of any length is the chunk kernel's: one launch)
   p.least = a.n_seqs == 1 ? 1 : (int)(kRows / group) + 1;
-  const int64_t rows = a.tokens * group;
   p.tiles = (int)std::min<int64_t>(a.n_seqs == 1 ? (rows + kPair - 1) / kPair : rows / kPair + a.n_seqs, INT32_MAX);
   const int64_t items = (int64_t)p.tiles * a.kv_heads;
   const int64_t span =
@@ -578,11 +622,12 @@ template <typename T, int D, int MODE>
 int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
   static unsigned char ready[2][Q4GPU_MAX_DEVICES];
   size_t rows_bytes;
-  const RowPlan few = row_plan(a, static_cast<char*>(a.workspace), &rows_bytes);
-  const bool chunks = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows;
-  ChunkPlan plan = chunk_plan(a, x, nullptr);
+  const RowPlan few = row_plan(a, x, static_cast<char*>(a.workspace), &rows_bytes);
+  ChunkPlan plan = chunk_plan<MODE>(a, x, nullptr);
+  const bool chunks = plan.tiles > 0;
   if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
-  const bool short_ones = !chunks || plan.least > 1;  // sequences for attn_rows_kernel
+  // sequences for attn_rows_kernel (with kShared it also looks at what only the device sees)
+  const bool short_ones = MODE == kShared || !chunks || plan.least > 1;
   int rc = Q4GPU_OK;
   if (short_ones) {
     rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D, MODE>), row_smem<D>(), ready[0]);
@@ -593,6 +638,7 @@ int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
     char* ws = static_cast<char*>(a.workspace) + (rows_bytes + 15) / 16 * 16;
     plan.ml = reinterpret_cast<float2*>(ws);
     plan.o = reinterpret_cast<float*>(plan.ml + (size_t)plan.tiles * a.kv_heads * plan.parts * kPair);
+    if constexpr (MODE == kShared) plan.o = nullptr, plan.ml = nullptr;
     rc = encode_map(&kmap, a, a.k_cache);
     if (rc == Q4GPU_OK) rc = encode_map(&vmap, a, a.v_cache);
     if (rc == Q4GPU_OK)
@@ -614,7 +660,12 @@ int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
     cfg.numAttrs = short_ones ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_chunk_kernel<T, D, MODE>, kmap, vmap, a, x, plan);
     if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: launch: %s", cudaGetErrorString(e));
-    if (plan.parts > 1) attn_join_kernel<T, D, MODE><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, x, plan);
+    if (MODE != kShared && plan.parts > 1) attn_join_kernel<T, D, MODE><<<dim3(a.kv_heads, plan.tiles, kPair / 8), 256, 0, s>>>(a, x, plan);
+  }
+  if constexpr (MODE == kShared) {
+    const int64_t rows = (int64_t)a.max_q * a.q_heads;
+    const dim3 grid(a.n_seqs, (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, 64)));
+    attn_shared_join_kernel<T, D><<<grid, 256, 0, s>>>(a, x, plan);
   }
   return q4gpu_check_launch();
 }
@@ -632,16 +683,75 @@ More settled_sinks(const q4gpu_attn_args& settled, int32_t sinks) {
   return x;
 }
 
+// The workspace behind the few-row kernel's: the two sets of parts and a word.  False: too large to count.
+struct SharedRoom {
+  size_t ml, o, word, bytes;
+};
+bool shared_room(const q4gpu_attn_args& a, const More& x, SharedRoom& r, int& own_parts) {
+  const ChunkPlan p = chunk_plan<kShared>(a, x, nullptr);
+  own_parts = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows ? p.parts : 1;
+  size_t rows_bytes;
+  row_plan(a, x, nullptr, &rows_bytes);
+  const size_t rows = (size_t)(own_parts + p.parts) * a.tokens * a.q_heads;
+  r.ml = (rows_bytes + 15) / 16 * 16;
+  r.o = r.ml + (rows * sizeof(float2) + 15) / 16 * 16;
+  r.word = r.o + rows * a.dim * sizeof(float);
+  r.bytes = r.word + 16;
+  return p.tiles <= 65535;
+}
+
+int check_shared(const q4gpu_attn_args* a, const q4gpu_shared_args* sh) {
+  if (!sh) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null arguments");
+  if (a->window) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: shared keys and a window do not go together");
+  if (sh->n_groups < 0 || sh->n_groups > 65535 || sh->max_prefix < 0)
+    return q4gpu_fail(Q4GPU_ERR_ARG, "attention: %d groups, shared keys up to %d", sh->n_groups, sh->max_prefix);
+  return Q4GPU_OK;
+}
+More settled_groups(const q4gpu_shared_args& sh) {
+  More x{};
+  x.cu_group = sh.cu_group, x.prefix_lens = sh.prefix_lens, x.n_groups = sh.n_groups;
+  return x;
+}
+
 }  // namespace
 
 extern "C" {
 
+size_t q4gpu_shared_attention_workspace_bytes(const q4gpu_attn_args* a, const q4gpu_shared_args* sh) {
+  if (check_sizes(a) != Q4GPU_OK || check_shared(a, sh) != Q4GPU_OK) return 0;
+  SharedRoom room;
+  int own_parts;
+  shared_room(settled(*a), settled_groups(*sh), room, own_parts);
+  return room.bytes;
+}
+
+int q4gpu_shared_attention(const q4gpu_attn_args* a, const q4gpu_shared_args* sh, void* stream) {
+  int rc = check_attn(a);
+  if (rc == Q4GPU_OK) rc = check_shared(a, sh);
+  if (rc != Q4GPU_OK) return rc;
+  if (sh->n_groups > 0 && (!sh->cu_group || !sh->prefix_lens))
+    return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null pointer");
+  if (a->n_seqs == 0 || a->tokens == 0) return Q4GPU_OK;
+  const q4gpu_attn_args b = settled(*a);
+  More x = settled_groups(*sh);
+  SharedRoom room;
+  if (!shared_room(b, x, room, x.own_parts)) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
+  if (a->workspace_bytes < room.bytes || !a->workspace)
+    return q4gpu_fail(Q4GPU_ERR_WORKSPACE, "attention: needs a workspace of %zu bytes", room.bytes);
+  if (!aligned(a->workspace, 16)) return q4gpu_fail(Q4GPU_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(a->workspace);
+  x.ml = reinterpret_cast<float2*>(ws + room.ml), x.o = reinterpret_cast<float*>(ws + room.o);
+  x.malformed = reinterpret_cast<int*>(ws + room.word);
+  return launch<kShared>(b, x, as_stream(stream));
+}
+
 size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args* a, int32_t sinks) {
   if (check_sizes(a) != Q4GPU_OK || sinks < 0) return 0;
   const q4gpu_attn_args b = settled(*a);
+  const More x = settled_sinks(b, sinks);
   size_t rows, chunks;
-  row_plan(b, nullptr, &rows);
-  chunk_plan(b, settled_sinks(b, sinks), &chunks);
+  row_plan(b, x, nullptr, &rows);
+  chunk_plan<kSinks>(b, x, &chunks);
   return (rows + 15) / 16 * 16 + chunks;
 }
 

@@ -37,10 +37,19 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
 __device__ __forceinline__ int64_t most_keys(const q4gpu_attn_args& a) { return (int64_t)a.table_pages * a.page_tokens; }
 
 // Which keys a query sees: those up to its own (through a window the last of them), or those and the first few keys of
-// the sequence as well.
-enum Mode { kPlain, kSinks };
+// the sequence as well, or, in two items of work that are joined afterwards, those that its group of sequences shares
+// and its sequence's own.
+enum Mode { kPlain, kSinks, kShared };
 struct More {  // what the modes need besides the arguments they share
   int sinks;   // kSinks: the first keys that every query sees
+  // kShared: group g is sequences cu_group[g] .. cu_group[g + 1] - 1, its first prefix_lens[g] keys are shared
+  const int32_t *cu_group, *prefix_lens;
+  int n_groups;
+  // what a row got from its own keys and from the shared ones: unnormalised sums [set][part][token][q_head][D], with
+  // the running maximum (log2 units) and sum; the own set has own_parts parts
+  float* o;
+  float2* ml;
+  int own_parts, *malformed;  // *malformed: cu_q or cu_group does not ascend
 };
 // A walk over a sequence's keys that leaves out `skip` keys from key `from` on.
 struct Gap {
@@ -67,22 +76,83 @@ __device__ __forceinline__ bool sequence_ok(const q4gpu_attn_args& a, int i) {
   return s >= 0 && s < a.n_slots && a.lens[s] >= 0 && a.lens[s] <= most_keys(a);
 }
 
-// Sequence and row pair of one grid index, and what its CTA needs to know of the
-// sequence: first query token, query tokens, cache slot, stored keys.
-struct ChunkTile {
-  int seq, row0, index, first, n, slot, len;
+// What a CTA needs to know of an item of work, which is a sequence, or with kShared (in this order) the own keys of a
+// sequence or the shared keys of a group.
+struct Item {
+  int slot, len, first, n;  // cache slot, end of the keys, first query token, query tokens
+  int lo;                   // kShared: the first key
+  bool flat;                // ... whether every query sees all of them (query t of n stands at len - n + t otherwise)
 };
-// Row pairs of sequence i (none where it has few rows); keys: about how many one walks.
-__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int group, int least, ChunkTile& t, int& keys) {
+template <int MODE>
+__device__ __forceinline__ int item_count(const q4gpu_attn_args& a, const More& x) {
+  return a.n_seqs + (MODE == kShared ? x.n_groups : 0);
+}
+__device__ __forceinline__ int keys_of(const q4gpu_attn_args& a, int slot) {
+  return slot >= 0 && slot < a.n_slots ? (int)max((int64_t)0, min((int64_t)a.lens[slot], most_keys(a))) : 0;
+}
+__device__ __forceinline__ int shared_keys(const q4gpu_attn_args& a, const More& x, int g) {
+  return (int)max((int64_t)0, min((int64_t)x.prefix_lens[g], most_keys(a)));
+}
+// The group of sequence i, or -1: the last that begins at or before it, if it reaches it.
+__device__ __forceinline__ int group_of(const More& x, int i) {
+  int g = 0, end = x.n_groups;
+  while (g < end) {
+    const int mid = (g + end) / 2;
+    if (x.cu_group[mid] <= i)
+      g = mid + 1;
+    else
+      end = mid;
+  }
+  return g > 0 && i < x.cu_group[g] ? g - 1 : -1;
+}
+template <int MODE>
+__device__ __forceinline__ Item item_of(const q4gpu_attn_args& a, const More& x, int i) {
+  Item s;
+  s.lo = 0, s.flat = false;
+  int last = i + 1;
+  if (MODE == kShared && i >= a.n_seqs) {
+    const int g = i - a.n_seqs;
+    s.flat = true;
+    i = max(0, min(x.cu_group[g], a.n_seqs)), last = max(i, min(x.cu_group[g + 1], a.n_seqs));
+    s.lo = shared_keys(a, x, g);  // (their end, for now)
+  }
+  s.first = max(0, min(a.cu_q[i], a.tokens));
+  s.n = max(0, min(a.cu_q[last], a.tokens) - s.first);
+  if (MODE == kShared && i == last) {  // a group without sequences: its first may not be there
+    s.slot = -1, s.len = s.lo = s.n = 0;
+    return s;
+  }
+  s.slot = a.seq_ids ? a.seq_ids[i] : i;
+  s.len = keys_of(a, s.slot);
+  if constexpr (MODE == kShared) {
+    if (s.flat) {
+      s.len = min(s.len, s.lo);
+      s.lo = 0;
+      if (s.len == 0) s.n = 0;
+    } else {
+      const int g = group_of(x, i);
+      s.lo = g < 0 ? 0 : shared_keys(a, x, g);
+      // its queries have to stand behind the shared keys (else its rows become zeros)
+      if (s.lo > 0 && s.lo > s.len - s.n) s.lo = s.len = 0;
+      if (s.n > a.max_q) s.n = 0;  // likewise
+    }
+  }
+  return s;
+}
+
+// Row pair of one grid index and its item.
+struct ChunkTile : Item {
+  int seq, row0, index;
+};
+// Row pairs of item i (none where it has few rows); keys: about how many one walks.
+template <int MODE>
+__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, const More& x, int i, int group, int least,
+                                        ChunkTile& t, int& keys) {
   keys = 0;
-  if (i >= a.n_seqs) return 0;
-  t.first = max(0, min(a.cu_q[i], a.tokens));
-  t.n = max(0, min(a.cu_q[i + 1], a.tokens) - t.first);
-  t.slot = a.seq_ids ? a.seq_ids[i] : i;
-  const bool known = t.slot >= 0 && t.slot < a.n_slots;
-  t.len = known ? (int)max((int64_t)0, min((int64_t)a.lens[t.slot], most_keys(a))) : 0;
+  if (i >= item_count<MODE>(a, x)) return 0;
+  static_cast<Item&>(t) = item_of<MODE>(a, x, i);
   if (t.n < least) return 0;
-  keys = a.window > 0 ? min(t.len, a.window) : t.len;  // (of sinks there are few)
+  keys = a.window > 0 ? min(t.len, a.window) : t.len - t.lo;  // (of sinks there are few)
   return (int)(((int64_t)t.n * group + kPair - 1) / kPair);
 }
 // The pair of grid row y; seq = -1 where there are fewer.  By one full warp.
@@ -90,19 +160,21 @@ __device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, int i, int gro
 // end: sequences in four classes (at least half, a quarter, an eighth of the most
 // keys, the rest), and within a class from its last row pair to its first, as
 // later rows see more keys.
-__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int least, int y) {
-  const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
-  ChunkTile t{-1, 0, y, 0, 0, 0, 0}, own;
+template <int MODE>
+__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, const More& x, int least, int y) {
+  const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads, items = item_count<MODE>(a, x);
+  ChunkTile t{}, own{};
+  t.seq = -1, t.index = y;
   int most = 0, keys;
-  for (int i = lane; i < a.n_seqs; i += 32) {
-    pairs_of(a, i, group, least, own, keys);
+  for (int i = lane; i < items; i += 32) {
+    pairs_of<MODE>(a, x, i, group, least, own, keys);
     most = max(most, keys);
   }
   most = __reduce_max_sync(~0u, most);
   auto rank = [&](int k) { return k >= most / 2 ? 0 : k >= most / 4 ? 1 : k >= most / 8 ? 2 : 3; };
   int count[4] = {0, 0, 0, 0};
-  for (int i = lane; i < a.n_seqs; i += 32) {
-    const int n = pairs_of(a, i, group, least, own, keys);
+  for (int i = lane; i < items; i += 32) {
+    const int n = pairs_of<MODE>(a, x, i, group, least, own, keys);
 #pragma unroll
     for (int c = 0; c < 4; ++c) count[c] += rank(keys) == c ? n : 0;
   }
@@ -118,8 +190,8 @@ __device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int lea
   }
   if (wanted < 0) return t;
   int before = 0;
-  for (int i0 = 0; i0 < a.n_seqs; i0 += 32) {
-    int mine = pairs_of(a, i0 + lane, group, least, own, keys);
+  for (int i0 = 0; i0 < items; i0 += 32) {
+    int mine = pairs_of<MODE>(a, x, i0 + lane, group, least, own, keys);
     if (rank(keys) != wanted) mine = 0;
     int run = mine;
 #pragma unroll
@@ -134,6 +206,7 @@ __device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, int lea
       t.row0 = (y - before - __shfl_sync(~0u, run - mine, k)) * kPair;
       t.first = __shfl_sync(~0u, own.first, k), t.n = __shfl_sync(~0u, own.n, k);
       t.slot = __shfl_sync(~0u, own.slot, k), t.len = __shfl_sync(~0u, own.len, k);
+      if constexpr (MODE == kShared) t.lo = __shfl_sync(~0u, own.lo, k), t.flat = t.seq >= a.n_seqs;
       return t;
     }
     before += __shfl_sync(~0u, run, 31);
@@ -374,7 +447,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (waits) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, plan.least, blockIdx.y);
+    const ChunkTile t = find_tile<MODE>(a, more, plan.least, blockIdx.y);
     if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
   }
   if (waits && warp == 11 && plan.least == 1 && a.err_flag)  // no other kernel in this call looks at the sequences
@@ -388,10 +461,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int64_t all_rows = (int64_t)n * group;
   const int rows = (int)min((int64_t)kPair, all_rows - tile.row0);
   const int t0 = tile.row0 / group, t1 = (tile.row0 + rows - 1) / group;  // first and last query of the pair
-  const int pos0 = len - n + t0, pos1 = len - n + t1;
+  const bool flat = MODE == kShared && tile.flat;
+  const int pos0 = flat ? len - 1 : len - n + t0, pos1 = flat ? len - 1 : len - n + t1;
   // keys that some row sees, and those that every row sees
-  const int lo = a.window > 0 ? first_seen(pos0, a.window) : 0, hi = max(0, pos1 + 1);
-  const int all_lo = a.window > 0 ? first_seen(pos1, a.window) : 0, all_hi = pos0 + 1;
+  const int item_lo = MODE == kShared ? tile.lo : 0;
+  const int lo = a.window > 0 ? first_seen(pos0, a.window) : item_lo, hi = max(0, pos1 + 1);
+  const int all_lo = a.window > 0 ? first_seen(pos1, a.window) : item_lo, all_hi = pos0 + 1;
   const Span span = span_of<MODE>(lo, hi, more);
   const int chunk = part_keys(plan, span.end - span.begin);
   const int parts = span.end > span.begin ? (span.end - span.begin + chunk - 1) / chunk : 1;
@@ -591,7 +666,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
     const uint32_t ts = tmem + lanes + kSCol + t * 2 * kStep, to = tmem + lanes + kOCol + t * D;
     const bool mine = r < rows;
-    const int pos = mine ? len - n + (tile.row0 + r) / group : -1;
+    const int pos = mine ? flat ? len - 1 : len - n + (tile.row0 + r) / group : -1;
     // (not 0: masked scores are -infinity before the factor; with the least number above 0 the exponents of finite
     // scores still vanish, and the weights are equal as a scale of 0 asks)
     const float c2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
@@ -623,7 +698,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tm_ld_wait32(s);
         tm_ld_wait32(s + 32);
         if (key < all_lo || key + kStep > all_hi || bad) {
-          const int last = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : 0;
+          const int last = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : MODE == kShared ? lo - key : 0;
           const int sunk = MODE == kSinks ? more.sinks - key : 0;
           unsigned ok = ~0u;  // pages that exist
           const int in_page = key & (a.page_tokens - 1);  // 64 in the second half of a 128-token page
@@ -702,12 +777,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int dt = (int)(((rem0 + r) * per_group) >> 20), q = t0 + dt, head = kvh * group + rem0 + r - dt * group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum, mm = m == -INFINITY ? 0.f : m * c2;
         const int64_t item = (int64_t)tile.index * a.kv_heads + kvh;
-        const int64_t at = (item * plan.parts + part) * kPair + r;
+        int64_t at = (item * plan.parts + part) * kPair + r;
+        if constexpr (MODE == kShared)
+          at = ((int64_t)((flat ? more.own_parts : 0) + part) * a.tokens + first + q) * a.q_heads + head;
+        float* const part_o = MODE == kShared ? more.o : plan.o;
+        const bool joined = MODE == kShared || parts > 1;  // by another kernel
         const bool odd = s_odd != 0;
-        if (mine && parts == 1 && a.lse)
+        if (mine && !joined && a.lse)
           a.lse[(int64_t)(first + q) * a.q_heads + head] =
               sum == 0.f ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
-        if (mine && parts > 1) plan.ml[at] = make_float2(m == -INFINITY ? m : mm, sum);
+        if (mine && joined) (MODE == kShared ? more.ml : plan.ml)[at] = make_float2(m == -INFINITY ? m : mm, sum);
         // The row goes through shared memory, where its queries were, so that whole rows are stored together.
         unsigned char* stage = smem + t * kTile;
 #pragma unroll
@@ -725,6 +804,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int w = begin; w < end; ++w) {
               const int k = key_at(w);
               if (k >= all_lo && k < all_hi) continue;  // went through the products
+              if (MODE == kShared && k < lo) continue;
               if (k > pos || (a.window > 0 && k <= pos - a.window && (MODE != kSinks || k >= more.sinks))) continue;
               const int id = table[k >> shift];
               if (id < 0 || id >= a.n_pages) continue;
@@ -740,11 +820,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               }
             }
           }
-          if (parts > 1) {
+          if (joined) {
             if (mine) {
 #pragma unroll
               for (int i = 0; i < 32; i += 4)
-                *reinterpret_cast<float4*>(plan.o + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                *reinterpret_cast<float4*>(part_o + at * D + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
           } else {
             const int row = r & (kMTile - 1);
@@ -756,7 +836,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                         ((((c + i) / 8 & 7) ^ (row & 7)) * 16)) = pack8<T>(o + i);
           }
         }
-        if (parts == 1) {
+        if (!joined) {
           __syncwarp();
           constexpr int kPieces = D / 8, kTogether = 32 / kPieces;  // 16-byte pieces of a row, rows at a time
           const int c = lane % kPieces, row0 = (warp & 3) * 32;
@@ -791,7 +871,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, More 
   __shared__ ChunkTile s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
   if (warp == 0) {
-    const ChunkTile t = find_tile(a, plan.least, blockIdx.y);
+    const ChunkTile t = find_tile<MODE>(a, more, plan.least, blockIdx.y);
     if (lane == 0) s_tile = t;
   }
   __syncthreads();
@@ -827,6 +907,55 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, More 
   for (int c = 0; c < D / 32; ++c) out[c * 32 + lane] = from_f32<T>(sum == 0.f ? 0.f : o[c] / sum);
   if (a.lse && lane == 0)
     a.lse[(int64_t)(first + t) * a.q_heads + head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Joins what each row got from its own keys and from the shared ones, part by part in order: one warp a row.  Rows of a
+// sequence that the others left out (an unknown slot, queries among the shared keys, more than max_q of them) become
+// zeros, and those of all where cu_q or cu_group does not ascend.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(q4gpu_attn_args a, More more, ChunkPlan plan) {
+  const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.q_heads / a.kv_heads, g = group_of(more, i);
+  const Item own = item_of<kShared>(a, more, i);
+  const bool valid = *more.malformed == 0 && own.n > 0 && own.len > 0;
+  const int all = max(0, min(a.cu_q[i + 1], a.tokens) - own.first);
+  Item pre{};
+  if (g >= 0) pre = item_of<kShared>(a, more, a.n_seqs + g);
+  auto parts_of = [&](int lo, int hi, const Item& s) {  // of a row pair
+    if (s.n < plan.least) return s.n > 0 ? 1 : 0;        // attn_rows_kernel's
+    const Span span = span_of<kShared>(lo, hi, more);
+    const int chunk = part_keys(plan, span.end - span.begin);
+    return span.end > span.begin ? (span.end - span.begin + chunk - 1) / chunk : 1;
+  };
+  for (int64_t y = (int64_t)blockIdx.y * 8 + warp; y < (int64_t)all * a.q_heads; y += (int64_t)gridDim.y * 8) {
+    const int t = (int)(y / a.q_heads), head = (int)(y - (int64_t)t * a.q_heads);
+    const int64_t row = (int64_t)(own.first + t) * a.q_heads + head, set = (int64_t)a.tokens * a.q_heads;
+    T* out = static_cast<T*>(a.out) + (int64_t)(own.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride;
+    float top = -INFINITY, sum = 0.f, o[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = 0.f;
+    int own_parts = 0, pre_parts = 0;
+    if (valid) {
+      const int64_t r = (int64_t)t * group + head % group, row0 = r / kPair * kPair;
+      const int rows = (int)min((int64_t)kPair, (int64_t)own.n * group - row0);
+      own_parts = parts_of(own.lo, max(0, own.len - own.n + (int)((row0 + rows - 1) / group) + 1), own);
+      pre_parts = g < 0 ? 0 : parts_of(0, pre.len, pre);
+    }
+    auto place = [&](int k) { return row + (k < own_parts ? k : more.own_parts + k - own_parts) * set; };
+    for (int k = 0; k < own_parts + pre_parts; ++k) top = fmaxf(top, more.ml[place(k)].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int k = 0; k < own_parts + pre_parts; ++k) {
+      const float2 w = more.ml[place(k)];
+      const float f = ex2(w.x - ref);
+      sum = fmaf(w.y, f, sum);
+      const float* p = more.o + place(k) * D + lane;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) o[c] = fmaf(p[c * 32], f, o[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) out[c * 32 + lane] = from_f32<T>(sum == 0.f ? 0.f : o[c] / sum);
+    if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+  }
 }
 
 }  // namespace paged

@@ -7,6 +7,7 @@ K/V cache, and what happens to the cache's pages between steps.
 * ``AddRmsNorm``  residual addition + RMS norm, 16-bit or 8-bit output with scales
 * ``RopeAppend``  q/k head norm, rotary positions, K/V stored in their pages
 * ``Attention``   a chunk of new tokens per sequence (or one) over the pages
+* ``SharedAttention``  the same where groups of sequences share their first keys
 * ``TokenLogprobs``  log probabilities of given tokens, entropy, likeliest tokens
 * ``Pages``       forking sequences, packing the pages in use
 * ``PagedCache``  a pool with its tables, and which pages are free
@@ -366,38 +367,51 @@ class Attention(_Err):
                     a.seq_ids = seq_ids.data_ptr()
                 return self._launch(out)
             self.layout = None
-            tokens = q.shape[0]
-            a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, "q")
-            a.out, a.out_token_stride, a.out_head_stride = self._heads(out, tokens, "out")
-            if cu_q.dtype != torch.int32 or cu_q.device != self.device or cu_q.dim() != 1 or cu_q.shape[0] < 1 or \
-                    not cu_q.is_contiguous():
-                raise ValueError(f"cu_q must be a contiguous int32 vector on {self.device}")
-            n = cu_q.shape[0] - 1
-            a.cu_q, a.n_seqs, a.tokens, a.max_q = cu_q.data_ptr(), n, tokens, max_q
-            a.max_ctx = max_ctx or min(a.table_pages * a.page_tokens, 2 ** 31 - 1)
-            a.seq_ids = a.lse = None
-            if seq_ids is not None:
-                _on(seq_ids, self.device, "seq_ids", torch.int32)
-                _need(seq_ids.shape == (n,) and seq_ids.is_contiguous(), f"seq_ids must be [{n}]")
-                a.seq_ids = seq_ids.data_ptr()
-            elif n > self.slots:
-                raise ValueError(f"{n} sequences over {self.slots} slots")
-            if lse is not None:
-                _on(lse, self.device, "lse", torch.float32)
-                if lse.shape != (tokens, self.q_heads) or not lse.is_contiguous():
-                    raise ValueError(f"lse must be contiguous [{tokens}, {self.q_heads}]")
-                a.lse = lse.data_ptr()
-            need = self._workspace_bytes(a)
-            if need > a.workspace_bytes:
-                if torch.cuda.is_current_stream_capturing():
-                    return self._launch_captured(out, need)
-                # the old ones stay: captured graphs know their addresses (each at least twice the last, so all
-                # together are less than two of the newest)
-                self.workspace = torch.zeros(max(need, 2 * a.workspace_bytes), dtype=torch.uint8, device=self.device)
-                self.own.append(self.workspace)
-                a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
-            self.layout = layout
-            return self._launch(out)
+            self._bind(q, out, cu_q, max_q, max_ctx, lse, seq_ids)
+            return self._run(out, layout)
+
+    def _bind(self, q: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, max_q: int, max_ctx: int,
+              lse: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor]) -> None:
+        """Checks a call's tensors and puts them into the arguments."""
+        a, tokens = self.args, q.shape[0]
+        a.q, a.q_token_stride, a.q_head_stride = self._heads(q, tokens, "q")
+        a.out, a.out_token_stride, a.out_head_stride = self._heads(out, tokens, "out")
+        a.cu_q, n = self._ends(cu_q, "cu_q")
+        a.n_seqs, a.tokens, a.max_q = n, tokens, max_q
+        a.max_ctx = max_ctx or min(a.table_pages * a.page_tokens, 2 ** 31 - 1)
+        a.seq_ids = a.lse = None
+        if seq_ids is not None:
+            _on(seq_ids, self.device, "seq_ids", torch.int32)
+            _need(seq_ids.shape == (n,) and seq_ids.is_contiguous(), f"seq_ids must be [{n}]")
+            a.seq_ids = seq_ids.data_ptr()
+        elif n > self.slots:
+            raise ValueError(f"{n} sequences over {self.slots} slots")
+        if lse is not None:
+            _on(lse, self.device, "lse", torch.float32)
+            if lse.shape != (tokens, self.q_heads) or not lse.is_contiguous():
+                raise ValueError(f"lse must be contiguous [{tokens}, {self.q_heads}]")
+            a.lse = lse.data_ptr()
+
+    def _ends(self, cu: torch.Tensor, name: str) -> tuple[int, int]:
+        if cu.dtype != torch.int32 or cu.device != self.device or cu.dim() != 1 or cu.shape[0] < 1 or \
+                not cu.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 vector on {self.device}")
+        return cu.data_ptr(), cu.shape[0] - 1
+
+    def _run(self, out: torch.Tensor, layout: tuple) -> torch.Tensor:
+        """Launches the checked call, with enough workspace; later calls of this layout need no checks."""
+        a = self.args
+        need = self._workspace_bytes(a)
+        if need > a.workspace_bytes:
+            if torch.cuda.is_current_stream_capturing():
+                return self._launch_captured(out, need)
+            # the old ones stay: captured graphs know their addresses (each at least twice the last, so all
+            # together are less than two of the newest)
+            self.workspace = torch.zeros(max(need, 2 * a.workspace_bytes), dtype=torch.uint8, device=self.device)
+            self.own.append(self.workspace)
+            a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
+        self.layout = layout
+        return self._launch(out)
 
     def _launch_captured(self, out: torch.Tensor, need: int) -> torch.Tensor:
         """A captured call that wants more workspace than there is: what is allocated now is zeroed by the graph's
@@ -430,6 +444,66 @@ class Attention(_Err):
         if t.shape != (tokens, self.q_heads, self.dim) or t.stride(2) != 1:
             raise ValueError(f"{name} must be [{tokens}, {self.q_heads}, {self.dim}] with contiguous head vectors")
         return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+class SharedAttention(Attention):
+    """``Attention`` of sequences that share their first keys: those are read once for all of a group.
+
+    Group g is the sequences cu_group[g] .. cu_group[g + 1] - 1 of a call and shares its
+    first prefix_lens[g] keys, which are read from the pages of the group's first
+    sequence.  Every query stands behind them.
+    """
+
+    def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                 q_heads: int, scale: Optional[float] = None):
+        super().__init__(k_cache, v_cache, table, lens, q_heads, scale)
+        self.groups = _native.SharedArgs()
+
+    def __call__(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,
+                 cu_group: Optional[torch.Tensor] = None, prefix_lens: Optional[torch.Tensor] = None, max_q: int = 1,
+                 max_ctx: int = 0, max_prefix: int = 0, lse: Optional[torch.Tensor] = None,
+                 seq_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """As ``Attention``, with cu_group int32 [groups + 1] and prefix_lens int32 [groups]; sequences in no
+        group share nothing; max_prefix: no prefix is longer (0: max_ctx).  A sequence whose queries do not
+        stand behind the shared keys is an error that `check` reports, and so are offsets that do not ascend."""
+        with self.lock:
+            a, g = self.args, self.groups
+            if cu_q is None or cu_group is None or prefix_lens is None:
+                raise ValueError("cu_q, cu_group and prefix_lens are needed")
+            if out is None:
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            # what the checks below look at: tensors laid out like the last call's need only their addresses
+            layout = (q.shape, q.stride(), q.dtype, q.device, out.shape, out.stride(), out.dtype, out.device,
+                      cu_q.shape, cu_q.stride(), cu_q.dtype, cu_q.device, max_q, max_ctx, max_prefix,
+                      cu_group.shape, cu_group.stride(), cu_group.dtype, cu_group.device,
+                      prefix_lens.shape, prefix_lens.stride(), prefix_lens.dtype, prefix_lens.device,
+                      None if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.device),
+                      None if seq_ids is None else (seq_ids.shape, seq_ids.stride(), seq_ids.dtype, seq_ids.device))
+            if layout == self.layout:
+                a.q, a.out, a.cu_q = q.data_ptr(), out.data_ptr(), cu_q.data_ptr()
+                g.cu_group, g.prefix_lens = cu_group.data_ptr(), prefix_lens.data_ptr()
+                if lse is not None:
+                    a.lse = lse.data_ptr()
+                if seq_ids is not None:
+                    a.seq_ids = seq_ids.data_ptr()
+                return self._launch(out)
+            self.layout = None
+            self._bind(q, out, cu_q, max_q, max_ctx, lse, seq_ids)
+            g.cu_group, g.n_groups = self._ends(cu_group, "cu_group")
+            _on(prefix_lens, self.device, "prefix_lens", torch.int32)
+            _need(prefix_lens.shape == (g.n_groups,) and prefix_lens.is_contiguous(),
+                  f"prefix_lens must be [{g.n_groups}]")
+            g.prefix_lens, g.max_prefix = prefix_lens.data_ptr(), max_prefix or a.max_ctx
+            return self._run(out, layout)
+
+    def _workspace_bytes(self, a: _native.AttnArgs) -> int:
+        return self.lib.q4gpu_shared_attention_workspace_bytes(a, self.groups)
+
+    def _launch(self, out: torch.Tensor) -> torch.Tensor:
+        rc = self.lib.q4gpu_shared_attention(self.args, self.groups, self._here())
+        if rc:
+            _native.check(rc, "q4gpu_shared_attention")
+        return out
 
 
 class TokenScores:

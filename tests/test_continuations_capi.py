@@ -72,3 +72,31 @@ def test_logprob_structure(tmp_path):
     assert int(out.pop("size")) == C.sizeof(_native.LogprobArgs)
     assert {k: int(v) for k, v in out.items()} == {n: getattr(_native.LogprobArgs, n).offset
                                                    for n, _ in _native.LogprobArgs._fields_}
+
+
+def shared(**kw):
+    return _native.SharedArgs(**(dict(cu_group=256, prefix_lens=256, n_groups=1, max_prefix=16) | kw))
+
+
+@pytest.mark.parametrize("kw,sh,rc", [
+    (dict(), dict(cu_group=None), ARG), (dict(), dict(prefix_lens=None), ARG), (dict(), dict(n_groups=-1), ARG),
+    (dict(), dict(n_groups=65536), ARG), (dict(), dict(max_prefix=-1), ARG), (dict(window=5), dict(), ARG),
+    (dict(dim=96), dict(), SHAPE), (dict(q=264), dict(), ALIGN), (dict(), dict(), WORKSPACE),
+    (dict(workspace=264, workspace_bytes=1 << 30), dict(), ALIGN),
+    (dict(tokens=2 ** 31 - 1, max_q=2 ** 31 - 1, q_heads=256, workspace=256, workspace_bytes=1 << 62), dict(), SHAPE)])
+def test_shared_refusals(lib, kw, sh, rc):
+    assert lib.q4gpu_shared_attention(attn(**kw), shared(**sh), None) == rc
+    assert lib.q4gpu_last_error().startswith(b"attention")
+
+
+def test_shared_sizes(lib):
+    size = lib.q4gpu_shared_attention_workspace_bytes
+    assert lib.q4gpu_shared_attention(attn(), None, None) == ARG and size(attn(), None) == 0
+    assert lib.q4gpu_shared_attention(attn(tokens=0), shared(), None) == 0
+    assert size(attn(window=3), shared()) == 0
+    one = size(attn(q_heads=16, kv_heads=8, dim=128, max_ctx=8192), shared())
+    # both sets of a row's unnormalised sums and statistics, beside the few-row kernel's own
+    many = dict(q_heads=16, kv_heads=8, dim=128, max_ctx=8192, n_seqs=64, tokens=64)
+    assert 0 < one < size(attn(**many), shared(max_prefix=8000)) < 1 << 26
+    assert size(attn(**many), shared()) >= 2 * 64 * 16 * (128 + 2) * 4
+    assert size(attn(tokens=2 ** 31 - 1, max_q=2 ** 31 - 1, q_heads=256), shared(n_groups=65535)) > 1 << 40
