@@ -322,25 +322,7 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* m, in
       : "memory");
 }
 
-// ---- pairs of float32 --------------------------------------------------------
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void split_pair(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
+// ---- exponentials -------------------------------------------------------------
 // 2^x of two values on the FMA pipe, for x <= 127.  Range reduction after Cody
 // and Waite: x = n + f with n = floor(x) from the low bits of x + 1.5 2^23
 // rounded down; 2^f on [0, 1] by the degree-4 polynomial with value 1 at 0 whose
