@@ -11,9 +11,12 @@ using namespace q4::paged;
 namespace {
 
 constexpr int kMostThreads = 512;
-constexpr int kMostParts = 16;    // CTAs of a row, a cluster
+constexpr int kMostParts = 8;  // CTAs of a row, a cluster
+constexpr int kUnit = 16;       // logits of a lane and step
+constexpr int kGroups = 64;     // of a row's threads, at most
 constexpr int kCandidates = 1024;
-constexpr float kLog2e = 1.4426950408889634f;
+static_assert(Q4GPU_TOP_MAX <= kGroups, "a group for each of the likeliest");
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Numbers that order like the logits: NaN above all, zeros of both signs alike.
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -40,25 +43,42 @@ __device__ __forceinline__ float largest(const float* x) {  // NaN if one is
   return m;
 }
 
-// 16 bytes of logits, which is how a row is read.
+// 16 neighbouring logits in pieces of 16 bytes, what a lane takes of a row at a time.
 template <typename T>
 struct Unit {
-  static constexpr int V = 16 / sizeof(T);
-  uint4 w;
+  static constexpr int kPieces = kUnit * sizeof(T) / 16;
+  static constexpr int kStages = sizeof(T) == 4 ? 3 : 4;  // steps of the ring: all but one of them in flight
+  uint4 w[kPieces];
   __device__ __forceinline__ void load(const uint4* p) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                 : "l"(p));
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                   : "l"(p + i));
   }
-  __device__ __forceinline__ void lowest() {  // all -infinity
+  __device__ __forceinline__ void take(int i, uint32_t at) {  // piece i from shared memory
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w)
+                 : "r"(at)
+                 : "memory");
+  }
+  // Place of piece c of lane r's unit among a warp's: neighbouring lanes' pieces lie in different banks.
+  static __device__ __forceinline__ int place(int r, int c) {
+    return r * kPieces + (c ^ (sizeof(T) == 4 ? (r >> 1) & 3 : (r >> 2) & 1));
+  }
+  static __device__ __forceinline__ void put_lowest(uint32_t at) {  // a piece of -infinities to shared memory
     const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
-    w = make_uint4(inf, inf, inf, inf);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(inf) : "memory");
   }
   __device__ __forceinline__ void get(float* x) const {
-    if constexpr (sizeof(T) == 4)
-      x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
-    else
-      unpack8<T>(w, x);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      if constexpr (sizeof(T) == 4)
+        x[4 * i] = __uint_as_float(w[i].x), x[4 * i + 1] = __uint_as_float(w[i].y),
+              x[4 * i + 2] = __uint_as_float(w[i].z), x[4 * i + 3] = __uint_as_float(w[i].w);
+      else
+        unpack8<T>(w[i], x + 8 * i);
+    }
   }
 };
 
@@ -72,16 +92,17 @@ struct Counter {  // two at a time: the halves of a mask of ones are -1 each, an
     return (uint32_t)b * 0x10001u;
   }
   __device__ __forceinline__ void add(const Unit<T>& u, uint32_t c) {
-    const uint32_t w[4] = {u.w.x, u.w.y, u.w.z, u.w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
+      const uint4& p = u.w[i / 4];
+      const uint32_t w = i % 4 == 0 ? p.x : i % 4 == 1 ? p.y : i % 4 == 2 ? p.z : p.w;
       if constexpr (__is_same(T, __half))
-        sum += __hge2_mask(*reinterpret_cast<const __half2*>(&w[i]), *reinterpret_cast<const __half2*>(&c));
+        sum += __hge2_mask(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&c));
       else
-        sum += __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), *reinterpret_cast<const __nv_bfloat162*>(&c));
+        sum += __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&c));
     }
   }
-  // sum = low (2^16 - 1) - high 2^16; at most 4 of each a unit
+  // sum = low (2^16 - 1) - high 2^16; at most 8 of each a unit
   __device__ __forceinline__ void flush() {
     const uint32_t low = (0u - sum) & 0xffffu, high = (low - (uint32_t)((sum + low) >> 16)) & 0xffffu;
     total += low + high, sum = 0;
@@ -92,8 +113,10 @@ struct Counter<float> {
   int total = 0;
   static __device__ __forceinline__ float bound(float v) { return v; }
   __device__ __forceinline__ void add(const Unit<float>& u, float c) {
-    total += (__uint_as_float(u.w.x) >= c) + (__uint_as_float(u.w.y) >= c) + (__uint_as_float(u.w.z) >= c) +
-             (__uint_as_float(u.w.w) >= c);
+    float x[kUnit];
+    u.get(x);
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) total += x[i] >= c;
   }
   __device__ __forceinline__ void flush() {}
 };
@@ -119,87 +142,39 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// What is known of some of a row's logits: the largest number m (-infinity: none), and over all but one place of it
-// S = sum e^(x - m) and T = sum e^(x - m) (x - m).
+// What a warp knows of its logits: m, the largest number of its own and of its CTA's first step (-infinity: none), and sums of
+// e^(x - m) and e^(x - m) (x - m).  One place of m is left out of the row's sums; `own`: it is one of this warp's.
 struct Sums {
   float m, s, t;
-  // The same against a larger m, with the place of the old one.
-  __device__ __forceinline__ void raise(float to) {
-    const float f = m == -INFINITY ? 0.f : ex2((m - to) * kLog2e);
-    t = f == 0.f ? 0.f : f * fmaf(m - to, s + 1.f, t);
-    s = f == 0.f ? 0.f : (s + 1.f) * f;
+  int own;
+  // The same against a larger m; `place`: with that of the old one.
+  __device__ __forceinline__ void raise(float to, bool place) {
+    const float f = m == -INFINITY ? 0.f : ex2((m - to) * kLog2e), all = place ? s + 1.f : s;
+    t = f == 0.f ? 0.f : f * fmaf(m - to, all, t);
+    s = f == 0.f ? 0.f : all * f;
     m = to;
   }
 };
-// The sums of each lane's logits joined; every lane gets them.
-__device__ __forceinline__ Sums join(Sums x) {
-  const float m = warp_max(x.m);
-  const unsigned first = __ballot_sync(~0u, x.m == m);
-  if ((threadIdx.x & 31) != (unsigned)(__ffs(first) - 1)) x.raise(m);
-  return Sums{m, warp_sum(x.s), warp_sum(x.t)};
-}
 
-// What a CTA knows of its part of a row.
-struct Part {
-  Sums sums;
-  int ahead, odd;
-  uint64_t top[Q4GPU_TOP_MAX];  // its first ones, falling; 0: no more
-};
+// What a lane holds of its warp's steps; s and t are the lane's share, the rest is the same in all.
+struct Held {
+  Sums sums{-INFINITY, 0.f, 0.f, 0};
+  bool left = false;  // the place to leave out is among the logits to come
+  bool odd = false;   // a NaN or +infinity (this lane's)
+  // The steps' reference, m log2e rounded, and what the rounding left out: e^(x - m) = 2^(x log2e - ref) 2^-rest.  Not
+  // for numbers so large that the rest is.
+  float ref = 0.f, rest = 0.f, back = 1.f;
+  bool tame = false;
 
-// `parts` CTAs a row (a cluster), each a stretch of its 16-byte units; what stands before the first and behind the last
-// boundary of 16 bytes is the first CTA's.  With m the row's largest logit,
-//   log p_t = (x_t - m) - log1p(S),   H = log1p(S) - T / (1 + S),
-// (see Sums) sums without cancellation however certain the row is.  The logits are read once: a warp
-// holds its sums against its own largest so far, which few steps change.
-// Of the likeliest only the largest of each thread is followed on the way.  The top-th of the largest of 32 groups of threads
-// bounds the top-th of all from below, and about as many logits as are wanted lie above
-// it: the few threads whose largest does are read again, from L2, and what lies above
-// the bound is ranked by counting.
-template <typename T>
-__global__ void __launch_bounds__(kMostThreads) token_logprobs_kernel(q4gpu_logprob_args a, int parts) {
-  constexpr int V = Unit<T>::V, U = 2;
-  __shared__ Part s_part;
-  __shared__ Sums s_sums[kMostThreads / 32];
-  __shared__ int s_ahead[kMostThreads / 32], s_odd, s_threads, s_found;
-  __shared__ uint64_t s_group[32], s_key[kCandidates];
-  __shared__ uint16_t s_thread[kMostThreads];
-  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
-  const int part = blockIdx.x % (unsigned)parts;
-  const int64_t row = blockIdx.x / (unsigned)parts;
-  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
-  const int head = min(a.vocab, (int)((0 - reinterpret_cast<uintptr_t>(x)) & 15) / (int)sizeof(T));
-  const uint4* body = reinterpret_cast<const uint4*>(x + head);
-  const int units = (a.vocab - head) / V, tail = head + units * V;  // where the last few begin
-  const int share = (units + parts - 1) / parts, u0 = min(units, part * share), u1 = min(units, u0 + share);
-
-  Unit<T> next[U];
-#pragma unroll
-  for (int j = 0; j < U; ++j) {
-    next[j].lowest();
-    if (u0 + tid + j * threads < u1) next[j].load(body + u0 + tid + j * threads);
+  __device__ __forceinline__ void raise(float to, bool own) {
+    sums.raise(to, sums.own && (threadIdx.x & 31) == 0);
+    sums.own = own;
+    ref = to * kLog2e, rest = fmaf(to, kLog2e, -ref), back = ex2(-rest);
+    tame = fabsf(to) < 65536.f;
   }
-  const int64_t given = a.targets ? a.targets[row] : -1;
-  const bool known = given >= 0 && given < a.vocab;
-  const T mine = known ? x[given] : from_f32<T>(__uint_as_float(0x7fffffffu));
-  // logits before the target's unit count from its value on, later ones above it
-  const int mine_unit = !known ? 0 : given < head ? -1 : given >= tail ? units : (int)(given - head) / V;
-  const auto from = Counter<T>::bound(mine), past = Counter<T>::bound(above(mine));
-  // the ends of the row, one logit a lane of one warp, and the logits before the target in its unit
-  const bool ends = part == 0 && warp == 0;
-  const int end_at = lane < 16 ? lane : tail + lane - 16;
-  const bool end_there = ends && (lane < 16 ? lane < head : end_at < a.vocab);
-  const float end = end_there ? to_f32(x[end_at]) : -INFINITY;
-  const int near_at = head + mine_unit * V + lane;
-  const bool tie = known && warp == 0 && mine_unit >= u0 && mine_unit < u1 && near_at < given &&
-                   to_f32(x[near_at]) == to_f32(mine);
-  if (tid == 0) s_odd = s_threads = s_found = 0;
-  if (tid < Q4GPU_TOP_MAX) s_part.top[tid] = 0;
-
-  Sums sums{-INFINITY, 0.f, 0.f};  // m: the warp's; s, t: this lane's share
-  bool odd = false;                // a NaN or +infinity
-  // N more logits of each lane (-infinity for none), where one reaches the warp's largest
-  auto careful = [&](float* v, auto count) {
-    constexpr int N = decltype(count)::value;
+  // N more logits of each lane (-infinity for none), where one may reach m.
+  template <int N>
+  __device__ __forceinline__ void careful(float* v) {
     float most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -207,247 +182,387 @@ __global__ void __launch_bounds__(kMostThreads) token_logprobs_kernel(q4gpu_logp
       most = fmaxf(most, v[i]);
     }
     most = warp_max(most);
-    int same = 0;  // one place of the largest is left out of the sums
-    if (most > sums.m) {
-      const float f = sums.m == -INFINITY ? 0.f : ex2((sums.m - most) * kLog2e);
-      const float place = lane == 0 ? 1.f : 0.f;  // that of the old largest comes in
-      sums.t = f == 0.f ? 0.f : f * fmaf(sums.m - most, sums.s + place, sums.t);
-      sums.s = f == 0.f ? 0.f : (sums.s + place) * f;
-      sums.m = most;
+    int same = 0;
+    if (most > sums.m) {  // one place of the largest is left out of the sums
+      raise(most, true);
       same = -1;
     }
-    if (most == -INFINITY && sums.m == -INFINITY) return;
-    int mine_same = 0;
+    if (sums.m == -INFINITY) return;
+    if (left) same = -1, left = false;
+    int mine = 0;
+    float s = 0.f, t[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = v[i] - sums.m, e = ex2(d * kLog2e);
-      if (v[i] == sums.m) {
-        ++mine_same;
-      } else if (e > 0.f) {
-        sums.s += e, sums.t = fmaf(e, d, sums.t);
+      const float d = v[i] - sums.m;
+      float e = ex2(d * kLog2e);
+      if (v[i] == sums.m) ++mine, e = 0.f;
+      s += e;
+      if (e > 0.f) t[i & 1] = fmaf(e, d, t[i & 1]);
+    }
+    same += __reduce_add_sync(~0u, mine);
+    sums.s += (threadIdx.x & 31) == 0 ? s + (float)same : s, sums.t += t[0] + t[1];
+  }
+};
+// Out of line: few steps come here, and the registers it takes cost the steps that do not.
+template <typename T>
+__device__ __noinline__ Held careful_step(Held h, uint32_t warp_at) {
+  Unit<T> now;
+#pragma unroll
+  for (int i = 0; i < Unit<T>::kPieces; ++i) now.take(i, warp_at + Unit<T>::place(threadIdx.x & 31, i) * 16);
+  float v[kUnit];
+  now.get(v);
+  h.careful<kUnit>(v);
+  return h;
+}
+
+// What the CTAs of a row tell each other.
+struct Board {
+  uint64_t group[kGroups];  // the largest of each group of threads
+  uint64_t key[kCandidates];
+  Sums sums[kMostParts * kMostThreads / 32];
+  int found, ahead, odd;
+};
+
+// `parts` CTAs a row (a cluster), each a stretch of its units of 16 logits; what stands before the first boundary of 16
+// bytes and behind the last whole unit is the first CTA's.  With m the row's largest logit, S the sum of e^(x - m) over all but one
+// place of it and T = sum e^(x - m) (x - m),
+//   log p_t = (x_t - m) - log1p(S),   H = log1p(S) - T / (1 + S),
+// sums without cancellation however certain the row is.  The logits are read once; a warp holds its
+// sums against the largest logit of its own and of the CTA's first step, which few steps change.
+// Of the likeliest only each thread's largest is followed on the way.  The top-th of the largest of 32 or 64 groups of threads
+// bounds the top-th of all from below, and about as many logits as are wanted lie above
+// it: the few threads whose largest does are read again, from L2, and what lies above
+// the bound is ranked by counting.
+template <typename T>
+__global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_logprob_args a, int parts) {
+  constexpr int P = Unit<T>::kPieces, S = Unit<T>::kStages;
+  extern __shared__ uint4 ring[];  // [warp][stage][Unit::place]
+  __shared__ Board s_board;
+  __shared__ uint64_t s_bound, s_top[Q4GPU_TOP_MAX];
+  __shared__ uint16_t s_thread[kMostThreads];
+  __shared__ int s_odd, s_threads;
+  __shared__ float s_first[kMostThreads / 32];
+  __shared__ Sums s_sums;
+  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+  const int part = blockIdx.x % (unsigned)parts;
+  const int64_t row = blockIdx.x / (unsigned)parts;
+  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+  const int head = min(a.vocab, (int)((0 - reinterpret_cast<uintptr_t>(x)) & 15) / (int)sizeof(T));
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  const int units = (a.vocab - head) / kUnit, tail = head + units * kUnit;  // where the last few begin
+  const int share = (units + parts - 1) / parts, u0 = min(units, part * share), u1 = min(units, u0 + share);
+  const int whole = (u1 - u0) / threads, steps = (u1 - u0 + threads - 1) / threads;
+
+  // A warp fetches its lanes' units together, neighbouring pieces by neighbouring lanes.
+  constexpr uint32_t kStage = 32 * P * 16;
+  const uint32_t warp_at = (uint32_t)__cvta_generic_to_shared(ring) + warp * S * kStage;
+  const uint32_t put_at = warp_at + Unit<T>::place(lane / P, lane % P) * 16;  // the next 32 pieces' are 512 bytes on
+  const uint4* source = body + (int64_t)(u0 + warp * 32) * P + lane;          // of the step that is fetched next
+  auto fetch = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) cp16(put_at + stage * kStage + i * 512, source + 32 * i, true);
+    cp_commit();
+    source += threads * P;
+  };
+  auto fetch_some = [&](int step) {  // that may not be whole, or not there
+    if (step < whole) return fetch(step % S);
+    if (step < steps) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const uint32_t to = put_at + step % S * kStage + i * 512;
+        if (u0 + step * threads + warp * 32 + (32 * i + lane) / P < u1)
+          cp16(to, source + 32 * i, true);
+        else
+          Unit<T>::put_lowest(to);
       }
     }
-    same += __reduce_add_sync(~0u, mine_same);
-    if (lane == 0) sums.s += (float)same;
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch_some(i);
+
+  const int64_t given = a.targets ? a.targets[row] : -1;
+  const bool known = given >= 0 && given < a.vocab;
+  const T mine = known ? x[given] : from_f32<T>(__uint_as_float(0x7fffffffu));
+  // logits before the target's unit count from its value on, later ones above it
+  const int mine_unit = !known ? 0 : given < head ? -1 : given >= tail ? units : (int)(given - head) / kUnit;
+  const auto from = Counter<T>::bound(mine), past = Counter<T>::bound(above(mine));
+  // the ends of the row, one logit a lane of one warp, and the logits before the target in its unit
+  const bool ends = part == 0 && warp == 0 && (head > 0 || tail < a.vocab);
+  const int end_at = lane < 8 ? lane : tail + lane - 8;
+  const bool end_there = ends && (lane < 8 ? lane < head : end_at < a.vocab);
+  const float end = end_there ? to_f32(x[end_at]) : -INFINITY;
+  const int near_at = head + mine_unit * kUnit + lane;
+  const bool tie = known && warp == 0 && mine_unit >= u0 && mine_unit < u1 && near_at < given &&
+                   to_f32(x[near_at]) == to_f32(mine);
+  if (tid < kGroups) s_board.group[tid] = 0;
+  if (tid == 0) s_board.found = s_board.ahead = s_board.odd = s_odd = s_threads = 0;
+  if (parts > 1)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  __syncthreads();
+  auto board = [&](int p) {  // part p's
+    Board* q = &s_board;
+    if (parts > 1) asm("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(&s_board), "r"(p));
+    return q;
   };
 
+  Held h;
   float most = -INFINITY;  // this thread's largest and the first unit that holds it
   int most_unit = u0 + tid;
   Counter<T> counter;
-  const int steps = (u1 - u0 + threads * U - 1) / (threads * U);
-  for (int step = 0; step < steps; ++step) {
-    Unit<T> now[U];
-    const int u = u0 + tid + step * U * threads;
+  int counted = 0;
+  const float target = known ? to_f32(mine) : INFINITY;
+  float limit = -INFINITY;  // m where the fast way may go up to it
+  uint32_t get_at[P];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      now[j] = next[j];
-      const int later = u + (U + j) * threads;
-      if (later < u1) next[j].load(body + later);
-      else next[j].lowest();
-    }
-    float v[U * V], tops[U];
+  for (int i = 0; i < P; ++i) get_at[i] = warp_at + Unit<T>::place(lane, i) * 16;
+  if (steps > 0) {  // the largest of the CTA's first step (of no later one, or it would depend on how far each warp is)
+    cp_wait<S - 2>();
+    __syncwarp();
+    Unit<T> now;
+    float v[kUnit];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      now[j].get(v + j * V);
-      tops[j] = largest<V>(v + j * V);
-      if (!(tops[j] <= most) && most == most) most = tops[j], most_unit = u + j * threads;
-      const int uj = u + j * threads;
-      if (uj < u1) counter.add(now[j], uj < mine_unit ? from : past);
+    for (int i = 0; i < P; ++i) now.take(i, get_at[i]);
+    now.get(v);
+    const float top = largest<kUnit>(v), w = warp_max(is_number(top) ? top : -INFINITY);
+    if (lane == 0) s_first[warp] = w;
+    __syncthreads();
+    const float m = lane < warps ? s_first[lane] : -INFINITY, all = warp_max(m);
+    h.left = __ffs(__ballot_sync(~0u, m == all)) - 1 == warp;
+    if (all > -INFINITY) h.raise(all, h.left);
+    limit = h.tame ? h.sums.m : -INFINITY;
+  }
+  int u = u0 + tid;
+  auto add = [&](int stage, auto whole_step, auto fetch_next) {
+    constexpr bool kWhole = decltype(whole_step)::value;
+    cp_wait<S - 2>();
+    __syncwarp();
+    Unit<T> now;
+#pragma unroll
+    for (int i = 0; i < P; ++i) now.take(i, get_at[i] + stage * kStage);
+    fetch_next();  // into the stage that was read a step before: the warp was whole since
+    float v[kUnit];
+    now.get(v);
+    const float top = largest<kUnit>(v);
+    if (!(top <= most) && most == most) most = top, most_unit = u;
+    if (__any_sync(~0u, !(top < target))) {  // a warp's logits mostly lie below the target's
+      if (kWhole || u < u1) counter.add(now, u < mine_unit ? from : past);
+      if ((++counted & 4095) == 0) counter.flush();
     }
-    if ((step & 4095) == 4095) counter.flush();
-    if (__any_sync(~0u, !(largest<U>(tops) < sums.m))) {
-      careful(v, std::integral_constant<int, U * V>());
+    if (__any_sync(~0u, !(top < limit))) {
+      h = careful_step<T>(h, warp_at + stage * kStage);
+      limit = h.tame ? h.sums.m : -INFINITY;
     } else {
-      const float before = sums.t;
-      const uint64_t m2 = pair_of(-sums.m, -sums.m), c2 = pair_of(kLog2e, kLog2e);
-      uint64_t s2 = 0, t2 = 0;
+      // e = 2^(x log2e - ref), a product and a sum with one rounding
+      const uint64_t r2 = pair_of(-h.ref, -h.ref), c2 = pair_of(kLog2e, kLog2e);
+      uint64_t s2 = 0, p2 = 0;
 #pragma unroll
-      for (int i = 0; i < U * V; i += 2) {
-        const uint64_t d = add_pair(pair_of(v[i], v[i + 1]), m2);
-        float ex, ey;
-        split_pair(mul_pair(d, c2), ex, ey);
-        const uint64_t e = pair_of(ex2(ex), ex2(ey));
-        s2 = add_pair(s2, e);
-        t2 = fma_pair(e, d, t2);
+      for (int i = 0; i < kUnit; i += 2) {
+        const uint64_t d = fma_pair(pair_of(v[i], v[i + 1]), c2, r2);
+        float x, y;
+        split_pair(d, x, y);
+        const uint64_t e = pair_of(ex2(x), ex2(y));
+        s2 = i ? add_pair(s2, e) : e;
+        p2 = fma_pair(e, d, p2);
       }
-      float p, q;
-      split_pair(s2, p, q);
-      sums.s += p + q;
-      split_pair(t2, p, q);
-      p += q;
-      if (!(p == p)) {  // 0 times -infinity
-        p = 0.f;
+      float s, p, x;
+      split_pair(s2, s, x);
+      s += x;
+      split_pair(p2, p, x);
+      p += x;
+      if (kWhole || u < u1) {
+        h.sums.s = fmaf(s, h.back, h.sums.s);
+        h.sums.t = fmaf(fmaf(-h.rest, s, p), h.back * kLn2, h.sums.t);
+      }
+    }
+    u += threads;
+  };
+  int step = 0;
+  for (; step + 2 * S - 1 <= whole; step += S) {
 #pragma unroll
-        for (int i = 0; i < U * V; ++i) {
-          const float d = v[i] - sums.m, e = ex2(d * kLog2e);
-          if (e > 0.f) p = fmaf(e, d, p);
-        }
+    for (int i = 0; i < S; ++i) add(i, std::true_type(), [&] { fetch((i + S - 1) % S); });
+  }
+  for (; step < steps; ++step) add(step % S, std::false_type(), [&] { fetch_some(step + S - 1); });
+  Sums sums = h.sums;
+  if (__any_sync(~0u, sums.t != sums.t)) {  // 0 times -infinity: rows with masks, whose sums are taken again
+    sums.t = 0.f;
+    for (int i = u0 + tid; i < u1; i += threads) {
+      Unit<T> now;
+      float v[kUnit];
+      now.load(body + (int64_t)i * P);
+      now.get(v);
+#pragma unroll
+      for (int k = 0; k < kUnit; ++k) {
+        const float d = v[k] - sums.m, e = ex2(d * kLog2e);
+        if (e > 0.f) sums.t = fmaf(e, d, sums.t);
       }
-      sums.t = before + p;
     }
   }
+  h.sums = sums;
   counter.flush();
-  int ahead = counter.total;
+  int ahead = counter.total + tie;
   const uint64_t end_key = end_there ? key_of(end, end_at) : 0, mine_key = known ? key_of(to_f32(mine), (int)given) : ~0ull;
   if (ends) {
     float v = end;
-    careful(&v, std::integral_constant<int, 1>());
+    h.careful<1>(&v);
     ahead += end_key > mine_key;
   }
-  if (odd) s_odd = 1;
-  {
-    Sums w = sums;
-    w.s = warp_sum(w.s), w.t = warp_sum(w.t);
-    ahead = __reduce_add_sync(~0u, ahead);
-    if (lane == 0) s_sums[warp] = w, s_ahead[warp] = ahead;
-  }
-  // the groups' largest: `warps` neighbouring lanes each
+  if (h.odd) s_odd = 1;
+  sums = h.sums;
+  sums.s = warp_sum(sums.s), sums.t = warp_sum(sums.t);
   uint64_t key = u0 + tid < u1 ? (uint64_t)order_of(most) << 32 | (uint32_t)~most_unit : 0;
+  const int groups = a.top <= kGroups / 4 ? kGroups / 2 : kGroups;  // (fewer for a few, whose bound is as good)
+  const int span = threads * parts / groups, lanes = min(span, 32);  // threads of a group, and those of them in a warp
+  uint64_t group = key;
+  if (a.top)
+    for (int o = 1; o < lanes; o <<= 1)
+      group = max(group, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)group, o));
+
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all boards are clean
+  Board* const first = board(0);
+  if (lane == 0) first->sums[part * warps + warp] = sums;
   if (a.top) {
-    uint64_t g = key;
-    for (int o = 1; o < warps; o <<= 1) g = max(g, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)g, o));
-    if (tid % warps == 0) s_group[tid / warps] = g;
+    const int g = (part * threads + tid) / span;
+    if (span > 32) {
+      if (lane < parts) atomicMax(reinterpret_cast<unsigned long long*>(&board(lane)->group[g]), (unsigned long long)group);
+    } else if (lane % lanes == 0) {
+      for (int p = 0; p < parts; ++p) board(p)->group[g] = group;
+    }
   }
-  __syncthreads();
+  auto meet = [&] {  // of the row's CTAs
+    if (parts > 1)
+      asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else
+      __syncthreads();
+  };
+  meet();
+  if (s_odd && known) {  // the order has NaNs, which comparisons leave out
+    ahead = end_key > mine_key;
+    for (int u = u0 + tid; u < u1; u += threads)
+      for (int i = head + u * kUnit; i < head + (u + 1) * kUnit; ++i) ahead += key_of(to_f32(x[i]), i) > mine_key;
+  }
+  ahead = __reduce_add_sync(~0u, ahead);
+  if (lane == 0 && ahead) atomicAdd(&first->ahead, ahead);
+  if (tid == 0 && s_odd) atomicOr(&first->odd, 1);
   if (a.top) {
-    const uint64_t g = s_group[lane];
+    // the group whose largest is the top-th: `peers` neighbouring lanes compare one with all
+    const int peers = threads / groups, g = tid / peers;
+    const uint64_t k = s_board.group[g];
     int before = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) before += s_group[i] > g || (s_group[i] == g && i < lane);
-    const unsigned at = __ballot_sync(~0u, before == a.top - 1);
-    const uint64_t bound = __shfl_sync(~0u, (unsigned long long)g, __ffs(at) - 1);
+    for (int i = tid % peers; i < groups; i += peers) before += s_board.group[i] > k || (s_board.group[i] == k && i < g);
+    for (int o = 1; o < peers; o <<= 1) before += __shfl_xor_sync(~0u, before, o);
+    if (before == a.top - 1) s_bound = k;
+    __syncthreads();
+    const uint64_t bound = s_bound;
     if (key && key >= bound) s_thread[atomicAdd(&s_threads, 1)] = (uint16_t)tid;
     auto found = [&](uint64_t k) {
-      const int n = atomicAdd(&s_found, 1);
-      if (n < kCandidates) s_key[n] = k;
+      const int n = atomicAdd(&first->found, 1);
+      if (n < kCandidates) first->key[n] = k;
     };
     if (end_there && end_key >= (bound & ~0xffffffffull)) found(end_key);
     __syncthreads();
+    const uint32_t bound_value = (uint32_t)(bound >> 32);
+    constexpr int kTogether = 8 / P;  // units on their way at a time
     for (int i = warp; i < s_threads; i += warps)
-      for (int u = u0 + s_thread[i] + lane * threads; u < u1; u += 32 * threads) {
-        Unit<T> w;
-        float v[V];
-        w.load(body + u);
-        w.get(v);
+      for (int u = u0 + s_thread[i] + lane * threads; u < u1; u += kTogether * 32 * threads) {
+        Unit<T> w[kTogether];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (((uint64_t)order_of(v[e]) << 32 | (uint32_t)~u) >= bound) found(key_of(v[e], head + u * V + e));
+        for (int j = 0; j < kTogether; ++j)
+          if (u + j * 32 * threads < u1) w[j].load(body + (int64_t)(u + j * 32 * threads) * P);
+#pragma unroll
+        for (int j = 0; j < kTogether; ++j) {
+          const int at = u + j * 32 * threads;
+          if (at >= u1) break;
+          float v[kUnit];
+          w[j].get(v);
+          if (order_of(largest<kUnit>(v)) < bound_value) continue;
+#pragma unroll
+          for (int e = 0; e < kUnit; ++e)
+            if (((uint64_t)order_of(v[e]) << 32 | (uint32_t)~at) >= bound) found(key_of(v[e], head + at * kUnit + e));
+        }
       }
-    __syncthreads();
-    const int n = s_found;
-    if (n <= kCandidates) {
-      for (int i = tid; i < n; i += threads) {
-        const uint64_t k = s_key[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += s_key[j] > k;
-        if (rank < a.top) s_part.top[rank] = k;
-      }
-    } else {  // many logits in few threads: one after another over the whole part
-      uint64_t last = ~0ull;
-      for (int k = 0; k < a.top; ++k) {
-        uint64_t best = end_key < last ? end_key : 0;
-        for (int u = u0 + tid; u < u1; u += threads)
-          for (int e = 0; e < V; ++e) {
-            const uint64_t c = key_of(to_f32(x[head + u * V + e]), head + u * V + e);
-            if (c < last) best = max(best, c);
-          }
-        for (int o = 16; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)best, o));
-        __syncthreads();
-        if (lane == 0) s_key[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < warps; ++w) best = max(best, s_key[w]);
-        if (tid == 0) s_part.top[k] = best;
-        last = best;
-      }
-    }
   }
-  if (s_odd && known) {  // the order has NaNs, which comparisons leave out
-    __syncthreads();
-    ahead = end_key > mine_key;
-    for (int u = u0 + tid; u < u1; u += threads)
-      for (int e = 0; e < V; ++e) ahead += key_of(to_f32(x[head + u * V + e]), head + u * V + e) > mine_key;
-    ahead = __reduce_add_sync(~0u, ahead);
-    if (lane == 0) s_ahead[warp] = ahead;
-    __syncthreads();
+  meet();
+  if (part != 0) return;
+
+  // the first CTA has everything
+  const int n = a.top ? s_board.found : 0;
+  if (n <= kCandidates) {
+    for (int i = tid; i < n; i += threads) {
+      const uint64_t k = s_board.key[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_board.key[j] > k;
+      if (rank < a.top) s_top[rank] = k;
+    }
+  } else {  // many of a few threads' logits: one after another over the whole row
+    uint64_t last = ~0ull;
+    for (int k = 0; k < a.top; ++k) {
+      uint64_t best = 0;
+      for (int i = tid; i < a.vocab; i += threads) {
+        const uint64_t c = key_of(to_f32(x[i]), i);
+        if (c < last) best = max(best, c);
+      }
+      for (int o = 16; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)best, o));
+      __syncthreads();
+      if (lane == 0) s_board.key[warp] = best;
+      __syncthreads();
+      for (int w = 0; w < warps; ++w) best = max(best, s_board.key[w]);
+      if (tid == 0) s_top[k] = best;
+      last = best;
+    }
   }
   if (warp == 0) {
-    Sums w{-INFINITY, 0.f, 0.f};
-    if (lane < warps) w = s_sums[lane];
-    w = join(w);
-    int n = (lane < warps ? s_ahead[lane] : 0) + (tie && !s_odd);
-    n = __reduce_add_sync(~0u, n);
-    if (lane == 0) s_part.sums = w, s_part.ahead = n, s_part.odd = s_odd;
-  }
-
-  // the parts joined by the first CTA
-  const Part* all = &s_part;
-  auto part_at = [&](int p) {
-    const Part* q = all;
-    if (parts > 1)
-      asm("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(all), "r"(p));
-    return q;
-  };
-  if (parts > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  } else {
-    __syncthreads();
-  }
-  if (part == 0) {
-    const float nan = __uint_as_float(0x7fffffffu);
-    if (warp == 0 || a.top) {  // (every warp that writes likeliest tokens needs the sums)
-      Sums w{-INFINITY, 0.f, 0.f};
-      int n = 0, no = 0;
-      if (lane < parts) {
-        const Part* q = part_at(lane);
-        w = q->sums, n = q->ahead, no = q->odd;
-      }
-      w = join(w);
-      n = __reduce_add_sync(~0u, n);
-      const bool bad = __any_sync(~0u, no), none = w.m == -INFINITY;
-      const float norm = log1pf(w.s);
-      auto logprob = [&](float v) { return bad ? nan : none ? -INFINITY : (v - w.m) - norm; };
-      if (tid == 0) {
-        if (a.targets) {
-          a.logprob[row] = known ? logprob(to_f32(mine)) : 0.f;
-          a.rank[row] = known ? n + 1 : 0;
-          if (given >= a.vocab && a.err_flag) *a.err_flag = 1;
-        }
-        a.entropy[row] = bad ? nan : none ? 0.f : norm - w.t / (1.f + w.s);
-      }
-      for (int i = tid; i < parts * a.top; i += threads) {
-        const int p = i / a.top, k = i - p * a.top;
-        const uint64_t c = part_at(p)->top[k];
-        int rank = k;
-        for (int q = 0; q < parts; ++q) {
-          if (q == p) continue;
-          const uint64_t* t = part_at(q)->top;
-          int lo = 0;  // how many of the part's are before this one
-#pragma unroll
-          for (int s = Q4GPU_TOP_MAX / 2; s; s >>= 1)
-            if (t[lo + s - 1] > c) lo += s;
-          rank += lo + (t[lo] > c);
-        }
-        if (c && rank < a.top) {
-          a.top_logprob[row * a.top + rank] = logprob(logit_of((uint32_t)(c >> 32)));
-          a.top_index[row * a.top + rank] = ~(int)(uint32_t)c;
-        }
-      }
+    const int all = parts * warps;
+    float m = -INFINITY;
+    for (int i = lane; i < all; i += 32) m = fmaxf(m, s_board.sums[i].m);
+    m = warp_max(m);
+    Sums w{m, 0.f, 0.f, 0};
+    int owners = 0;  // of places of m, one of which is left out
+    for (int i = lane; i < all; i += 32) {
+      Sums v = s_board.sums[i];
+      if (v.m == m)
+        owners += v.own;
+      else
+        v.raise(m, v.own);
+      w.s += v.s, w.t += v.t;
     }
+    owners = __reduce_add_sync(~0u, owners);
+    w.s = warp_sum(w.s) + (float)max(owners - 1, 0), w.t = warp_sum(w.t);
+    if (lane == 0) s_sums = w;
   }
-  if (parts > 1)  // the first CTA has read the others' memory
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  __syncthreads();
+  const Sums w = s_sums;
+  const bool bad = s_board.odd, none = w.m == -INFINITY;
+  const float norm = log1pf(w.s), nan = __uint_as_float(0x7fffffffu);
+  auto logprob = [&](float v) { return bad ? nan : none ? -INFINITY : (v - w.m) - norm; };
+  if (tid == 0) {
+    if (a.targets) {
+      a.logprob[row] = known ? logprob(to_f32(mine)) : 0.f;
+      a.rank[row] = known ? s_board.ahead + 1 : 0;
+      if (given >= a.vocab && a.err_flag) *a.err_flag = 1;
+    }
+    a.entropy[row] = bad ? nan : none ? 0.f : norm - w.t / (1.f + w.s);
+  }
+  if (tid < a.top) {
+    a.top_logprob[row * a.top + tid] = logprob(logit_of((uint32_t)(s_top[tid] >> 32)));
+    a.top_index[row * a.top + tid] = ~(int)(uint32_t)s_top[tid];
+  }
 }
 
-// CTAs of a row and threads of a CTA.
+// CTAs of a row and threads of a CTA.  A thread has at least two units where there are as many, since a warp's start and
+// end take as long as six steps (us; 700 rows of 4099: 8.7 with 128 threads, 11.4 with 256; 4000 of 32000: 128 with 256,
+// 137 with 128, 157 with 512; 2048 of 151936: 164 with 512, 171 with 256).  Few rows take a cluster each, as long as
+// that gives no SM a second CTA: clusters wait for one another's SMs (one row of 151936 floats: 17.1 alone, 14.3, 12.1 and 11.1
+// with 2, 4 and 8 CTAs; 64 rows: 21.2, 17.6, 18.7, 30.2).
 struct Shape {
   int parts, threads;
 };
 Shape shape_of(const q4gpu_logprob_args& a) {
-  const int64_t units = (int64_t)a.vocab * (a.dtype == Q4GPU_F32 ? 4 : 2) / 16;
-  Shape s{1, kMostThreads};
-  while (s.threads > 32 && units <= s.threads * 2) s.threads /= 4;
-  if (s.threads < 32) s.threads = 32;
-  while (s.parts < kMostParts && a.rows * s.parts * s.threads < 148 * 1024 && units / s.parts >= 4 * s.threads)
+  const int64_t units = a.vocab / kUnit;
+  Shape s{1, 64};
+  while (s.threads < kMostThreads && units >= (s.threads < 128 ? 2 : 8) * s.threads) s.threads *= 2;
+  while (s.parts < kMostParts && a.rows * s.parts * s.threads * 2 <= 148 * kMostThreads &&
+         units / s.parts >= 2 * s.threads)
     s.parts *= 2;
   return s;
 }
@@ -456,22 +571,24 @@ template <typename T>
 int launch(const q4gpu_logprob_args& a, cudaStream_t stream) {
   const Shape s = shape_of(a);
   if (a.rows * s.parts > INT32_MAX) return q4gpu_fail(Q4GPU_ERR_SHAPE, "logprobs: too many rows");
+  constexpr int kPerThread = kUnit * (int)sizeof(T) * Unit<T>::kStages;  // of the ring
   static unsigned char ready[Q4GPU_MAX_DEVICES];
-  if (s.parts > 8) {  // more CTAs than any cluster may have: once per device
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && !(dev < Q4GPU_MAX_DEVICES && ready[dev]))
-      e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "logprobs: cluster size: %s", cudaGetErrorString(e));
-    if (dev < Q4GPU_MAX_DEVICES) ready[dev] = 1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(dev < Q4GPU_MAX_DEVICES && ready[dev])) {  // once per device
+    e = cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kPerThread * kMostThreads);
+    if (e == cudaSuccess && dev < Q4GPU_MAX_DEVICES) ready[dev] = 1;
   }
+  if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "logprobs: attributes: %s", cudaGetErrorString(e));
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = s.parts, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.rows * s.parts)), cfg.blockDim = dim3(s.threads);
+  cfg.dynamicSmemBytes = (size_t)kPerThread * s.threads;
   cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = s.parts > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, s.parts);
+  e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, s.parts);
   if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "logprobs: launch: %s", cudaGetErrorString(e));
   return q4gpu_check_launch();
 }
