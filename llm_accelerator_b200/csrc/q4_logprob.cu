@@ -463,15 +463,17 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     __syncthreads();
     const uint32_t bound_value = (uint32_t)(bound >> 32);
     constexpr int kTogether = 8 / P;  // units on their way at a time
-    for (int i = warp; i < s_threads; i += warps)
-      for (int u = u0 + s_thread[i] + lane * threads; u < u1; u += kTogether * 32 * threads) {
+    // a thread's units by as many lanes, up to a warp
+    const int peer_lanes = steps > 16 ? 32 : steps > 8 ? 16 : steps > 4 ? 8 : steps > 2 ? 4 : 2, across = 32 / peer_lanes;
+    for (int i = warp * across + lane / peer_lanes; i < s_threads; i += warps * across)
+      for (int u = u0 + s_thread[i] + lane % peer_lanes * threads; u < u1; u += kTogether * peer_lanes * threads) {
         Unit<T> w[kTogether];
 #pragma unroll
         for (int j = 0; j < kTogether; ++j)
-          if (u + j * 32 * threads < u1) w[j].load(body + (int64_t)(u + j * 32 * threads) * P);
+          if (u + j * peer_lanes * threads < u1) w[j].load(body + (int64_t)(u + j * peer_lanes * threads) * P);
 #pragma unroll
         for (int j = 0; j < kTogether; ++j) {
-          const int at = u + j * 32 * threads;
+          const int at = u + j * peer_lanes * threads;
           if (at >= u1) break;
           float v[kUnit];
           w[j].get(v);
