@@ -20,9 +20,6 @@ inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uint
 // ---------------------------------------------------------------------------
 // few query rows (decode): at most 16 (token, head) pairs share a key head
 // ---------------------------------------------------------------------------
-constexpr int kRows = 16;        // rows of one mma.sync tile
-constexpr int kTileKeys = 16;    // keys of a warp's step; a page holds whole steps
-constexpr int kRowWarps = 8;
 constexpr int kRowStages = 3;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -66,69 +63,7 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
 // longest sequence does not decide; a stretch's ends cut at most two (sequence,
 // head) items, whose pieces are joined by the CTA that finishes last, in the
 // order of the pieces.
-constexpr int kUnitKeys = kRowWarps * kTileKeys;
-constexpr int kPieceCost = 3;
-constexpr int kMostCtas = 1024;   // counters, always at the workspace's start: no other call's data gets there
-constexpr int kLeastStretch = 6;  // units: shorter pieces cost more to join than they save
-
-struct RowPlan {
-  int ctas;
-  float* o;       // [cta][2][kRows][D] unnormalised sums: of a piece begun earlier, of one that goes on
-  float2* ml;     // [cta][2][kRows] their running maximum (log2 units) and sum
-  int32_t* done;  // [cta] finished pieces of the item whose first piece goes on from this CTA
-};
-
-// Keys that the kernel below walks for item s, from `lo` on; -1: not its
-// item (no queries, or more rows than a tile).  With sinks the walk starts
-// at key 0 and leaves out `gap.skip` keys from key gap.from on.
-template <int MODE>
-__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const More& x, const Item& s, int group, int& lo,
-                                        Gap& gap) {
-  lo = 0;
-  gap = Gap{0, 0};
-  if (s.n == 0 || s.n > kRows / group) return -1;
-  if (a.window > 0) lo = first_seen(s.len - s.n, a.window) & ~(kTileKeys - 1);
-  if constexpr (MODE == kSinks) {
-    gap = gap_before(lo, x.sinks, kTileKeys);
-    lo = 0;
-  } else if constexpr (MODE == kShared) {
-    lo = s.lo & ~(kTileKeys - 1);
-  }
-  return max(0, s.len - gap.skip - lo);
-}
-template <int MODE>
-__device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, const More& x, int i, int group) {  // of one head
-  int lo;
-  Gap gap;
-  const int keys = row_keys<MODE>(a, x, item_of<MODE>(a, x, i), group, lo, gap);
-  return keys < 0 ? 0 : kPieceCost + (keys + kUnitKeys - 1) / kUnitKeys;
-}
-
-// With kShared: whether cu_q and cu_group ascend at item i, within what they index.
-__device__ __forceinline__ bool ascends(const q4gpu_attn_args& a, const More& x, int i) {
-  const bool group = i >= a.n_seqs;
-  const int32_t* cu = group ? x.cu_group + (i - a.n_seqs) : a.cu_q + i;
-  return cu[0] >= 0 && cu[1] >= cu[0] && cu[1] <= (group ? a.n_seqs : a.tokens);
-}
-// Whether what only the device sees of item i is in range.
-template <int MODE>
-__device__ __forceinline__ bool item_ok(const q4gpu_attn_args& a, const More& x, int i) {
-  if (i < a.n_seqs) {
-    if (!sequence_ok(a, i)) return false;
-    if constexpr (MODE == kShared) {
-      const int n = a.cu_q[i + 1] - a.cu_q[i], g = group_of(x, i);
-      if (n > 0 && g >= 0 && x.prefix_lens[g] > 0 && x.prefix_lens[g] > a.lens[a.seq_ids ? a.seq_ids[i] : i] - n)
-        return false;
-    }
-    return true;
-  }
-  const int g = i - a.n_seqs, c = x.cu_group[g];
-  if (!ascends(a, x, i) || x.prefix_lens[g] < 0) return false;
-  if (c == x.cu_group[g + 1] || x.prefix_lens[g] == 0) return true;
-  const int s = a.seq_ids ? a.seq_ids[c] : c;  // whose pages hold the shared keys
-  return s >= 0 && s < a.n_slots && x.prefix_lens[g] <= keys_of(a, s);
-}
-
+constexpr int kCounters = 4096;  // always at the workspace's start: no other call's data gets there
 // Each warp runs over its own 16-key steps of a piece with its own running
 // maximum and sum, so no barrier stands in the loop; the eight are joined at its
 // end.  (Eight warps and one CTA per SM for heads of 128, two for 64; four warps
@@ -137,15 +72,24 @@ __device__ __forceinline__ bool item_ok(const q4gpu_attn_args& a, const More& x,
 // against 94 for 16 of 64-value heads.)  Bound by memory: every key and value is
 // read once, for all heads of its group; 16 decodes at 16384 keys stream 6.1 TB/s.
 template <typename T, int D, int MODE>
-__global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_args a, More x, RowPlan plan) {
-  constexpr int kThreads = kRowWarps * 32;
+__global__ void __launch_bounds__(kRowWarps * 32, D == 64 ? 2 : 1)
+    attn_rows_kernel(q4gpu_attn_args a, More x, RowPlan plan) {
+  constexpr int W = kRowWarps, kThreads = W * 32;
+  const int heads = MODE == kPlain ? 1 : 1 << plan.heads_log;  // of a piece; each has `slices` of the warps
+  const int slices = MODE == kPlain ? W : W >> plan.heads_log, unit_keys = slices * kTileKeys;
+  const int blocks = MODE == kPlain ? a.kv_heads : a.kv_heads >> plan.heads_log;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ float s_m[kRowWarps][kRows], s_l[kRowWarps][kRows];
-  __shared__ int64_t s_sum[kRowWarps], s_start;
-  __shared__ int s_most[kRowWarps], s_seq, s_last;
+  __shared__ float s_m[W][kRows], s_l[W][kRows];
+  __shared__ int64_t s_sum[W], s_start;
+  __shared__ int s_most[W], s_seq, s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.q_heads / a.kv_heads;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the chunk kernel reads nothing of this one
+  __shared__ __align__(16) unsigned char s_staged[MODE != kPlain ? sizeof(Staged) : 16];
+  __shared__ Item s_item[MODE != kPlain ? 2 * kStaged : 1];
+  const bool known = few<MODE>(a, x);
+  const Where where = where_of<MODE>(a, x, reinterpret_cast<Staged*>(s_staged));
+  if constexpr (MODE != kPlain) __syncthreads();
   // the axis: each thread adds up a run of sequences
   const int items = item_count<MODE>(a, x), per = (items + kThreads - 1) / kThreads;
   const int run0 = min(items, (int)threadIdx.x * per), run1 = min(items, run0 + per);
@@ -157,15 +101,19 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   const bool alone = MODE != kShared && (int64_t)a.max_q * group <= kRows;
   bool over = false;
   for (int i = run0; i < run1; ++i) {
-    over |= alone && item_of<MODE>(a, x, i).n > kRows / group;
-    if (blockIdx.x == 0) {
-      if (MODE == kShared && !ascends(a, x, i)) malformed = true;
-      if (a.err_flag && !item_ok<MODE>(a, x, i)) *a.err_flag = 1;
+    const Item s = item_of<MODE>(a, x, where, i);
+    if (MODE != kPlain && known) s_item[i] = s;
+    over |= alone && s.n > kRows / group;
+    if constexpr (MODE == kShared) {  // (which the joining kernel reports)
+      if (blockIdx.x == 0 && !few<MODE>(a, x)) malformed |= !ascends(a, where, i);
+    } else if constexpr (MODE == kPlain) {
+      if (blockIdx.x == 0 && a.err_flag && !sequence_ok(a, i)) *a.err_flag = 1;
     }
-    const int c = row_cost<MODE>(a, x, i, group);
-    mine_cost += (int64_t)c * a.kv_heads;
+    const int c = row_cost<MODE>(a, x, plan, s, group);
+    mine_cost += (int64_t)c * blocks * row_tiles<MODE>(s, group);
     most = max(most, c);
   }
+  auto item = [&](int i) { return MODE != kPlain && known ? s_item[i] : item_of<MODE>(a, x, where, i); };
   int64_t upto = mine_cost;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -177,95 +125,111 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
   if (lane == 0) s_most[warp] = most;
   if constexpr (MODE == kShared) {
     malformed = __syncthreads_or(malformed);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *x.malformed = malformed;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !few<MODE>(a, x)) *x.malformed = malformed;
   } else {
     over = __syncthreads_or(over);
   }
   int64_t total = 0, before = upto - mine_cost;
 #pragma unroll
-  for (int w = 0; w < kRowWarps; ++w) {
+  for (int w = 0; w < W; ++w) {
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
     most = max(most, s_most[w]);
   }
-  // (32-bit divisions where the numbers allow them)
-  auto quotient = [](int64_t x, int64_t y) {
-    return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
-  };
-  const int64_t stretch = max(quotient(total + plan.ctas - 1, plan.ctas), (int64_t)min(most, kLeastStretch));
+  const int64_t stretch = stretch_of(plan, total, most);
   const int64_t first_unit = blockIdx.x * stretch, last_unit = min(total, first_unit + stretch);
   if (first_unit < last_unit) {
     if (before <= first_unit && first_unit < before + mine_cost) {  // one thread's run holds it
       int i = run0;
-      for (int64_t c; before + (c = (int64_t)row_cost<MODE>(a, x, i, group) * a.kv_heads) <= first_unit; ++i) before += c;
+      for (;; ++i) {
+        const Item s = item(i);
+        const int64_t c = (int64_t)row_cost<MODE>(a, x, plan, s, group) * blocks * row_tiles<MODE>(s, group);
+        if (before + c > first_unit) break;
+        before += c;
+      }
       s_seq = i, s_start = before;
     }
     __syncthreads();
     int seq = s_seq, lo;
     Gap gap;
     int64_t start = s_start;  // where the sequence's first head begins
-    Item s = item_of<MODE>(a, x, seq);
-    int keys = row_keys<MODE>(a, x, s, group, lo, gap), cost = row_cost<MODE>(a, x, seq, group), kvh = (int)quotient(first_unit - start, cost);
+    Item s = item(seq);
+    const int piece_cost = MODE == kPlain ? kPieceCost : plan.piece_cost;
+    row_keys<MODE>(a, x, s, group, lo, gap);
+    int cost = row_cost<MODE>(a, x, plan, s, group), tiles = row_tiles<MODE>(s, group);
+    int sub = (int)quotient(first_unit - start, cost);  // block of heads, tile of rows
     for (;;) {
-      const int64_t head_start = start + (int64_t)kvh * cost + kPieceCost;  // of its first real unit
-      if (head_start - kPieceCost >= last_unit) break;
-      const int units = cost - kPieceCost;
+      const int64_t head_start = start + (int64_t)sub * cost + piece_cost;  // of its first real unit
+      if (head_start - piece_cost >= last_unit) break;
+      const int units = MODE != kPlain && s.len - gap.skip - lo <= 0 ? 0 : cost - piece_cost;
       const int u0 = (int)max((int64_t)0, first_unit - head_start);
       const int u1 = (int)min((int64_t)units, last_unit - head_start);
       // (a sequence without keys: its zeros are written by the CTA where its cost begins)
-      if (u1 > u0 || (units == 0 && head_start - kPieceCost >= first_unit)) {
-        const int rows = s.n * group;
+      if (u1 > u0 || (units == 0 && head_start - piece_cost >= first_unit)) {
+        const int tile = MODE == kShared ? sub % tiles : 0;
+        const int kvh = (MODE == kShared ? sub / tiles : sub) * heads;  // the first of the piece's heads
+        const int row0 = tile * kRows, rows = MODE == kShared ? min(kRows, s.n * group - row0) : s.n * group;
+        const int my_kvh = kvh + (MODE == kPlain ? 0 : warp % heads), slice = MODE == kPlain ? warp : warp / heads;
         const int64_t cta0 = quotient(head_start, stretch),
                       cta1 = units == 0 ? cta0 : quotient(head_start + units - 1, stretch);
         const int parts = (int)(cta1 - cta0) + 1, part = (int)(blockIdx.x - cta0);
-        const int pos0 = MODE == kShared && s.flat ? s.len - 1 : s.len - s.n, pos1 = s.len - 1;  // first, last query
+        // of the first and the last query
+        const int pos0 = MODE != kShared ? s.len - s.n : s.flat ? s.len - 1 : s.len - s.n + row0 / group, pos1 = s.len - 1;
         // along the walk; key_at gives the key
-        const int begin = lo + u0 * kUnitKeys, end = min(s.len - gap.skip, lo + u1 * kUnitKeys);
+        const int begin = lo + u0 * unit_keys, end = min(s.len - gap.skip, lo + u1 * unit_keys);
         auto key_at = [&](int walk) { return MODE == kSinks && walk >= gap.from ? walk + gap.skip : walk; };
         auto unseen = [&](int j, int p) {
           if (MODE == kShared && j < s.lo) return true;
           return j > p || (a.window > 0 && j <= p - a.window && (MODE != kSinks || j >= x.sinks));
         };
 
-        // the queries as A fragments: row g and g + 8, 16 values of a head per step
         const int g = lane >> 2, tq = lane & 3;
         uint32_t qf[D / 16][4];
         int row_pos[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = g + 8 * h, t = r / group;
-          row_pos[h] = r >= rows ? -1 : MODE == kShared && s.flat ? pos0 : pos0 + t;
-          const T* qp = static_cast<const T*>(a.q) + (int64_t)(s.first + t) * a.q_token_stride +
-                        (int64_t)(kvh * group + r - t * group) * a.q_head_stride + 2 * tq;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            qf[k][h] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k) : 0u;
-            qf[k][h + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * k + 8) : 0u;
-          }
+          const int r = g + 8 * h, t = (row0 + r) / group;
+          row_pos[h] = r >= rows ? -1 : MODE == kShared && s.flat ? pos0 : s.len - s.n + t;
         }
 
         const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kRowStages * 2 * kTileKeys * D * 2);
         constexpr int kTileBytes = kTileKeys * D * 2;
         const int32_t* table = a.table + (int64_t)max(0, min(s.slot, a.n_slots - 1)) * a.table_stride;
         const int steps = units > 0 ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
-        const int mine = steps > warp ? (steps - warp + kRowWarps - 1) / kRowWarps : 0;
+        const int mine = steps > slice ? (steps - slice + slices - 1) / slices : 0;
         const int shift = 31 - __clz(a.page_tokens);
         auto page_of = [&](int i) {
           if (i >= mine) return -1;
-          const int p = table[key_at(begin + kTileKeys * (warp + kRowWarps * i)) >> shift];
+          const int p = table[key_at(begin + kTileKeys * (slice + slices * i)) >> shift];
           if (p >= 0 && p < a.n_pages) return p;
           if (a.err_flag) *a.err_flag = 1;
           return -1;
         };
         int next_page = page_of(0);
+        // the queries of the warp's head come through the last stage, which the keys need last
+        const uint32_t q_at = ring + (kRowStages - 1) * 2 * kTileBytes;
+        {
+          constexpr int kPieces = D / 8, kPer = 32 / kPieces;
+          const int c = lane % kPieces;
+#pragma unroll
+          for (int r0 = 0; r0 < kRows; r0 += kPer) {
+            const int r = r0 + lane / kPieces, t = (row0 + r) / group;
+            const bool there = r < rows;
+            const int64_t at = there ? (int64_t)(s.first + t) * a.q_token_stride +
+                                           (int64_t)(my_kvh * group + row0 + r - t * group) * a.q_head_stride + c * 8
+                                     : 0;
+            cp16(q_at + piece<D>(r, c), static_cast<const T*>(a.q) + at, there);
+          }
+          cp_commit();
+        }
         uint32_t valid = 0;  // bit i % 32: step i's page exists
         auto load = [&](int i) {
           const int page = next_page;
           next_page = page_of(i + 1);
           if (i < mine) valid = (valid & ~(1u << (i & 31))) | ((page >= 0 ? 1u : 0u) << (i & 31));
           if (i < mine && page >= 0) {
-            const int walk = begin + kTileKeys * (warp + kRowWarps * i), key = key_at(walk);
-            const int64_t off = page * a.page_stride + kvh * a.head_stride + (key & (a.page_tokens - 1)) * a.row_stride;
+            const int walk = begin + kTileKeys * (slice + slices * i), key = key_at(walk);
+            const int64_t off = page * a.page_stride + my_kvh * a.head_stride + (key & (a.page_tokens - 1)) * a.row_stride;
             const uint32_t at = ring + (i % kRowStages) * 2 * kTileBytes;
             constexpr int kPieces = D / 8, kPer = 32 / kPieces;  // lanes per row, rows per pass
             const int c = lane % kPieces;
@@ -284,6 +248,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
 #pragma unroll
         for (int i = 0; i < kRowStages - 1; ++i) load(i);
 
+        cp_wait<kRowStages - 1>();
+        __syncwarp();
+        // as A fragments: rows g and g + 8, 16 values of a head per step
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) ldsm4(qf[k], q_at + piece<D>(lane & 15, 2 * k + (lane >> 4)));
+        __syncwarp();
+
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -294,7 +265,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           load(i + kRowStages - 1);
           if (!((valid >> (i & 31)) & 1u)) continue;
           const uint32_t kt = ring + (i % kRowStages) * 2 * kTileBytes, vt = kt + kTileBytes;
-          const int key = key_at(begin + kTileKeys * (warp + kRowWarps * i));
+          const int key = key_at(begin + kTileKeys * (slice + slices * i));
           float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -383,6 +354,83 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
         for (int h = 0; h < 2; ++h) {
           l[h] += __shfl_xor_sync(~0u, l[h], 1);
           l[h] += __shfl_xor_sync(~0u, l[h], 2);
+        }
+        const bool joined_here = !(MODE == kShared && known);  // else the joining kernel finds the pieces itself
+        if (MODE != kPlain && slices == 1) {
+          // The warp has its head to itself: no barrier stands in the walk from piece to piece, and while one waits for
+          // its first keys the others compute.
+          const int hw = warp;
+          __syncwarp();  // every lane is done with the ring
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = g + 8 * h, t = (row0 + r) / group, head = my_kvh * group + row0 + r - t * group;
+            if (r >= rows) continue;
+            const int64_t row = (int64_t)(s.first + t) * a.q_heads + head;
+            if (parts > 1 || MODE == kShared) {
+              const int64_t at = parts > 1 ? ((2 * (int64_t)blockIdx.x + (part == 0)) * heads + hw) * kRows + r
+                                           : (int64_t)(s.flat ? x.own_parts : 0) * a.tokens * a.q_heads + row;
+              float* to = (parts > 1 ? plan.o : x.o) + at * D + 2 * tq;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(to + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+              if (tq == 0) (parts > 1 ? plan.ml : x.ml)[at] = make_float2(l[h] == 0.f ? -INFINITY : m[h], l[h]);
+            } else {
+              T* to = static_cast<T*>(a.out) + (int64_t)(s.first + t) * a.out_token_stride +
+                      (int64_t)head * a.out_head_stride + 2 * tq;
+              const bool none = l[h] == 0.f;
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<uint32_t*>(to + 8 * n) =
+                    pack2<T>(none ? 0.f : o[n][2 * h] / l[h], none ? 0.f : o[n][2 * h + 1] / l[h]);
+              if (a.lse && tq == 0) a.lse[row] = none ? -INFINITY : (m[h] + log2f(l[h])) * kLn2;
+            }
+          }
+          if (parts > 1 && joined_here) {
+            __threadfence();
+            __syncwarp();
+            int last = 0;
+            if (lane == 0) {
+              int32_t* const done = plan.done + cta0 * heads + hw;
+              last = atomicAdd(done, 1) == parts - 1;
+              if (last) *done = 0;
+            }
+            if (__shfl_sync(~0u, last, 0)) {
+              __threadfence();
+              for (int i = lane; i < rows * (D / 4); i += 32) {
+                const int r = i / (D / 4), d = (i - r * (D / 4)) * 4, t = (row0 + r) / group;
+                const int head = my_kvh * group + row0 + r - t * group;
+                auto slot = [&](int k) { return ((2 * (cta0 + k) + (k == 0)) * heads + hw) * kRows + r; };
+                float top = -INFINITY, sum = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+                for (int k = 0; k < parts; ++k) {
+                  const float2 w = __ldcg(&plan.ml[slot(k)]);
+                  const float f = ex2(w.x - base);
+                  const float4 p = __ldcg(reinterpret_cast<const float4*>(plan.o + slot(k) * D + d));
+                  sum = fmaf(w.y, f, sum);
+                  v.x = fmaf(p.x, f, v.x), v.y = fmaf(p.y, f, v.y), v.z = fmaf(p.z, f, v.z), v.w = fmaf(p.w, f, v.w);
+                }
+                if constexpr (MODE == kShared) {
+                  const int64_t at = ((int64_t)(s.flat ? x.own_parts : 0) * a.tokens + s.first + t) * a.q_heads + head;
+                  *reinterpret_cast<float4*>(x.o + at * D + d) = v;
+                  if (d == 0) x.ml[at] = make_float2(sum == 0.f ? -INFINITY : base, sum);
+                  continue;
+                }
+                const bool none = sum == 0.f;
+                *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.first + t) * a.out_token_stride +
+                                          (int64_t)head * a.out_head_stride + d) =
+                    make_uint2(pack2<T>(none ? 0.f : v.x / sum, none ? 0.f : v.y / sum),
+                               pack2<T>(none ? 0.f : v.z / sum, none ? 0.f : v.w / sum));
+                if (a.lse && d == 0)
+                  a.lse[(int64_t)(s.first + t) * a.q_heads + head] = none ? -INFINITY : (base + log2f(sum)) * kLn2;
+              }
+            }
+          }
+        } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           if (tq == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
         }
         __syncthreads();  // every warp is done with its ring
@@ -396,40 +444,50 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
               *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
                   make_float2(o[n][2 * h], o[n][2 * h + 1]);
         __syncthreads();
-        auto put = [&](int r, int d, float m_all, float l_all, float v) {
-          const int t = r / group, head = kvh * group + r - t * group;
+        // four neighbouring values a thread
+        auto put = [&](int hw, int r, int d, float m_all, float l_all, const float4& v) {
+          const int t = (row0 + r) / group, head = (kvh + hw) * group + row0 + r - t * group;
           if constexpr (MODE == kShared) {
             const int64_t at = ((int64_t)(s.flat ? x.own_parts : 0) * a.tokens + s.first + t) * a.q_heads + head;
-            x.o[at * D + d] = v;
+            *reinterpret_cast<float4*>(x.o + at * D + d) = v;
             if (d == 0) x.ml[at] = make_float2(l_all == 0.f ? -INFINITY : m_all, l_all);
             return;
           }
-          static_cast<T*>(a.out)[(int64_t)(s.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride + d] =
-              from_f32<T>(l_all == 0.f ? 0.f : v / l_all);
+          const bool none = l_all == 0.f;
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.first + t) * a.out_token_stride +
+                                    (int64_t)head * a.out_head_stride + d) =
+              make_uint2(pack2<T>(none ? 0.f : v.x / l_all, none ? 0.f : v.y / l_all),
+                         pack2<T>(none ? 0.f : v.z / l_all, none ? 0.f : v.w / l_all));
           if (a.lse && d == 0)
-            a.lse[(int64_t)(s.first + t) * a.q_heads + head] = l_all == 0.f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+            a.lse[(int64_t)(s.first + t) * a.q_heads + head] = none ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
         };
-        for (int i = threadIdx.x; i < rows * D; i += kRowWarps * 32) {
-          const int r = i / D, d = i - r * D;
-          float top = -INFINITY, sum = 0.f, v = 0.f;
+        auto add = [](float4& v, const float4& w, float f) {
+          v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
+        };
+        for (int i = threadIdx.x; i < heads * rows * (D / 4); i += W * 32) {
+          const int hr = i / (D / 4), d = (i - hr * (D / 4)) * 4, hw = MODE == kPlain ? 0 : hr / rows, r = hr - hw * rows;
+          float top = -INFINITY, sum = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, s_m[w][r]);
+          for (int w = 0; w < W; ++w)
+            if (MODE == kPlain || w % heads == hw) top = fmaxf(top, s_m[w][r]);
           const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-          for (int w = 0; w < kRowWarps; ++w) {
+          for (int w = 0; w < W; ++w) {
+            if (MODE != kPlain && w % heads != hw) continue;
             const float f = ex2(s_m[w][r] - base);
             sum = fmaf(s_l[w][r], f, sum);
-            v = fmaf(so[(w * kRows + r) * D + d], f, v);
+            add(v, *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + d), f);
           }
           if (parts == 1) {
-            put(r, d, base, sum, v);
+            put(hw, r, d, base, sum, v);
           } else {
-            const int64_t at = (2 * (int64_t)blockIdx.x + (part == 0)) * kRows + r;
-            plan.o[at * D + d] = v;
+            const int64_t at = ((2 * (int64_t)blockIdx.x + (part == 0)) * heads + hw) * kRows + r;
+            *reinterpret_cast<float4*>(plan.o + at * D + d) = v;
             if (d == 0) plan.ml[at] = make_float2(top, sum);
           }
         }
-        if (parts > 1) {
+        if (parts > 1 && joined_here) {
           __threadfence();
           __syncthreads();
           if (threadIdx.x == 0) {
@@ -439,11 +497,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
           __syncthreads();
           if (s_last) __threadfence();
         }
-        if (parts > 1 && s_last)
-          for (int i = threadIdx.x; i < rows * D; i += kRowWarps * 32) {
-            const int r = i / D, d = i - r * D;
-            auto slot = [&](int k) { return (2 * (cta0 + k) + (k == 0)) * kRows + r; };
-            float top = -INFINITY, sum = 0.f, v = 0.f;
+        if (parts > 1 && joined_here && s_last)
+          for (int i = threadIdx.x; i < heads * rows * (D / 4); i += W * 32) {
+            const int hr = i / (D / 4), d = (i - hr * (D / 4)) * 4, hw = MODE == kPlain ? 0 : hr / rows, r = hr - hw * rows;
+            auto slot = [&](int k) { return ((2 * (cta0 + k) + (k == 0)) * heads + hw) * kRows + r; };
+            float top = -INFINITY, sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
             for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
             const float base = top == -INFINITY ? 0.f : top;
@@ -452,28 +511,32 @@ __global__ void __launch_bounds__(kRowWarps * 32) attn_rows_kernel(q4gpu_attn_ar
               const float2 w = __ldcg(&plan.ml[slot(k)]);
               const float f = ex2(w.x - base);
               sum = fmaf(w.y, f, sum);
-              v = fmaf(__ldcg(&plan.o[slot(k) * D + d]), f, v);
+              add(v, __ldcg(reinterpret_cast<const float4*>(plan.o + slot(k) * D + d)), f);
             }
-            put(r, d, base, sum, v);
+            put(hw, r, d, base, sum, v);
           }
         __syncthreads();  // the ring and the shared words are free for the next piece
+        }
       }
-      if (++kvh == a.kv_heads) {
-        kvh = 0;
-        start += (int64_t)cost * a.kv_heads;
+      if (++sub == blocks * tiles) {
+        sub = 0;
+        start += (int64_t)cost * blocks * tiles;
         do {
           if (++seq >= items) break;
-          s = item_of<MODE>(a, x, seq);
-          keys = row_keys<MODE>(a, x, s, group, lo, gap);
-          cost = row_cost<MODE>(a, x, seq, group);
+          s = item(seq);
+          row_keys<MODE>(a, x, s, group, lo, gap);
+          cost = row_cost<MODE>(a, x, plan, s, group), tiles = row_tiles<MODE>(s, group);
         } while (cost == 0);
         if (seq >= items) break;
       }
     }
   }
+  if (MODE == kSinks && blockIdx.x == 0 && a.err_flag)
+    for (int i = threadIdx.x; i < a.n_seqs; i += kThreads)
+      if (!sequence_ok(a, i)) *a.err_flag = 1;
   if (over)
     for (int i = blockIdx.x; i < a.n_seqs; i += gridDim.x) {
-      const Item s = item_of<MODE>(a, x, i);
+      const Item s = item_of<MODE>(a, x, where, i);
       if (s.n <= kRows / group) continue;
       for (int64_t e = threadIdx.x; e < (int64_t)s.n * a.q_heads * D; e += kThreads) {
         const int64_t row = e / D, t = s.first + row / a.q_heads, head = row % a.q_heads;
@@ -528,22 +591,6 @@ q4gpu_attn_args settled(const q4gpu_attn_args& a) {
   return b;
 }
 
-RowPlan row_plan(const q4gpu_attn_args& a, const More& x, char* ws, size_t* bytes) {
-  RowPlan p{};
-  const size_t items = (size_t)(a.n_seqs + x.n_groups) * a.kv_heads;
-  // no CTA without at least one (sequence, head) or kLeastStretch units of one
-  const int64_t units = ((int64_t)a.max_ctx + kUnitKeys - 1) / kUnitKeys + kPieceCost;
-  const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + kLeastStretch - 1) / kLeastStretch + 1);
-  p.ctas = (int)std::min<int64_t>(most, kSms * (a.dim == 64 ? 2 : 1));
-  static_assert(kSms * 4 <= kMostCtas, "a counter a CTA");
-  const size_t done = kMostCtas * sizeof(int32_t), rows = (size_t)p.ctas * 2 * kRows;
-  if (bytes) *bytes = done + rows * (8 + (size_t)a.dim * 4);
-  p.done = reinterpret_cast<int32_t*>(ws);
-  p.ml = reinterpret_cast<float2*>(ws + done);
-  p.o = reinterpret_cast<float*>(p.ml + rows);
-  return p;
-}
-
 // Parts of a chunk's keys: one where the (row pair, key head) items fill the
 // GPU, else as many as fill it once, each of at least kMinPart keys.  (Cutting
 // the last wave of many items in two evens the SMs out, 348 steps on the longest
@@ -555,14 +602,20 @@ ChunkPlan chunk_plan(const q4gpu_attn_args& a, const More& x, size_t* bytes) {
   const int64_t group = a.q_heads / a.kv_heads, rows = a.tokens * group;
   if constexpr (MODE == kShared) {
     // a group's queries count together: tiles for its shared keys, and for own keys of long chunks
-    p.least = (int)(kRows / group) + 1, p.parts = 1;
+    p.least = (int)(kMostTiles * kRows / group) + 1, p.parts = 1;
     const int64_t most = a.tokens / p.least;  // items of so many queries
     int64_t tiles = 0;
-    if (rows > kRows) tiles = rows / kPair + std::min<int64_t>(x.n_groups, most);
-    if (a.max_q * group > kRows) tiles += rows / kPair + std::min<int64_t>(a.n_seqs, most);
+    if (rows > kMostTiles * kRows) tiles = rows / kPair + std::min<int64_t>(x.n_groups, most);
+    if (a.max_q * group > kMostTiles * kRows) tiles += rows / kPair + std::min<int64_t>(a.n_seqs, most);
     p.tiles = (int)std::min<int64_t>(tiles, INT32_MAX);
+    // The shared keys get SMs of their own, beside attn_rows_kernel's: half of them, or more where they are most of the
+    // keys.  (64 sequences, 8192 shared keys and up to 512 own ones: 29.6 us with half, 33.1 with 65 %, 36 with 35 %, 49.8
+    // after one another; 2 groups of 32 x 4 tokens, 4096 and 100 keys: 66.6 with 72 %, 95 with half.)
+    const double shared = (double)tiles * std::min(x.max_prefix, a.max_ctx);
+    const double own = (double)a.n_seqs * std::max(1, a.max_ctx - x.max_prefix);
+    const int sms = (int)(kSms * std::min(0.8, std::max(0.5, shared / (shared + own))));
     if (tiles)
-      p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / (tiles * a.kv_heads), a.max_ctx / kMinPart));
+      p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(sms / (tiles * a.kv_heads), a.max_ctx / kMinPart));
     return p;
   }
   if (a.max_q * group <= kRows || a.n_seqs == 0 || a.tokens == 0) {  // nothing for the chunk kernel
@@ -577,6 +630,51 @@ ChunkPlan chunk_plan(const q4gpu_attn_args& a, const More& x, size_t* bytes) {
       a.window > 0 ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + kPair + kNTile + x.sinks) : a.max_ctx;
   p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / items, span / kMinPart));
   if (bytes) *bytes = p.parts > 1 ? (size_t)p.tiles * a.kv_heads * p.parts * kPair * (8 + (size_t)a.dim * 4) : 0;
+  return p;
+}
+
+template <int MODE>
+RowPlan row_plan(const q4gpu_attn_args& a, const More& x, char* ws, size_t* bytes) {
+  RowPlan p{};
+  const int64_t seqs = a.n_seqs + x.n_groups;
+  p.least_stretch = 6, p.piece_cost = kPieceCost;
+  if constexpr (MODE != kPlain) {
+    // Several key heads a piece, a warp or a few each, where there are sequences enough: pieces are fewer (64 decodes
+    // through a window of 2048 over 1 to 8704 keys: 46 us with one, 38.5 with two, 41 with eight, whose pieces are
+    // cut and joined more often; 64 sequences of 1 to 512 own keys beside 8192 shared ones, which another kernel
+    // joins: 40.8 with two, 32.2 with eight).
+    const int most = MODE == kSinks ? 160 : 32;
+    while (2 << p.heads_log <= kRowWarps && a.kv_heads % (2 << p.heads_log) == 0 &&
+           seqs * (a.kv_heads >> (p.heads_log + 1)) >= most)
+      ++p.heads_log;
+    // Where a unit a CTA is all there is, that is how it is cut (one token of 1028 seen keys: 12.0 us, 16.4 in
+    // stretches of 6).
+    const int64_t unit = (kRowWarps * kTileKeys) >> p.heads_log, blocks = a.kv_heads >> p.heads_log;
+    const int64_t shared = MODE == kShared ? std::min(x.max_prefix, a.max_ctx) : 0;
+    const int64_t seen = MODE == kSinks ? std::min<int64_t>(a.max_ctx, (int64_t)a.window + a.max_q + x.sinks + 2 * unit)
+                                        : a.max_ctx - shared;
+    const int64_t all = blocks * (a.n_seqs * ((seen + unit - 1) / unit) + x.n_groups * ((shared + unit - 1) / unit));
+    if (all <= kSms) p.piece_cost = 0, p.least_stretch = 1;
+  }
+  p.unit_log = 31 - __builtin_clz((kRowWarps * kTileKeys) >> p.heads_log);
+  const size_t items = (size_t)seqs * (a.kv_heads >> p.heads_log) * (MODE == kShared ? kMostTiles : 1);
+  // no CTA without at least one item or least_stretch units of one
+  const int unit = (kRowWarps * kTileKeys) >> p.heads_log;
+  const int64_t units = ((int64_t)a.max_ctx + unit - 1) / unit + p.piece_cost;
+  const int64_t most = (int64_t)items * std::max<int64_t>(1, (units + p.least_stretch - 1) / p.least_stretch + 1);  // (of a stretch's two ends)
+  int sms = kSms;
+  if (MODE == kShared && (int64_t)a.tokens * (a.q_heads / a.kv_heads) > (int64_t)kMostTiles * kRows * x.n_groups) {
+    // groups for the chunk kernel, which runs beside this one
+    const ChunkPlan c = chunk_plan<MODE>(a, x, nullptr);
+    sms = (int)std::max<int64_t>(kSms / 4, kSms - (int64_t)c.tiles * a.kv_heads * c.parts);
+  }
+  p.ctas = (int)std::min<int64_t>(most, sms * (a.dim == 64 ? 2 : 1));
+  static_assert(kSms * 2 * kRowWarps <= kCounters, "a counter a CTA and head");
+  const size_t done = kCounters * sizeof(int32_t), rows = ((size_t)p.ctas * 2 * kRows) << p.heads_log;  // (even)
+  if (bytes) *bytes = done + rows * (8 + (size_t)a.dim * 4);
+  p.done = reinterpret_cast<int32_t*>(ws);
+  p.ml = reinterpret_cast<float2*>(ws + done);
+  p.o = reinterpret_cast<float*>(p.ml + rows);
   return p;
 }
 
@@ -620,19 +718,15 @@ int allow_smem(const void* kernel, int bytes, unsigned char* ready) {
 
 template <typename T, int D, int MODE>
 int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
-  static unsigned char ready[2][Q4GPU_MAX_DEVICES];
+  static unsigned char ready[Q4GPU_MAX_DEVICES];
   size_t rows_bytes;
-  const RowPlan few = row_plan(a, x, static_cast<char*>(a.workspace), &rows_bytes);
+  const RowPlan few = row_plan<MODE>(a, x, static_cast<char*>(a.workspace), &rows_bytes);
   ChunkPlan plan = chunk_plan<MODE>(a, x, nullptr);
   const bool chunks = plan.tiles > 0;
   if (plan.tiles > 65535) return q4gpu_fail(Q4GPU_ERR_SHAPE, "attention: too many query rows");
   // sequences for attn_rows_kernel (with kShared it also looks at what only the device sees)
   const bool short_ones = MODE == kShared || !chunks || plan.least > 1;
   int rc = Q4GPU_OK;
-  if (short_ones) {
-    rc = allow_smem(reinterpret_cast<const void*>(attn_rows_kernel<T, D, MODE>), row_smem<D>(), ready[0]);
-    if (rc != Q4GPU_OK) return rc;
-  }
   CUtensorMap kmap, vmap;
   if (chunks) {
     char* ws = static_cast<char*>(a.workspace) + (rows_bytes + 15) / 16 * 16;
@@ -642,10 +736,16 @@ int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
     rc = encode_map(&kmap, a, a.k_cache);
     if (rc == Q4GPU_OK) rc = encode_map(&vmap, a, a.v_cache);
     if (rc == Q4GPU_OK)
-      rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D, MODE>), chunk_smem<D>(), ready[1]);
+      rc = allow_smem(reinterpret_cast<const void*>(attn_chunk_kernel<T, D, MODE>), chunk_smem<D>(), ready);
     if (rc != Q4GPU_OK) return rc;
   }
-  if (short_ones) attn_rows_kernel<T, D, MODE><<<few.ctas, kRowWarps * 32, row_smem<D>(), s>>>(a, x, few);
+  if (short_ones) {
+    static unsigned char ready[Q4GPU_MAX_DEVICES];
+    const auto kernel = attn_rows_kernel<T, D, MODE>;
+    rc = allow_smem(reinterpret_cast<const void*>(kernel), row_smem<D>(), ready);
+    if (rc == Q4GPU_OK) kernel<<<few.ctas, kRowWarps * 32, row_smem<D>(), s>>>(a, x, few);
+    if (rc != Q4GPU_OK) return rc;
+  }
   if (chunks) {
     // starts beside the short sequences' kernel, on the SMs that it leaves free
     cudaLaunchAttribute attr[1];
@@ -664,8 +764,15 @@ int launch(const q4gpu_attn_args& a, const More& x, cudaStream_t s) {
   }
   if constexpr (MODE == kShared) {
     const int64_t rows = (int64_t)a.max_q * a.q_heads;
-    const dim3 grid(a.n_seqs, (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, 64)));
-    attn_shared_join_kernel<T, D><<<grid, 256, 0, s>>>(a, x, plan);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // it waits for the others itself
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.n_seqs, (unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + 7) / 8, 64)));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s, cfg.attrs = attr, cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_shared_join_kernel<T, D>, a, x, plan, few);
+    if (e != cudaSuccess) return q4gpu_fail(Q4GPU_ERR_CUDA, "attention: launch: %s", cudaGetErrorString(e));
   }
   return q4gpu_check_launch();
 }
@@ -689,9 +796,9 @@ struct SharedRoom {
 };
 bool shared_room(const q4gpu_attn_args& a, const More& x, SharedRoom& r, int& own_parts) {
   const ChunkPlan p = chunk_plan<kShared>(a, x, nullptr);
-  own_parts = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kRows ? p.parts : 1;
+  own_parts = (int64_t)a.max_q * (a.q_heads / a.kv_heads) > kMostTiles * kRows ? p.parts : 1;
   size_t rows_bytes;
-  row_plan(a, x, nullptr, &rows_bytes);
+  row_plan<kShared>(a, x, nullptr, &rows_bytes);
   const size_t rows = (size_t)(own_parts + p.parts) * a.tokens * a.q_heads;
   r.ml = (rows_bytes + 15) / 16 * 16;
   r.o = r.ml + (rows * sizeof(float2) + 15) / 16 * 16;
@@ -709,7 +816,7 @@ int check_shared(const q4gpu_attn_args* a, const q4gpu_shared_args* sh) {
 }
 More settled_groups(const q4gpu_shared_args& sh) {
   More x{};
-  x.cu_group = sh.cu_group, x.prefix_lens = sh.prefix_lens, x.n_groups = sh.n_groups;
+  x.cu_group = sh.cu_group, x.prefix_lens = sh.prefix_lens, x.n_groups = sh.n_groups, x.max_prefix = sh.max_prefix;
   return x;
 }
 
@@ -750,7 +857,7 @@ size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args* a, int32_t si
   const q4gpu_attn_args b = settled(*a);
   const More x = settled_sinks(b, sinks);
   size_t rows, chunks;
-  row_plan(b, x, nullptr, &rows);
+  row_plan<kSinks>(b, x, nullptr, &rows);
   chunk_plan<kSinks>(b, x, &chunks);
   return (rows + 15) / 16 * 16 + chunks;
 }

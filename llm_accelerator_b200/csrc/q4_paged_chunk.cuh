@@ -44,7 +44,7 @@ struct More {  // what the modes need besides the arguments they share
   int sinks;   // kSinks: the first keys that every query sees
   // kShared: group g is sequences cu_group[g] .. cu_group[g + 1] - 1, its first prefix_lens[g] keys are shared
   const int32_t *cu_group, *prefix_lens;
-  int n_groups;
+  int n_groups, max_prefix;
   // what a row got from its own keys and from the shared ones: unnormalised sums [set][part][token][q_head][D], with
   // the running maximum (log2 units) and sum; the own set has own_parts parts
   float* o;
@@ -90,48 +90,80 @@ __device__ __forceinline__ int item_count(const q4gpu_attn_args& a, const More& 
 __device__ __forceinline__ int keys_of(const q4gpu_attn_args& a, int slot) {
   return slot >= 0 && slot < a.n_slots ? (int)max((int64_t)0, min((int64_t)a.lens[slot], most_keys(a))) : 0;
 }
-__device__ __forceinline__ int shared_keys(const q4gpu_attn_args& a, const More& x, int g) {
-  return (int)max((int64_t)0, min((int64_t)x.prefix_lens[g], most_keys(a)));
+// The index arrays of a call, in global memory or staged.
+struct Where {
+  const int32_t *cu_q, *slots, *keys;  // keys (staged): of each sequence's slot
+  const int32_t *cu_group, *prefix_lens;
+};
+// A CTA looks at several of them for each item, one after another: with few sequences it first brings them into shared
+// memory, which takes two trips.
+constexpr int kStaged = 128;
+struct Staged {
+  int32_t cu_q[kStaged + 1], slots[kStaged], keys[kStaged], cu_group[kStaged + 1], prefix_lens[kStaged];
+};
+template <int MODE>
+__device__ __forceinline__ bool few(const q4gpu_attn_args& a, const More& x) {
+  return MODE != kPlain && a.n_seqs <= kStaged && x.n_groups <= kStaged;
+}
+// By all threads of a CTA; a barrier has to follow.
+template <int MODE>
+__device__ __forceinline__ Where where_of(const q4gpu_attn_args& a, const More& x, Staged* s) {
+  if (!few<MODE>(a, x)) return Where{a.cu_q, a.seq_ids, nullptr, x.cu_group, x.prefix_lens};
+  for (int i = threadIdx.x; i <= a.n_seqs; i += blockDim.x) {
+    s->cu_q[i] = a.cu_q[i];
+    if (i == a.n_seqs) break;
+    const int slot = a.seq_ids ? a.seq_ids[i] : i;
+    s->slots[i] = slot, s->keys[i] = keys_of(a, slot);
+  }
+  if (x.n_groups > 0)
+    for (int i = threadIdx.x; i <= x.n_groups; i += blockDim.x) {
+      s->cu_group[i] = x.cu_group[i];
+      if (i < x.n_groups) s->prefix_lens[i] = x.prefix_lens[i];
+    }
+  return Where{s->cu_q, s->slots, s->keys, s->cu_group, s->prefix_lens};
+}
+__device__ __forceinline__ int shared_keys(const q4gpu_attn_args& a, const Where& w, int g) {
+  return (int)max((int64_t)0, min((int64_t)w.prefix_lens[g], most_keys(a)));
 }
 // The group of sequence i, or -1: the last that begins at or before it, if it reaches it.
-__device__ __forceinline__ int group_of(const More& x, int i) {
+__device__ __forceinline__ int group_of(const More& x, const Where& w, int i) {
   int g = 0, end = x.n_groups;
   while (g < end) {
     const int mid = (g + end) / 2;
-    if (x.cu_group[mid] <= i)
+    if (w.cu_group[mid] <= i)
       g = mid + 1;
     else
       end = mid;
   }
-  return g > 0 && i < x.cu_group[g] ? g - 1 : -1;
+  return g > 0 && i < w.cu_group[g] ? g - 1 : -1;
 }
 template <int MODE>
-__device__ __forceinline__ Item item_of(const q4gpu_attn_args& a, const More& x, int i) {
+__device__ __forceinline__ Item item_of(const q4gpu_attn_args& a, const More& x, const Where& w, int i) {
   Item s;
   s.lo = 0, s.flat = false;
   int last = i + 1;
   if (MODE == kShared && i >= a.n_seqs) {
     const int g = i - a.n_seqs;
     s.flat = true;
-    i = max(0, min(x.cu_group[g], a.n_seqs)), last = max(i, min(x.cu_group[g + 1], a.n_seqs));
-    s.lo = shared_keys(a, x, g);  // (their end, for now)
+    i = max(0, min(w.cu_group[g], a.n_seqs)), last = max(i, min(w.cu_group[g + 1], a.n_seqs));
+    s.lo = shared_keys(a, w, g);  // (their end, for now)
   }
-  s.first = max(0, min(a.cu_q[i], a.tokens));
-  s.n = max(0, min(a.cu_q[last], a.tokens) - s.first);
+  s.first = max(0, min(w.cu_q[i], a.tokens));
+  s.n = max(0, min(w.cu_q[last], a.tokens) - s.first);
   if (MODE == kShared && i == last) {  // a group without sequences: its first may not be there
     s.slot = -1, s.len = s.lo = s.n = 0;
     return s;
   }
-  s.slot = a.seq_ids ? a.seq_ids[i] : i;
-  s.len = keys_of(a, s.slot);
+  s.slot = w.slots ? w.slots[i] : i;
+  s.len = MODE != kPlain && w.keys ? w.keys[i] : keys_of(a, s.slot);
   if constexpr (MODE == kShared) {
     if (s.flat) {
       s.len = min(s.len, s.lo);
       s.lo = 0;
       if (s.len == 0) s.n = 0;
     } else {
-      const int g = group_of(x, i);
-      s.lo = g < 0 ? 0 : shared_keys(a, x, g);
+      const int g = group_of(x, w, i);
+      s.lo = g < 0 ? 0 : shared_keys(a, w, g);
       // its queries have to stand behind the shared keys (else its rows become zeros)
       if (s.lo > 0 && s.lo > s.len - s.n) s.lo = s.len = 0;
       if (s.n > a.max_q) s.n = 0;  // likewise
@@ -146,11 +178,11 @@ struct ChunkTile : Item {
 };
 // Row pairs of item i (none where it has few rows); keys: about how many one walks.
 template <int MODE>
-__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, const More& x, int i, int group, int least,
-                                        ChunkTile& t, int& keys) {
+__device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, const More& x, const Where& w, int i, int group,
+                                        int least, ChunkTile& t, int& keys) {
   keys = 0;
   if (i >= item_count<MODE>(a, x)) return 0;
-  static_cast<Item&>(t) = item_of<MODE>(a, x, i);
+  static_cast<Item&>(t) = item_of<MODE>(a, x, w, i);
   if (t.n < least) return 0;
   keys = a.window > 0 ? min(t.len, a.window) : t.len - t.lo;  // (of sinks there are few)
   return (int)(((int64_t)t.n * group + kPair - 1) / kPair);
@@ -161,20 +193,23 @@ __device__ __forceinline__ int pairs_of(const q4gpu_attn_args& a, const More& x,
 // keys, the rest), and within a class from its last row pair to its first, as
 // later rows see more keys.
 template <int MODE>
-__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, const More& x, int least, int y) {
+__device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, const More& x, const Where& w, int least,
+                                               int y) {
   const int lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads, items = item_count<MODE>(a, x);
+  // where no sequence has so many queries only groups have
+  const int first = MODE == kShared && a.max_q < least ? a.n_seqs : 0;
   ChunkTile t{}, own{};
   t.seq = -1, t.index = y;
   int most = 0, keys;
-  for (int i = lane; i < items; i += 32) {
-    pairs_of<MODE>(a, x, i, group, least, own, keys);
+  for (int i = first + lane; i < items; i += 32) {
+    pairs_of<MODE>(a, x, w, i, group, least, own, keys);
     most = max(most, keys);
   }
   most = __reduce_max_sync(~0u, most);
   auto rank = [&](int k) { return k >= most / 2 ? 0 : k >= most / 4 ? 1 : k >= most / 8 ? 2 : 3; };
   int count[4] = {0, 0, 0, 0};
-  for (int i = lane; i < items; i += 32) {
-    const int n = pairs_of<MODE>(a, x, i, group, least, own, keys);
+  for (int i = first + lane; i < items; i += 32) {
+    const int n = pairs_of<MODE>(a, x, w, i, group, least, own, keys);
 #pragma unroll
     for (int c = 0; c < 4; ++c) count[c] += rank(keys) == c ? n : 0;
   }
@@ -190,8 +225,8 @@ __device__ __forceinline__ ChunkTile find_tile(const q4gpu_attn_args& a, const M
   }
   if (wanted < 0) return t;
   int before = 0;
-  for (int i0 = 0; i0 < items; i0 += 32) {
-    int mine = pairs_of<MODE>(a, x, i0 + lane, group, least, own, keys);
+  for (int i0 = first; i0 < items; i0 += 32) {
+    int mine = pairs_of<MODE>(a, x, w, i0 + lane, group, least, own, keys);
     if (rank(keys) != wanted) mine = 0;
     int run = mine;
 #pragma unroll
@@ -227,6 +262,65 @@ __device__ __forceinline__ Span span_of(int lo, int hi, const More& more) {
     return Span{0, hi - gap.skip, gap};
   }
   return Span{base, hi, Gap{0, 0}};
+}
+
+// attn_rows_kernel's work lies on one axis: item by item, subitem by subitem, in units of keys (q4_paged_attn.cu).
+constexpr int kRows = 16;      // rows of one mma.sync tile
+constexpr int kTileKeys = 16;  // keys of a warp's step; a page holds whole steps
+constexpr int kRowWarps = 8;   // of a CTA, at most
+constexpr int kPieceCost = 3;
+constexpr int kMostTiles = 4;  // kShared: tiles of 16 rows that an item may have there; more are attn_chunk_kernel's
+struct RowPlan {
+  int ctas, unit_log;  // log2 of the keys of a unit
+  int heads_log;      // log2 of the key heads of a piece, which share the CTA's warps
+  int least_stretch;  // units: shorter pieces cost more to join than they save
+  int piece_cost;     // units
+  float* o;       // [cta][2][head][kRows][D] unnormalised sums: of a piece begun earlier, of one that goes on
+  float2* ml;     // [cta][2][head][kRows] their running maximum (log2 units) and sum
+  int32_t* done;  // [cta] finished pieces of the item whose first piece goes on from this CTA
+};
+
+// Keys that the kernel below walks for item s, from `lo` on; -1: not its
+// item (no queries, or more rows than a tile).  With sinks the walk starts
+// at key 0 and leaves out `gap.skip` keys from key gap.from on.
+template <int MODE>
+__device__ __forceinline__ int row_keys(const q4gpu_attn_args& a, const More& x, const Item& s, int group, int& lo,
+                                        Gap& gap) {
+  lo = 0;
+  gap = Gap{0, 0};
+  if (s.n == 0 || s.n > (MODE == kShared ? kMostTiles : 1) * kRows / group) return -1;
+  if (a.window > 0) lo = first_seen(s.len - s.n, a.window) & ~(kTileKeys - 1);
+  if constexpr (MODE == kSinks) {
+    gap = gap_before(lo, x.sinks, kTileKeys);
+    lo = 0;
+  } else if constexpr (MODE == kShared) {
+    lo = s.lo & ~(kTileKeys - 1);
+  }
+  return max(0, s.len - gap.skip - lo);
+}
+// Cost of one of an item's subitems, which are its tiles of rows for each block of key heads (0: not this kernel's).
+template <int MODE>
+__device__ __forceinline__ int row_cost(const q4gpu_attn_args& a, const More& x, const RowPlan& plan, const Item& s,
+                                        int group) {
+  int lo;
+  Gap gap;
+  const int keys = row_keys<MODE>(a, x, s, group, lo, gap);
+  constexpr int kUnit = kRowWarps * kTileKeys;
+  if constexpr (MODE == kPlain) return keys < 0 ? 0 : kPieceCost + (keys + kUnit - 1) / kUnit;
+  return keys < 0 ? 0 : plan.piece_cost + max(1, (keys + (1 << plan.unit_log) - 1) >> plan.unit_log);
+}
+template <int MODE>
+__device__ __forceinline__ int row_tiles(const Item& s, int group) {
+  return MODE == kShared ? (s.n * group + kRows - 1) / kRows : 1;
+}
+
+// (32-bit divisions where the numbers allow them)
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+// Units of each CTA of an axis of `total`, whose longest subitem has `most`.
+__device__ __forceinline__ int64_t stretch_of(const RowPlan& plan, int64_t total, int most) {
+  return max(quotient(total + plan.ctas - 1, plan.ctas), (int64_t)min(most, plan.least_stretch));
 }
 
 // ---- tensor memory, 32 columns at a time ---------------------------------------
@@ -428,8 +522,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   auto wait_before = [&] {
     if (waits) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
+  if constexpr (MODE == kShared) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const Where where = where_of<MODE>(a, more, reinterpret_cast<Staged*>(smem));  // (where the queries go later)
+  if constexpr (MODE != kPlain) __syncthreads();
   if (warp == 0) {
-    const ChunkTile t = find_tile<MODE>(a, more, plan.least, blockIdx.y);
+    const ChunkTile t = find_tile<MODE>(a, more, where, plan.least, blockIdx.y);
     if (lane == 0) s_tile = t, s_bad = s_odd = s_dead = 0;
   }
   if (waits && warp == 11 && plan.least == 1 && a.err_flag)  // no other kernel in this call looks at the sequences
@@ -853,7 +950,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, More 
   __shared__ ChunkTile s_tile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.x;
   if (warp == 0) {
-    const ChunkTile t = find_tile<MODE>(a, more, plan.least, blockIdx.y);
+    const ChunkTile t =
+        find_tile<MODE>(a, more, where_of<kPlain>(a, more, nullptr), plan.least, blockIdx.y);
     if (lane == 0) s_tile = t;
   }
   __syncthreads();
@@ -891,52 +989,202 @@ __global__ void __launch_bounds__(256) attn_join_kernel(q4gpu_attn_args a, More 
     a.lse[(int64_t)(first + t) * a.q_heads + head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Joins what each row got from its own keys and from the shared ones, part by part in order: one warp a row.  Rows of a
+// Whether cu_q (i < n_seqs) or cu_group ascends at item i, within what it indexes.
+__device__ __forceinline__ bool ascends(const q4gpu_attn_args& a, const Where& w, int i) {
+  const bool group = i >= a.n_seqs;
+  const int32_t* cu = group ? w.cu_group + (i - a.n_seqs) : w.cu_q + i;
+  return cu[0] >= 0 && cu[1] >= cu[0] && cu[1] <= (group ? a.n_seqs : a.tokens);
+}
+// Whether what only the device sees of a call with shared keys is in range, for a sequence or a group.
+__device__ __forceinline__ bool shared_ok(const q4gpu_attn_args& a, const More& x, const Where& w, int i) {
+  if (i < a.n_seqs) {
+    if (!sequence_ok(a, i)) return false;
+    const int n = a.cu_q[i + 1] - a.cu_q[i], g = group_of(x, w, i);
+    return n == 0 || g < 0 || w.prefix_lens[g] <= 0 ||
+           w.prefix_lens[g] <= a.lens[a.seq_ids ? a.seq_ids[i] : i] - n;
+  }
+  const int g = i - a.n_seqs, c = w.cu_group[g];
+  if (!ascends(a, w, i) || w.prefix_lens[g] < 0) return false;
+  if (c == w.cu_group[g + 1] || w.prefix_lens[g] == 0) return true;
+  const int s = a.seq_ids ? a.seq_ids[c] : c;  // whose pages hold the shared keys
+  return s >= 0 && s < a.n_slots && w.prefix_lens[g] <= keys_of(a, s);
+}
+
+// Joins what each row got from its own keys and from the shared ones, part by part in order: one warp a row.  It works out
+// for itself where the pieces of attn_rows_kernel lie (with many sequences that kernel joins them, which takes it a fence,
+// a counter and a trip of its own).  Rows of a
 // sequence that the others left out (an unknown slot, queries among the shared keys, more than max_q of them) become
-// zeros, and those of all where cu_q or cu_group does not ascend.
+// zeros, and those of all where cu_q or cu_group does not ascend.  It also reports what only the device sees.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) attn_shared_join_kernel(q4gpu_attn_args a, More more, ChunkPlan plan) {
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(q4gpu_attn_args a, More more, ChunkPlan plan,
+                                                                RowPlan rows) {
+  constexpr int V = D / 32;  // neighbouring values of a lane
+  __shared__ Staged s_staged;
+  __shared__ int64_t s_before[2 * kStaged], s_sum[8];
+  __shared__ int s_most[8];
   const int i = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.q_heads / a.kv_heads, g = group_of(more, i);
-  const Item own = item_of<kShared>(a, more, i);
-  const bool valid = *more.malformed == 0 && own.n > 0 && own.len > 0;
-  const int all = max(0, min(a.cu_q[i + 1], a.tokens) - own.first);
+  const Where where = where_of<kShared>(a, more, &s_staged);
+  const bool known = few<kShared>(a, more);
+  __syncthreads();
+  const int group = a.q_heads / a.kv_heads, g = group_of(more, where, i), blocks = a.kv_heads >> rows.heads_log;
+  bool malformed = false;
+  int64_t stretch = 1;
+  if (known) {  // the axis: an item a thread
+    static_assert(2 * kStaged <= 256, "an item a thread");
+    const int k = threadIdx.x;
+    int64_t cost = 0;
+    int most = 0;
+    if (k < a.n_seqs + more.n_groups) {
+      malformed = !ascends(a, where, k);
+      const Item s = item_of<kShared>(a, more, where, k);
+      most = row_cost<kShared>(a, more, rows, s, group);
+      cost = (int64_t)most * blocks * row_tiles<kShared>(s, group);
+    }
+    int64_t upto = cost;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += v;
+    }
+    most = __reduce_max_sync(~0u, most);
+    if (lane == 31) s_sum[warp] = upto;
+    if (lane == 0) s_most[warp] = most;
+    malformed = __syncthreads_or(malformed);
+    int64_t total = 0, before = upto - cost;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp) before += s_sum[w];
+      total += s_sum[w], most = max(most, s_most[w]);
+    }
+    s_before[k] = before;
+    stretch = max((int64_t)1, stretch_of(rows, total, most));
+    __syncthreads();
+  }
+  if (blockIdx.y == 0 && a.err_flag) {
+    if (threadIdx.x == 0 && !shared_ok(a, more, where, i)) *a.err_flag = 1;
+    for (int64_t k = i + (int64_t)threadIdx.x * gridDim.x; k < more.n_groups; k += (int64_t)256 * gridDim.x)
+      if (!shared_ok(a, more, where, a.n_seqs + (int)k)) *a.err_flag = 1;
+  }
+  const Item own = item_of<kShared>(a, more, where, i);
+  const int all = max(0, min(where.cu_q[i + 1], a.tokens) - own.first);
   Item pre{};
-  if (g >= 0) pre = item_of<kShared>(a, more, a.n_seqs + g);
-  auto parts_of = [&](int lo, int hi, const Item& s) {  // of a row pair
-    if (s.n < plan.least) return s.n > 0 ? 1 : 0;        // attn_rows_kernel's
-    const Span span = span_of<kShared>(lo, hi, more);
-    const int chunk = part_keys(plan, span.end - span.begin);
-    return span.end > span.begin ? (span.end - span.begin + chunk - 1) / chunk : 1;
+  if (g >= 0) pre = item_of<kShared>(a, more, where, a.n_seqs + g);
+
+  // What a row has of item s: `n` parts, `step` rows of the sums apart from `first` on (of the sets', or of the pieces').
+  struct Parts {
+    int n;
+    bool pieces;
+    int64_t first, step;
   };
+  auto parts_of = [&](const Item& s, int id, int64_t token, int head, int set0) {
+    Parts p{0, false, 0, 0};
+    if (s.n == 0) return p;
+    const int64_t set = (int64_t)a.tokens * a.q_heads;
+    p.first = set0 * set + token * a.q_heads + head, p.step = set;
+    const int64_t r = (token - s.first) * group + head % group;  // the row's number in its key head
+    if (s.n >= plan.least) {                                     // attn_chunk_kernel's
+      const int64_t row0 = r / kPair * kPair;
+      const int n = (int)min((int64_t)kPair, (int64_t)s.n * group - row0);
+      const int hi = s.flat ? s.len : max(0, s.len - s.n + (int)((row0 + n - 1) / group) + 1);
+      const Span span = span_of<kShared>(s.lo, hi, more);
+      const int chunk = part_keys(plan, span.end - span.begin);
+      p.n = span.end > span.begin ? (span.end - span.begin + chunk - 1) / chunk : 1;
+      return p;
+    }
+    p.n = 1;
+    if (!known) return p;
+    const int kvh = head / group, heads = 1 << rows.heads_log, tiles = row_tiles<kShared>(s, group);
+    const int cost = row_cost<kShared>(a, more, rows, s, group);
+    int lo;
+    Gap gap;
+    if (row_keys<kShared>(a, more, s, group, lo, gap) <= 0) return p;
+    const int64_t start = s_before[id] + (int64_t)((kvh >> rows.heads_log) * tiles + (int)(r / kRows)) * cost +
+                          rows.piece_cost;  // of its first real unit
+    const int64_t cta0 = quotient(start, stretch), cta1 = quotient(start + cost - rows.piece_cost - 1, stretch);
+    if (cta0 == cta1) return p;
+    p.n = (int)(cta1 - cta0) + 1, p.pieces = true, p.step = 2 * heads * kRows;
+    p.first = (2 * cta0 * heads + (kvh & (heads - 1))) * kRows + r % kRows;  // (the first piece lies `heads` rows on)
+    return p;
+  };
+  bool waited = false;
   for (int64_t y = (int64_t)blockIdx.y * 8 + warp; y < (int64_t)all * a.q_heads; y += (int64_t)gridDim.y * 8) {
-    const int t = (int)(y / a.q_heads), head = (int)(y - (int64_t)t * a.q_heads);
-    const int64_t row = (int64_t)(own.first + t) * a.q_heads + head, set = (int64_t)a.tokens * a.q_heads;
-    T* out = static_cast<T*>(a.out) + (int64_t)(own.first + t) * a.out_token_stride + (int64_t)head * a.out_head_stride;
-    float top = -INFINITY, sum = 0.f, o[D / 32];
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) o[c] = 0.f;
-    int own_parts = 0, pre_parts = 0;
-    if (valid) {
-      const int64_t r = (int64_t)t * group + head % group, row0 = r / kPair * kPair;
-      const int rows = (int)min((int64_t)kPair, (int64_t)own.n * group - row0);
-      own_parts = parts_of(own.lo, max(0, own.len - own.n + (int)((row0 + rows - 1) / group) + 1), own);
-      pre_parts = g < 0 ? 0 : parts_of(0, pre.len, pre);
+    const int t = (int)quotient(y, a.q_heads), head = (int)(y - (int64_t)t * a.q_heads);
+    const int64_t token = own.first + t, row = token * a.q_heads + head;
+    Parts mine = parts_of(own, i, token, head, 0), shared{0, false, 0, 0};
+    if (g >= 0) shared = parts_of(pre, a.n_seqs + g, token, head, more.own_parts);
+    if (!waited) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");  // now the parts are there
+      if (!known) malformed = *more.malformed != 0;
+      waited = true;
     }
-    auto place = [&](int k) { return row + (k < own_parts ? k : more.own_parts + k - own_parts) * set; };
-    for (int k = 0; k < own_parts + pre_parts; ++k) top = fmaxf(top, more.ml[place(k)].x);
-    const float ref = top == -INFINITY ? 0.f : top;
-    for (int k = 0; k < own_parts + pre_parts; ++k) {
-      const float2 w = more.ml[place(k)];
-      const float f = ex2(w.x - ref);
-      sum = fmaf(w.y, f, sum);
-      const float* p = more.o + place(k) * D + lane;
+    if (malformed || own.n == 0 || own.len == 0) mine.n = shared.n = 0;
+    const int parts = mine.n + shared.n;
+    auto place = [&](int k, bool& pieces) {
+      const bool first = k < mine.n;
+      const Parts& p = first ? mine : shared;
+      const int j = first ? k : k - mine.n;
+      pieces = p.pieces;
+      return p.first + j * p.step + (p.pieces && j == 0 ? (int64_t)kRows << rows.heads_log : 0);
+    };
+    float top = -INFINITY, sum = 0.f, o[V];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) o[c] = fmaf(p[c * 32], f, o[c]);
+    for (int c = 0; c < V; ++c) o[c] = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += 32) {  // a lane a part
+      bool pieces = false;
+      const int64_t at = k0 + lane < parts ? place(k0 + lane, pieces) : 0;
+      const float2 w = k0 + lane < parts ? (pieces ? rows.ml : more.ml)[at] : make_float2(-INFINITY, 0.f);
+      const float* const from = (pieces ? rows.o : more.o) + at * D;
+      float most = w.x;
+      bool nan = w.x != w.x || w.y != w.y;
+#pragma unroll
+      for (int s = 16; s; s >>= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, s));
+      nan = __any_sync(~0u, nan);
+      const float next = fmaxf(top, most), ref = next == -INFINITY ? 0.f : next;
+      const float shrink = top == -INFINITY ? 0.f : ex2(top - ref), f = ex2(w.x - ref);
+      sum *= shrink;
+#pragma unroll
+      for (int c = 0; c < V; ++c) o[c] *= shrink;
+      top = next;
+      const float part = nan ? w.x * 0.f + w.y : f * w.y;
+      float total = part;
+#pragma unroll
+      for (int s = 16; s; s >>= 1) total += __shfl_xor_sync(~0u, total, s);
+      sum += total;
+      const int n = min(32, parts - k0);
+      for (int k1 = 0; k1 < n; k1 += 8) {  // eight loads on their way at a time
+        float v[8][V];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float* p = reinterpret_cast<const float*>(
+                               __shfl_sync(~0u, reinterpret_cast<unsigned long long>(from), (k1 + k) & 31)) + lane * V;
+          if (k1 + k >= n) {
+#pragma unroll
+            for (int c = 0; c < V; ++c) v[k][c] = 0.f;
+          } else if constexpr (V == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p);
+            v[k][0] = q.x, v[k][1] = q.y, v[k][2] = q.z, v[k][3] = q.w;
+          } else {
+            const float2 q = *reinterpret_cast<const float2*>(p);
+            v[k][0] = q.x, v[k][1] = q.y;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float weight = __shfl_sync(~0u, f, (k1 + k) & 31);
+          if (k1 + k < n)
+#pragma unroll
+            for (int c = 0; c < V; ++c) o[c] = fmaf(v[k][c], weight, o[c]);
+        }
+      }
     }
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) out[c * 32 + lane] = from_f32<T>(sum == 0.f ? 0.f : o[c] / sum);
-    if (a.lse && lane == 0) a.lse[row] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T* out = static_cast<T*>(a.out) + token * a.out_token_stride + (int64_t)head * a.out_head_stride + lane * V;
+    if constexpr (V == 4)
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+    else
+      *reinterpret_cast<uint32_t*>(out) = pack2<T>(o[0] * inv, o[1] * inv);
+    if (a.lse && lane == 0)
+      a.lse[row] = sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.6931471805599453f;
   }
 }
 
