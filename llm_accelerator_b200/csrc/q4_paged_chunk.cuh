@@ -63,6 +63,9 @@ __device__ __forceinline__ Gap gap_before(int lo, int sinks, int step) {
   return g;
 }
 
+// The lowest n bits of 64 (none where n is negative, all from 64 on).
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
 // First key that a query at position pos (negative: before all keys) sees through a window.
 __device__ __forceinline__ int first_seen(int pos, int window) { return (int)max((int64_t)0, (int64_t)pos - window + 1); }
 
@@ -777,18 +780,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tm_ld_wait32(s);
         tm_ld_wait32(s + 32);
         if (key < all_lo || key + kStep > all_hi || bad) {
-          const int last = pos - key, low = a.window > 0 ? pos - a.window + 1 - key : MODE == kShared ? lo - key : 0;
-          const int sunk = MODE == kSinks ? more.sinks - key : 0;
-          unsigned ok = ~0u;  // pages that exist
-          const int in_page = key & (a.page_tokens - 1);  // 64 in the second half of a 128-token page
-          if (bad) {
-            ok = 0;
+          // a bit for each key of the step that the row sees
+          const int low = a.window > 0 ? pos - a.window + 1 - key : MODE == kShared ? lo - key : 0;
+          uint64_t seen = bits_below(pos - key + 1) & ~bits_below(low);
+          if constexpr (MODE == kSinks) seen |= bits_below(min(pos + 1, more.sinks) - key);
+          if (bad) {  // pages that exist
+            uint64_t there = 0;
             for (int p = key >> shift; p << shift < min(key + kStep, key_end); ++p)
-              ok |= (table[p] >= 0 && table[p] < a.n_pages ? 1u : 0u) << (p - (key >> shift));
+              if (table[p] >= 0 && table[p] < a.n_pages)
+                there |= bits_below(((p + 1) << shift) - key) & ~bits_below((p << shift) - key);
+            seen &= there;
           }
+          const uint32_t words[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
 #pragma unroll
           for (int c = 0; c < kStep; ++c)
-            if (c > last || (c < low && (MODE != kSinks || c >= sunk)) || !((ok >> ((in_page + c) >> shift)) & 1u)) s[c] = -INFINITY;
+            if (!(words[c / 32] & (1u << (c & 31)))) s[c] = -INFINITY;
         }
 #pragma unroll
         for (int c = 0; c < kStep; c += 8)
