@@ -4,17 +4,21 @@ a serving loop uses them.
 The fixed-point path is the product's arithmetic; ``fp32_diag`` judges it against
 a float32 forward of the same weights, one position at a time.  ``PagedDecoder`` is
 that float model at serving speed: prompts enter in chunks, sequences of
-different lengths step together, prompts are shared by forking, and the cache is
-packed when sequences end.  Per layer (H/common.py:231-298 in the reference):
+different lengths step together, prompts are shared by forking (and their keys read once
+for neighbouring forks), texts may grow past a window whose first tokens stay visible,
+tokens are judged by their log probabilities, and the cache is packed when sequences
+end.  Per layer (H/common.py:231-298 in the reference):
 
     residual add + norm            paged.AddRmsNorm
     q, k, v product                torch.matmul (cuBLAS)
     q/k norm, rotary, K/V store    paged.RopeAppend
-    attention over the pages       paged.Attention
+    attention over the pages       paged.Attention, or paged.SharedAttention for forks
     o product, residual + norm     torch.matmul, paged.AddRmsNorm
     gate/up, SiLU, down products   torch.matmul; with ``eight_bit`` the gate/up input is
                                    normed straight into e4m3 with a scale per row and
                                    multiplied in 8 bits
+
+and of the logits                  paged.TokenLogprobs
 
     python -m llm_accelerator_b200.paged_decode [prompt tokens] [continuations]
 """
@@ -28,22 +32,24 @@ import torch
 
 from . import _native, tables
 from .fp32_diag import EPS, HEAD_DIM, HEADS, INTER, KV_HEADS, THETA
-from .paged import AddRmsNorm, Attention, PagedCache, RopeAppend
+from .paged import AddRmsNorm, Attention, PagedCache, RopeAppend, SharedAttention, Step, TokenLogprobs, TokenScores
 
 
 class PagedDecoder:
     """A Qwen3 layer stack with its paged cache.
 
     ``weights``: the dict of ``fp32_diag.float_weights``.  ``rope_factor`` above 1 stretches
-    the rotary frequencies over ``max_ctx`` (``tables.rope_float_tables``).
+    the rotary frequencies over ``max_ctx`` (``tables.rope_float_tables``).  With ``window`` a
+    token sees the last ``window`` ones up to itself, and the first ``sinks``.
     """
 
     def __init__(self, weights: dict, max_seqs: int = 8, max_ctx: int = 4096, n_pages: Optional[int] = None,
                  page_tokens: int = 64, dtype: torch.dtype = torch.bfloat16, rope_factor: float = 1.0,
-                 eight_bit: bool = False):
+                 eight_bit: bool = False, window: int = 0, sinks: int = 0):
         T, dev = _native, weights["embed"].device
         layers = weights["layers"]
-        self.dtype, self.eight_bit = dtype, eight_bit
+        self.dtype, self.eight_bit, self.window = dtype, eight_bit, window
+        self._logprobs: dict[int, TokenLogprobs] = {}
         self.embed = weights["embed"].to(dtype)
         per_seq = -(-max_ctx // page_tokens)
         self.cache = PagedCache(len(layers), n_pages or max_seqs * per_seq, page_tokens, KV_HEADS, HEAD_DIM, max_seqs,
@@ -61,7 +67,8 @@ class PagedDecoder:
                                        out_dtype=torch.float8_e4m3fn if eight_bit else None),
                    "rope": RopeAppend(cos, sin, q_gamma=w[T.T_Q_GAMMA].to(dtype), k_gamma=w[T.T_K_GAMMA].to(dtype),
                                       eps=EPS),
-                   "attn": Attention(k, v, self.cache.table, self.cache.lens, q_heads=HEADS), "k": k, "v": v}
+                   "attn": Attention(k, v, self.cache.table, self.cache.lens, q_heads=HEADS, window=window, sinks=sinks),
+                   "k": k, "v": v}
             if eight_bit:
                 top = lay["gu"].float().abs().amax(1, keepdim=True) / 448.0
                 top[top == 0] = 1.0  # a row of zeros stays zeros
@@ -69,14 +76,25 @@ class PagedDecoder:
                 lay["gu8_scale"] = top.t().contiguous()
             self.layers.append(lay)
 
-    def forward(self, seqs: Sequence[int], tokens: Sequence[Sequence[int]]) -> torch.Tensor:
-        """Appends tokens[i] to sequence seqs[i]; float32 logits [sequences, vocab] after each one's last token."""
-        counts = [len(t) for t in tokens]
-        if min(counts, default=0) < 1:
-            raise ValueError("every sequence of a step needs a token")
+    def _attend(self, lay: dict, q: torch.Tensor, step: Step) -> torch.Tensor:
+        if step.cu_group is None or self.window:
+            return lay["attn"](q, None, step.cu_q, max_q=step.max_q, max_ctx=step.max_ctx, seq_ids=step.seq_ids)
+        if "shared" not in lay:
+            lay["shared"] = SharedAttention(lay["k"], lay["v"], self.cache.table, self.cache.lens, q_heads=HEADS)
+        return lay["shared"](q, None, step.cu_q, step.cu_group, step.prefix_lens, max_q=step.max_q,
+                             max_ctx=step.max_ctx, max_prefix=step.max_prefix, seq_ids=step.seq_ids)
+
+    def _known(self, tokens: Sequence[Sequence[int]]) -> None:
         vocab = self.embed.shape[0]
         if not all(0 <= t < vocab for one in tokens for t in one):
             raise ValueError(f"a token is outside the vocabulary of {vocab}")
+
+    def _layers(self, seqs: Sequence[int], tokens: Sequence[Sequence[int]]) -> tuple[torch.Tensor, torch.Tensor, Step]:
+        """Appends tokens[i] to sequence seqs[i]; the last layer's residual stream and what is still to be added to it."""
+        counts = [len(t) for t in tokens]
+        if min(counts, default=0) < 1:
+            raise ValueError("every sequence of a step needs a token")
+        self._known(tokens)
         flat = torch.tensor([t for one in tokens for t in one], dtype=torch.long).pin_memory()
         step = self.cache.extend(seqs, counts)
         h = self.embed[flat.to(self.embed.device, non_blocking=True)]
@@ -89,16 +107,39 @@ class PagedDecoder:
             qkv = (x @ lay["qkv"].t()).view(n, HEADS + 2 * KV_HEADS, HEAD_DIM)
             q, k, v = qkv[:, :HEADS], qkv[:, HEADS:HEADS + KV_HEADS], qkv[:, HEADS + KV_HEADS:]
             lay["rope"](q, k, v, step.positions, step.rows, lay["k"], lay["v"])
-            o = lay["attn"](q, None, step.cu_q, max_q=step.max_q, max_ctx=step.max_ctx, seq_ids=step.seq_ids)
-            add = o.view(n, HEADS * HEAD_DIM) @ lay["o"].t()
+            add = self._attend(lay, q, step).view(n, HEADS * HEAD_DIM) @ lay["o"].t()
             if self.eight_bit:
                 x8, s8 = lay["norm2"](add, residual=h, residual_out=h)
                 gu = torch._scaled_mm(x8, lay["gu8"].t(), scale_a=s8, scale_b=lay["gu8_scale"], out_dtype=self.dtype)
             else:
                 gu = lay["norm2"](add, residual=h, residual_out=h) @ lay["gu"].t()
             add = (torch.nn.functional.silu(gu[:, :INTER]) * gu[:, INTER:]) @ lay["down"].t()
+        return h, add, step
+
+    def forward(self, seqs: Sequence[int], tokens: Sequence[Sequence[int]]) -> torch.Tensor:
+        """Appends tokens[i] to sequence seqs[i]; float32 logits [sequences, vocab] after each one's last token."""
+        h, add, step = self._layers(seqs, tokens)
         last = step.cu_q[1:].long() - 1
         return (self.final(add[last], residual=h[last]) @ self.embed.t()).float()
+
+    def logprobs(self, top: int = 0) -> TokenLogprobs:
+        """The decoder's ``TokenLogprobs`` with ``top`` alternatives."""
+        if top not in self._logprobs:
+            self._logprobs[top] = TokenLogprobs(top, self.embed.device)
+        return self._logprobs[top]
+
+    def score(self, seq: int, tokens: Sequence[int], chunk: int = 512, top: int = 0) -> list[TokenScores]:
+        """Appends `tokens` to a sequence in chunks and judges each by the one before it: row i of a chunk is about the
+        token that follows its token i (the last row of all about none: logprob 0, rank 0)."""
+        if not len(tokens) or chunk < 1:
+            raise ValueError("a text has a token and a chunk at least one")
+        self._known([tokens])
+        judge, scores = self.logprobs(top), []
+        targets = torch.tensor(list(tokens[1:]) + [-1], dtype=torch.long).to(self.embed.device)
+        for at in range(0, len(tokens), chunk):
+            h, add, _ = self._layers([seq], [tokens[at:at + chunk]])
+            scores.append(judge(self.final(add, residual=h) @ self.embed.t(), targets[at:at + chunk]))
+        return scores
 
     def prefill(self, seq: int, prompt: Sequence[int], chunk: int = 512) -> torch.Tensor:
         """A prompt in chunks; the logits after its last token."""
@@ -110,20 +151,29 @@ class PagedDecoder:
 
     def generate(self, seqs: Sequence[int], logits: torch.Tensor, n: int) -> list[list[int]]:
         """n greedy tokens of every sequence, from the logits after its last one."""
-        out = [[] for _ in seqs]
+        return self.generate_scored(seqs, logits, n)[0]
+
+    def generate_scored(self, seqs: Sequence[int], logits: torch.Tensor, n: int) -> \
+            tuple[list[list[int]], list[list[float]]]:
+        """n greedy tokens of every sequence and their log probabilities."""
+        out, scores, judge = [[] for _ in seqs], [[] for _ in seqs], self.logprobs(1)
+        logits = logits.to(self.embed.device)
         for i in range(n):
-            pick = logits.argmax(-1).tolist()
-            for o, t in zip(out, pick):
-                o.append(t)
+            best = judge(logits)
+            pick = best.top_index[:, 0].tolist()
+            for o, s, token, score in zip(out, scores, pick, best.top_logprob[:, 0].tolist()):
+                o.append(token)
+                s.append(score)
             if i + 1 < n:
                 logits = self.forward(seqs, [[t] for t in pick])
-        return out
+        return out, scores
 
 
 def run(prompt_tokens: int = 1500, continuations: int = 4, new_tokens: int = 8, n_layers: int = 4, vocab: int = 4096,
         seed: int = 0, chunk: int = 512) -> dict:
     """One prompt shared by several continuations on the synthetic model: prefilled in chunks,
-    forked, continued by different first tokens together, ended but one, packed, continued."""
+    forked, continued by different first tokens together, ended but one, packed, continued; with the mean log
+    probability of each continuation's tokens."""
     from .fp32_diag import float_weights
 
     class Shape:  # what float_weights asks of a model
@@ -137,14 +187,15 @@ def run(prompt_tokens: int = 1500, continuations: int = 4, new_tokens: int = 8, 
     kids = list(range(1, continuations + 1))
     d.cache.fork(0, kids)
     starts = logits[0].topk(continuations).indices.tolist()
-    texts = d.generate(kids, d.forward(kids, [[t] for t in starts]), new_tokens)
+    texts, scores = d.generate_scored(kids, d.forward(kids, [[t] for t in starts]), new_tokens)
     used = d.cache.pool.shape[0] - d.cache.free_pages
     for s in [0] + kids[:-1]:
         d.cache.free(s)
     live = d.cache.compact()
     more = d.generate(kids[-1:], d.forward(kids[-1:], [[texts[-1][-1]]]), new_tokens)
     d.cache.pages.check()
-    return {"prompt_tokens": prompt_tokens, "continuations": {t: x for t, x in zip(starts, texts)}, "pages_used": used,
+    return {"prompt_tokens": prompt_tokens, "continuations": {t: x for t, x in zip(starts, texts)},
+            "logprobs": {t: sum(s) / len(s) for t, s in zip(starts, scores)}, "pages_used": used,
             "pages_after_compaction": live, "continued": more[0]}
 
 
