@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     uint64_t last = ~0ull;
     for (int k = 0; k < a.top; ++k) {
       uint64_t best = 0;
-      for (int i = tid; i < a.vocab; i += threads) {
-        const uint64_t c = key_of(to_f32(x[i]), i);
+      for (int64_t i = tid; i < a.vocab; i += threads) {
+        const uint64_t c = key_of(to_f32(x[i]), (int)i);
         if (c < last) best = max(best, c);
       }
       for (int o = 16; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)best, o));

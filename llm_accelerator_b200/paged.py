@@ -175,8 +175,8 @@ class _Err:
         if what == 2:
             raise _native.Q4GpuError(f"{type(self).__name__}: a wait inside a kernel ran out; its output is incomplete")
         if what:
-            raise _native.Q4GpuError(f"{type(self).__name__}: a position, row, page, slot, length or query range was "
-                                     "out of range; what it named was left untouched")
+            raise _native.Q4GpuError(f"{type(self).__name__}: a position, row, page, slot, length, query range or "
+                                     "token was out of range; what it named was left untouched")
 
 
 class RopeAppend(_Err):

@@ -67,6 +67,10 @@ def check(pool, table, lens, cu, q, window, sinks, scale=None, err=0):
     return out, lse
 
 
+def off(a, b):
+    return float((a.float() - b.float()).norm() / b.float().norm())
+
+
 HEADS = [(16, 8, 128, 64), (4, 4, 64, 16), (7, 1, 128, 32), (8, 1, 64, 128)]
 
 
@@ -147,6 +151,43 @@ def test_empty_rows(new):
     lens[1], lens[2] = max(0, new - 3), 0
     out, _ = check(pool, table, lens, cu, q, 7, 3)
     assert not out[cu[2]:].any()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("seqs", [3, 200])  # more than the kernels keep in shared memory
+def test_out_of_range_is_reported(new, seqs):
+    """Unknown slots, lengths that the table cannot hold, more queries than max_q, offsets past the tokens."""
+    def fresh():
+        return make([new] * seqs, [90] * seqs, 4, 2, 64, 32, BF, 11)
+
+    def call(max_q=new, seq_ids=None, cu=None, lens=None):
+        pool, table, lens0, cu0, q = fresh()
+        lens = lens0 if lens is None else lens
+        op = paged.Attention(pool[:, 0], pool[:, 1], table, lens, q_heads=4, window=20, sinks=3)
+        lse = torch.full(q.shape[:2], 5.0, device="cuda")
+        out = op(q, torch.full_like(q, 5.0), cu0 if cu is None else cu, max_q=max_q, max_ctx=512, lse=lse,
+                 seq_ids=seq_ids)
+        return out, lse, int(op.err.item())
+
+    pool, table, lens, cu, q = fresh()
+    want, lse = attend(pool, table, lens, cu, q, 20, 3)
+    ids = list(range(seqs))
+    for bad in (-1, seqs):
+        out, l, err = call(seq_ids=i32([ids[0], bad] + ids[2:]))
+        assert err == 1 and not out[new:2 * new].any() and (l[new:2 * new] == -math.inf).all()
+        assert off(out[:new], want[:new]) < 0.01 and off(out[2 * new:], want[2 * new:]) < 0.01
+    long = lens.clone()
+    long[1] = 10 ** 6
+    out, _, err = call(lens=long)
+    assert err == 1 and off(out[:new], want[:new]) < 0.01 and out.isfinite()[:new].all()
+    ends = cu.clone()
+    ends[-1] += 5
+    out, _, err = call(cu=ends)
+    assert err == 1 and off(out, want) < 0.01
+    if new > 1:
+        out, l, err = call(max_q=new - 1)
+        assert err == 1 and all(off(out[a:b], want[a:b]) < 0.01 or not out[a:b].any()
+                                for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()))
 
 
 def test_captured_with_growing_lengths():
