@@ -56,17 +56,21 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Work is laid out on one axis: sequence by sequence, key head by key head, in
-// units of 128 keys, each (sequence, head) behind kPieceCost units that stand for
+// Work is laid out on one axis: item by item (a sequence, or with kShared the own
+// keys of one or the shared keys of a group), block of key heads by block, tile
+// of 16 rows by tile, in units of keys (128 keys of one head, or as many of all of
+// a block's together), each such subitem behind kPieceCost units that stand for
 // what starting it costs (64 decodes at 1 to 8704 keys: 59.3 us with 2, 56.7 with
 // 3, 60.2 with 4).  Every CTA takes an equal stretch of that axis, so the
-// longest sequence does not decide; a stretch's ends cut at most two (sequence,
-// head) items, whose pieces are joined by the CTA that finishes last, in the
-// order of the pieces.
+// longest sequence does not decide; a stretch's ends cut at most two subitems,
+// whose pieces are joined in the order of the pieces, by the CTA that finishes
+// last, or with kShared by the kernel that joins own and shared keys.
 constexpr int kCounters = 4096;  // always at the workspace's start: no other call's data gets there
+
 // Each warp runs over its own 16-key steps of a piece with its own running
-// maximum and sum, so no barrier stands in the loop; the eight are joined at its
-// end.  (Eight warps and one CTA per SM for heads of 128, two for 64; four warps
+// maximum and sum, so no barrier stands in the loop; those of a head are joined at
+// its end (with a head a warp there is nothing to join, and no barrier at all).
+// (Eight warps and one CTA per SM for heads of 128, two for 64; four warps
 // and twice the CTAs start short pieces a little faster, 64 decodes at 1 to 8704
 // keys 55.6 us against 57.0, but take 33.0 against 24.0 for one at 16384 and 122
 // against 94 for 16 of 64-value heads.)  Bound by memory: every key and value is
@@ -430,92 +434,92 @@ __global__ void __launch_bounds__(kRowWarps * 32, D == 64 ? 2 : 1)
           }
         } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (tq == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
-        }
-        __syncthreads();  // every warp is done with its ring
-        // the warps' sums, side by side in the ring's memory
-        float* so = reinterpret_cast<float*>(smem);
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (g + 8 * h < rows)
-              *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
-                  make_float2(o[n][2 * h], o[n][2 * h + 1]);
-        __syncthreads();
-        // four neighbouring values a thread
-        auto put = [&](int hw, int r, int d, float m_all, float l_all, const float4& v) {
-          const int t = (row0 + r) / group, head = (kvh + hw) * group + row0 + r - t * group;
-          if constexpr (MODE == kShared) {
-            const int64_t at = ((int64_t)(s.flat ? x.own_parts : 0) * a.tokens + s.first + t) * a.q_heads + head;
-            *reinterpret_cast<float4*>(x.o + at * D + d) = v;
-            if (d == 0) x.ml[at] = make_float2(l_all == 0.f ? -INFINITY : m_all, l_all);
-            return;
+          for (int h = 0; h < 2; ++h) {
+            if (tq == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
           }
-          const bool none = l_all == 0.f;
-          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.first + t) * a.out_token_stride +
-                                    (int64_t)head * a.out_head_stride + d) =
-              make_uint2(pack2<T>(none ? 0.f : v.x / l_all, none ? 0.f : v.y / l_all),
-                         pack2<T>(none ? 0.f : v.z / l_all, none ? 0.f : v.w / l_all));
-          if (a.lse && d == 0)
-            a.lse[(int64_t)(s.first + t) * a.q_heads + head] = none ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
-        };
-        auto add = [](float4& v, const float4& w, float f) {
-          v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
-        };
-        for (int i = threadIdx.x; i < heads * rows * (D / 4); i += W * 32) {
-          const int hr = i / (D / 4), d = (i - hr * (D / 4)) * 4, hw = MODE == kPlain ? 0 : hr / rows, r = hr - hw * rows;
-          float top = -INFINITY, sum = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          __syncthreads();  // every warp is done with its ring
+          // the warps' sums, side by side in the ring's memory
+          float* so = reinterpret_cast<float*>(smem);
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (MODE == kPlain || w % heads == hw) top = fmaxf(top, s_m[w][r]);
-          const float base = top == -INFINITY ? 0.f : top;
+          for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-          for (int w = 0; w < W; ++w) {
-            if (MODE != kPlain && w % heads != hw) continue;
-            const float f = ex2(s_m[w][r] - base);
-            sum = fmaf(s_l[w][r], f, sum);
-            add(v, *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + d), f);
-          }
-          if (parts == 1) {
-            put(hw, r, d, base, sum, v);
-          } else {
-            const int64_t at = ((2 * (int64_t)blockIdx.x + (part == 0)) * heads + hw) * kRows + r;
-            *reinterpret_cast<float4*>(plan.o + at * D + d) = v;
-            if (d == 0) plan.ml[at] = make_float2(top, sum);
-          }
-        }
-        if (parts > 1 && joined_here) {
-          __threadfence();
+            for (int h = 0; h < 2; ++h)
+              if (g + 8 * h < rows)
+                *reinterpret_cast<float2*>(so + (warp * kRows + g + 8 * h) * D + 8 * n + 2 * tq) =
+                    make_float2(o[n][2 * h], o[n][2 * h + 1]);
           __syncthreads();
-          if (threadIdx.x == 0) {
-            s_last = atomicAdd(plan.done + cta0, 1) == parts - 1;
-            if (s_last) plan.done[cta0] = 0;
-          }
-          __syncthreads();
-          if (s_last) __threadfence();
-        }
-        if (parts > 1 && joined_here && s_last)
+          // four neighbouring values a thread
+          auto put = [&](int hw, int r, int d, float m_all, float l_all, const float4& v) {
+            const int t = (row0 + r) / group, head = (kvh + hw) * group + row0 + r - t * group;
+            if constexpr (MODE == kShared) {
+              const int64_t at = ((int64_t)(s.flat ? x.own_parts : 0) * a.tokens + s.first + t) * a.q_heads + head;
+              *reinterpret_cast<float4*>(x.o + at * D + d) = v;
+              if (d == 0) x.ml[at] = make_float2(l_all == 0.f ? -INFINITY : m_all, l_all);
+              return;
+            }
+            const bool none = l_all == 0.f;
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (int64_t)(s.first + t) * a.out_token_stride +
+                                      (int64_t)head * a.out_head_stride + d) =
+                make_uint2(pack2<T>(none ? 0.f : v.x / l_all, none ? 0.f : v.y / l_all),
+                           pack2<T>(none ? 0.f : v.z / l_all, none ? 0.f : v.w / l_all));
+            if (a.lse && d == 0)
+              a.lse[(int64_t)(s.first + t) * a.q_heads + head] = none ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+          };
+          auto add = [](float4& v, const float4& w, float f) {
+            v.x = fmaf(w.x, f, v.x), v.y = fmaf(w.y, f, v.y), v.z = fmaf(w.z, f, v.z), v.w = fmaf(w.w, f, v.w);
+          };
           for (int i = threadIdx.x; i < heads * rows * (D / 4); i += W * 32) {
             const int hr = i / (D / 4), d = (i - hr * (D / 4)) * 4, hw = MODE == kPlain ? 0 : hr / rows, r = hr - hw * rows;
-            auto slot = [&](int k) { return ((2 * (cta0 + k) + (k == 0)) * heads + hw) * kRows + r; };
             float top = -INFINITY, sum = 0.f;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+              if (MODE == kPlain || w % heads == hw) top = fmaxf(top, s_m[w][r]);
             const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll 8
-            for (int k = 0; k < parts; ++k) {
-              const float2 w = __ldcg(&plan.ml[slot(k)]);
-              const float f = ex2(w.x - base);
-              sum = fmaf(w.y, f, sum);
-              add(v, __ldcg(reinterpret_cast<const float4*>(plan.o + slot(k) * D + d)), f);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+              if (MODE != kPlain && w % heads != hw) continue;
+              const float f = ex2(s_m[w][r] - base);
+              sum = fmaf(s_l[w][r], f, sum);
+              add(v, *reinterpret_cast<const float4*>(so + (w * kRows + r) * D + d), f);
             }
-            put(hw, r, d, base, sum, v);
+            if (parts == 1) {
+              put(hw, r, d, base, sum, v);
+            } else {
+              const int64_t at = ((2 * (int64_t)blockIdx.x + (part == 0)) * heads + hw) * kRows + r;
+              *reinterpret_cast<float4*>(plan.o + at * D + d) = v;
+              if (d == 0) plan.ml[at] = make_float2(top, sum);
+            }
           }
-        __syncthreads();  // the ring and the shared words are free for the next piece
+          if (parts > 1 && joined_here) {
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+              s_last = atomicAdd(plan.done + cta0, 1) == parts - 1;
+              if (s_last) plan.done[cta0] = 0;
+            }
+            __syncthreads();
+            if (s_last) __threadfence();
+          }
+          if (parts > 1 && joined_here && s_last)
+            for (int i = threadIdx.x; i < heads * rows * (D / 4); i += W * 32) {
+              const int hr = i / (D / 4), d = (i - hr * (D / 4)) * 4, hw = MODE == kPlain ? 0 : hr / rows, r = hr - hw * rows;
+              auto slot = [&](int k) { return ((2 * (cta0 + k) + (k == 0)) * heads + hw) * kRows + r; };
+              float top = -INFINITY, sum = 0.f;
+              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+              for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(&plan.ml[slot(k)]).x);
+              const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+              for (int k = 0; k < parts; ++k) {
+                const float2 w = __ldcg(&plan.ml[slot(k)]);
+                const float f = ex2(w.x - base);
+                sum = fmaf(w.y, f, sum);
+                add(v, __ldcg(reinterpret_cast<const float4*>(plan.o + slot(k) * D + d)), f);
+              }
+              put(hw, r, d, base, sum, v);
+            }
+          __syncthreads();  // the ring and the shared words are free for the next piece
         }
       }
       if (++sub == blocks * tiles) {
