@@ -215,12 +215,17 @@ __device__ __noinline__ Held careful_step(Held h, uint32_t warp_at) {
   return h;
 }
 
+// What a warp knows in the end: its sums, its logits before the target, whether there is a NaN or +infinity among them.
+struct Record {
+  Sums sums;
+  int ahead, odd;
+};
 // What the CTAs of a row tell each other.
 struct Board {
   uint64_t group[kGroups];  // the largest of each group of threads
   uint64_t key[kCandidates];
-  Sums sums[kMostParts * kMostThreads / 32];
-  int found, ahead, odd;
+  Record record[kMostParts * kMostThreads / 32];
+  int found;
 };
 
 // `parts` CTAs a row (a cluster), each a stretch of its units of 16 logits; what stands before the first boundary of 16
@@ -240,9 +245,9 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   __shared__ Board s_board;
   __shared__ uint64_t s_bound, s_top[Q4GPU_TOP_MAX];
   __shared__ uint16_t s_thread[kMostThreads];
-  __shared__ int s_odd, s_threads;
+  __shared__ int s_threads;
   __shared__ float s_first[kMostThreads / 32];
-  __shared__ Sums s_sums;
+  __shared__ Record s_all;
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
   const int part = blockIdx.x % (unsigned)parts;
   const int64_t row = blockIdx.x / (unsigned)parts;
@@ -293,13 +298,12 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   const bool end_there = ends && (lane < 8 ? lane < head : end_at < a.vocab);
   const float end = end_there ? to_f32(x[end_at]) : -INFINITY;
   const int near_at = head + mine_unit * kUnit + lane;
-  const bool tie = known && warp == 0 && mine_unit >= u0 && mine_unit < u1 && near_at < given &&
-                   to_f32(x[near_at]) == to_f32(mine);
+  const bool tie = known && mine_unit >= u0 && mine_unit < u1 && warp == ((mine_unit - u0) & (threads - 1)) >> 5 &&
+                   near_at < given && to_f32(x[near_at]) == to_f32(mine);
   if (tid < kGroups) s_board.group[tid] = 0;
-  if (tid == 0) s_board.found = s_board.ahead = s_board.odd = s_odd = s_threads = 0;
+  if (tid == 0) s_board.found = s_threads = 0;
   if (parts > 1)
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  __syncthreads();
   auto board = [&](int p) {  // part p's
     Board* q = &s_board;
     if (parts > 1) asm("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(&s_board), "r"(p));
@@ -407,7 +411,13 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     h.careful<1>(&v);
     ahead += end_key > mine_key;
   }
-  if (h.odd) s_odd = 1;
+  const bool odd = __any_sync(~0u, h.odd);
+  if (odd && known) {  // the order has NaNs, which comparisons leave out
+    ahead = end_key > mine_key;
+    for (int u = u0 + tid; u < u1; u += threads)
+      for (int i = head + u * kUnit; i < head + (u + 1) * kUnit; ++i) ahead += key_of(to_f32(x[i]), i) > mine_key;
+  }
+  ahead = __reduce_add_sync(~0u, ahead);
   sums = h.sums;
   sums.s = warp_sum(sums.s), sums.t = warp_sum(sums.t);
   uint64_t key = u0 + tid < u1 ? (uint64_t)order_of(most) << 32 | (uint32_t)~most_unit : 0;
@@ -420,7 +430,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
 
   if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all boards are clean
   Board* const first = board(0);
-  if (lane == 0) first->sums[part * warps + warp] = sums;
+  if (lane == 0) first->record[part * warps + warp] = Record{sums, ahead, odd};
   if (a.top) {
     const int g = (part * threads + tid) / span;
     if (span > 32) {
@@ -436,14 +446,6 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
       __syncthreads();
   };
   meet();
-  if (s_odd && known) {  // the order has NaNs, which comparisons leave out
-    ahead = end_key > mine_key;
-    for (int u = u0 + tid; u < u1; u += threads)
-      for (int i = head + u * kUnit; i < head + (u + 1) * kUnit; ++i) ahead += key_of(to_f32(x[i]), i) > mine_key;
-  }
-  ahead = __reduce_add_sync(~0u, ahead);
-  if (lane == 0 && ahead) atomicAdd(&first->ahead, ahead);
-  if (tid == 0 && s_odd) atomicOr(&first->odd, 1);
   if (a.top) {
     // the group whose largest is the top-th: `peers` neighbouring lanes compare one with all
     const int peers = threads / groups, g = tid / peers;
@@ -516,31 +518,33 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   if (warp == 0) {
     const int all = parts * warps;
     float m = -INFINITY;
-    for (int i = lane; i < all; i += 32) m = fmaxf(m, s_board.sums[i].m);
+    for (int i = lane; i < all; i += 32) m = fmaxf(m, s_board.record[i].sums.m);
     m = warp_max(m);
     Sums w{m, 0.f, 0.f, 0};
-    int owners = 0;  // of places of m, one of which is left out
+    int owners = 0, ahead = 0, odd = 0;  // owners: of places of m, one of which is left out
     for (int i = lane; i < all; i += 32) {
-      Sums v = s_board.sums[i];
+      Sums v = s_board.record[i].sums;
+      ahead += s_board.record[i].ahead, odd |= s_board.record[i].odd;
       if (v.m == m)
         owners += v.own;
       else
         v.raise(m, v.own);
       w.s += v.s, w.t += v.t;
     }
-    owners = __reduce_add_sync(~0u, owners);
+    owners = __reduce_add_sync(~0u, owners), ahead = __reduce_add_sync(~0u, ahead);
+    odd = __any_sync(~0u, odd);
     w.s = warp_sum(w.s) + (float)max(owners - 1, 0), w.t = warp_sum(w.t);
-    if (lane == 0) s_sums = w;
+    if (lane == 0) s_all = Record{w, ahead, odd};
   }
   __syncthreads();
-  const Sums w = s_sums;
-  const bool bad = s_board.odd, none = w.m == -INFINITY;
+  const Sums w = s_all.sums;
+  const bool bad = s_all.odd, none = w.m == -INFINITY;
   const float norm = log1pf(w.s), nan = __uint_as_float(0x7fffffffu);
   auto logprob = [&](float v) { return bad ? nan : none ? -INFINITY : (v - w.m) - norm; };
   if (tid == 0) {
     if (a.targets) {
       a.logprob[row] = known ? logprob(to_f32(mine)) : 0.f;
-      a.rank[row] = known ? s_board.ahead + 1 : 0;
+      a.rank[row] = known ? s_all.ahead + 1 : 0;
       if (given >= a.vocab && a.err_flag) *a.err_flag = 1;
     }
     a.entropy[row] = bad ? nan : none ? 0.f : norm - w.t / (1.f + w.s);
