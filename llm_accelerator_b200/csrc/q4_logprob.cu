@@ -236,8 +236,8 @@ struct Board {
 // sums against the largest logit of its own and of the CTA's first step, which few steps change.
 // Of the likeliest only each thread's largest is followed on the way.  The top-th of the largest of 32 or 64 groups of threads
 // bounds the top-th of all from below, and about as many logits as are wanted lie above
-// it: the few threads whose largest does are read again, from L2, and what lies above
-// the bound is ranked by counting.
+// it: the units with the few threads' largest that do are read again, from L2 (all of a thread's units where a second one's
+// does), and what lies above the bound is ranked by counting.
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_logprob_args a, int parts) {
   constexpr int P = Unit<T>::kPieces, S = Unit<T>::kStages;
@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   Held h;
   float most = -INFINITY;  // this thread's largest and the first unit that holds it
   int most_unit = u0 + tid;
+  float second = -INFINITY;  // no other unit of the thread has a larger one
   Counter<T> counter;
   int counted = 0;
   const float target = known ? to_f32(mine) : INFINITY;
@@ -348,6 +349,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     float v[kUnit];
     now.get(v);
     const float top = largest<kUnit>(v);
+    second = fmaxf(second, fminf(top, most));
     if (!(top <= most) && most == most) most = top, most_unit = u;
     if (__any_sync(~0u, !(top < target))) {  // a warp's logits mostly lie below the target's
       if (kWhole || u < u1) counter.add(now, u < mine_unit ? from : past);
@@ -456,14 +458,30 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     if (before == a.top - 1) s_bound = k;
     __syncthreads();
     const uint64_t bound = s_bound;
-    if (key && key >= bound) s_thread[atomicAdd(&s_threads, 1)] = (uint16_t)tid;
+    const uint32_t bound_value = (uint32_t)(bound >> 32);
     auto found = [&](uint64_t k) {
       const int n = atomicAdd(&first->found, 1);
       if (n < kCandidates) first->key[n] = k;
     };
+    auto look = [&](const Unit<T>& w, int u) {
+      float v[kUnit];
+      w.get(v);
+      if (order_of(largest<kUnit>(v)) < bound_value) return;
+#pragma unroll
+      for (int e = 0; e < kUnit; ++e)
+        if (((uint64_t)order_of(v[e]) << 32 | (uint32_t)~u) >= bound) found(key_of(v[e], head + u * kUnit + e));
+    };
     if (end_there && end_key >= (bound & ~0xffffffffull)) found(end_key);
+    if (key && key >= bound) {
+      if (most == most && order_of(second) < bound_value) {  // mostly one unit is all there is to look at
+        Unit<T> w;
+        w.load(body + (int64_t)most_unit * P);
+        look(w, most_unit);
+      } else {
+        s_thread[atomicAdd(&s_threads, 1)] = (uint16_t)tid;
+      }
+    }
     __syncthreads();
-    const uint32_t bound_value = (uint32_t)(bound >> 32);
     constexpr int kTogether = 8 / P;  // units on their way at a time
     // a thread's units by as many lanes, up to a warp
     const int peer_lanes = steps > 16 ? 32 : steps > 8 ? 16 : steps > 4 ? 8 : steps > 2 ? 4 : 2, across = 32 / peer_lanes;
@@ -476,13 +494,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
 #pragma unroll
         for (int j = 0; j < kTogether; ++j) {
           const int at = u + j * peer_lanes * threads;
-          if (at >= u1) break;
-          float v[kUnit];
-          w[j].get(v);
-          if (order_of(largest<kUnit>(v)) < bound_value) continue;
-#pragma unroll
-          for (int e = 0; e < kUnit; ++e)
-            if (((uint64_t)order_of(v[e]) << 32 | (uint32_t)~at) >= bound) found(key_of(v[e], head + at * kUnit + e));
+          if (at < u1) look(w[j], at);
         }
       }
   }
