@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   __shared__ Board s_board;
   __shared__ uint64_t s_bound, s_top[Q4GPU_TOP_MAX];
   __shared__ uint16_t s_thread[kMostThreads];
-  __shared__ int s_threads;
+  __shared__ int s_unit[kMostThreads], s_threads, s_units;
   __shared__ float s_first[kMostThreads / 32];
   __shared__ Record s_all;
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   const bool tie = known && mine_unit >= u0 && mine_unit < u1 && warp == ((mine_unit - u0) & (threads - 1)) >> 5 &&
                    near_at < given && to_f32(x[near_at]) == to_f32(mine);
   if (tid < kGroups) s_board.group[tid] = 0;
-  if (tid == 0) s_board.found = s_threads = 0;
+  if (tid == 0) s_board.found = s_threads = s_units = 0;
   if (parts > 1)
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   auto board = [&](int p) {  // part p's
@@ -460,43 +460,38 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     const uint64_t bound = s_bound;
     const uint32_t bound_value = (uint32_t)(bound >> 32);
     auto found = [&](uint64_t k) {
-      const int n = atomicAdd(&first->found, 1);
-      if (n < kCandidates) first->key[n] = k;
+      const int n = atomicAdd(&s_board.found, 1);
+      if (n < kCandidates) s_board.key[n] = k;
     };
-    auto look = [&](const Unit<T>& w, int u) {
+    if (end_there && end_key >= (bound & ~0xffffffffull)) found(end_key);
+    if (key && key >= bound) {  // mostly one unit is all there is to look at
+      if (most == most && order_of(second) < bound_value)
+        s_unit[atomicAdd(&s_units, 1)] = most_unit;
+      else
+        s_thread[atomicAdd(&s_threads, 1)] = (uint16_t)tid;
+    }
+    __syncthreads();
+    const int single = s_units, looks = single + s_threads * steps;
+    for (int i = tid; i < looks; i += threads) {
+      const int j = i - single, k = j / max(steps, 1);
+      const int u = j < 0 ? s_unit[i] : u0 + s_thread[k] + (j - k * steps) * threads;
+      if (u >= u1) continue;
+      Unit<T> w;
       float v[kUnit];
+      w.load(body + (int64_t)u * P);
       w.get(v);
-      if (order_of(largest<kUnit>(v)) < bound_value) return;
+      if (order_of(largest<kUnit>(v)) < bound_value) continue;
 #pragma unroll
       for (int e = 0; e < kUnit; ++e)
         if (((uint64_t)order_of(v[e]) << 32 | (uint32_t)~u) >= bound) found(key_of(v[e], head + u * kUnit + e));
-    };
-    if (end_there && end_key >= (bound & ~0xffffffffull)) found(end_key);
-    if (key && key >= bound) {
-      if (most == most && order_of(second) < bound_value) {  // mostly one unit is all there is to look at
-        Unit<T> w;
-        w.load(body + (int64_t)most_unit * P);
-        look(w, most_unit);
-      } else {
-        s_thread[atomicAdd(&s_threads, 1)] = (uint16_t)tid;
-      }
     }
-    __syncthreads();
-    constexpr int kTogether = 8 / P;  // units on their way at a time
-    // a thread's units by as many lanes, up to a warp
-    const int peer_lanes = steps > 16 ? 32 : steps > 8 ? 16 : steps > 4 ? 8 : steps > 2 ? 4 : 2, across = 32 / peer_lanes;
-    for (int i = warp * across + lane / peer_lanes; i < s_threads; i += warps * across)
-      for (int u = u0 + s_thread[i] + lane % peer_lanes * threads; u < u1; u += kTogether * peer_lanes * threads) {
-        Unit<T> w[kTogether];
-#pragma unroll
-        for (int j = 0; j < kTogether; ++j)
-          if (u + j * peer_lanes * threads < u1) w[j].load(body + (int64_t)(u + j * peer_lanes * threads) * P);
-#pragma unroll
-        for (int j = 0; j < kTogether; ++j) {
-          const int at = u + j * peer_lanes * threads;
-          if (at < u1) look(w[j], at);
-        }
-      }
+    if (part != 0) {  // to the first CTA together: one trip for the place, one for the keys
+      __syncthreads();
+      if (tid == 0) s_units = atomicAdd(&first->found, s_board.found);
+      __syncthreads();
+      for (int i = tid; i < min(s_board.found, kCandidates); i += threads)
+        if (s_units + i < kCandidates) first->key[s_units + i] = s_board.key[i];
+    }
   }
   meet();
   if (part != 0) return;
