@@ -510,12 +510,12 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
       if (rank < a.top) s_top[rank] = k;
     }
   } else {  // many of a few threads' logits: one after another over the whole row
-    uint64_t last = ~0ull;
+    uint64_t last = 0;
     for (int k = 0; k < a.top; ++k) {
       uint64_t best = 0;
       for (int64_t i = tid; i < a.vocab; i += threads) {
         const uint64_t c = key_of(to_f32(x[i]), (int)i);
-        if (c < last) best = max(best, c);
+        if (k == 0 || c < last) best = max(best, c);  // (no key is above a NaN's at index 0)
       }
       for (int o = 16; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)best, o));
       __syncthreads();

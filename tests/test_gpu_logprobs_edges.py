@@ -1,0 +1,67 @@
+"""Rows of logits whose likeliest tokens are hard to tell apart.  Whole numbers are exact: falling logits, NaN before
+all, equal ones by rising index."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from llm_accelerator_b200 import paged  # noqa: E402
+
+BF, HF, SF = torch.bfloat16, torch.float16, torch.float32
+
+
+def likeliest(x, top):
+    """The order by definition: a stable sort, NaN as more than everything."""
+    v = x.double()
+    first = v.isnan().double().sort(stable=True, dim=-1, descending=True).indices  # NaNs, then the others
+    nans = v.isnan().sum(-1)
+    rest = torch.where(v.isnan(), -math.inf, v)
+    # (a NaN's place in `rest` counts as the lowest; the others' order is cut behind the NaNs)
+    order = rest.sort(stable=True, dim=-1, descending=True).indices
+    out = torch.empty(x.shape[0], top, dtype=torch.int64, device="cuda")
+    for r in range(x.shape[0]):
+        n = int(nans[r])
+        mine = order[r][~v[r].isnan()[order[r]]]
+        out[r] = torch.cat((first[r][:min(n, top)], mine[:max(0, top - n)]))
+    return out
+
+
+def normal(rows, vocab, dtype, seed=0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return (torch.randn(rows, vocab, device="cuda", generator=g) * 3).to(dtype)
+
+
+def check(x, top):
+    op = paged.TokenLogprobs(top=top)
+    got = op(x)
+    assert torch.equal(got.top_index.long(), likeliest(x, top))
+    op.check()
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF])
+@pytest.mark.parametrize("rows", [1, 64, 300])
+@pytest.mark.parametrize("top", [1, 2, 5, 32])
+def test_rows_of_nan(dtype, rows, top):
+    x = normal(rows, 151936, dtype)
+    x[0] = math.nan
+    x[-1, : 5000] = math.nan
+    got = check(x, top)
+    assert got.top_index[0].tolist() == list(range(top))
+    assert got.top_logprob[0].isnan().all() and got.entropy[0].isnan()
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("what", [math.nan, 50.0])
+@pytest.mark.parametrize("top", [5, 32])
+def test_many_large_ones_in_a_few_threads(dtype, what, top):
+    """Every 512th unit of 16 and the three behind it: more than 1024 logits of four threads."""
+    x = normal(300, 151936, dtype)
+    x[7].view(-1, 16)[torch.arange(151936 // 16, device="cuda") % 512 < 4] = what
+    check(x, top)
