@@ -811,6 +811,16 @@ bool shared_room(const q4gpu_attn_args& a, const More& x, SharedRoom& r, int& ow
   return p.tiles <= 65535;
 }
 
+// The workspace of a call without shared keys: the few-row kernel's, and the chunk kernel's parts behind it.  By the
+// plans of the mode that is launched, which lay it out.
+template <int MODE>
+size_t room_of(const q4gpu_attn_args& a, const More& x) {
+  size_t rows, chunks;
+  row_plan<MODE>(a, x, nullptr, &rows);
+  chunk_plan<MODE>(a, x, &chunks);
+  return (rows + 15) / 16 * 16 + chunks;
+}
+
 int check_shared(const q4gpu_attn_args* a, const q4gpu_shared_args* sh) {
   if (!sh) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: null arguments");
   if (a->window) return q4gpu_fail(Q4GPU_ERR_ARG, "attention: shared keys and a window do not go together");
@@ -860,10 +870,7 @@ size_t q4gpu_sink_attention_workspace_bytes(const q4gpu_attn_args* a, int32_t si
   if (check_sizes(a) != Q4GPU_OK || sinks < 0) return 0;
   const q4gpu_attn_args b = settled(*a);
   const More x = settled_sinks(b, sinks);
-  size_t rows, chunks;
-  row_plan<kSinks>(b, x, nullptr, &rows);
-  chunk_plan<kSinks>(b, x, &chunks);
-  return (rows + 15) / 16 * 16 + chunks;
+  return x.sinks ? room_of<kSinks>(b, x) : room_of<kPlain>(b, x);
 }
 
 int q4gpu_sink_attention(const q4gpu_attn_args* a, int32_t sinks, void* stream) {
