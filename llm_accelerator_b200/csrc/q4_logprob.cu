@@ -297,12 +297,13 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   const auto from = Counter<T>::bound(mine), past = Counter<T>::bound(above(mine));
   // the ends of the row, one logit a lane of one warp, and the logits before the target in its unit
   const bool ends = part == 0 && warp == 0 && (head > 0 || tail < a.vocab);
-  const int end_at = lane < 8 ? lane : tail + lane - 8;
-  const bool end_there = ends && (lane < 8 ? lane < head : end_at < a.vocab);
+  // (places are compared by their distance: next to 2^31 a sum with the lane would wrap)
+  const bool end_there = ends && (lane < 8 ? lane < head : lane - 8 < a.vocab - tail);
+  const int end_at = !end_there ? 0 : lane < 8 ? lane : tail + lane - 8;
   const float end = end_there ? to_f32(x[end_at]) : -INFINITY;
-  const int near_at = head + mine_unit * kUnit + lane;
+  const int near = head + mine_unit * kUnit;
   const bool tie = known && mine_unit >= u0 && mine_unit < u1 && warp == ((mine_unit - u0) & (threads - 1)) >> 5 &&
-                   near_at < given && to_f32(x[near_at]) == to_f32(mine);
+                   lane < (int)given - near && to_f32(x[near + lane]) == to_f32(mine);
   if (tid < kGroups) s_board.group[tid] = 0;
   if (tid == 0) s_board.found = s_threads = s_units = 0;
   if (parts > 1)

@@ -65,3 +65,26 @@ def test_many_large_ones_in_a_few_threads(dtype, what, top):
     x = normal(300, 151936, dtype)
     x[7].view(-1, 16)[torch.arange(151936 // 16, device="cuda") % 512 < 4] = what
     check(x, top)
+
+
+@pytest.mark.parametrize("first", [0, 1, 7])
+def test_vocabularies_next_to_2_to_the_31(first):
+    """Equal logits but for three: sums and ranks of the last unit of 16 and of what stands behind it."""
+    vocab = 2 ** 31 - 1
+    store = torch.zeros(vocab + 16, dtype=BF, device="cuda")
+    x = store[first:first + vocab].view(1, vocab)
+    lp = paged.TokenLogprobs()
+    for t in (vocab - 1, vocab - 15, vocab - 16, vocab - 17, vocab - 30, 2 ** 30, 0):
+        got = lp(x, torch.tensor([t], device="cuda"))
+        assert got.rank.item() == t + 1
+        # 2^31 - 2 ones in 32 bits: each of the few additions a warp and its partners make is off by 2^-24 at most
+        assert abs(got.logprob.item() + math.log(vocab)) < 1e-4 and abs(got.entropy.item() - math.log(vocab)) < 1e-4
+    best = {vocab - 1: 32.0, vocab - 17: 31.0, 0: 30.0}
+    for at, v in best.items():
+        x[0, at] = v
+    got = paged.TokenLogprobs(top=3)(x, torch.tensor([vocab - 2], device="cuda"))
+    assert got.top_index[0].tolist() == list(best) and got.rank.item() == vocab
+    want = torch.tensor(list(best.values()), dtype=torch.float64)
+    norm = math.log(vocab - 3 + sum(math.exp(v) for v in best.values()))
+    assert (got.top_logprob[0].double().cpu() - (want - norm)).abs().max() < 1e-4
+    lp.check()
