@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
                    lane < (int)given - near && to_f32(x[near + lane]) == to_f32(mine);
   if (tid < kGroups) s_board.group[tid] = 0;
   if (tid == 0) s_board.found = s_threads = s_units = 0;
-  if (parts > 1)
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  __syncwarp();  // (the cluster's barriers are for whole warps, and lanes have taken ways of their own)
+  if (parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   auto board = [&](int p) {  // part p's
     Board* q = &s_board;
     if (parts > 1) asm("mapa.u64 %0, %1, %2;" : "=l"(q) : "l"(&s_board), "r"(p));
@@ -435,6 +435,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     for (int o = 1; o < lanes; o <<= 1)
       group = max(group, (uint64_t)__shfl_xor_sync(~0u, (unsigned long long)group, o));
 
+  __syncwarp();
   if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all boards are clean
   Board* const first = board(0);
   if (lane == 0) first->record[part * warps + warp] = Record{sums, ahead, odd};
@@ -447,6 +448,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     }
   }
   auto meet = [&] {  // of the row's CTAs
+    __syncwarp();
     if (parts > 1)
       asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
     else

@@ -88,3 +88,17 @@ def test_vocabularies_next_to_2_to_the_31(first):
     norm = math.log(vocab - 3 + sum(math.exp(v) for v in best.values()))
     assert (got.top_logprob[0].double().cpu() - (want - norm)).abs().max() < 1e-4
     lp.check()
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("rows", [1, 20, 64])
+def test_candidates_of_single_lanes(dtype, rows):
+    """Rows over clusters whose candidates lie in one lane of a warp, in one warp, in the last CTA: lanes that have no
+    more to look at wait for the others before the CTAs meet."""
+    x = normal(rows, 151936, dtype)
+    units = x.view(rows, -1, 16)
+    units[0, 5::512, 3] = 40.0
+    units[rows // 2, 32:64, 0] = 41.0
+    units[-1, -7:, 9] = 42.0
+    for _ in range(3):
+        check(x, 20)
