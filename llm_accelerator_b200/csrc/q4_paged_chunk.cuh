@@ -1194,6 +1194,9 @@ __global__ void __launch_bounds__(256) attn_shared_join_kernel(q4gpu_attn_args a
     if (a.lse && lane == 0)
       a.lse[row] = sum == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(sum)) * 0.6931471805599453f;
   }
+  // Where no sequence has a row nobody has waited: one CTA does, so that this kernel is not complete before the others
+  // and what comes next in the stream may change their inputs.
+  if (!waited && blockIdx.x == 0 && blockIdx.y == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace paged
