@@ -276,7 +276,7 @@ int q4gpu_rope_append(const q4gpu_rope_args *a, void *stream);
  * outside 0 .. n_pages - 1, which hold no keys) gets zeros and -infinity.
  * *err_flag (optional) becomes 1 where a page of a seen key, the slot of a
  * sequence with queries (it holds no keys then), its lens (cut off at what its
- * row of the table can name) or cu_q (cut off at 0 .. tokens) is out of range,
+ * row of the table can name, and at 2^30) or cu_q (cut off at 0 .. tokens) is out of range,
  * and where a sequence has more than max_q queries (its rows are then complete
  * or zeros and -infinity).
  * What stands in a key or value row that a query does not see does not reach

@@ -591,7 +591,7 @@ q4gpu_attn_args settled(const q4gpu_attn_args& a) {
   q4gpu_attn_args b = a;
   if (b.table_pages == 0) b.table_pages = (int32_t)std::min<int64_t>(b.table_stride, INT32_MAX);
   // a window that no slot's keys fill is none (position - window would pass 31 bits for queries before the first key)
-  if (b.window >= std::min<int64_t>((int64_t)b.table_pages * b.page_tokens, INT32_MAX)) b.window = 0;
+  if (b.window >= most_keys(b)) b.window = 0;
   return b;
 }
 

@@ -33,8 +33,13 @@ __device__ __forceinline__ int part_keys(const ChunkPlan& plan, int keys) {
   return max(kMinPart, ((keys + plan.parts - 1) / plan.parts + kNTile - 1) & ~(kNTile - 1));
 }
 
-// Keys that a slot's row of the table can name.
-__device__ __forceinline__ int64_t most_keys(const q4gpu_attn_args& a) { return (int64_t)a.table_pages * a.page_tokens; }
+// Keys that a slot's row of the table can name, and that sums of two places of a walk in 31 bits allow (as many
+// different keys of the smallest kind, 256 bytes with their values, are more than the memory holds).
+constexpr int kMostKeys = 1 << 30;
+__host__ __device__ __forceinline__ int64_t most_keys(const q4gpu_attn_args& a) {
+  const int64_t named = (int64_t)a.table_pages * a.page_tokens;
+  return named < kMostKeys ? named : kMostKeys;
+}
 
 // Which keys a query sees: those up to its own (through a window the last of them), or those and the first few keys of
 // the sequence as well, or, in two items of work that are joined afterwards, those that its group of sequences shares
