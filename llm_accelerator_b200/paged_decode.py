@@ -151,21 +151,30 @@ class PagedDecoder:
 
     def generate(self, seqs: Sequence[int], logits: torch.Tensor, n: int) -> list[list[int]]:
         """n greedy tokens of every sequence, from the logits after its last one."""
-        return self.generate_scored(seqs, logits, n)[0]
+        return self._greedy(seqs, logits, n, lambda x: (x.argmax(-1).tolist(), None))[0]
 
     def generate_scored(self, seqs: Sequence[int], logits: torch.Tensor, n: int) -> \
             tuple[list[list[int]], list[list[float]]]:
         """n greedy tokens of every sequence and their log probabilities."""
-        out, scores, judge = [[] for _ in seqs], [[] for _ in seqs], self.logprobs(1)
-        logits = logits.to(self.embed.device)
+        judge = self.logprobs(1)
+
+        def pick(x: torch.Tensor) -> tuple[list[int], list[float]]:
+            best = judge(x)
+            return best.top_index[:, 0].tolist(), best.top_logprob[:, 0].tolist()
+        return self._greedy(seqs, logits.to(self.embed.device), n, pick)
+
+    def _greedy(self, seqs: Sequence[int], logits: torch.Tensor, n: int, pick) -> \
+            tuple[list[list[int]], list[list[float]]]:
+        """n tokens of every sequence by `pick`, which gives those of one step's logits, and their scores or None."""
+        out, scores = [[] for _ in seqs], [[] for _ in seqs]
         for i in range(n):
-            best = judge(logits)
-            pick = best.top_index[:, 0].tolist()
-            for o, s, token, score in zip(out, scores, pick, best.top_logprob[:, 0].tolist()):
-                o.append(token)
-                s.append(score)
+            tokens, values = pick(logits)
+            for o, t in zip(out, tokens):
+                o.append(t)
+            for s, v in zip(scores, values or ()):
+                s.append(v)
             if i + 1 < n:
-                logits = self.forward(seqs, [[t] for t in pick])
+                logits = self.forward(seqs, [[t] for t in tokens])
         return out, scores
 
 
