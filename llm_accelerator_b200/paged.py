@@ -689,6 +689,10 @@ class PagedCache:
     # and 9.4, of 1024 11.7 and 15.2; 16 of 256 15.4 and 10.0, of 1024 18.0 and 21.4; 64 of 256 19.0 and 27.4, of 8192
     # 25.4 and 259.8).
     SHARED_KEYS, SAVED_KEYS = 1024, 16384
+    # ... and new tokens of a sequence up to which they can be: longer chunks fill tiles by themselves, so that sharing
+    # saves no time and joining costs some (alone against together, 16 of 8192 keys: 112 and 59 us with 16 tokens, 113 and
+    # 173 with 64; 64 of 1024: 94 and 71 with 16, 94 and 142 with 32, 243 and 750 with 256).
+    NEW_TOKENS = 16
 
     def __init__(self, n_layers: int, n_pages: int, page_tokens: int, kv_heads: int, head_dim: int, max_seqs: int,
                  max_ctx: int, dtype: torch.dtype = torch.bfloat16, device: Optional[torch.device] = None):
@@ -762,10 +766,9 @@ class PagedCache:
             rows.append(held[p // self.page_tokens] * self.page_tokens + p % self.page_tokens if n else p)
             self._len[s] += n
         runs = shared_runs([self._held[s] for s in seqs], self._users) if len(seqs) > 1 else []
-        prefix = max((p for _, p in runs), default=0) * self.page_tokens
-        saved = sum((n - 1) * p for n, p in runs) * self.page_tokens
+        prefix = self._together(runs, counts)
         groups = {}
-        if prefix >= self.SHARED_KEYS or saved >= self.SAVED_KEYS:
+        if prefix:
             ends = np.cumsum([0] + [n for n, _ in runs])
             groups = dict(cu_group=self._up(ends.astype(np.int32)), max_prefix=prefix,
                           prefix_lens=self._up(np.asarray([p * self.page_tokens for _, p in runs], dtype=np.int32)))
@@ -777,6 +780,14 @@ class PagedCache:
         return Step(ids, self._up(np.concatenate(([0], np.cumsum(counts))).astype(np.int32)),
                     self._up(np.concatenate(pos).astype(np.int32)), self._up(np.concatenate(rows)), max(counts),
                     max(max(lens), 1), **groups)
+
+    def _together(self, runs: Sequence[tuple[int, int]], counts: Sequence[int]) -> int:
+        """The most keys that a run of a step shares, if its runs are worth attending to together, else 0."""
+        if max(counts) > self.NEW_TOKENS:
+            return 0
+        prefix = max((p for _, p in runs), default=0) * self.page_tokens
+        saved = sum((n - 1) * p for n, p in runs) * self.page_tokens
+        return prefix if prefix >= self.SHARED_KEYS or saved >= self.SAVED_KEYS else 0
 
     def fork(self, parent: int, children: Sequence[int]) -> None:
         """Empty sequences `children` continue `parent`: full pages are shared, its last one copied."""
