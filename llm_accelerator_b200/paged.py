@@ -684,12 +684,17 @@ class PagedCache:
     and are never written again; a partly filled last page belongs to one.
     """
 
-    # Shared keys from which on a step's neighbouring forks are worth attending to together: of one group, or in all
-    # those that are not read again (us a layer, 16 heads on 8 of 128, together against alone: 2 forks of 256 tokens 10.9
-    # and 9.4, of 1024 11.7 and 15.2; 16 of 256 15.4 and 10.0, of 1024 18.0 and 21.4; 64 of 256 19.0 and 27.4, of 8192
-    # 25.4 and 259.8).
-    SHARED_KEYS, SAVED_KEYS = 1024, 16384
-    # ... and new tokens of a sequence up to which they can be: longer chunks fill tiles by themselves, so that sharing
+    # Whether a step's neighbouring forks attend together (us a layer of 16 heads on 8 of 128, then of 28 on 4 of 64, one
+    # new token each, alone and together).  A few sequences do from SHARED_KEYS on: alone their keys are cut into many
+    # pieces (2 forks of 256 keys 9.3 and 10.3, 8.2 and 10.0; of 1024 15.0 and 11.8, 13.6 and 10.6; 8 of 1024 16.5 and 15.5, 13.9
+    # and 13.5; 12 of 1024 18.5 and 17.0, 14.4 and 19.1).  Otherwise they do where enough is not read again: SAVED_KEYS
+    # of 8 heads of 128, of smaller ones more by the square of a key's values, as those are read in less time but joined in
+    # the same (16 of 256 10.0 and 15.4; 32 of 256 20.3 and 15.9; 64 of 256 27.1 and 18.4, 10.3 and 21.1; 64 of 1024 50.5 and
+    # 21.6, 22.1 and 25.3; 64 of 8192 261 and 31, 80 and 35), and more by the new tokens of a sequence (16 of 512 keys
+    # 17.9 and 16.5 with one, 18.5 and 22.1 with 4; 32 of 1024 33.4 and 27.8 with 4).
+    SHARED_KEYS, SAVED_KEYS = 1024, 7500
+    FEW = 8, 4  # sequences, new tokens of each
+    # New tokens of a sequence up to which it can pay: longer chunks fill tiles by themselves, so that sharing
     # saves no time and joining costs some (alone against together, 16 of 8192 keys: 112 and 59 us with 16 tokens, 113 and
     # 173 with 64; 64 of 1024: 94 and 71 with 16, 94 and 142 with 32, 243 and 750 with 256).
     NEW_TOKENS = 16
@@ -783,11 +788,15 @@ class PagedCache:
 
     def _together(self, runs: Sequence[tuple[int, int]], counts: Sequence[int]) -> int:
         """The most keys that a run of a step shares, if its runs are worth attending to together, else 0."""
-        if max(counts) > self.NEW_TOKENS:
+        new = max(counts)
+        if new > self.NEW_TOKENS:
             return 0
         prefix = max((p for _, p in runs), default=0) * self.page_tokens
         saved = sum((n - 1) * p for n, p in runs) * self.page_tokens
-        return prefix if prefix >= self.SHARED_KEYS or saved >= self.SAVED_KEYS else 0
+        values = self.pool.shape[3] * self.pool.shape[5]  # of a key
+        few = len(counts) <= self.FEW[0] and new <= self.FEW[1]
+        enough = saved * values ** 2 >= self.SAVED_KEYS * new * 1024 ** 2
+        return prefix if few and prefix >= self.SHARED_KEYS or enough else 0
 
     def fork(self, parent: int, children: Sequence[int]) -> None:
         """Empty sequences `children` continue `parent`: full pages are shared, its last one copied."""
