@@ -307,11 +307,13 @@ class Attention(_Err):
     the keys a slot holds, the new ones included.  ``scale`` defaults to
     dim ** -0.5; with ``window`` a query sees the last ``window`` keys up to its own, and
     the first ``sinks`` keys of its sequence up to its own (pages that hold neither are
-    not read).
+    not read).  ``share``: another of them (a layer before, say) whose workspace this one
+    uses as well; their calls then follow one another like those of one object.
     """
 
     def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
-                 q_heads: int, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
+                 q_heads: int, scale: Optional[float] = None, window: int = 0, sinks: int = 0,
+                 share: Optional["Attention"] = None):
         self.lib = _native.load()
         self.device = _cuda(k_cache, "k_cache")
         self.dtype = k_cache.dtype
@@ -328,8 +330,12 @@ class Attention(_Err):
         _need(window > 0 or sinks == 0, "sinks need a window")
         self.q_heads, self.dim, self.slots, self.sinks = q_heads, dim, table.shape[0], sinks
         self.k_cache, self.v_cache, self.table, self.lens = k_cache, v_cache, table, lens
+        _need(share is None or share.device == self.device, "a workspace is shared on one device")
         self.workspace = self.layout = None
-        self.lock = threading.Lock()
+        # workspaces, the newest last.  The old ones stay: captured graphs know their addresses (each is at least twice
+        # the last, so all together are less than two of the newest)
+        self.room: list[torch.Tensor] = [] if share is None else share.room
+        self.lock = threading.Lock() if share is None else share.lock
         self._new_err()
         self.args = _native.AttnArgs(
             k_cache=k_cache.data_ptr(), v_cache=v_cache.data_ptr(), table=table.data_ptr(), lens=lens.data_ptr(),
@@ -403,11 +409,14 @@ class Attention(_Err):
         a = self.args
         need = self._workspace_bytes(a)
         if need > a.workspace_bytes:
-            if torch.cuda.is_current_stream_capturing():
-                return self._launch_captured(out, need)
-            # the old ones stay: captured graphs know their addresses (each at least twice the last, so all
-            # together are less than two of the newest)
-            self.workspace = torch.zeros(max(need, 2 * a.workspace_bytes), dtype=torch.uint8, device=self.device)
+            if not self.room or self.room[-1].numel() < need:
+                if torch.cuda.is_current_stream_capturing():
+                    return self._launch_captured(out, need)
+                held = self.room[-1].numel() if self.room else 0
+                self.room.append(torch.zeros(max(need, 2 * held), dtype=torch.uint8, device=self.device))
+            else:  # made by a call of another operator, on whatever stream
+                self.room[-1].record_stream(torch.cuda.current_stream(self.device))
+            self.workspace = self.room[-1]
             self.own.append(self.workspace)
             a.workspace, a.workspace_bytes = self.workspace.data_ptr(), self.workspace.numel()
         self.layout = layout
@@ -455,8 +464,8 @@ class SharedAttention(Attention):
     """
 
     def __init__(self, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
-                 q_heads: int, scale: Optional[float] = None):
-        super().__init__(k_cache, v_cache, table, lens, q_heads, scale)
+                 q_heads: int, scale: Optional[float] = None, share: Optional[Attention] = None):
+        super().__init__(k_cache, v_cache, table, lens, q_heads, scale, share=share)
         self.groups = _native.SharedArgs()
 
     def __call__(self, q: torch.Tensor, out: Optional[torch.Tensor] = None, cu_q: Optional[torch.Tensor] = None,

@@ -80,7 +80,8 @@ class PagedDecoder:
         if step.cu_group is None or self.window:
             return lay["attn"](q, None, step.cu_q, max_q=step.max_q, max_ctx=step.max_ctx, seq_ids=step.seq_ids)
         if "shared" not in lay:
-            lay["shared"] = SharedAttention(lay["k"], lay["v"], self.cache.table, self.cache.lens, q_heads=HEADS)
+            lay["shared"] = SharedAttention(lay["k"], lay["v"], self.cache.table, self.cache.lens, q_heads=HEADS,
+                                            share=self.layers[0].get("shared"))  # the layers run one after another
         return lay["shared"](q, None, step.cu_q, step.cu_group, step.prefix_lens, max_q=step.max_q,
                              max_ctx=step.max_ctx, max_prefix=step.max_prefix, seq_ids=step.seq_ids)
 
