@@ -14,7 +14,10 @@ constexpr int kMostThreads = 512;
 constexpr int kMostParts = 8;  // CTAs of a row, a cluster
 constexpr int kUnit = 16;       // logits of a lane and step
 constexpr int kGroups = 64;     // of a row's threads, at most
-constexpr int kCandidates = 1024;
+constexpr int kCandidates = 1024;  // of a CTA, for the likeliest
+constexpr int kReach = 48;         // threads whose largest reach the bound that are looked at without a better one
+constexpr int kFew = 64;           // ... that go to the first CTA as they are
+static_assert(Q4GPU_TOP_MAX <= kFew && kCandidates * 8 <= 64 * kUnit * 2 * 4, "the candidates fit in the smallest ring");
 static_assert(Q4GPU_TOP_MAX <= kGroups, "a group for each of the likeliest");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -223,7 +226,7 @@ struct Record {
 // What the CTAs of a row tell each other.
 struct Board {
   uint64_t group[kGroups];  // the largest of each group of threads
-  uint64_t key[kCandidates];
+  uint64_t key[kMostParts * kFew];
   Record record[kMostParts * kMostThreads / 32];
   int found;
 };
@@ -237,7 +240,9 @@ struct Board {
 // Of the likeliest only each thread's largest is followed on the way.  The top-th of the largest of 32 or 64 groups of
 // threads bounds the top-th of all from below, and about as many logits as are wanted lie above it: the units with the
 // few threads' largest that do are read again, from L2 (all of a thread's units where a second one's does), and what
-// lies above the bound is ranked by counting.
+// lies above the bound is ranked by counting.  A CTA whose many threads reach the bound goes by the top-th of those.
+// Only where a few threads hold more than 1024 of the logits above it (large ones at a distance that is a multiple of
+// 16 times the threads) the first CTA takes one after another over the whole row.
 // 2048 rows of 151936 in bf16 take 160 us (3.9 TB/s), bound by instructions (63400 of a warp's a row with a target and 5
 // alternatives, which fill 64 % of the issue slots) and by a row's beginning and end, 11 of its 24 us beside one other
 // CTA; 1024 rows in float32 112 us (5.6 TB/s), bound by memory.
@@ -248,7 +253,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   __shared__ Board s_board;
   __shared__ uint64_t s_bound, s_top[Q4GPU_TOP_MAX];
   __shared__ uint16_t s_thread[kMostThreads];
-  __shared__ int s_unit[kMostThreads], s_threads, s_units;
+  __shared__ int s_unit[kMostThreads], s_threads, s_units, s_found;
   __shared__ float s_first[kMostThreads / 32];
   __shared__ Record s_all;
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   const bool tie = known && mine_unit >= u0 && mine_unit < u1 && warp == ((mine_unit - u0) & (threads - 1)) >> 5 &&
                    lane < (int)given - near && to_f32(x[near + lane]) == to_f32(mine);
   if (tid < kGroups) s_board.group[tid] = 0;
-  if (tid == 0) s_board.found = s_threads = s_units = 0;
+  if (tid == 0) s_board.found = s_threads = s_units = s_found = 0;
   __syncwarp();  // (the cluster's barriers are for whole warps, and lanes have taken ways of their own)
   if (parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   auto board = [&](int p) {  // part p's
@@ -447,6 +452,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
       for (int p = 0; p < parts; ++p) board(p)->group[g] = group;
     }
   }
+  uint64_t* const list = reinterpret_cast<uint64_t*>(ring);  // (its logits are read) this CTA's candidates
   auto meet = [&] {  // of the row's CTAs
     __syncwarp();
     if (parts > 1)
@@ -464,20 +470,42 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     for (int o = 1; o < peers; o <<= 1) before += __shfl_xor_sync(~0u, before, o);
     if (before == a.top - 1) s_bound = k;
     __syncthreads();
-    const uint64_t bound = s_bound;
-    const uint32_t bound_value = (uint32_t)(bound >> 32);
-    auto found = [&](uint64_t k) {
-      const int n = atomicAdd(&s_board.found, 1);
-      if (n < kCandidates) s_board.key[n] = k;
-    };
-    if (end_there && end_key >= (bound & ~0xffffffffull)) found(end_key);
-    if (key && key >= bound) {  // mostly one unit is all there is to look at
-      if (most == most && order_of(second) < bound_value)
+    uint64_t bound = s_bound;
+    auto look = [&] {  // threads that reach the bound; mostly one unit is all there is to look at
+      if (!key || key < bound) return;
+      if (most == most && order_of(second) < (uint32_t)(bound >> 32))
         s_unit[atomicAdd(&s_units, 1)] = most_unit;
       else
         s_thread[atomicAdd(&s_threads, 1)] = (uint16_t)tid;
-    }
+    };
+    look();
     __syncthreads();
+    // Mostly they are few.  Where they are many (equal logits, as masks leave them, or logits that fall or rise along the
+    // row) the top-th of theirs is the better bound: this CTA has no more to offer.
+    const int reach = s_units + s_threads;
+    if (reach > kReach) {
+      __syncthreads();
+      if (tid == 0) s_units = s_threads = 0;
+      __syncthreads();
+      if (key && key >= bound) list[atomicAdd(&s_threads, 1)] = key;
+      __syncthreads();
+      if (key && key >= bound) {
+        int rank = 0;
+        for (int i = 0; i < reach; ++i) rank += list[i] > key;
+        if (rank == a.top - 1) s_bound = key;
+      }
+      if (tid == 0) s_threads = 0;
+      __syncthreads();
+      bound = s_bound;
+      look();
+      __syncthreads();
+    }
+    const uint32_t bound_value = (uint32_t)(bound >> 32);
+    auto found = [&](uint64_t k) {
+      const int n = atomicAdd(&s_found, 1);
+      if (n < kCandidates) list[n] = k;
+    };
+    if (end_there && end_key >= (bound & ~0xffffffffull)) found(end_key);
     const int single = s_units, looks = single + s_threads * steps;
     for (int i = tid; i < looks; i += threads) {
       const int j = i - single, k = j / max(steps, 1);
@@ -494,22 +522,35 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
     }
     if (part != 0) {  // to the first CTA together: one trip for the place, one for the keys
       __syncthreads();
-      if (tid == 0) s_units = atomicAdd(&first->found, s_board.found);
+      const int n = s_found;
+      const uint64_t* from = list;
+      int give = n;
+      if (n > kFew && n <= kCandidates) {  // the first `top` of them
+        for (int i = tid; i < n; i += threads) {
+          const uint64_t k = list[i];
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += list[j] > k;
+          if (rank < a.top) s_top[rank] = k;
+        }
+        from = s_top, give = a.top;
+      }
+      if (tid == 0) s_units = atomicAdd(&first->found, n > kCandidates ? kMostParts * kFew + 1 : give);
       __syncthreads();
-      for (int i = tid; i < min(s_board.found, kCandidates); i += threads)
-        if (s_units + i < kCandidates) first->key[s_units + i] = s_board.key[i];
+      if (n <= kCandidates)
+        for (int i = tid; i < give; i += threads) first->key[min(s_units + i, kMostParts * kFew - 1)] = from[i];
     }
   }
   meet();
   if (part != 0) return;
 
   // the first CTA has everything
-  const int n = a.top ? s_board.found : 0;
-  if (n <= kCandidates) {
+  const int own = a.top ? s_found : 0, n = own + (a.top ? s_board.found : 0);
+  if (own <= kCandidates && n - own <= kMostParts * kFew) {
     for (int i = tid; i < n; i += threads) {
-      const uint64_t k = s_board.key[i];
+      const uint64_t k = i < own ? list[i] : s_board.key[i - own];
       int rank = 0;
-      for (int j = 0; j < n; ++j) rank += s_board.key[j] > k;
+      for (int j = 0; j < own; ++j) rank += list[j] > k;
+      for (int j = own; j < n; ++j) rank += s_board.key[j - own] > k;
       if (rank < a.top) s_top[rank] = k;
     }
   } else {  // many of a few threads' logits: one after another over the whole row

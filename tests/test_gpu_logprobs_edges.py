@@ -102,3 +102,52 @@ def test_candidates_of_single_lanes(dtype, rows):
     units[-1, -7:, 9] = 42.0
     for _ in range(3):
         check(x, 20)
+
+
+@pytest.mark.parametrize("rows,every,width", [(1, 512, 24), (64, 512, 8), (300, 512, 4)])
+@pytest.mark.parametrize("what", [math.nan, 50.0])
+def test_many_large_ones_in_a_few_threads_of_a_cluster(rows, every, width, what):
+    """Likewise where 8, 2 or one CTA share a row, and in other rows not."""
+    x = normal(rows, 151936, SF, 1)
+    for r in {0, rows // 2}:
+        x[r].view(-1, 16)[torch.arange(151936 // 16, device="cuda") % every < width] = what
+    check(x, 5)
+    check(x, 32)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF])
+@pytest.mark.parametrize("rows,vocab", [(1, 151936), (64, 151936), (300, 151936), (1, 1100), (40, 32001), (700, 4099)])
+@pytest.mark.parametrize("left", [0, 1, 3, 10, 40])
+@pytest.mark.parametrize("low", ["infinity", "lowest"])
+def test_masks_that_leave_few(dtype, rows, vocab, left, low):
+    """Fewer tokens are allowed than alternatives are asked for: what is masked follows by rising index."""
+    x = torch.full((rows, vocab), -math.inf if low == "infinity" else torch.finfo(dtype).min, dtype=dtype, device="cuda")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(left)
+    for r in range(min(rows, 8)):
+        at = torch.randperm(vocab, device="cuda", generator=g)[:left]
+        x[r, at] = torch.randn(left, device="cuda", generator=g).to(dtype)
+    for top in (1, 5, 20, 32):
+        check(x, top)
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("rows", [1, 64, 300])
+@pytest.mark.parametrize("kind", ["block", "rising", "falling", "constant", "stairs", "two values"])
+def test_likeliest_that_stand_together(dtype, rows, kind):
+    """A block of allowed tokens, logits in order, equal ones: many threads reach what a group's largest bounds."""
+    vocab = 151936
+    x = normal(rows, vocab, dtype, 2)
+    at = torch.arange(vocab, device="cuda")
+    if kind == "block":
+        x[:, :5000], x[:, 9000:] = -math.inf, -math.inf
+    elif kind == "constant":
+        x[:] = 1.5
+    elif kind == "stairs":
+        x[:] = (at // 1000).to(dtype)
+    elif kind == "two values":
+        x[:] = (x > 0).to(dtype)
+    else:
+        x[:] = (at if kind == "rising" else -at).float().mul(1e-4).to(dtype)
+    for top in (1, 5, 20, 32):
+        check(x, top)
