@@ -797,7 +797,7 @@ class PagedCache:
 
     def _together(self, runs: Sequence[tuple[int, int]], counts: Sequence[int]) -> int:
         """The most keys that a run of a step shares, if its runs are worth attending to together, else 0."""
-        new = max(counts)
+        new = max(1, *counts)
         if new > self.NEW_TOKENS:
             return 0
         prefix = max((p for _, p in runs), default=0) * self.page_tokens

@@ -48,3 +48,9 @@ def test_the_rule_can_be_moved():
     assert c._together([(2, 1)], [1, 1]) == 0
     c.SHARED_KEYS = 16
     assert c._together([(2, 1)], [1, 1]) == 16 and c._together([(1, 0), (1, 0)], [1, 1]) == 0
+
+
+def test_a_step_without_tokens():
+    """Weighs what is not read again like a step of single tokens."""
+    assert together(2, 256, [0, 0]) == 0 and together(16, 256, [0] * 16) == 0
+    assert together(64, 256, [0] * 64) == 64 * 4
