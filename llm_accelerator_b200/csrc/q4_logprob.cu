@@ -610,8 +610,8 @@ __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_l
   }
 }
 
-// CTAs of a row and threads of a CTA.  A thread has at least two units where there are as many, since a warp's start
-// and end take as long as six steps (us; 700 rows of 4099: 8.7 with 128 threads, 11.4 with 256; 4000 of 32000: 128 with
+// CTAs of a row and threads of a CTA.  More than 128 threads have at least four units each (alone, one in a cluster),
+// since a warp's start and end take as long as six steps (us; 700 rows of 4099: 8.7 with 128 threads, 11.4 with 256; 4000 of 32000: 128 with
 // 256, 137 with 128, 157 with 512; 2048 of 151936: 164 with 512, 171 with 256).  Few rows take a cluster each, as long
 // as that gives no SM a second CTA: clusters wait for one another's SMs (one row of 151936 floats: 17.1 alone, 14.3,
 // 12.1 and 11.1 with 2, 4 and 8 CTAs; 64 rows: 21.2, 17.6, 18.7, 30.2).
