@@ -323,7 +323,7 @@ int q4gpu_sink_attention(const q4gpu_attn_args *a, int32_t sinks, void *stream);
  * Results are those of q4gpu_paged_attention (window = 0) over tables that name
  * the same keys.  What only the device sees is checked as there; besides, *err_flag becomes 1
  * where cu_group or prefix_lens is out of range (where cu_group or cu_q does not
- * ascend, all rows become zeros and -infinity), where the first sequence's slot
+ * ascend, the rows of all sequences become zeros and -infinity), where the first sequence's slot
  * holds fewer keys than are shared (those that are there count), and where a sequence's
  * queries do not stand behind the shared keys (its rows become zeros and
  * -infinity, as do those of a sequence with more than max_q queries).

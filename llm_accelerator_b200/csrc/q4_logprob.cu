@@ -243,8 +243,8 @@ struct Board {
 // lies above the bound is ranked by counting.  A CTA whose many threads reach the bound goes by the top-th of those.
 // Only where a few threads hold more than 1024 of the logits above it (large ones at a distance that is a multiple of
 // 16 times the threads) the first CTA takes one after another over the whole row.
-// 2048 rows of 151936 in bf16 take 160 us (3.9 TB/s), bound by instructions (63400 of a warp's a row with a target and 5
-// alternatives, which fill 64 % of the issue slots) and by a row's beginning and end, 11 of its 24 us beside one other
+// 2048 rows of 151936 in bf16 take 165 us (3.8 TB/s), bound by instructions (63700 of a warp's a row with a target and 5
+// alternatives, which fill 65 % of the issue slots) and by a row's beginning and end, 11 of its 24 us beside one other
 // CTA; 1024 rows in float32 112 us (5.6 TB/s), bound by memory.
 template <typename T>
 __global__ void __launch_bounds__(kMostThreads, 2) token_logprobs_kernel(q4gpu_logprob_args a, int parts) {
