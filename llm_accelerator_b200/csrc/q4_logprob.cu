@@ -123,12 +123,13 @@ struct Counter<float> {
   }
   __device__ __forceinline__ void flush() {}
 };
-// The next value of the type above v (NaN above infinity).
+// The next value of the type above v (NaN above infinity, and above NaN, whose next bits may be those of a zero).
 template <typename T>
 __device__ __forceinline__ T above(T v) {
   using B = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
   constexpr B kSign = (B)1 << (sizeof(T) * 8 - 1);
   B b = *reinterpret_cast<const B*>(&v);
+  if (to_f32(v) != to_f32(v)) return v;
   if (b == kSign) b = 0;  // the zeros are one
   b = b & kSign ? b - 1 : b + 1;
   return *reinterpret_cast<const T*>(&b);

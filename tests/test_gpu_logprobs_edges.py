@@ -151,3 +151,24 @@ def test_likeliest_that_stand_together(dtype, rows, kind):
         x[:] = (at if kind == "rising" else -at).float().mul(1e-4).to(dtype)
     for top in (1, 5, 20, 32):
         check(x, top)
+
+
+@pytest.mark.parametrize("dtype,ints,patterns", [
+    (BF, torch.int16, (0x7fc0, 0x7fff, 0x7f81, -0x40, -1)), (HF, torch.int16, (0x7e00, 0x7fff, 0x7c01, -0x200, -1)),
+    (SF, torch.int32, (0x7fc00000, 0x7fffffff, 0x7f800001, -0x400000, -1))])
+@pytest.mark.parametrize("rows,vocab", [(40, 570), (3, 40), (64, 5000), (1, 151936)])
+def test_targets_that_are_nan(dtype, ints, patterns, rows, vocab):
+    """NaN of any bits comes first in the order: its rank counts the NaNs before it and nothing else."""
+    for bits in patterns:
+        x = normal(rows, vocab, dtype, 3)
+        at = sorted({vocab // 7, vocab // 2, vocab - 1})
+        for i in at:
+            x.view(ints)[:, i] = bits
+        assert x[0, at].isnan().all()
+        op = paged.TokenLogprobs()
+        for k, i in enumerate(at):
+            got = op(x, torch.full((rows,), i, device="cuda"))
+            assert (got.rank == k + 1).all() and got.logprob.isnan().all()
+        rest = op(x, torch.zeros(rows, dtype=torch.int64, device="cuda"))  # and before every number
+        v = x.double()
+        assert torch.equal(rest.rank.long(), 1 + ((v > v[:, :1]) | v.isnan()).sum(-1))
